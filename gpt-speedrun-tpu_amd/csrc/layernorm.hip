@@ -1,0 +1,484 @@
+// Layer normalisation over the last dimension, forward and backward:
+//   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r
+//   y  = h scale + bias
+//   g  = dy scale;  dx = r (g - mean(g) - h mean(g h))
+//   dscale = sum over rows of dy h;  dbias = sum over rows of dy
+// Everything between the loads and the stores is float32 (the mean first, then
+// the squares of the differences from it), so each output is rounded once, to
+// its own type.  Rows of any width, row stride and alignment: a row is read in
+// 16-byte pieces wherever it starts (the loads need no alignment here), its last
+// few values one by one.
+#include "common.h"
+
+namespace {
+
+enum { kBf16 = GPTRIG_TYPE_BF16, kF32 = GPTRIG_TYPE_F32 };
+
+// N values of type T from a place of any alignment.
+template <typename T, int N>
+struct __attribute__((packed)) Piece {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_piece(float (&out)[N], const T* __restrict__ row, int at, int d) {
+  if (at + N <= d) {
+    const Piece<T, N> p = *reinterpret_cast<const Piece<T, N>*>(row + at);
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = (float)p.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = at + j < d ? (float)row[at + j] : 0.f;
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_piece(T* __restrict__ row, const float (&v)[N], int at, int d) {
+  if (at + N <= d) {
+    Piece<T, N> p;
+#pragma unroll
+    for (int j = 0; j < N; ++j) p.v[j] = (T)v[j];
+    *reinterpret_cast<Piece<T, N>*>(row + at) = p;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (at + j < d) row[at + j] = (T)v[j];
+  }
+}
+
+// Sum over the L lanes that share a row; every one of them gets it.  L = 256 (a
+// whole workgroup) goes through red[4], which the caller keeps apart from the
+// previous sum's.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = (L < 64 ? L : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0] + red[1] + red[2] + red[3];
+  }
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// Forward: L lanes hold a row, C pieces of V = 16 bytes each.
+// ---------------------------------------------------------------------------
+template <typename T, typename P, int L, int C>
+__global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx,
+                                                            const P* __restrict__ scale, const P* __restrict__ bias,
+                                                            T* __restrict__ y, float* __restrict__ mean,
+                                                            float* __restrict__ rstd, int64_t rows, int d, float eps) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float red[2][4];
+  const int lane = threadIdx.x % L;
+  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (row >= rows) return;  // (with L = 256 the whole workgroup)
+  const T* xr = x + row * ldx;
+  float v[C][V];
+  float sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    load_piece<T, V>(v[c], xr, V * (lane + L * c), d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum += v[c][j];
+  }
+  const float mu = row_sum<L>(sum, red[0]) / (float)d;
+  float sq = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      v[c][j] -= mu;
+      if (V * (lane + L * c) + j < d) sq += v[c][j] * v[c][j];
+    }
+  const float r = rsqrtf(row_sum<L>(sq, red[1]) / (float)d + eps);
+  if (lane == 0 && mean) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int at = V * (lane + L * c);
+    if (at >= d) break;
+    float s[V], b[V];
+    load_piece<P, V>(s, scale, at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) b[j] = 0.f;
+    if (bias) load_piece<P, V>(b, bias, at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = fmaf(v[c][j] * r, s[j], b[j]);
+    store_piece<T, V>(y + row * d, s, at, d);
+  }
+}
+
+// Rows wider than the registers of a workgroup: three passes over the row, the
+// later two from the caches.
+template <typename T, typename P>
+__global__ void __launch_bounds__(256) layernorm_fwd_wide_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                 const P* __restrict__ scale,
+                                                                 const P* __restrict__ bias, T* __restrict__ y,
+                                                                 float* __restrict__ mean, float* __restrict__ rstd,
+                                                                 int d, float eps) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float red[2][4];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  float v[V];
+  float sum = 0.f;
+  for (int64_t at = V * threadIdx.x; at < d; at += V * 256) {
+    load_piece<T, V>(v, xr, (int)at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum += v[j];
+  }
+  const float mu = row_sum<256>(sum, red[0]) / (float)d;
+  float sq = 0.f;
+  for (int64_t at = V * threadIdx.x; at < d; at += V * 256) {
+    load_piece<T, V>(v, xr, (int)at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (at + j < d) sq += (v[j] - mu) * (v[j] - mu);
+  }
+  const float r = rsqrtf(row_sum<256>(sq, red[1]) / (float)d + eps);
+  if (threadIdx.x == 0 && mean) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+  for (int64_t at = V * threadIdx.x; at < d; at += V * 256) {
+    float s[V], b[V];
+    load_piece<T, V>(v, xr, (int)at, d);
+    load_piece<P, V>(s, scale, (int)at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) b[j] = 0.f;
+    if (bias) load_piece<P, V>(b, bias, (int)at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = fmaf((v[j] - mu) * r, s[j], b[j]);
+    store_piece<T, V>(y + row * d, s, (int)at, d);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward.  A workgroup walks rows with the same columns in the same lanes, so
+// the column sums of dy h and dy stay in registers; they are joined over the
+// workgroup in LDS at the end and leave as one partial row, and
+// layernorm_columns_kernel adds the partial rows in a fixed order (no atomics:
+// the gradients are the same on every run).
+// ---------------------------------------------------------------------------
+template <typename T, typename P, int L, int C>
+__global__ void __launch_bounds__(256)
+    layernorm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
+                         const P* __restrict__ scale, const float* __restrict__ mean, const float* __restrict__ rstd,
+                         T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int d) {
+  constexpr int V = 16 / sizeof(T), G = 256 / L;  // G rows at a time
+  __shared__ float red[2][2][4];
+  __shared__ float join[G > 1 ? G : 1][G > 1 ? L * V : 1];
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  float ds[C][V], db[C][V], s[C][V];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    load_piece<P, V>(s[c], scale, V * (lane + L * c), d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) ds[c][j] = db[c][j] = 0.f;
+  }
+  const float inv_d = 1.f / (float)d;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * G + group; row < rows; row += (int64_t)gridDim.x * G, turn ^= 1) {
+    const T* gr = dy + row * lddy;
+    const T* xr = x + row * ldx;
+    const float mu = mean[row], r = rstd[row];
+    float g[C][V], h[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      load_piece<T, V>(g[c], gr, V * (lane + L * c), d);
+      load_piece<T, V>(h[c], xr, V * (lane + L * c), d);
+    }
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        // (Past the row's end dy is 0 and so is everything summed here.)
+        h[c][j] = (h[c][j] - mu) * r;
+        db[c][j] += g[c][j];
+        ds[c][j] = fmaf(g[c][j], h[c][j], ds[c][j]);
+        g[c][j] *= s[c][j];
+        a += g[c][j];
+        b = fmaf(g[c][j], h[c][j], b);
+      }
+    if (dx) {
+      a = row_sum<L>(a, red[turn][0]) * inv_d;
+      b = row_sum<L>(b, red[turn][1]) * inv_d;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int at = V * (lane + L * c);
+        if (at < d) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[c][j] = r * (g[c][j] - a - h[c][j] * b);
+          store_piece<T, V>(dx + row * d, g[c], at, d);
+        }
+      }
+    }
+  }
+  if (!partial) return;
+  float* const out = partial + (size_t)blockIdx.x * 2 * d;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      if constexpr (G > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) join[group][V * lane + j] = which ? db[c][j] : ds[c][j];
+        __syncthreads();
+        for (int i = threadIdx.x; i < L * V; i += 256) {
+          float t = 0.f;
+#pragma unroll
+          for (int k = 0; k < G; ++k) t += join[k][i];
+          if (L * V * c + i < d) out[(size_t)which * d + L * V * c + i] = t;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int at = V * (lane + L * c) + j;
+          if (at < d) out[(size_t)which * d + at] = which ? db[c][j] : ds[c][j];
+        }
+      }
+    }
+}
+
+// Wide rows: dx with two passes over each row ...
+template <typename T, typename P>
+__global__ void __launch_bounds__(256)
+    layernorm_bwd_wide_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
+                              const P* __restrict__ scale, const float* __restrict__ mean,
+                              const float* __restrict__ rstd, T* __restrict__ dx, int d) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float red[2][4];
+  const int64_t row = blockIdx.x;
+  const T* gr = dy + row * lddy;
+  const T* xr = x + row * ldx;
+  const float mu = mean[row], r = rstd[row];
+  float g[V], h[V], s[V];
+  float a = 0.f, b = 0.f;
+  for (int64_t at = V * threadIdx.x; at < d; at += V * 256) {
+    load_piece<T, V>(g, gr, (int)at, d);
+    load_piece<T, V>(h, xr, (int)at, d);
+    load_piece<P, V>(s, scale, (int)at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float t = g[j] * s[j];
+      a += t;
+      b = fmaf(t, (h[j] - mu) * r, b);
+    }
+  }
+  a = row_sum<256>(a, red[0]) / (float)d;
+  b = row_sum<256>(b, red[1]) / (float)d;
+  for (int64_t at = V * threadIdx.x; at < d; at += V * 256) {
+    load_piece<T, V>(g, gr, (int)at, d);
+    load_piece<T, V>(h, xr, (int)at, d);
+    load_piece<P, V>(s, scale, (int)at, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) g[j] = r * (g[j] * s[j] - a - (h[j] - mu) * r * b);
+    store_piece<T, V>(dx + row * d, g, (int)at, d);
+  }
+}
+
+// ... and the column sums over blocks of rows: blockIdx.x the columns (V a
+// thread), blockIdx.y the block of rows.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    layernorm_bwd_wide_columns_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
+                                      const float* __restrict__ mean, const float* __restrict__ rstd,
+                                      float* __restrict__ partial, int64_t rows, int d) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t at = (int64_t)V * (blockIdx.x * 256 + threadIdx.x);
+  if (at >= d) return;
+  float ds[V], db[V], g[V], h[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) ds[j] = db[j] = 0.f;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    load_piece<T, V>(g, dy + row * lddy, (int)at, d);
+    load_piece<T, V>(h, x + row * ldx, (int)at, d);
+    const float mu = mean[row], r = rstd[row];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ds[j] = fmaf(g[j], (h[j] - mu) * r, ds[j]);
+      db[j] += g[j];
+    }
+  }
+  float* const out = partial + (size_t)blockIdx.y * 2 * d;
+  store_piece<float, V>(out, ds, (int)at, d);
+  store_piece<float, V>(out + d, db, (int)at, d);
+}
+
+// dscale and dbias from the partial rows: 16 columns of one of the two by 16
+// slices of the partial rows per workgroup.
+template <typename P>
+__global__ void __launch_bounds__(256) layernorm_columns_kernel(const float* __restrict__ partial, int parts, int d,
+                                                                P* __restrict__ dscale, P* __restrict__ dbias) {
+  __shared__ float red[16][17];
+  P* const out = blockIdx.y ? dbias : dscale;
+  if (!out) return;
+  const int lane = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + lane;
+  float s = 0.f;
+  if (col < d) {
+    const float* p = partial + (size_t)blockIdx.y * d + col;
+#pragma unroll 8
+    for (int i = slice; i < parts; i += 16) s += p[(size_t)i * 2 * d];
+  }
+  red[slice][lane] = s;
+  __syncthreads();
+  if (slice == 0 && col < d) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][lane];
+    out[col] = (P)s;
+  }
+}
+
+// Lanes a row and pieces a lane for pieces of V values: the fewest idle lanes
+// among 32 lanes of up to 4 pieces, then 64, then a workgroup of up to 4; {0, 0}
+// for wider rows.
+struct Shape {
+  int lanes, pieces;
+};
+Shape row_shape(int d, int v) {
+  const int pieces = ceil_div(d, v);
+  if (pieces <= 128) return {32, ceil_div(pieces, 32)};
+  if (pieces <= 256) return {64, ceil_div(pieces, 64)};
+  if (pieces <= 1024) return {256, ceil_div(pieces, 256)};
+  return {0, 0};
+}
+
+constexpr int kParts = 512;  // partial rows at most: two workgroups a CU
+
+int parts_of(int64_t rows, int d, int v) {
+  const Shape s = row_shape(d, v);
+  const int64_t groups = s.lanes ? (rows + 256 / s.lanes - 1) / (256 / s.lanes) : rows;
+  return (int)(groups < 1 ? 1 : groups < kParts ? groups : kParts);
+}
+
+#define LN_SHAPES(CALL)                                                                             \
+  switch (sh.lanes * 8 + sh.pieces) {                                                               \
+    case 32 * 8 + 1: CALL(32, 1); break;                                                            \
+    case 32 * 8 + 2: CALL(32, 2); break;                                                            \
+    case 32 * 8 + 3: CALL(32, 3); break;                                                            \
+    case 32 * 8 + 4: CALL(32, 4); break;                                                            \
+    case 64 * 8 + 3: CALL(64, 3); break;                                                            \
+    case 64 * 8 + 4: CALL(64, 4); break;                                                            \
+    case 256 * 8 + 2: CALL(256, 2); break;                                                          \
+    case 256 * 8 + 3: CALL(256, 3); break;                                                          \
+    case 256 * 8 + 4: CALL(256, 4); break;                                                          \
+  }
+
+template <typename T, typename P>
+void launch_fwd(const void* x, int64_t ldx, const void* scale, const void* bias, void* y, float* mean, float* rstd,
+                int64_t rows, int d, float eps, hipStream_t st) {
+  const Shape sh = row_shape(d, 16 / sizeof(T));
+  if (!sh.lanes) {
+    layernorm_fwd_wide_kernel<T, P><<<(unsigned)rows, 256, 0, st>>>((const T*)x, ldx, (const P*)scale, (const P*)bias,
+                                                                    (T*)y, mean, rstd, d, eps);
+    return;
+  }
+  const unsigned grid = (unsigned)((rows + 256 / sh.lanes - 1) / (256 / sh.lanes));
+#define LN_FWD(L, C)                                                                                             \
+  layernorm_fwd_kernel<T, P, L, C><<<grid, 256, 0, st>>>((const T*)x, ldx, (const P*)scale, (const P*)bias, (T*)y, \
+                                                         mean, rstd, rows, d, eps)
+  LN_SHAPES(LN_FWD)
+#undef LN_FWD
+}
+
+template <typename T, typename P>
+void launch_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* scale, const float* mean,
+                const float* rstd, void* dx, void* dscale, void* dbias, float* partial, int64_t rows, int d,
+                hipStream_t st) {
+  const Shape sh = row_shape(d, 16 / sizeof(T));
+  const int parts = parts_of(rows, d, 16 / sizeof(T));
+  if (!dscale && !dbias) partial = nullptr;
+  if (rows > 0) {
+    if (sh.lanes) {
+#define LN_BWD(L, C)                                                                                              \
+  layernorm_bwd_kernel<T, P, L, C><<<dx && !partial ? (unsigned)((rows + 256 / L - 1) / (256 / L)) : (unsigned)parts, \
+                                     256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx, (const P*)scale, mean, rstd, \
+                                                   (T*)dx, partial, rows, d)
+      LN_SHAPES(LN_BWD)
+#undef LN_BWD
+    } else {
+      if (dx)
+        layernorm_bwd_wide_kernel<T, P><<<(unsigned)rows, 256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx,
+                                                                        (const P*)scale, mean, rstd, (T*)dx, d);
+      if (partial)
+        layernorm_bwd_wide_columns_kernel<T>
+            <<<dim3(ceil_div(d, 256 * (16 / sizeof(T))), parts), 256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx, mean,
+                                                                              rstd, partial, rows, d);
+    }
+  }
+  if (partial)
+    layernorm_columns_kernel<P><<<dim3(ceil_div(d, 16), 2), 256, 0, st>>>(partial, rows > 0 ? parts : 0, d, (P*)dscale,
+                                                                          (P*)dbias);
+}
+
+bool type_ok(int t) { return t == kBf16 || t == kF32; }
+bool aligned(const void* p, int type) { return ((uintptr_t)p & (type == kBf16 ? 1 : 3)) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int gptrig_layernorm_fwd(const void* x, int64_t ldx, int x_type, const void* scale, const void* bias, int param_type,
+                         void* y, float* mean, float* rstd, int64_t rows, int d, float eps, void* stream) {
+  if (!x || !scale || !y || (mean == nullptr) != (rstd == nullptr)) return GPTRIG_E_NULL;
+  if (!type_ok(x_type) || !type_ok(param_type)) return GPTRIG_E_DTYPE;
+  if (rows < 0 || rows > INT32_MAX || d <= 0 || d > (1 << 30) || ldx < 0 || !(eps >= 0.f)) return GPTRIG_E_SHAPE;
+  if (!aligned(x, x_type) || !aligned(y, x_type) || !aligned(scale, param_type) || !aligned(bias, param_type))
+    return GPTRIG_E_SHAPE;
+  if (rows == 0) return GPTRIG_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (x_type == kBf16 && param_type == kBf16)
+    launch_fwd<bf16, bf16>(x, ldx, scale, bias, y, mean, rstd, rows, d, eps, s);
+  else if (x_type == kBf16)
+    launch_fwd<bf16, float>(x, ldx, scale, bias, y, mean, rstd, rows, d, eps, s);
+  else if (param_type == kBf16)
+    launch_fwd<float, bf16>(x, ldx, scale, bias, y, mean, rstd, rows, d, eps, s);
+  else
+    launch_fwd<float, float>(x, ldx, scale, bias, y, mean, rstd, rows, d, eps, s);
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
+}
+
+size_t gptrig_layernorm_bwd_workspace_bytes(int64_t rows, int d, int x_type) {
+  if (rows < 0 || d <= 0 || !type_ok(x_type)) return 0;
+  return (size_t)parts_of(rows, d, x_type == kBf16 ? 8 : 4) * 2 * d * sizeof(float);
+}
+
+int gptrig_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int x_type, const void* scale,
+                         int param_type, const float* mean, const float* rstd, void* dx, void* dscale, void* dbias,
+                         void* workspace, size_t workspace_bytes, int64_t rows, int d, void* stream) {
+  if (!dy || !x || !scale || !mean || !rstd) return GPTRIG_E_NULL;
+  if (!type_ok(x_type) || !type_ok(param_type)) return GPTRIG_E_DTYPE;
+  if (rows < 0 || rows > INT32_MAX || d <= 0 || d > (1 << 30) || ldx < 0 || lddy < 0) return GPTRIG_E_SHAPE;
+  if (!aligned(dy, x_type) || !aligned(x, x_type) || !aligned(dx, x_type) || !aligned(scale, param_type) ||
+      !aligned(dscale, param_type) || !aligned(dbias, param_type) || ((uintptr_t)workspace & 15))
+    return GPTRIG_E_SHAPE;
+  if (dscale || dbias) {
+    if (!workspace) return GPTRIG_E_NULL;
+    if (workspace_bytes < gptrig_layernorm_bwd_workspace_bytes(rows, d, x_type)) return GPTRIG_E_WORKSPACE;
+  } else if (!dx || rows == 0) {
+    return GPTRIG_OK;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  float* const ws = (float*)workspace;
+  if (x_type == kBf16 && param_type == kBf16)
+    launch_bwd<bf16, bf16>(dy, lddy, x, ldx, scale, mean, rstd, dx, dscale, dbias, ws, rows, d, s);
+  else if (x_type == kBf16)
+    launch_bwd<bf16, float>(dy, lddy, x, ldx, scale, mean, rstd, dx, dscale, dbias, ws, rows, d, s);
+  else if (param_type == kBf16)
+    launch_bwd<float, bf16>(dy, lddy, x, ldx, scale, mean, rstd, dx, dscale, dbias, ws, rows, d, s);
+  else
+    launch_bwd<float, float>(dy, lddy, x, ldx, scale, mean, rstd, dx, dscale, dbias, ws, rows, d, s);
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
+}
+
+}  // extern "C"

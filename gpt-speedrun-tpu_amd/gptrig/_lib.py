@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p, c_char_p
+from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p, c_char_p
 
 import torch
 
@@ -20,6 +20,8 @@ I = c_int
 L = c_int64
 F = c_float
 Z = c_size_t
+N = c_double
+U = c_uint32
 
 
 class WGrad(ctypes.Structure):
@@ -63,6 +65,9 @@ SIGNATURES: dict[str, tuple] = {
     "gptrig_add_bias_rmsnorm_fwd": (I, [P, P, P, F, P, P, P, P, I, I, P]),
     "gptrig_rmsnorm_bwd_workspace_bytes": (Z, [I, I]),
     "gptrig_rmsnorm_bwd": (I, [P, P, P, P, P, P, P, I, P, Z, I, I, P]),
+    "gptrig_layernorm_fwd": (I, [P, L, I, P, P, I, P, P, P, L, I, F, P]),
+    "gptrig_layernorm_bwd_workspace_bytes": (Z, [L, I, I]),
+    "gptrig_layernorm_bwd": (I, [P, L, P, L, I, P, I, P, P, P, P, P, P, Z, L, I, P]),
     "gptrig_bias_grad": (I, [P, I, I, P, P]),
     "gptrig_weight_grad": (I, [P, P, P, P, I, I, I, P]),
     "gptrig_weight_grads": (I, [ctypes.POINTER(WGrad), I, I, P]),
@@ -82,6 +87,7 @@ SIGNATURES: dict[str, tuple] = {
     "gptrig_embedding_fwd": (I, [P, P, P, I, I, I, P]),
     "gptrig_embedding_bwd": (I, [P, P, P, I, I, I, P]),
     "gptrig_adamw": (I, [P, P, P, P, P, P, P, L, I, F, F, F, I, P, P, P]),
+    "gptrig_adamw_tensors": (I, [P, I, I, I, P, N, N, N, I, P, U, P]),
     "gptrig_sq_norm_partials": (I, [P, L, I, P, P]),
     "gptrig_finalize_norm": (I, [P, I, F, P, P, P, F, P, P]),
     "gptrig_transpose_bf16": (I, [P, P, I, I, P]),
@@ -141,6 +147,16 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed: {text} (status {status})")
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call(name, *args, stream)`` on ``device``'s current stream, with that device the current one."""
+
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream())
+        return
+    with torch.cuda.device(device):
+        call(name, *args, stream())
+
+
 def query(name: str, *args) -> int:
     return int(getattr(lib(), name)(*args))
 
@@ -161,6 +177,15 @@ def require_device(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("gptrig kernels run on the GPU; got a CPU tensor")
+
+
+def require_one_device(*tensors: torch.Tensor | None) -> None:
+    """All of them on one GPU."""
+
+    require_device(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise RuntimeError(f"the tensors lie on several devices: {sorted(map(str, devices))}")
 
 
 def workspace(nbytes: int, device) -> torch.Tensor:

@@ -1,17 +1,24 @@
 """Optimizer schedule and per-tensor AdamW hyper-parameters, mirroring
 ``recipes/reference/train.py:1219-1345``.
 
-The update itself is the fused ``gptrig_adamw`` kernel; this module resolves
-the host-side scalars (learning rate per step, bias corrections) and the
-per-tensor table ``{lr_mult, epsilon, decay}`` the kernel reads.
+The update itself is the fused ``gptrig_adamw`` kernel over one arena; this
+module resolves the host-side scalars (learning rate per step, bias corrections)
+and the per-tensor table ``{lr_mult, epsilon, decay}`` the kernel reads.
+``adamw_tensors`` is the same update over tensors that lie anywhere, with float32
+or 8-bit moments.
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
+from typing import Sequence
 
 import numpy as np
+import torch
+
+from . import _lib
 
 
 @dataclass(frozen=True)
@@ -104,3 +111,115 @@ def tensor_hparams(paths, cfg: OptimizerConfig, parameterization: str, width: fl
         decay = cfg.weight_decay * dec_h * dec_m if decays(path) else 0.0
         rows.append((lr_m, eps, decay))
     return np.asarray(rows, dtype=np.float32)
+
+
+# Consecutive values of a tensor that share a scale of the 8-bit moments.
+STATE_BLOCK = 256
+_STATE_TYPES = {torch.float32: 32, torch.float8_e4m3fn: 8}
+
+
+def adamw_tensors_state(params: Sequence[torch.Tensor], bits: int = 32) -> dict[str, list[torch.Tensor]]:
+    """Zero moments for ``adamw_tensors`` under its argument names: float32, or
+    float8_e4m3fn codes and their scales with ``bits=8``."""
+
+    if bits not in (8, 32):
+        raise ValueError(f"moments are held in 8 or 32 bits, got {bits}")
+    names = ("exp_avg", "exp_avg_sq")
+    if bits == 32:
+        return {n: [torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in params] for n in names}
+    state = {n: [torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn) for p in params]
+             for n in names}
+    state.update({n + "_scale": [torch.zeros(-(-p.numel() // STATE_BLOCK), dtype=torch.float32, device=p.device)
+                                 for p in params] for n in names})
+    return state
+
+
+def _list_of(name: str, tensors, like: Sequence[torch.Tensor], sizes: Sequence, dtypes, device) -> torch.dtype | None:
+    """Checks a list of tensors beside ``like``; its type (None for an empty list)."""
+
+    if len(tensors) != len(like):
+        raise ValueError(f"{name} has {len(tensors)} tensors, params {len(like)}")
+    types = {t.dtype for t in tensors}
+    if len(types) > 1 or not types <= dtypes:
+        raise TypeError(f"{name} must all be one of {sorted(map(str, dtypes))}, got {sorted(map(str, types))}")
+    for i, (t, size) in enumerate(zip(tensors, sizes)):
+        if t.shape != size:
+            raise ValueError(f"{name}[{i}] must be {tuple(size)}, got {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}[{i}] must be contiguous")
+        if t.device != device:
+            raise RuntimeError(f"{name}[{i}] is on {t.device}, params[0] on {device}")
+    return types.pop() if types else None
+
+
+def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
+                  exp_avg_sq: Sequence[torch.Tensor], hparams: torch.Tensor, *, lr: float, beta1: float, beta2: float,
+                  step: int, exp_avg_scale: Sequence[torch.Tensor] | None = None,
+                  exp_avg_sq_scale: Sequence[torch.Tensor] | None = None, clip_scale: torch.Tensor | None = None,
+                  shadow: Sequence[torch.Tensor] | None = None, seed: int | None = None) -> None:
+    """One AdamW step, in place, over a list of contiguous float32 tensors.
+
+    The update of ``GPTTrainer`` (``recipes/reference/train.py:1386-1445``), in a
+    few launches however many tensors there are.  ``hparams``: float32 ``[tensors,
+    3]`` on the device, the rows ``{lr_mult, epsilon, decay}`` of
+    ``tensor_hparams``.  ``grads``: all float32 or all bfloat16.  ``exp_avg`` and
+    ``exp_avg_sq``: both float32, or both float8_e4m3fn with the scales of their
+    blocks of ``STATE_BLOCK`` values (``adamw_tensors_state`` makes either).  8-bit
+    moments are rounded stochastically from ``seed`` (0 to 2^32 - 1; default
+    ``step``), which every step needs another of; the same call gives the same
+    result.  ``clip_scale``: a float32 scalar on the device that multiplies the
+    gradients.  ``shadow``: bfloat16 tensors that receive the rounded parameters.
+    No two of the tensors written may overlap.  ``lr``, ``step`` and ``seed`` are
+    fixed in a captured graph.
+    """
+
+    if not params:
+        raise ValueError("adamw_tensors needs at least one tensor")
+    f32 = {torch.float32}
+    device = params[0].device
+    shapes = [p.shape for p in params]
+    _list_of("params", params, params, shapes, f32, device)
+    grad_type = _list_of("grads", grads, params, shapes, {torch.float32, torch.bfloat16}, device)
+    kind = _list_of("exp_avg", exp_avg, params, shapes, set(_STATE_TYPES), device)
+    _list_of("exp_avg_sq", exp_avg_sq, params, shapes, {kind}, device)
+    bits = _STATE_TYPES[kind]
+    counts = [p.numel() for p in params]
+    if (exp_avg_scale is None) != (bits == 32) or (exp_avg_sq_scale is None) != (bits == 32):
+        raise ValueError("8-bit moments, and only those, come with exp_avg_scale and exp_avg_sq_scale")
+    if bits == 8:
+        blocks = [(-(-n // STATE_BLOCK),) for n in counts]
+        _list_of("exp_avg_scale", exp_avg_scale, params, blocks, f32, device)
+        _list_of("exp_avg_sq_scale", exp_avg_sq_scale, params, blocks, f32, device)
+    if shadow is not None:
+        _list_of("shadow", shadow, params, shapes, {torch.bfloat16}, device)
+    if hparams.dtype != torch.float32 or hparams.shape != (len(params), 3) or not hparams.is_contiguous():
+        raise ValueError(f"hparams must be contiguous float32 [{len(params)}, 3], got {hparams.dtype} "
+                         f"{tuple(hparams.shape)}")
+    if clip_scale is not None and (clip_scale.dtype != torch.float32 or clip_scale.numel() != 1):
+        raise ValueError("clip_scale must be one float32 value")
+    if not 0.0 <= beta1 < 1.0 or not 0.0 <= beta2 < 1.0:
+        raise ValueError(f"beta1 and beta2 must be in [0, 1), got {beta1} and {beta2}")
+    if step < 1:
+        raise ValueError(f"step counts from 1, got {step}")
+    seed = step % 2 ** 32 if seed is None else seed
+    if not 0 <= seed < 2 ** 32:
+        raise ValueError(f"seed must be in [0, 2^32), got {seed}")
+
+    def addresses(tensors):
+        return [0] * len(params) if tensors is None else [t.data_ptr() for t in tensors]
+
+    lists = [addresses(t) for t in (params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, shadow)]
+    sizes = (4, None, bits // 8, bits // 8, 4 / STATE_BLOCK, 4 / STATE_BLOCK, 2)
+    written = sorted((a, a + n * size) for addr, size in zip(lists, sizes) if size
+                     for a, n in zip(addr, counts) if n and a)
+    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
+        raise ValueError("tensors that the step writes overlap")
+    _lib.require_one_device(params[0], hparams, clip_scale)
+    # One row of gptrig_adamw_tensor a tensor: seven addresses and the count.
+    table = [0] * (8 * len(params))
+    for column, values in enumerate((*lists, counts)):
+        table[column::8] = values
+    _lib.call_on(device, "gptrig_adamw_tensors", (ctypes.c_int64 * len(table))(*table), len(params),
+                 1 if grad_type == torch.float32 else 0, bits, hparams.data_ptr(), float(lr), float(beta1), float(beta2),
+                 int(step), _lib.ptr(clip_scale), seed)
+    torch.autograd.graph.increment_version(params)  # (a graph that saved one of them must not run backward now)

@@ -33,6 +33,10 @@ extern "C" {
 #define GPTRIG_E_LAUNCH (-5)      /* the HIP launch failed */
 #define GPTRIG_E_WORKSPACE (-6)   /* workspace smaller than the query says */
 
+/* Element types, where an entry point takes more than one. */
+#define GPTRIG_TYPE_BF16 0
+#define GPTRIG_TYPE_F32 1
+
 /* Library identity and status text. */
 const char* gptrig_version(void);
 const char* gptrig_status_string(int status);
@@ -219,6 +223,26 @@ int gptrig_rmsnorm_bwd(const void* dy, const void* x, const void* scale, const f
                        void* dx, float* dscale, int accumulate_dscale, void* workspace, size_t workspace_bytes,
                        int rows, int d, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Layer normalisation over the last dimension (no counterpart in the reference,
+ * whose models use rms_norm): with mu the mean and r = 1 / sqrt(variance + eps)
+ * of a row, y = (x - mu) r scale + bias, in float32 throughout and rounded once.
+ * x and y of type x_type [rows, d], x with row stride ldx (any; 0 repeats a row),
+ * y contiguous; scale and bias (nullable) of type param_type [d]; mean, rstd f32
+ * [rows], both NULL or both written, for the backward.  Pointers aligned to
+ * their element; rows below 2^31, d at most 2^30.
+ * The backward writes dx (of x_type, contiguous), dscale and dbias (of
+ * param_type, summed in float32 in a fixed order), each nullable;
+ * gptrig_layernorm_bwd_workspace_bytes of workspace, 16-byte aligned, where
+ * dscale or dbias is asked for.
+ * ---------------------------------------------------------------------- */
+int gptrig_layernorm_fwd(const void* x, int64_t ldx, int x_type, const void* scale, const void* bias, int param_type,
+                         void* y, float* mean, float* rstd, int64_t rows, int d, float eps, void* stream);
+size_t gptrig_layernorm_bwd_workspace_bytes(int64_t rows, int d, int x_type);
+int gptrig_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int x_type, const void* scale,
+                         int param_type, const float* mean, const float* rstd, void* dx, void* dscale, void* dbias,
+                         void* workspace, size_t workspace_bytes, int64_t rows, int d, void* stream);
+
 /* Weight and bias gradients of rig/nn.py:55-56 (linear, y = x W + b):
  * dw f32 [rows_in, cols_out] += x^T dy for x bf16 [n, rows_in], dy bf16
  * [n, cols_out] (rows_in, cols_out multiples of 8), and, when db is not NULL,
@@ -338,6 +362,30 @@ int gptrig_embedding_bwd(const int32_t* tokens, const void* dout, float* dtable,
 int gptrig_adamw(float* param, const float* grad, float* m, float* v, void* param_bf16, const int32_t* chunk_tensor,
                  const float* tensor_hparams, int64_t n_chunks, int chunk, float lr, float beta1, float beta2,
                  int step, const float* clip_scale, float* sq_partials, void* stream);
+/* The same update over a list of tensors that lie anywhere, in one launch per 48
+ * of them (tensors is host memory, read before the call returns), with float32
+ * moments (state_bits 32) or 8-bit ones (state_bits 8: e4m3 codes and one f32
+ * scale per 256 consecutive values of a tensor, m_scale and v_scale
+ * [ceil(n / 256)]; a moment is code x scale, zeros to begin with).  8-bit moments
+ * are rounded stochastically, from a hash of seed, the tensor's place in the
+ * list and the element's in the tensor: give every step another seed.  An
+ * infinite or NaN moment is kept as a NaN code.  grad_type of all gradients;
+ * tensor_hparams f32 [count, 3] = {lr_mult, epsilon, decay} in device memory;
+ * clip_scale a nullable device scalar.  Pointers aligned to their element; no
+ * two tensors' memory may overlap; at most 2^40 elements a tensor. */
+typedef struct {
+  float* param;    /* f32 [n], updated */
+  const void* grad;
+  void* m;         /* f32 or e4m3 [n], updated */
+  void* v;
+  float* m_scale;  /* 8 bits only */
+  float* v_scale;
+  void* shadow;    /* bf16 [n] = bf16(updated param), or NULL */
+  int64_t n;
+} gptrig_adamw_tensor;
+int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
+                         const float* tensor_hparams, double lr, double beta1, double beta2, int step,
+                         const float* clip_scale, uint32_t seed, void* stream);
 /* Per-chunk sums of squares of an f32 arena (for clipping before the update). */
 int gptrig_sq_norm_partials(const float* x, int64_t n_chunks, int chunk, float* partials, void* stream);
 /* norm = sqrt(sum partials); clip = min(1, grad_clip/(norm+1e-6)) (1 if grad_clip <= 0);

@@ -1,0 +1,134 @@
+"""What ``layer_norm`` and ``adamw_tensors`` refuse, on the host, before any launch (CPU tensors)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from gptrig import _lib
+from gptrig.nn import layer_norm
+from gptrig.optim import adamw_tensors, adamw_tensors_state
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def test_layer_norm_refusals():
+    x, s = torch.zeros((2, 8)), torch.ones(8)
+    for bad in (x.half(), x.double(), x.int()):
+        with pytest.raises(TypeError, match="bfloat16 or float32"):
+            layer_norm(bad, s)
+    with pytest.raises(TypeError, match="both"):
+        layer_norm(x, s, torch.zeros(8, dtype=BF16))
+    with pytest.raises(TypeError, match="both"):
+        layer_norm(x, s.half())
+    for bad in (torch.ones(7), torch.ones((1, 8)), torch.ones(())):
+        with pytest.raises(ValueError, match=r"must be \[8\]"):
+            layer_norm(x, bad)
+        with pytest.raises(ValueError, match=r"must be \[8\]"):
+            layer_norm(x, s, bad)
+    for bad in (torch.zeros(()), torch.zeros((3, 0))):
+        with pytest.raises(ValueError, match="last dimension"):
+            layer_norm(bad, s)
+    for eps in (-1e-5, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            layer_norm(x, s, eps=eps)
+    with pytest.raises(RuntimeError, match="GPU"):
+        layer_norm(x, s)
+
+
+def step(n=2, bits=32, **change):
+    shapes = [(3, 4), (300,)][:n]
+    p = [torch.zeros(s) for s in shapes]
+    args = dict(params=p, grads=[torch.zeros(s) for s in shapes], hparams=torch.zeros((n, 3)), lr=0.1, beta1=0.9, beta2=0.95,
+                step=1, **adamw_tensors_state(p, bits))
+    args.update(change)
+    adamw_tensors(**args)
+
+
+def test_adamw_tensors_refusals():
+    with pytest.raises(RuntimeError, match="GPU"):
+        step()
+    with pytest.raises(RuntimeError, match="GPU"):
+        step(bits=8)
+    with pytest.raises(ValueError, match="at least one"):
+        step(params=[])
+    with pytest.raises(ValueError, match="grads has 1"):
+        step(grads=[torch.zeros((3, 4))])
+    with pytest.raises(ValueError, match=r"grads\[1\] must be"):
+        step(grads=[torch.zeros((3, 4)), torch.zeros(299)])
+    with pytest.raises(ValueError, match=r"grads\[0\] must be contiguous"):
+        step(grads=[torch.zeros((4, 3)).t(), torch.zeros(300)])
+    with pytest.raises(TypeError, match="grads must all"):
+        step(grads=[torch.zeros((3, 4)), torch.zeros(300, dtype=BF16)])
+    with pytest.raises(TypeError, match="params must all"):
+        step(params=[torch.zeros((3, 4), dtype=BF16), torch.zeros(300, dtype=BF16)])
+    with pytest.raises(TypeError, match="exp_avg must all"):
+        step(exp_avg=[torch.zeros((3, 4), dtype=BF16), torch.zeros(300, dtype=BF16)])
+    with pytest.raises(TypeError, match="exp_avg_sq must all"):
+        step(exp_avg_sq=adamw_tensors_state([torch.zeros((3, 4)), torch.zeros(300)], 8)["exp_avg_sq"])
+    with pytest.raises(ValueError, match="come with"):
+        step(bits=8, exp_avg_scale=None)
+    with pytest.raises(ValueError, match="come with"):
+        step(exp_avg_scale=[torch.zeros(1), torch.zeros(2)])
+    with pytest.raises(ValueError, match=r"exp_avg_sq_scale\[1\] must be \(2,\)"):
+        step(bits=8, exp_avg_sq_scale=[torch.zeros(1), torch.zeros(1)])
+    with pytest.raises(TypeError, match="shadow"):
+        step(shadow=[torch.zeros((3, 4)), torch.zeros(300)])
+    for bad in (torch.zeros((2, 2)), torch.zeros((1, 3)), torch.zeros((2, 3), dtype=torch.float64), torch.zeros((3, 2)).t()):
+        with pytest.raises(ValueError, match="hparams"):
+            step(hparams=bad)
+    for bad in (torch.zeros(2), torch.zeros(1, dtype=torch.float64)):
+        with pytest.raises(ValueError, match="clip_scale"):
+            step(clip_scale=bad)
+    for name in ("beta1", "beta2"):
+        for bad in (1.0, -0.1, float("nan")):
+            with pytest.raises(ValueError, match="beta1"):
+                step(**{name: bad})
+    with pytest.raises(ValueError, match="counts from 1"):
+        step(step=0)
+    for bad in (-1, 2 ** 32):
+        with pytest.raises(ValueError, match="seed"):
+            step(seed=bad)
+    p = torch.zeros(300)
+    with pytest.raises(ValueError, match="overlap"):
+        adamw_tensors([p, p], [p, p], [torch.zeros(300) for _ in range(2)], [torch.zeros(300) for _ in range(2)],
+                      torch.zeros((2, 3)), lr=0.1, beta1=0.9, beta2=0.9, step=1)
+    big = torch.zeros(400)
+    with pytest.raises(ValueError, match="overlap"):
+        step(n=1, params=[big[:12].view(3, 4)], exp_avg=[big[8:20].view(3, 4)])
+    with pytest.raises(ValueError, match="8 or 32"):
+        adamw_tensors_state([p], 16)
+
+
+def test_entry_points_refuse_on_the_host():
+    lib = _lib.lib()
+    at = ctypes.c_void_p(1 << 12)
+    odd = ctypes.c_void_p((1 << 12) + 1)
+    fwd = lib.gptrig_layernorm_fwd
+    assert fwd(None, 8, 0, at, None, 1, at, None, None, 2, 8, 1e-5, None) == -1
+    assert fwd(at, 8, 2, at, None, 1, at, None, None, 2, 8, 1e-5, None) == -3
+    assert fwd(at, 8, 0, at, None, 1, at, at, None, 2, 8, 1e-5, None) == -1
+    for ld, rows, d in ((-1, 2, 8), (8, -1, 8), (8, 2, 0), (8, 1 << 31, 8), (8, 2, (1 << 30) + 1)):
+        assert fwd(at, ld, 0, at, None, 1, at, None, None, rows, d, 1e-5, None) == -2
+    assert fwd(at, 8, 0, at, None, 1, at, None, None, 2, 8, float("nan"), None) == -2
+    assert fwd(odd, 8, 0, at, None, 1, at, None, None, 2, 8, 1e-5, None) == -2
+    assert fwd(at, 8, 0, at, None, 1, at, None, None, 0, 8, 1e-5, None) == 0
+    bwd = lib.gptrig_layernorm_bwd
+    need = lib.gptrig_layernorm_bwd_workspace_bytes(100, 64, 0)
+    assert need >= 2 * 64 * 4
+    assert bwd(at, 64, at, 64, 0, at, 1, at, at, None, at, None, None, 0, 100, 64, None) == -1
+    assert bwd(at, 64, at, 64, 0, at, 1, at, at, None, at, None, at, need - 1, 100, 64, None) == -6
+    assert bwd(at, 64, at, 64, 0, at, 1, at, at, None, None, None, None, 0, 100, 64, None) == 0
+    adamw = lib.gptrig_adamw_tensors
+    row = (ctypes.c_int64 * 8)(1 << 12, 1 << 12, 1 << 12, 1 << 12, 0, 0, 0, 100)
+    assert adamw(None, 1, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -1
+    assert adamw(row, 1, 1, 8, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -1  # no scales
+    assert adamw(row, 1, 2, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -3
+    assert adamw(row, 1, 1, 16, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -4
+    assert adamw(row, 1, 1, 32, at, 0.1, 1.0, 0.95, 1, None, 0, None) == -2
+    assert adamw(row, 1, 1, 32, at, 0.1, 0.9, 0.95, 0, None, 0, None) == -2
+    assert adamw(row, 0, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == 0
+    row[0] += 2
+    assert adamw(row, 1, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -2

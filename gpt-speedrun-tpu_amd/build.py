@@ -19,7 +19,7 @@ OUT_DIR = os.path.join(HERE, "gptrig")
 LIB = os.path.join(OUT_DIR, "libgptrig.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 SOURCES = ("capi.hip", "elementwise.hip", "attention.hip", "flce.hip", "flce32.hip", "moe.hip", "linear.hip",
-           "layernorm.hip", "adamw_tensors.hip")
+           "layernorm.hip", "adamw_tensors.hip", "scored_attention_fwd.hip", "scored_attention_bwd.hip")
 
 FLAGS = [
     "--offload-arch=gfx950",

@@ -1,0 +1,222 @@
+// Attention whose scores are capped by a tanh or get a bias that depends on
+// distance, over causal, prefix and document masks, with heads that may share
+// keys and values.  For query i and key j of one (batch, head):
+//   u_ij = scale q_i . k_j
+//   s_ij = c tanh(u_ij / c) - slope |i - j|     (without a cap: u_ij - slope |i - j|)
+//   visible(i, j): j <= max(i, prefix - 1) and segment_i == segment_j
+//   P = softmax of s over the visible j, o = P v, L_i = log2 sum_j 2^(s_ij log2 e)
+//   dS = P (do v^T - delta), delta_i = o_i . do_i;  dU = dS (1 - tanh^2(u / c))
+//   dv = P^T do, dk = scale dU^T q, dq = scale dU k
+// Scores are taken in units of log2 e from the start, so every exponential is one
+// v_exp_f32.  With w = 1 / (1 + exp(2 u / c)): tanh(u / c) = 1 - 2 w and
+// 1 - tanh^2 = 4 w (1 - w); w saturates to 0 and 1 without an overflow.
+// The matrix products take bf16 operands: P and dU are rounded to bf16 for them
+// (half a step is 2^-8 of the value, the rounding of the results themselves); all
+// else is float32.
+//
+// A pair that is not visible adds nothing, whatever its k, v, q or do hold.  Its P
+// and dU are set to 0; but 0 x inf is not 0, so a tile that holds hidden pairs is
+// searched for infinities and NaN before its rows are summed over (Dirty, below).
+#pragma once
+
+#include "attn_common.h"
+
+namespace {
+
+constexpr int kRows = 64;  // rows of an LDS tile
+
+struct ScoreArgs {
+  float raw;            // scale log2 e; with a cap 2 log2 e scale / cap
+  float cap2;           // cap log2 e
+  const float* slopes;  // [heads], nullable
+  const int32_t* prefix;  // [batch], nullable
+};
+
+// The score of raw product r in units of log2 e, without the bias; w as above.
+template <bool kCap>
+__device__ __forceinline__ float base_score(float r, const ScoreArgs& a, float& w) {
+  if constexpr (kCap) {
+    w = __builtin_amdgcn_rcpf(1.0f + fast_exp2(r * a.raw));
+    return fmaf(-2.0f * a.cap2, w, a.cap2);
+  } else {
+    return r * a.raw;
+  }
+}
+
+// The row of accumulator element i (of 16) in the lower half of the wave; the upper half adds 4.
+__host__ __device__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+__device__ __forceinline__ int prefix_of(const ScoreArgs& a, int b, int S) {
+  return a.prefix ? min(max(a.prefix[b], 0), S) : 0;
+}
+
+// Element offset of 16-byte chunk c16 of row `row` in a tile of kRows rows: a
+// tile of 128 columns is two swizzled ones of 64.
+__device__ __forceinline__ int tile_at(int row, int c16) { return (c16 >> 3) * kRows * 64 + at64::swz(row, c16 & 7); }
+__device__ __forceinline__ bf16x8 tile_row(const at64::lds_t* t, int row, int c16) {
+  return *(const at64::lds_x8*)(t + tile_at(row, c16));
+}
+// Transposed operand of columns 32 db .. +31, rows in accumulator order from r0.
+__device__ __forceinline__ bf16x8 tile_col(const at64::lds_t* t, int db, int r0, int lane) {
+  return at64::trfrag<true>(t + (db >> 1) * kRows * 64, 32 * (db & 1), r0, lane);
+}
+
+// 16 bytes a lane, or 4, global -> LDS: lane l's land at lds + 16 l (4 l).
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, at64::lds_t* lds, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)lds, 16, offset, 0, 0, 0);
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, void* lds, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)lds, 4, offset, 0, 0, 0);
+}
+
+// One tile of 64 rows x D columns, global -> LDS by the DMA path.  Wave w of 4
+// fills 1 KB blocks D/32 w .. of 8 rows each; rows at or past S and columns at
+// or past `dim` read as zeros.
+template <int D>
+struct Fill {
+  static constexpr int NB = D / 32;
+  int off[NB];
+  int stride;  // bytes a row
+  __device__ __forceinline__ void init(int64_t row_stride, int dim, int wave, int lane) {
+    stride = (int)row_stride * 2;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int blk = NB * wave + j;
+      const int row = 8 * (blk & 7) + (lane >> 3);
+      const int t = (row >> 1) & 7;
+      const int c = 8 * (blk >> 3) + ((lane & 7) ^ (((t & 1) << 2) | (t >> 1)));
+      off[j] = 8 * c < dim ? row * stride + 16 * c : INT32_MIN;  // (past every buffer)
+    }
+  }
+  __device__ __forceinline__ void operator()(__amdgpu_buffer_rsrc_t rs, at64::lds_t* tile, int row0, int wave) const {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) dma16(rs, tile + (NB * wave + j) * 512, off[j] + row0 * stride);
+  }
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t slice(const bf16* base, int S, int64_t row_stride, int dim) {
+  return make_rsrc(base, (uint32_t)(((int64_t)(S - 1) * row_stride + dim) * 2));
+}
+
+// Rows of an LDS tile that hold an infinity or NaN, for tiles with hidden pairs
+// (at the causal border and where documents meet): each of the 4 waves searches 16
+// rows, four lanes a row, and one barrier shares what they found.  Where there
+// is such a row, the caller records which of its own results it reaches, and
+// clear() puts zeros in the place of its infinities and NaN; nothing else of a
+// kernel knows of it.
+// (One 1 KB read and two operations a word per wave, on two tiles of a workgroup.)
+template <int D>
+struct Dirty {
+  uint64_t* found;  // LDS, [4]: bit l of wave w's word: row 16 w + l / 4
+
+  __device__ __forceinline__ bool find(const at64::lds_t* tile, int wave, int lane) const {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = u16x2{};
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const u32x4 w = __builtin_bit_cast(u32x4, tile_row(tile, 16 * wave + (lane >> 2), (lane & 3) + 4 * j));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[e] & 0x7FFF7FFFu));
+    }
+    const uint64_t mine = __ballot(top[0] >= 0x7F80u || top[1] >= 0x7F80u);
+    if (lane == 0) found[wave] = mine;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane((found[0] | found[1] | found[2] | found[3]) != 0);
+  }
+  __device__ __forceinline__ bool row(int r) const { return (found[r >> 4] >> 4 * (r & 15) & 15) != 0; }
+  // (Every wave has recorded what it needs of the tile by the first barrier.)
+  __device__ __forceinline__ void clear(at64::lds_t* tile, int wave, int lane) const {
+    __syncthreads();
+    const int r = 16 * wave + (lane >> 2);
+    if (row(r))
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        at64::lds_x8* const at = (at64::lds_x8*)(tile + tile_at(r, (lane & 3) + 4 * j));
+        bf16x8 v = *at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fabsf((float)v[e]) < INFINITY ? v[e] : (bf16)0.f;
+        *at = v;
+      }
+    __syncthreads();
+  }
+};
+
+// acc[db] += (columns of `tile`, rows r0 .. r0 + 31)^T x, x the wave's 32 x 32
+// operand in accumulator order (16 rows of this lane's column as bf16).
+template <int DB>
+__device__ __forceinline__ void product(f32x16 (&acc)[DB], const at64::lds_t* tile, int r0, const bf16x8 (&x)[2],
+                                        int lane) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = mfma32(tile_col(tile, db, r0 + 16 * c, lane), x[c], acc[db]);
+}
+
+// ---------------------------------------------------------------------------
+// Host side: what every entry point checks, and the choice of a kernel
+// ---------------------------------------------------------------------------
+struct ScoredCall {
+  const void* p[9];
+  int64_t st[27];
+  ScoreArgs args;
+  int dim;
+  bool cap;
+
+  View view(int i) const { return {(const bf16*)p[i], st[3 * i], st[3 * i + 1], st[3 * i + 2]}; }
+  MutView out(int i) const { return {(bf16*)const_cast<void*>(p[i]), st[3 * i], st[3 * i + 1], st[3 * i + 2]}; }
+
+  // kv: bit i set where tensor i has kv_heads heads (for its default strides).
+  int init(const void* const* tensors, int n, uint32_t kv, int batch, int heads, int kv_heads, int seq, int head_dim,
+           const int64_t* strides, float softmax_scale, float score_cap, const float* slopes, const int32_t* prefix) {
+    for (int i = 0; i < n; ++i) {
+      if (!tensors[i]) return GPTRIG_E_NULL;
+      if ((uintptr_t)tensors[i] & 15) return GPTRIG_E_SHAPE;
+      p[i] = tensors[i];
+    }
+    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq <= 0 || head_dim <= 0 || head_dim % 8)
+      return GPTRIG_E_SHAPE;
+    if (head_dim > 128) return GPTRIG_E_UNSUPPORTED;
+    if (!(softmax_scale > 0.f) || !(softmax_scale <= 3.0e38f)) return GPTRIG_E_SHAPE;
+    if (!(score_cap >= 0.f) || score_cap > 1000.f) return GPTRIG_E_SHAPE;
+    dim = head_dim;
+    for (int i = 0; i < n; ++i) {
+      const int64_t hn = kv >> i & 1 ? kv_heads : heads;
+      const int64_t plain[3] = {hn * seq * head_dim, (int64_t)seq * head_dim, head_dim};
+      for (int j = 0; j < 3; ++j) {
+        const int64_t s = strides ? strides[3 * i + j] : plain[j];
+        if (s < 0 || (s & 7)) return GPTRIG_E_SHAPE;
+        st[3 * i + j] = s;
+      }
+      // A (batch, head) slice is addressed by 32-bit byte offsets, a tile past its end included.
+      if (((long long)seq + 64) * st[3 * i + 2] * 2 >= (1ll << 31)) return GPTRIG_E_SHAPE;
+    }
+    cap = score_cap > 0.f;
+    args.raw = softmax_scale * GPTRIG_LOG2E;
+    args.cap2 = score_cap * GPTRIG_LOG2E;
+    if (cap) {
+      args.raw = 2.0f * GPTRIG_LOG2E * (softmax_scale / score_cap);
+      if (!(args.raw > 0.f && args.raw <= 3.0e38f)) return GPTRIG_E_SHAPE;
+    }
+    args.slopes = slopes;
+    args.prefix = prefix;
+    return GPTRIG_OK;
+  }
+};
+
+// CALL(head dim of the kernel, cap, bias, segment ids) for a call c.
+#define SCORED_BIAS_SEG(CALL, c, D, CAP, seg)                                                          \
+  do {                                                                                                 \
+    if (c.args.slopes && seg) { CALL(D, CAP, true, true); }                                            \
+    else if (c.args.slopes) { CALL(D, CAP, true, false); }                                             \
+    else if (seg) { CALL(D, CAP, false, true); }                                                       \
+    else { CALL(D, CAP, false, false); }                                                               \
+  } while (0)
+#define SCORED_DISPATCH(CALL, c, seg)                                                                  \
+  do {                                                                                                 \
+    if (c.dim <= 64 && c.cap) SCORED_BIAS_SEG(CALL, c, 64, true, seg);                                 \
+    else if (c.dim <= 64) SCORED_BIAS_SEG(CALL, c, 64, false, seg);                                    \
+    else if (c.cap) SCORED_BIAS_SEG(CALL, c, 128, true, seg);                                          \
+    else SCORED_BIAS_SEG(CALL, c, 128, false, seg);                                                    \
+  } while (0)
+
+}  // namespace

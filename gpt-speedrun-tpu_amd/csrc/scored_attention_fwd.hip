@@ -1,0 +1,246 @@
+// Forward of the attention of scored_attention.h.  A workgroup owns 128 queries
+// of one head (4 waves x 32) and walks the tiles of 64 keys that any of them can
+// see.  Each wave computes S^T = K Q^T, so a lane holds one query and 16 of 32
+// keys: the softmax is lane-local but for one exchange between the half-waves,
+// and P^T is already the operand of o^T = V^T P^T.
+#include "scored_attention.h"
+
+namespace {
+
+constexpr int kQueries = 128;
+
+template <int D, bool kCap, bool kBias, bool kSeg>
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
+    scored_fwd_kernel(View Q, View K, View V, MutView O, float* __restrict__ lse2, const int32_t* __restrict__ seg,
+                      ScoreArgs a, int B, int H, int Hk, int S, int dim) {
+  constexpr int KC = D / 16, DB = D / 32;
+  constexpr bool kRaw = !kCap && !kBias;  // the softmax scales the raw products itself
+  __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
+  __shared__ __attribute__((aligned(16))) bf16 fk1[kRows * D];
+  __shared__ __attribute__((aligned(16))) bf16 fv0[kRows * D];
+  __shared__ __attribute__((aligned(16))) bf16 fv1[kRows * D];
+
+  const int nq = (S + kQueries - 1) / kQueries;
+  int bh, qb;
+  xcd_map(blockIdx.x, nq, B * H, bh, qb);
+  qb = nq - 1 - qb;
+  const int b = bh / H, h = bh % H, hk = h / (H / Hk);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hl = lane >> 5, l32 = lane & 31;
+  const int q0 = qb * kQueries, qw0 = q0 + 32 * wave, my_q = qw0 + l32;
+  const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
+  const int my_last = min(max(my_q, last_prefix), S - 1);  // the last key this lane's query may see
+  const int all_see = max(qw0, last_prefix);               // keys up to here are behind no query of the wave
+  const int wave_last = max(qw0 + 31, last_prefix);
+  const int ntiles = max(min(q0 + kQueries, S) - 1, last_prefix) / kRows + 1;
+  const float slope2 = kBias ? a.slopes[h] * GPTRIG_LOG2E : 0.f;
+
+  bf16x8 qreg[KC];
+#pragma unroll
+  for (int kc = 0; kc < KC; ++kc)
+    qreg[kc] = my_q < S && 16 * kc + 8 * hl < dim
+                   ? *reinterpret_cast<const bf16x8*>(Q.row(b, h, my_q) + 16 * kc + 8 * hl) : bf16x8{};
+  const int seg_q = (kSeg && my_q < S) ? seg[(size_t)b * S + my_q] : 0;
+  __shared__ uint64_t scan_s[2];
+  SegScan<4> scan;
+  if constexpr (kSeg) scan.template init<kQueries / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+  float m_run = kMinusBig, l_run = 0.f;
+
+  const __amdgpu_buffer_rsrc_t k_rs = slice(K.row(b, hk, 0), S, K.ss, dim);
+  const __amdgpu_buffer_rsrc_t v_rs = slice(V.row(b, hk, 0), S, V.ss, dim);
+  Fill<D> kf, vf;
+  kf.init(K.ss, dim, wave, lane);
+  vf.init(V.ss, dim, wave, lane);
+
+  // One half of a tile, keys kh0 .. kh0 + 31.  same: no id needs a compare.
+  auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, int kv0, int sb,
+                  bool same) __attribute__((always_inline)) {
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) s = mfma32(tile_row(kt, 32 * sb + l32, 2 * kc + hl), qreg[kc], s);
+    const int kh0 = kv0 + 32 * sb;
+    if constexpr (!kRaw) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float w;
+        s[i] = base_score<kCap>(s[i], a, w);
+      }
+    }
+    if constexpr (kBias) {
+      const float x = (float)(my_q - kh0 - 4 * hl);
+      if (kh0 + 31 > qw0 && last_prefix > qw0) {  // keys after their query are visible
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope2, fabsf(x - (float)acc_row(i)), s[i]);
+      } else {
+        const float b0 = -slope2 * x;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] += fmaf(slope2, (float)acc_row(i), b0);
+      }
+    }
+    const bool masked = kh0 + 31 > all_see || kh0 + 32 > S || (kSeg && !same);
+    if (masked) {
+      const int lim = my_last - kh0 - 4 * hl;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        bool vis = acc_row(i) <= lim;
+        if (kSeg && !same) vis = vis && seg[(size_t)b * S + min(kh0 + 4 * hl + acc_row(i), S - 1)] == seg_q;
+        s[i] = vis ? s[i] : -INFINITY;
+      }
+    }
+    float m_tile = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
+    m_tile = fmaxf(m_tile, __shfl_xor(m_tile, 32));
+    if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
+    // The running maximum moves only when a row's maximum exceeds it by more
+    // than 8 (log2): P stays below 2^8 and most halves rescale nothing.
+    const bool grow = m_tile > m_run + 8.0f;
+    const float m_new = grow ? m_tile : m_run;
+    if (__ballot(grow)) {
+      const float alpha = fast_exp2(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+    }
+    m_run = m_new;
+    bf16x8 pb[2];
+    float lsum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, -m_new) : s[i] - m_new);
+      lsum += p;
+      pb[i >> 3][i & 7] = (bf16)p;
+    }
+    l_run += lsum;
+    product<DB>(acc, vt, 32 * sb, pb, lane);
+  };
+
+  // Infinities and NaN of visible v rows in tiles that clear() changed: a bit per
+  // accumulator element, for +inf and for -inf (both: NaN).
+  __shared__ uint64_t dirty_s[4];
+  uint64_t plus = 0, minus = 0;
+  auto clean = [&](at64::lds_t* vt, int kv0, bool same) {
+    const Dirty<D> dirty{dirty_s};
+    if (!dirty.find(vt, wave, lane)) return;
+#pragma unroll 1
+    for (int r = 0; r < kRows; ++r) {
+      if (!__builtin_amdgcn_readfirstlane(dirty.row(r))) continue;
+      const int key = kv0 + r;
+      bool vis = key <= my_last;
+      if (kSeg && !same) vis = vis && seg[(size_t)b * S + min(key, S - 1)] == seg_q;
+#pragma unroll 1
+      for (int e = 0; e < 16 * DB; ++e) {
+        const int col = 32 * (e >> 4) + acc_row(e & 15) + 4 * hl;
+        const float v = (float)*(vt + tile_at(r, col >> 3) + (col & 7));
+        if (vis && !(v < INFINITY)) plus |= 1ull << e;    // (+inf or NaN)
+        if (vis && !(v > -INFINITY)) minus |= 1ull << e;
+      }
+    }
+    dirty.clear(vt, wave, lane);
+  };
+
+  // Tile `it` from (kt, vt), the next one, nx, on its way to (nkt, nvt).
+  auto tile = [&](const at64::lds_t* kt, at64::lds_t* vt, at64::lds_t* nkt, at64::lds_t* nvt, int it, int nx,
+                  bool same) __attribute__((always_inline)) {
+    const int kv0 = it * kRows;
+    if (nx < ntiles) {
+      kf(k_rs, nkt, nx * kRows, wave);
+      vf(v_rs, nvt, nx * kRows, wave);
+    }
+    if (kv0 + kRows - 1 > max(q0, last_prefix) || (kSeg && !same)) clean(vt, kv0, same);
+    if (kv0 <= wave_last) half(kt, vt, kv0, 0, same);
+    __builtin_amdgcn_sched_barrier(0);  // keep the halves' live ranges apart
+    if (kv0 + 32 <= wave_last) half(kt, vt, kv0, 1, same);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
+    __syncthreads();
+  };
+
+  at64::lds_t* const k0s = gemm::lds_cast(fk0);
+  at64::lds_t* const k1s = gemm::lds_cast(fk1);
+  at64::lds_t* const v0s = gemm::lds_cast(fv0);
+  at64::lds_t* const v1s = gemm::lds_cast(fv1);
+  auto next = [&](int t, bool& same) {
+    if constexpr (kSeg) return scan.next(t, ntiles, wave, lane, same);
+    same = true;
+    return t;
+  };
+  bool same = true, same_n = true;
+  int it = next(0, same);
+  kf(k_rs, k0s, it * kRows, wave);
+  vf(v_rs, v0s, it * kRows, wave);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  while (true) {  // (A workgroup's own positions hold visible pairs: there is a first tile.)
+    int nx = next(it + 1, same_n);
+    tile(k0s, v0s, k1s, v1s, it, nx, same);
+    if (nx >= ntiles) break;
+    it = nx;
+    nx = next(it + 1, same);
+    tile(k1s, v1s, k0s, v0s, it, nx, same_n);
+    if (nx >= ntiles) break;
+    it = nx;
+  }
+
+  const float l_tot = l_run + __shfl_xor(l_run, 32);
+  if (__ballot((plus | minus) != 0)) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool p = plus >> (16 * db + i) & 1, m = minus >> (16 * db + i) & 1;
+        if (p || m) acc[db][i] += p && m ? __builtin_nanf("") : p ? INFINITY : -INFINITY;
+      }
+  }
+  if (my_q < S) {
+    const float inv = 1.0f / l_tot;
+    bf16* orow = O.row(b, h, my_q);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d0 = 32 * db + 8 * r + 4 * hl;
+        if (d0 >= dim) continue;
+        bf16x4 o4;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o4[t] = (bf16)(acc[db][4 * r + t] * inv);
+        *reinterpret_cast<bf16x4*>(orow + d0) = o4;
+      }
+    if (hl == 0 && lse2) lse2[((size_t)b * H + h) * S + my_q] = m_run + __log2f(l_tot);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const int32_t* segment_ids,
+                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, float* lse2,
+                           int batch, int heads, int kv_heads, int seq, int head_dim, const int64_t* strides,
+                           float softmax_scale, float score_cap, void* stream) {
+  ScoredCall c;
+  const void* tensors[4] = {q, k, v, o};
+  const int status = c.init(tensors, 4, 0b0110u, batch, heads, kv_heads, seq, head_dim, strides, softmax_scale,
+                            score_cap, distance_slopes, prefix_lengths);
+  if (status != GPTRIG_OK) return status;
+  const long long grid = (long long)batch * heads * ceil_div(seq, kQueries);
+  if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
+  hipStream_t s = (hipStream_t)stream;
+  const View Q = c.view(0), K = c.view(1), V = c.view(2);
+  const MutView O = c.out(3);
+#define SCORED_FWD(D, CAP, BIAS, SEG)                                                                             \
+  scored_fwd_kernel<D, CAP, BIAS, SEG><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, lse2, segment_ids, c.args, batch, \
+                                                                      heads, kv_heads, seq, head_dim)
+  SCORED_DISPATCH(SCORED_FWD, c, segment_ids != nullptr);
+#undef SCORED_FWD
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
+}
+
+}  // extern "C"

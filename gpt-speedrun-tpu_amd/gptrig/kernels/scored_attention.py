@@ -1,0 +1,151 @@
+"""Attention whose scores are capped by a tanh or biased by distance, on gfx950.
+
+Beside ``make_causal_attention``, which is the reference's operator:
+``make_scored_attention(ScoredAttentionConfig)`` returns ``attention(q, k, v,
+segment_ids=None, *, prefix_lengths=None, distance_slopes=None)`` over BHSD
+tensors, with key and value heads that query heads may share.  For query i and
+key j of one head
+
+    u = softmax_scale * q_i . k_j
+    score = score_cap * tanh(u / score_cap) - slope * |i - j|   (u without a cap)
+    visible: (j <= i or j < prefix) and segment_i == segment_j
+
+It runs the kernels of ``csrc/scored_attention_fwd.hip`` and
+``csrc/scored_attention_bwd.hip``; head dims up to 128 and sequences of any length
+are handled in-kernel.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Callable
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .flash_attention import _kernel_view, _strides
+
+MAX_CAP = 1000.0  # float32 tells tanh scores of a larger cap apart less well than bfloat16 operands do
+
+
+@dataclass(frozen=True)
+class ScoredAttentionConfig:
+    """``softmax_scale``: default ``head_dim ** -0.5``; ``score_cap``: default none."""
+
+    softmax_scale: float | None = None
+    score_cap: float | None = None
+
+    def __post_init__(self) -> None:
+        if self.softmax_scale is not None and not 0.0 < self.softmax_scale < math.inf:
+            raise ValueError(f"softmax_scale must be positive and finite, got {self.softmax_scale}")
+        if self.score_cap is not None and not 0.0 < self.score_cap <= MAX_CAP:
+            raise ValueError(f"score_cap must be in (0, {MAX_CAP:g}], got {self.score_cap}")
+
+
+def _validate(q, k, v, segment_ids, prefix_lengths, distance_slopes) -> None:
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError(
+            f"q, k, and v must use BHSD rank-4 layout; got {tuple(q.shape)}, {tuple(k.shape)}, and {tuple(v.shape)}"
+        )
+    if not all(q.shape) or not all(k.shape):
+        raise ValueError(f"q/k/v dimensions must be nonzero, got {tuple(q.shape)} and {tuple(k.shape)}")
+    B, H, S, D = q.shape
+    if k.shape != v.shape or (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D) or H % k.shape[1]:
+        raise ValueError("k and v must be [batch, kv_heads, seq, head_dim] of q's batch, seq and head_dim, kv_heads "
+                         f"dividing q's heads; got {tuple(q.shape)}, {tuple(k.shape)}, and {tuple(v.shape)}")
+    if D > 128 or D % 8:
+        raise ValueError(f"the kernel requires head_dim <= 128 and divisible by 8; got {D}")
+    if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+        raise TypeError(f"the HIP attention kernels take bfloat16 q/k/v; got {q.dtype}, {k.dtype}, {v.dtype}")
+    for name, t, shape in (("segment_ids", segment_ids, (B, S)), ("prefix_lengths", prefix_lengths, (B,))):
+        if t is None:
+            continue
+        if t.dtype not in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
+            raise TypeError(f"{name} must be integers, got {t.dtype}")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {list(shape)}; got {tuple(t.shape)}")
+    if distance_slopes is not None:
+        if distance_slopes.dtype != torch.float32:
+            raise TypeError(f"distance_slopes must be float32, got {distance_slopes.dtype}")
+        if tuple(distance_slopes.shape) != (H,):
+            raise ValueError(f"distance_slopes must be [{H}], one a head; got {tuple(distance_slopes.shape)}")
+        if distance_slopes.requires_grad:
+            raise ValueError("distance_slopes are constants: no gradient is computed for them")
+
+
+def _view(t: torch.Tensor) -> torch.Tensor:
+    """A view the kernels accept: as the causal kernels', and a (batch, head) slice within 32-bit offsets."""
+
+    t = _kernel_view(t)
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t if (t.shape[2] + 64) * t.stride(2) < 1 << 30 else t.contiguous()
+
+
+class _ScoredAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, segment_ids, prefix_lengths, slopes, scale, cap):
+        q, k, v = (_view(t) for t in (q, k, v))
+        B, H, S, D = q.shape
+        o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+        keep = any(ctx.needs_input_grad)
+        lse2 = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if keep else None
+        _lib.call_on(q.device, "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(lse2),
+                     B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
+        if keep:
+            ctx.save_for_backward(q, k, v, o, lse2, segment_ids, prefix_lengths, slopes)
+            ctx.scalars = (scale, cap)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse2, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
+        B, H, S, D = q.shape
+        Hk = k.shape[1]
+        do = _view(do)
+        dq = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+        dk = torch.empty((B, Hk, S, D), dtype=q.dtype, device=q.device)
+        dv = torch.empty_like(dk)
+        ws = _lib.workspace(_lib.query("gptrig_scored_attn_bwd_workspace_bytes", B, H, Hk, S, D), q.device)
+        _lib.call_on(q.device, "gptrig_scored_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                     do.data_ptr(), lse2.data_ptr(), _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes),
+                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), B, H, Hk, S, D,
+                     _strides(q, k, v, o, do, dq, dk, dv), *ctx.scalars)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def make_scored_attention(config: ScoredAttentionConfig = ScoredAttentionConfig()) -> Callable:
+    """The attention of this module for one configuration.
+
+    ``q`` ``[batch, heads, seq, head_dim]``, ``k`` and ``v`` ``[batch, kv_heads,
+    seq, head_dim]`` bfloat16 of any strides, ``heads`` a multiple of ``kv_heads``
+    (head h reads kv head ``h // (heads // kv_heads)``).  ``segment_ids``: integers
+    ``[batch, seq]``; ``prefix_lengths``: integers ``[batch]``, the positions that
+    every query of the sequence sees; ``distance_slopes``: float32 ``[heads]``,
+    constants.  Differentiable once in q, k and v; the same call gives the same
+    bits.  Pairs that are not visible add nothing, whatever they hold.
+    """
+
+    def attention(q, k, v, segment_ids=None, *, prefix_lengths=None, distance_slopes=None):
+        _validate(q, k, v, segment_ids, prefix_lengths, distance_slopes)
+        S = q.shape[2]
+        if segment_ids is not None:
+            segment_ids = segment_ids.to(torch.int32).contiguous()
+        if prefix_lengths is not None:
+            if prefix_lengths.dtype == torch.int64:
+                prefix_lengths = prefix_lengths.clamp(0, S)
+            prefix_lengths = prefix_lengths.to(torch.int32).contiguous()
+        if distance_slopes is not None:
+            distance_slopes = distance_slopes.contiguous()
+        _lib.require_one_device(q, k, v, segment_ids, prefix_lengths, distance_slopes)
+        if (S + 64) * q.shape[3] >= 1 << 30:
+            raise ValueError(f"a head's tensors must stay below 2 GiB, got {tuple(q.shape)}")
+        scale = q.shape[3] ** -0.5 if config.softmax_scale is None else config.softmax_scale
+        return _ScoredAttention.apply(q, k, v, segment_ids, prefix_lengths, distance_slopes, float(scale),
+                                      float(config.score_cap or 0.0))
+
+    return attention

@@ -82,6 +82,35 @@ int gptrig_attn_bwd_rope(const void* q, const void* k, const void* v, const void
                          const void* rope_cos, const void* rope_sin, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Attention with capped or biased scores, prefix and document masks, and heads
+ * that share keys and values (no counterpart in the reference, whose attention is
+ * the one above).  q, o, dout, dq: logical [batch, heads, seq, head_dim]; k, v, dk,
+ * dv: [batch, kv_heads, seq, head_dim], head h reading kv head h / (heads /
+ * kv_heads); bf16, head_dim contiguous, a multiple of 8 up to 128.  With u =
+ * softmax_scale q_i . k_j the score of a pair is
+ *   score_cap tanh(u / score_cap) - distance_slopes[h] |i - j|
+ * (score_cap 0: no cap, else at most 1000; distance_slopes f32 [heads] or NULL).
+ * Query i sees key j where j <= i or j < prefix_lengths[batch] (i32 [batch] or
+ * NULL; values are clamped to [0, seq]) and, with segment_ids (i32 [batch, seq] or
+ * NULL), the ids are equal.  `strides` as above (order q, k, v, o; in the backward q,
+ * k, v, o, dout, dq, dk, dv); all tensors 16-byte aligned.  lse2 f32 [batch, heads,
+ * seq]: log2 of the sum of exponentials (NULL where no backward follows).
+ * Hidden pairs add nothing even where their values are infinite or NaN.
+ * Results do not depend on the order of the workgroups (no atomics).
+ * ---------------------------------------------------------------------- */
+int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const int32_t* segment_ids,
+                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, float* lse2,
+                           int batch, int heads, int kv_heads, int seq, int head_dim,
+                           const int64_t* strides /* q,k,v,o */, float softmax_scale, float score_cap, void* stream);
+size_t gptrig_scored_attn_bwd_workspace_bytes(int batch, int heads, int kv_heads, int seq, int head_dim);
+int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                           const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
+                           const float* distance_slopes, void* dq, void* dk, void* dv, void* workspace,
+                           size_t workspace_bytes, int batch, int heads, int kv_heads, int seq, int head_dim,
+                           const int64_t* strides /* q,k,v,o,dout,dq,dk,dv */, float softmax_scale, float score_cap,
+                           void* stream);
+
+/* ------------------------------------------------------------------------
  * Fused linear cross-entropy (LM head + online log-sum-exp + loss + dh/dW).
  * Replaces rig/kernels/linear_cross_entropy.py:
  *   forward  _losses_and_residual   (:115-179)

@@ -1,4 +1,4 @@
-"""What ``layer_norm`` and ``adamw_tensors`` refuse, on the host, before any launch (CPU tensors)."""
+"""What ``layer_norm``, ``adamw_tensors`` and the scored attention refuse, on the host, before any launch (CPU tensors)."""
 
 from __future__ import annotations
 
@@ -132,3 +132,83 @@ def test_entry_points_refuse_on_the_host():
     assert adamw(row, 0, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == 0
     row[0] += 2
     assert adamw(row, 1, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -2
+
+
+def test_scored_attention_refusals():
+    from gptrig.kernels import ScoredAttentionConfig, make_scored_attention
+
+    for bad in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="softmax_scale"):
+            ScoredAttentionConfig(softmax_scale=bad)
+        with pytest.raises(ValueError, match="score_cap"):
+            ScoredAttentionConfig(score_cap=bad)
+    with pytest.raises(ValueError, match="score_cap"):
+        ScoredAttentionConfig(score_cap=1001.0)
+    attention = make_scored_attention(ScoredAttentionConfig(score_cap=30.0))
+    q = torch.zeros((2, 4, 16, 64), dtype=BF16)
+    k = torch.zeros((2, 2, 16, 64), dtype=BF16)
+    with pytest.raises(ValueError, match="rank-4"):
+        attention(q[0], k, k)
+    for bad in (k[:1], k[:, :, :8], k[..., :32], torch.zeros((2, 3, 16, 64), dtype=BF16), torch.zeros((2, 8, 16, 64), dtype=BF16)):
+        with pytest.raises(ValueError, match="kv_heads"):
+            attention(q, bad, bad)
+    with pytest.raises(ValueError, match="kv_heads"):
+        attention(q, k, k[:, :1])
+    with pytest.raises(ValueError, match="nonzero"):
+        attention(q[:, :, :0], k[:, :, :0], k[:, :, :0])
+    for D in (136, 60):
+        t = torch.zeros((1, 1, 4, D), dtype=BF16)
+        with pytest.raises(ValueError, match="head_dim"):
+            attention(t, t, t)
+    with pytest.raises(TypeError, match="bfloat16"):
+        attention(q.half(), k.half(), k.half())
+    with pytest.raises(TypeError, match="bfloat16"):
+        attention(q, k, k.float())
+    for bad in (torch.zeros((2, 16)), torch.zeros((2, 16), dtype=torch.bool)):
+        with pytest.raises(TypeError, match="segment_ids"):
+            attention(q, k, k, bad)
+    with pytest.raises(ValueError, match="segment_ids"):
+        attention(q, k, k, torch.zeros((2, 15), dtype=torch.int32))
+    with pytest.raises(TypeError, match="prefix_lengths"):
+        attention(q, k, k, prefix_lengths=torch.zeros(2))
+    with pytest.raises(ValueError, match="prefix_lengths"):
+        attention(q, k, k, prefix_lengths=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(TypeError, match="distance_slopes"):
+        attention(q, k, k, distance_slopes=torch.zeros(4, dtype=BF16))
+    with pytest.raises(ValueError, match="distance_slopes"):
+        attention(q, k, k, distance_slopes=torch.zeros(2))
+    with pytest.raises(ValueError, match="constants"):
+        attention(q, k, k, distance_slopes=torch.zeros(4, requires_grad=True))
+    with pytest.raises(RuntimeError, match="GPU"):
+        attention(q, k, k)
+
+
+def test_scored_attention_entry_points_refuse_on_the_host():
+    lib = _lib.lib()
+    at, odd = ctypes.c_void_p(1 << 12), ctypes.c_void_p((1 << 12) + 8)
+
+    def fwd(q=at, o=at, B=1, H=4, Hk=2, S=16, D=64, strides=None, scale=0.125, cap=0.0):
+        return lib.gptrig_scored_attn_fwd(q, at, at, None, None, None, o, None, B, H, Hk, S, D, strides, scale, cap, None)
+
+    assert fwd(q=None) == -1 and fwd(q=odd) == -2
+    assert fwd(Hk=3) == -2 and fwd(Hk=0) == -2 and fwd(S=0) == -2 and fwd(B=-1) == -2
+    assert fwd(D=60) == -2 and fwd(D=136) == -4
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert fwd(scale=scale) == -2
+    for cap in (-1.0, 1001.0, float("nan"), 1e-42):
+        assert fwd(cap=cap) == -2
+    assert fwd(S=1 << 24) == -2  # a head's slice past 2 GiB
+    for change in (4, -64):
+        st = (ctypes.c_int64 * 12)(*[4096, 1024, 64] * 4)
+        st[2] = change
+        assert fwd(strides=st) == -2
+    big = ctypes.c_size_t(1 << 40)
+    need = lib.gptrig_scored_attn_bwd_workspace_bytes(1, 4, 2, 16, 64)
+    assert need >= 4 * 16 * 4
+
+    def bwd(ws=at, size=big, lse=at, dv=at):
+        return lib.gptrig_scored_attn_bwd(at, at, at, at, at, lse, None, None, None, at, at, dv, ws, size, 1, 4, 2, 16, 64, None,
+                                          0.125, 0.0, None)
+
+    assert bwd(ws=None) == -1 and bwd(lse=None) == -1 and bwd(dv=None) == -1
+    assert bwd(size=need - 1) == -6 and bwd(ws=odd) == -2

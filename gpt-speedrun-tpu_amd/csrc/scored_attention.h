@@ -32,19 +32,20 @@ struct ScoreArgs {
   const int32_t* prefix;  // [batch], nullable
 };
 
-// The score of raw product r in units of log2 e, without the bias; w as above.
-template <bool kCap>
-__device__ __forceinline__ float base_score(float r, const ScoreArgs& a, float& w) {
-  if constexpr (kCap) {
-    w = __builtin_amdgcn_rcpf(1.0f + fast_exp2(r * a.raw));
-    return fmaf(-2.0f * a.cap2, w, a.cap2);
-  } else {
-    return r * a.raw;
-  }
+// The w of raw product r.
+__device__ __forceinline__ float cap_w(float r, const ScoreArgs& a) {
+  return __builtin_amdgcn_rcpf(1.0f + fast_exp2(r * a.raw));
 }
 
 // The row of accumulator element i (of 16) in the lower half of the wave; the upper half adds 4.
 __host__ __device__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+// slope x acc_row(i), the same for every lane: kept in scalar registers.
+__device__ __forceinline__ void row_bias(float (&bias)[16], float slope) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    bias[i] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, slope * (float)acc_row(i))));
+}
 
 __device__ __forceinline__ int prefix_of(const ScoreArgs& a, int b, int S) {
   return a.prefix ? min(max(a.prefix[b], 0), S) : 0;
@@ -97,6 +98,33 @@ struct Fill {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t slice(const bf16* base, int S, int64_t row_stride, int dim) {
   return make_rsrc(base, (uint32_t)(((int64_t)(S - 1) * row_stride + dim) * 2));
 }
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// What the ids of a tile's 64 rows mean for one wave's own 32 positions, where the
+// document test of the whole workgroup could not tell: per half of the tile
+// whether any pair may be visible, and whether ids have to be compared for it.
+struct WaveIds {
+  int lo, hi;  // the wave's own ids (each in both half-waves)
+  __device__ __forceinline__ void init(int own) {
+    lo = hi = own;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor(lo, o));
+      hi = max(hi, __shfl_xor(hi, o));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+  }
+  // Bits 0 and 1: the halves with a visible pair; docs: those whose ids have to be compared.
+  __device__ __forceinline__ int look(const int* ids, int lane, int& docs) const {
+    const int id = ids[lane];
+    const uint64_t within = __ballot(id >= lo && id <= hi);
+    const uint32_t in0 = (uint32_t)within, in1 = (uint32_t)(within >> 32);
+    docs = (lo != hi || in0 != ~0u ? 1 : 0) | (lo != hi || in1 != ~0u ? 2 : 0);
+    return (in0 ? 1 : 0) | (in1 ? 2 : 0);
+  }
+};
 
 // Rows of an LDS tile that hold an infinity or NaN, for tiles with hidden pairs
 // (at the causal border and where documents meet): each of the 4 waves searches 16

@@ -16,16 +16,20 @@ namespace {
 
 constexpr int kOwn = 128;  // queries or keys of a workgroup: 4 waves x 32
 
+// The dq pass leaves two numbers a query for the other pass: the constant of its
+// exponents, cap log2 e - L_i (with a bias less slope (i mod 64), the part of the
+// bias that is the query's own in its tile), and -delta_i.
 template <int D, bool kCap, bool kBias, bool kSeg>
 __global__ void __launch_bounds__(256, 2)
     scored_dq_kernel(View Q, View K, View V, View O, View dO, const float* __restrict__ lse2,
-                     const int32_t* __restrict__ seg, float* __restrict__ delta, MutView dQ, ScoreArgs a, int B, int H,
-                     int Hk, int S, int dim, float scale) {
+                     const int32_t* __restrict__ seg, float* __restrict__ shifts, float* __restrict__ minus_delta,
+                     MutView dQ, ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
   constexpr int KC = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fk1[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fv0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fv1[kRows * D];
+  __shared__ __attribute__((aligned(16))) int sg0[kRows], sg1[kRows];
   __shared__ uint64_t dirty_s[4], scan_s[2];
 
   const int nq = (S + kOwn - 1) / kOwn;
@@ -39,13 +43,17 @@ __global__ void __launch_bounds__(256, 2)
   const int q0 = qb * kOwn, qw0 = q0 + 32 * wave, my_q = qw0 + l32;
   const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
   const int my_last = min(max(my_q, last_prefix), S - 1);
-  const int all_see = max(qw0, last_prefix);
   const int wave_last = max(qw0 + 31, last_prefix);
   const int ntiles = max(min(q0 + kOwn, S) - 1, last_prefix) / kRows + 1;
   const float slope2 = kBias ? a.slopes[h] * GPTRIG_LOG2E : 0.f;
+  float bias[16], raw = a.raw, twice = -2.0f * a.cap2;
+  if constexpr (kBias) {
+    row_bias(bias, slope2);
+    asm("" : "+v"(raw), "+v"(twice));
+  }
 
   bf16x8 qreg[KC], greg[KC];
-  float my_delta = 0.f;
+  float delta = 0.f;
 #pragma unroll
   for (int kc = 0; kc < KC; ++kc) {
     const int c = 16 * kc + 8 * hl;
@@ -54,15 +62,22 @@ __global__ void __launch_bounds__(256, 2)
     greg[kc] = ok ? *reinterpret_cast<const bf16x8*>(dO.row(b, h, my_q) + c) : bf16x8{};
     const bf16x8 o = ok ? *reinterpret_cast<const bf16x8*>(O.row(b, h, my_q) + c) : bf16x8{};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) my_delta = fmaf((float)o[j], (float)greg[kc][j], my_delta);
+    for (int j = 0; j < 8; ++j) delta = fmaf((float)o[j], (float)greg[kc][j], delta);
   }
-  my_delta += __shfl_xor(my_delta, 32);
+  delta += __shfl_xor(delta, 32);
   const size_t my_row = (size_t)bh * S + my_q;
-  const float my_lse = my_q < S ? lse2[my_row] : 0.f;
-  if (my_q < S && hl == 0) delta[my_row] = my_delta;
-  const int seg_q = (kSeg && my_q < S) ? seg[(size_t)b * S + my_q] : 0;
+  const float shift = my_q < S ? (kCap ? a.cap2 : 0.f) - lse2[my_row] : 0.f;
+  if (my_q < S && hl == 0) {
+    shifts[my_row] = kBias ? fmaf(-slope2, (float)(my_q & (kRows - 1)), shift) : shift;
+    minus_delta[my_row] = -delta;
+  }
+  const int seg_q = kSeg ? seg[(size_t)b * S + min(my_q, S - 1)] : 0;
+  WaveIds ids;
   SegScan<4> scan;
-  if constexpr (kSeg) scan.template init<kOwn / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+  if constexpr (kSeg) {
+    ids.init(seg_q);
+    scan.template init<kOwn / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+  }
 
   f32x16 acc[DB];
 #pragma unroll
@@ -74,9 +89,14 @@ __global__ void __launch_bounds__(256, 2)
   Fill<D> kf, vf;
   kf.init(K.ss, dim, wave, lane);
   vf.init(V.ss, dim, wave, lane);
+  auto fill = [&](at64::lds_t* kt, at64::lds_t* vt, int* sg, int kv0) {
+    kf(k_rs, kt, kv0, wave);
+    vf(v_rs, vt, kv0, wave);
+    if (kSeg && wave == 2) dma4(make_rsrc(seg + (size_t)b * S, (uint32_t)S * 4u), sg, (kv0 + lane) * 4);
+  };
 
-  auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, int kv0, int sb,
-                  bool same) __attribute__((always_inline)) {
+  auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, const int* sg, int kv0, int sb,
+                  int docs) __attribute__((always_inline)) {
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
@@ -85,28 +105,39 @@ __global__ void __launch_bounds__(256, 2)
     }
     const int kh0 = kv0 + 32 * sb;
     const float x = (float)(my_q - kh0 - 4 * hl);
-    const bool both_ways = kBias && kh0 + 31 > qw0 && last_prefix > qw0;
-    const float b0 = -slope2 * x - my_lse;
+    const float off = kBias ? fmaf(-slope2, x, shift) : shift;
+    float w[kCap ? 16 : 1];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float w, t = base_score<kCap>(s[i], a, w);
-      if constexpr (kBias) {
-        if (both_ways) t = fmaf(-slope2, fabsf(x - (float)acc_row(i)), t) - my_lse;
-        else t += fmaf(slope2, (float)acc_row(i), b0);
+      if constexpr (kCap) {
+        w[i] = cap_w(s[i], a);
+        s[i] = kBias ? fmaf(twice, w[i], bias[i]) + off : fmaf(twice, w[i], off);
       } else {
-        t -= my_lse;
+        s[i] = kBias ? fmaf(s[i], raw, bias[i]) + off : fmaf(s[i], raw, off);
       }
-      float ds = fast_exp2(t) * (dp[i] - my_delta);
-      if constexpr (kCap) ds *= fmaf(-w, w, w);  // (1 - tanh^2) / 4
-      s[i] = ds;
     }
-    if (kh0 + 31 > all_see || kh0 + 32 > S || (kSeg && !same)) {
-      const int lim = my_last - kh0 - 4 * hl;
+    if (kBias && kh0 + 31 > qw0 && last_prefix > qw0) {  // keys after their query
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        bool vis = acc_row(i) <= lim;
-        if (kSeg && !same) vis = vis && seg[(size_t)b * S + min(kh0 + 4 * hl + acc_row(i), S - 1)] == seg_q;
-        s[i] = vis ? s[i] : 0.f;
+      for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f * slope2, fmaxf((float)acc_row(i) - x, 0.f), s[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = fast_exp2(s[i]) * (dp[i] - delta);
+      if constexpr (kCap) s[i] *= fmaf(-w[i], w[i], w[i]);  // (1 - tanh^2) / 4
+    }
+    if (kh0 + 31 > qw0 || kh0 + 32 > S || (kSeg && docs)) {
+      const int lim = my_last - kh0 - 4 * hl;
+      if (kSeg && docs) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const i32x4 id = *reinterpret_cast<const i32x4*>(sg + 32 * sb + 8 * r + 4 * hl);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            s[4 * r + t] = acc_row(4 * r + t) <= lim && id[t] == seg_q ? s[4 * r + t] : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = acc_row(i) <= lim ? s[i] : 0.f;
       }
     }
     bf16x8 ds8[2];
@@ -115,30 +146,35 @@ __global__ void __launch_bounds__(256, 2)
     product<DB>(acc, kt, 32 * sb, ds8, lane);
   };
 
-  auto clean = [&](at64::lds_t* kt, int kv0, bool same) {
+  auto clean = [&](at64::lds_t* kt, const int* sg, int kv0, bool same) {
     const Dirty<D> dirty{dirty_s};
     if (!dirty.find(kt, wave, lane)) return;
 #pragma unroll 1
     for (int r = 0; r < kRows; ++r) {
       if (!__builtin_amdgcn_readfirstlane(dirty.row(r))) continue;
       bool vis = kv0 + r <= my_last;
-      if (kSeg && !same) vis = vis && seg[(size_t)b * S + min(kv0 + r, S - 1)] == seg_q;
+      if (kSeg && !same) vis = vis && sg[r] == seg_q;
       spoilt |= vis;
     }
     dirty.clear(kt, wave, lane);
   };
 
-  auto tile = [&](at64::lds_t* kt, const at64::lds_t* vt, at64::lds_t* nkt, at64::lds_t* nvt, int it, int nx,
-                  bool same) __attribute__((always_inline)) {
+  auto tile = [&](at64::lds_t* kt, const at64::lds_t* vt, const int* sg, at64::lds_t* nkt, at64::lds_t* nvt, int* nsg,
+                  int it, int nx, bool same) __attribute__((always_inline)) {
     const int kv0 = it * kRows;
-    if (nx < ntiles) {
-      kf(k_rs, nkt, nx * kRows, wave);
-      vf(v_rs, nvt, nx * kRows, wave);
+    int sb = 0, end = 0, docs = 0;
+    if (it < ntiles) {
+      if (nx < ntiles) fill(nkt, nvt, nsg, nx * kRows);
+      if (kv0 + kRows - 1 > max(q0, last_prefix) || (kSeg && !same)) clean(kt, sg, kv0, same);
+      end = kv0 > wave_last ? 0 : kv0 + 32 > wave_last ? 1 : 2;
+      if (kSeg && !same) {
+        const int in = ids.look(sg, lane, docs);
+        sb = in & 1 ? 0 : 1;
+        end = min(end, in & 2 ? 2 : in);
+      }
     }
-    if (kv0 + kRows - 1 > max(q0, last_prefix) || (kSeg && !same)) clean(kt, kv0, same);
-    if (kv0 <= wave_last) half(kt, vt, kv0, 0, same);
-    __builtin_amdgcn_sched_barrier(0);  // keep the halves' live ranges apart
-    if (kv0 + 32 <= wave_last) half(kt, vt, kv0, 1, same);
+#pragma unroll 1
+    for (; sb < end; ++sb) half(kt, vt, sg, kv0, sb, docs >> sb & 1);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   };
@@ -154,19 +190,14 @@ __global__ void __launch_bounds__(256, 2)
   };
   bool same = true, same_n = true;
   int it = next(0, same);
-  kf(k_rs, k0s, it * kRows, wave);
-  vf(v_rs, v0s, it * kRows, wave);
+  fill(k0s, v0s, sg0, it * kRows);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  while (true) {
-    int nx = next(it + 1, same_n);
-    tile(k0s, v0s, k1s, v1s, it, nx, same);
-    if (nx >= ntiles) break;
-    it = nx;
-    nx = next(it + 1, same);
-    tile(k1s, v1s, k0s, v0s, it, nx, same_n);
-    if (nx >= ntiles) break;
-    it = nx;
+  while (it < ntiles) {
+    const int nx = next(it + 1, same_n);
+    tile(k0s, v0s, sg0, k1s, v1s, sg1, it, nx, same);
+    it = next(nx + 1, same);
+    tile(k1s, v1s, sg1, k0s, v0s, sg0, nx, it, same_n);
   }
 
   if (my_q < S) {
@@ -191,9 +222,10 @@ __global__ void __launch_bounds__(256, 2)
 // dk^T += Q^T dU over the queries.
 template <int D, bool kCap, bool kBias, bool kSeg>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
-    scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ lse2,
-                      const float* __restrict__ delta, const int32_t* __restrict__ seg, MutView dK, MutView dV,
-                      ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
+    scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ shifts,
+                      const float* __restrict__ minus_delta, const int32_t* __restrict__ seg, MutView dK, MutView dV,
+                      float* __restrict__ partial, int parts, ScoreArgs a, int B, int H, int Hk, int S, int dim,
+                      float scale) {
   constexpr int KC = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(16))) bf16 fq0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fq1[kRows * D];
@@ -203,10 +235,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   __shared__ __attribute__((aligned(16))) int sg0[kRows], sg1[kRows];
   __shared__ uint64_t dirty_s[4], scan_s[2];
 
-  const int nkv = (S + kOwn - 1) / kOwn, G = H / Hk;
+  // parts workgroups share the heads of a group where there are few keys to own.
+  const int nkv = (S + kOwn - 1) / kOwn, G = H / Hk / parts;
   int bh, kb;
-  xcd_map(blockIdx.x, nkv, B * Hk, bh, kb);
-  const int b = bh / Hk, hk = bh % Hk;
+  xcd_map(blockIdx.x, nkv, B * Hk * parts, bh, kb);
+  const int part = bh % parts, b = bh / parts / Hk, hk = bh / parts % Hk, h0 = hk * (H / Hk) + part * G;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
@@ -221,9 +254,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     kfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(K.row(b, hk, my_k) + c) : bf16x8{};
     vfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(V.row(b, hk, my_k) + c) : bf16x8{};
   }
-  const int seg_k = (kSeg && my_k < S) ? seg[(size_t)b * S + my_k] : 0;
+  const int seg_k = kSeg ? seg[(size_t)b * S + min(my_k, S - 1)] : 0;
+  WaveIds ids;
   SegScan<4> scan;
-  if constexpr (kSeg) scan.template init<kOwn / 64>(seg + (size_t)b * S, scan_s, S, k0, lane);
+  if constexpr (kSeg) {
+    ids.init(seg_k);
+    scan.template init<kOwn / 64>(seg + (size_t)b * S, scan_s, S, k0, lane);
+  }
 
   f32x16 dv_acc[DB], dk_acc[DB];
 #pragma unroll
@@ -236,68 +273,78 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   Fill<D> qf, gf;
   qf.init(Q.ss, dim, wave, lane);
   gf.init(dO.ss, dim, wave, lane);
-  // Rows of head h: past the last one lse and delta read as zeros like q and do.
+  // Rows of head h: past the last one everything reads as zeros.
   auto fill = [&](at64::lds_t* qt, at64::lds_t* gt, float* ls, float* dl, int* sg, int h, int qq0) {
     qf(slice(Q.row(b, h, 0), S, Q.ss, dim), qt, qq0, wave);
     gf(slice(dO.row(b, h, 0), S, dO.ss, dim), gt, qq0, wave);
     const size_t row = ((size_t)b * H + h) * S;
     if (wave == 0)
-      dma4(make_rsrc(lse2 + row, (uint32_t)S * 4u), ls, (qq0 + lane) * 4);
+      dma4(make_rsrc(shifts + row, (uint32_t)S * 4u), ls, (qq0 + lane) * 4);
     if (wave == 1)
-      dma4(make_rsrc(delta + row, (uint32_t)S * 4u), dl, (qq0 + lane) * 4);
+      dma4(make_rsrc(minus_delta + row, (uint32_t)S * 4u), dl, (qq0 + lane) * 4);
     if (kSeg && wave == 2)
       dma4(make_rsrc(seg + (size_t)b * S, (uint32_t)S * 4u), sg, (qq0 + lane) * 4);
   };
 
   // 32 queries qq0 + 32 qs .. of the tile.
+  float raw = a.raw, twice = -2.0f * a.cap2;
   auto half = [&](const at64::lds_t* qt, const at64::lds_t* gt, const float* ls, const float* dl, const int* sg,
-                  int qq0, int qs, float slope2, bool same) __attribute__((always_inline)) {
-    f32x16 s = f32x16{}, dp = f32x16{};
+                  int qq0, int qs, float slope2, int docs) __attribute__((always_inline)) {
+    const int own = 32 * qs + 4 * hl;  // row of element 0
+    f32x16 s = f32x16{}, dp;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 d4 = *reinterpret_cast<const f32x4*>(dl + own + 8 * r);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) dp[4 * r + t] = d4[t];
+    }
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
       s = mfma32(tile_row(qt, 32 * qs + l32, 2 * kc + hl), kfr[kc], s);
       dp = mfma32(tile_row(gt, 32 * qs + l32, 2 * kc + hl), vfr[kc], dp);
     }
     const int qh0 = qq0 + 32 * qs;
-    const float x = (float)(qh0 + 4 * hl - my_k);  // the distance of element 0
-    const bool both_ways = kBias && kw0 + 31 > qh0 && last_prefix > qh0;
-    const float b0 = -slope2 * x;
-    float p[16];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 32 * qs + 8 * r + 4 * hl);
-      const f32x4 d4 = *reinterpret_cast<const f32x4*>(dl + 32 * qs + 8 * r + 4 * hl);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int i = 4 * r + t;
-        float w, u = base_score<kCap>(s[i], a, w);
-        if constexpr (kBias) {
-          if (both_ways) u = fmaf(-slope2, fabsf(x + (float)acc_row(i)), u);
-          else u += fmaf(-slope2, (float)acc_row(i), b0);
-        }
-        p[i] = fast_exp2(u - l4[t]);
-        float ds = p[i] * (dp[i] - d4[t]);
-        if constexpr (kCap) ds *= fmaf(-w, w, w);  // (1 - tanh^2) / 4
-        s[i] = ds;
-      }
-    }
-    if (kw0 + 31 > max(qh0, last_prefix) || qh0 + 32 > S || (kSeg && !same)) {
-      // Query qh0 + 4 hl + c sees my_k from c = first on, all of them inside the prefix.
+    __builtin_amdgcn_sched_barrier(0);
+    const float off = -slope2 * (float)(qq0 - my_k);
+    const bool border = kw0 + 31 > qh0 || qh0 + 32 > S || (kSeg && docs);
+    bf16x8 p8[2], ds8[2];
+    auto middle = [&](auto tag) __attribute__((always_inline)) {
+      constexpr bool kBorder = decltype(tag)::value;
+      // Query own + c sees my_k from c = first on, all of them inside the prefix.
       const int first = my_k <= last_prefix ? -64 : my_k - qh0 - 4 * hl, end = S - qh0 - 4 * hl;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        bool vis = acc_row(i) >= first && acc_row(i) < end;
-        if (kSeg && !same) vis = vis && sg[32 * qs + 4 * hl + acc_row(i)] == seg_k;
-        p[i] = vis ? p[i] : 0.f;
-        s[i] = vis ? s[i] : 0.f;
-      }
-    }
-    bf16x8 p8[2], ds8[2];
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + own + 8 * r);
+        const i32x4 id = kBorder && kSeg ? *reinterpret_cast<const i32x4*>(sg + own + 8 * r) : i32x4{};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      p8[i >> 3][i & 7] = (bf16)p[i];
-      ds8[i >> 3][i & 7] = (bf16)s[i];
-    }
+        for (int t = 0; t < 4; ++t) {
+          const int i = 4 * r + t, c = acc_row(i);
+          float e, w = 0.f;
+          if constexpr (kCap) {
+            w = cap_w(s[i], a);
+            e = fmaf(twice, w, l4[t]);
+          } else {
+            e = fmaf(s[i], raw, l4[t]);
+          }
+          if constexpr (kBias) e += off;
+          if constexpr (kBias && kBorder)  // keys after their query, where a prefix shows them
+            e = fmaf(-2.0f * slope2, fmaxf((float)(my_k - qh0 - 4 * hl - c), 0.f), e);
+          float p = fast_exp2(e), ds = p * dp[i];
+          if constexpr (kCap) ds *= fmaf(-w, w, w);  // (1 - tanh^2) / 4
+          if constexpr (kBorder) {
+            bool vis = c >= first && c < end;
+            if (kSeg) vis = vis && (!docs || id[t] == seg_k);
+            p = vis ? p : 0.f;
+            ds = vis ? ds : 0.f;
+          }
+          p8[i >> 3][i & 7] = (bf16)p;
+          ds8[i >> 3][i & 7] = (bf16)ds;
+        }
+      }
+    };
+    if (border) middle(std::true_type{});
+    else middle(std::false_type{});
+    __builtin_amdgcn_sched_barrier(0);
     product<DB>(dv_acc, gt, 32 * qs, p8, lane);
     product<DB>(dk_acc, qt, 32 * qs, ds8, lane);
   };
@@ -316,18 +363,27 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     }
   };
 
-  auto tile = [&](at64::lds_t* qt, at64::lds_t* gt, const float* ls, const float* dl, const int* sg, int qb, float slope2,
+  auto tile = [&](at64::lds_t* qt, at64::lds_t* gt, const float* ls, const float* dl, const int* sg, int qb, int g,
                   bool same) __attribute__((always_inline)) {
     const int qq0 = qb * kRows;
-    if (k0 + kOwn - 1 > max(qq0, last_prefix) || (kSeg && !same)) {
-      clean(qt, sg, qq0, same);
-      __syncthreads();  // (the second search reuses the first one's words)
-      clean(gt, sg, qq0, same);
+    const float slope2 = kBias ? a.slopes[h0 + min(g, G - 1)] * GPTRIG_LOG2E : 0.f;
+    int qs = 0, end = 0, docs = 0;
+    if (g < G) {
+      if (k0 + kOwn - 1 > max(qq0, last_prefix) || (kSeg && !same)) {
+        clean(qt, sg, qq0, same);
+        __syncthreads();  // (the second search reuses the first one's words)
+        clean(gt, sg, qq0, same);
+      }
+      qs = kw0 <= max(qq0 + 31, last_prefix) ? 0 : kw0 <= qq0 + 63 ? 1 : 2;
+      end = kw0 < S ? 2 : 0;
+      if (kSeg && !same) {
+        const int in = ids.look(sg, lane, docs);
+        qs = max(qs, in & 1 ? 0 : 1);
+        end = min(end, in & 2 ? 2 : in);
+      }
     }
-    const bool here = kw0 < S;
-    if (here && kw0 <= max(qq0 + 31, last_prefix)) half(qt, gt, ls, dl, sg, qq0, 0, slope2, same);
-    __builtin_amdgcn_sched_barrier(0);  // keep the halves' live ranges apart
-    if (here && kw0 <= max(qq0 + 63, last_prefix)) half(qt, gt, ls, dl, sg, qq0, 1, slope2, same);
+#pragma unroll 1
+    for (; qs < end; ++qs) half(qt, gt, ls, dl, sg, qq0, qs, slope2, docs >> qs & 1);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   };
@@ -354,30 +410,45 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     }
     return t;
   };
-  auto slope_of = [&](int g) { return kBias ? a.slopes[hk * G + g] * GPTRIG_LOG2E : 0.f; };
-  int g = 0, gn = 0;
+  int g = 0;
   bool same = true, same_n = true;
-  int qb = next(start, g, same), nx;
-  gn = g;
-  fill(q0s, g0s, ls0, dl0, sg0, hk * G + g, qb * kRows);
+  int qb = next(start, g, same);
+  fill(q0s, g0s, ls0, dl0, sg0, h0 + g, qb * kRows);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  while (true) {  // (The workgroup's own positions hold visible pairs: every head has a first tile.)
-    nx = next(qb + 1, gn, same_n);
-    if (gn < G) fill(q1s, g1s, ls1, dl1, sg1, hk * G + gn, nx * kRows);
-    tile(q0s, g0s, ls0, dl0, sg0, qb, slope_of(g), same);
-    if (gn >= G) break;
-    qb = nx, g = gn;
-    nx = next(qb + 1, gn, same);
-    if (gn < G) fill(q0s, g0s, ls0, dl0, sg0, hk * G + gn, nx * kRows);
-    tile(q1s, g1s, ls1, dl1, sg1, qb, slope_of(g), same_n);
-    if (gn >= G) break;
-    qb = nx, g = gn;
+  while (g < G) {  // (The workgroup's own positions hold visible pairs: every head has a first tile.)
+    int gn = g;
+    const int nx = next(qb + 1, gn, same_n);
+    if (gn < G) fill(q1s, g1s, ls1, dl1, sg1, h0 + gn, nx * kRows);
+    tile(q0s, g0s, ls0, dl0, sg0, qb, g, same);
+    g = gn;
+    qb = next(nx + 1, g, same);
+    if (g < G) fill(q0s, g0s, ls0, dl0, sg0, h0 + g, qb * kRows);
+    tile(q1s, g1s, ls1, dl1, sg1, nx, gn, same_n);
   }
 
   if (my_k < S) {
     const float bad = spoilt ? __builtin_nanf("") : 1.0f;
     const float f = bad * (kCap ? 4.0f * scale : scale);
+    if (parts > 1) {
+      const size_t rows = (size_t)B * Hk * parts * S, row = (size_t)bh * S + my_k;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d0 = 32 * db + 8 * r + 4 * hl;
+          if (d0 >= dim) continue;
+          f32x4 k4, v4;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            k4[t] = dk_acc[db][4 * r + t] * f;
+            v4[t] = dv_acc[db][4 * r + t] * bad;
+          }
+          *reinterpret_cast<f32x4*>(partial + row * dim + d0) = k4;
+          *reinterpret_cast<f32x4*>(partial + (rows + row) * dim + d0) = v4;
+        }
+      return;
+    }
     bf16* krow = dK.row(b, hk, my_k);
     bf16* vrow = dV.row(b, hk, my_k);
 #pragma unroll
@@ -398,13 +469,51 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   }
 }
 
+// dk and dv from the parts' sums: a thread adds 8 columns of one row of either, the parts in order.
+__global__ void __launch_bounds__(256) scored_join_kernel(const float* __restrict__ partial, int parts, MutView dK,
+                                                          MutView dV, int B, int Hk, int S, int dim) {
+  const int per = dim / 8;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)B * Hk * S;
+  const bool values = t >= rows * per;
+  const int64_t u = values ? t - rows * per : t;
+  if (u >= rows * per) return;
+  const int64_t row = u / per;
+  const int c = 8 * (int)(u % per), s = (int)(row % S), bh = (int)(row / S);
+  f32x4 lo = f32x4{}, hi = f32x4{};
+  for (int p = 0; p < parts; ++p) {
+    const float* at = partial + ((values ? rows * parts : 0) + ((int64_t)bh * parts + p) * S + s) * dim + c;
+    lo += *reinterpret_cast<const f32x4*>(at);
+    hi += *reinterpret_cast<const f32x4*>(at + 4);
+  }
+  const bf16x8 o = {(bf16)lo[0], (bf16)lo[1], (bf16)lo[2], (bf16)lo[3],
+                    (bf16)hi[0], (bf16)hi[1], (bf16)hi[2], (bf16)hi[3]};
+  *reinterpret_cast<bf16x8*>((values ? dV : dK).row(bh / Hk, bh % Hk, s) + c) = o;
+}
+
+// Parts of each group of heads: the fewest that divide it and give kWant
+// workgroups (they are of uneven length, so several a CU).
+constexpr long long kWant = 1024;
+int parts_of(int batch, int heads, int kv_heads, int seq) {
+  const int G = heads / kv_heads;
+  const long long blocks = (long long)batch * kv_heads * ceil_div(seq, kOwn);
+  for (int p = 1; p < G; ++p)
+    if (G % p == 0 && blocks * p >= kWant) return p;
+  return G;
+}
+
+size_t row_numbers_bytes(int batch, int heads, int seq) {
+  return ((size_t)batch * heads * seq * sizeof(float) + 255) & ~(size_t)255;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t gptrig_scored_attn_bwd_workspace_bytes(int batch, int heads, int kv_heads, int seq, int head_dim) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || seq <= 0 || head_dim <= 0) return 0;
-  return (size_t)batch * heads * seq * sizeof(float);
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq <= 0 || head_dim <= 0) return 0;
+  const int parts = parts_of(batch, heads, kv_heads, seq);
+  const size_t sums = parts > 1 ? (size_t)2 * batch * kv_heads * parts * seq * head_dim * sizeof(float) : 0;
+  return 2 * row_numbers_bytes(batch, heads, seq) + sums;
 }
 
 int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
@@ -423,19 +532,28 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
   if ((uintptr_t)workspace & 15) return GPTRIG_E_SHAPE;
   const long long grid = (long long)batch * heads * ceil_div(seq, kOwn);
   if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
-  const unsigned kv_grid = (unsigned)((long long)batch * kv_heads * ceil_div(seq, kOwn));
+  const int parts = parts_of(batch, heads, kv_heads, seq);
+  const unsigned kv_grid = (unsigned)((long long)batch * kv_heads * parts * ceil_div(seq, kOwn));
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2), O = c.view(3), dO = c.view(4);
   const MutView dQ = c.out(5), dK = c.out(6), dV = c.out(7);
-  float* const delta = (float*)workspace;
-#define SCORED_BWD(D, CAP, BIAS, SEG)                                                                              \
-  scored_dq_kernel<D, CAP, BIAS, SEG><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, dO, lse2, segment_ids, delta, dQ,   \
-                                                                     c.args, batch, heads, kv_heads, seq, head_dim,  \
-                                                                     softmax_scale);                                 \
-  scored_dkv_kernel<D, CAP, BIAS, SEG><<<kv_grid, 256, 0, s>>>(Q, K, V, dO, lse2, delta, segment_ids, dK, dV, c.args, \
-                                                               batch, heads, kv_heads, seq, head_dim, softmax_scale)
+  float* const shifts = (float*)workspace;
+  float* const minus_delta = shifts + row_numbers_bytes(batch, heads, seq) / sizeof(float);
+  float* const partial = minus_delta + row_numbers_bytes(batch, heads, seq) / sizeof(float);
+#define SCORED_BWD(D, CAP, BIAS, SEG)                                                                                \
+  scored_dq_kernel<D, CAP, BIAS, SEG><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, dO, lse2, segment_ids, shifts,        \
+                                                                     minus_delta, dQ, c.args, batch, heads, kv_heads,  \
+                                                                     seq, head_dim, softmax_scale);                    \
+  scored_dkv_kernel<D, CAP, BIAS, SEG><<<kv_grid, 256, 0, s>>>(Q, K, V, dO, shifts, minus_delta, segment_ids, dK, dV,  \
+                                                               partial, parts, c.args, batch, heads, kv_heads, seq,    \
+                                                               head_dim, softmax_scale)
   SCORED_DISPATCH(SCORED_BWD, c, segment_ids != nullptr);
 #undef SCORED_BWD
+  if (parts > 1) {
+    const long long threads = 2ll * batch * kv_heads * seq * (head_dim / 8);
+    if (threads > 256ll * INT32_MAX) return GPTRIG_E_SHAPE;
+    scored_join_kernel<<<ceil_div(threads, 256), 256, 0, s>>>(partial, parts, dK, dV, batch, kv_heads, seq, head_dim);
+  }
   GPTRIG_CHECK_LAUNCH();
   return GPTRIG_OK;
 }

@@ -9,7 +9,13 @@ namespace {
 
 constexpr int kQueries = 128;
 
-template <int D, bool kCap, bool kBias, bool kSeg>
+// With a cap and no bias every score lies within +-cap, so up to kFixedCap a fixed
+// reference in place of the running maximum keeps every P within [2^-100, 1].
+constexpr float kFixedCap = 34.0f;
+
+enum { kRunning = 0, kFixed = 1 };
+
+template <int D, bool kCap, bool kBias, bool kSeg, int kMax>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     scored_fwd_kernel(View Q, View K, View V, MutView O, float* __restrict__ lse2, const int32_t* __restrict__ seg,
                       ScoreArgs a, int B, int H, int Hk, int S, int dim) {
@@ -19,6 +25,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   __shared__ __attribute__((aligned(16))) bf16 fk1[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fv0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fv1[kRows * D];
+  __shared__ __attribute__((aligned(16))) int sg0[kRows], sg1[kRows];
 
   const int nq = (S + kQueries - 1) / kQueries;
   int bh, qb;
@@ -31,90 +38,119 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   const int q0 = qb * kQueries, qw0 = q0 + 32 * wave, my_q = qw0 + l32;
   const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
   const int my_last = min(max(my_q, last_prefix), S - 1);  // the last key this lane's query may see
-  const int all_see = max(qw0, last_prefix);               // keys up to here are behind no query of the wave
   const int wave_last = max(qw0 + 31, last_prefix);
   const int ntiles = max(min(q0 + kQueries, S) - 1, last_prefix) / kRows + 1;
   const float slope2 = kBias ? a.slopes[h] * GPTRIG_LOG2E : 0.f;
+
+  float bias[16];  // of a key acc_row(i) after element 0's
+  // (An instruction reads one scalar register: the bias's, so the factors are vectors.)
+  float raw = a.raw, twice = -2.0f * a.cap2;
+  if constexpr (kBias) {
+    row_bias(bias, slope2);
+    asm("" : "+v"(raw), "+v"(twice));
+  }
 
   bf16x8 qreg[KC];
 #pragma unroll
   for (int kc = 0; kc < KC; ++kc)
     qreg[kc] = my_q < S && 16 * kc + 8 * hl < dim
                    ? *reinterpret_cast<const bf16x8*>(Q.row(b, h, my_q) + 16 * kc + 8 * hl) : bf16x8{};
-  const int seg_q = (kSeg && my_q < S) ? seg[(size_t)b * S + my_q] : 0;
+  const int seg_q = kSeg ? seg[(size_t)b * S + min(my_q, S - 1)] : 0;
+  WaveIds ids;
   __shared__ uint64_t scan_s[2];
   SegScan<4> scan;
-  if constexpr (kSeg) scan.template init<kQueries / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+  if constexpr (kSeg) {
+    ids.init(seg_q);
+    scan.template init<kQueries / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+  }
 
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
-  float m_run = kMinusBig, l_run = 0.f;
+  float m_run = kMax == kFixed ? a.cap2 : kMinusBig, l_run = 0.f;
 
   const __amdgpu_buffer_rsrc_t k_rs = slice(K.row(b, hk, 0), S, K.ss, dim);
   const __amdgpu_buffer_rsrc_t v_rs = slice(V.row(b, hk, 0), S, V.ss, dim);
   Fill<D> kf, vf;
   kf.init(K.ss, dim, wave, lane);
   vf.init(V.ss, dim, wave, lane);
+  auto fill = [&](at64::lds_t* kt, at64::lds_t* vt, int* sg, int kv0) {
+    kf(k_rs, kt, kv0, wave);
+    vf(v_rs, vt, kv0, wave);
+    if (kSeg && wave == 2) dma4(make_rsrc(seg + (size_t)b * S, (uint32_t)S * 4u), sg, (kv0 + lane) * 4);
+  };
 
-  // One half of a tile, keys kh0 .. kh0 + 31.  same: no id needs a compare.
-  auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, int kv0, int sb,
-                  bool same) __attribute__((always_inline)) {
+  // One half of a tile, keys kh0 .. kh0 + 31.  docs: ids have to be compared.
+  auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, const int* sg, int kv0, int sb,
+                  int docs) __attribute__((always_inline)) {
     f32x16 s = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) s = mfma32(tile_row(kt, 32 * sb + l32, 2 * kc + hl), qreg[kc], s);
     const int kh0 = kv0 + 32 * sb;
+    // Scores less `off`, which is the same for all of a lane's keys: what a score
+    // has in common with the others of its query costs no operation here.
+    float off = kCap && kMax == kRunning ? a.cap2 : 0.f;
     if constexpr (!kRaw) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float w;
-        s[i] = base_score<kCap>(s[i], a, w);
+        if constexpr (kCap) {
+          const float w = cap_w(s[i], a);
+          s[i] = kBias ? fmaf(twice, w, bias[i]) : twice * w;
+        } else {
+          s[i] = fmaf(s[i], raw, bias[i]);
+        }
       }
+      if constexpr (kBias) off = fmaf(-slope2, (float)(my_q - kh0 - 4 * hl), off);  // element 0's
     }
-    if constexpr (kBias) {
-      const float x = (float)(my_q - kh0 - 4 * hl);
-      if (kh0 + 31 > qw0 && last_prefix > qw0) {  // keys after their query are visible
+    // (One branch for everything that the halves behind every query go without.)
+    if (kh0 + 31 > qw0 || kh0 + 32 > S || (kSeg && docs)) {
+      if constexpr (kBias) {  // keys after their query, where a prefix shows them
+        const float x = (float)(my_q - kh0 - 4 * hl);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope2, fabsf(x - (float)acc_row(i)), s[i]);
-      } else {
-        const float b0 = -slope2 * x;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] += fmaf(slope2, (float)acc_row(i), b0);
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f * slope2, fmaxf((float)acc_row(i) - x, 0.f), s[i]);
       }
-    }
-    const bool masked = kh0 + 31 > all_see || kh0 + 32 > S || (kSeg && !same);
-    if (masked) {
       const int lim = my_last - kh0 - 4 * hl;
+      if (kSeg && docs) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        bool vis = acc_row(i) <= lim;
-        if (kSeg && !same) vis = vis && seg[(size_t)b * S + min(kh0 + 4 * hl + acc_row(i), S - 1)] == seg_q;
-        s[i] = vis ? s[i] : -INFINITY;
+        for (int r = 0; r < 4; ++r) {
+          const i32x4 id = *reinterpret_cast<const i32x4*>(sg + 32 * sb + 8 * r + 4 * hl);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            s[4 * r + t] = acc_row(4 * r + t) <= lim && id[t] == seg_q ? s[4 * r + t] : -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = acc_row(i) <= lim ? s[i] : -INFINITY;
       }
     }
-    float m_tile = -INFINITY;
+    float shift = 0.f;  // of the exponents
+    if constexpr (kMax == kRunning) {
+      float m_tile = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
-    m_tile = fmaxf(m_tile, __shfl_xor(m_tile, 32));
-    if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
-    // The running maximum moves only when a row's maximum exceeds it by more
-    // than 8 (log2): P stays below 2^8 and most halves rescale nothing.
-    const bool grow = m_tile > m_run + 8.0f;
-    const float m_new = grow ? m_tile : m_run;
-    if (__ballot(grow)) {
-      const float alpha = fast_exp2(m_run - m_new);
-      l_run *= alpha;
+      for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
+      if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
+      m_tile += off;  // (with a bias each half-wave has its own)
+      m_tile = fmaxf(m_tile, __shfl_xor(m_tile, 32));
+      // The running maximum moves only when a row's maximum exceeds it by more
+      // than 8 (log2): P stays below 2^8 and most halves rescale nothing.
+      const bool grow = m_tile > m_run + 8.0f;
+      const float m_new = grow ? m_tile : m_run;
+      if (__ballot(grow)) {
+        const float alpha = fast_exp2(m_run - m_new);
+        l_run *= alpha;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+          for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+      }
+      m_run = m_new;
+      shift = off - m_new;
     }
-    m_run = m_new;
     bf16x8 pb[2];
     float lsum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, -m_new) : s[i] - m_new);
+      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, shift) : kMax == kFixed ? s[i] : s[i] + shift);
       lsum += p;
       pb[i >> 3][i & 7] = (bf16)p;
     }
@@ -126,15 +162,14 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   // accumulator element, for +inf and for -inf (both: NaN).
   __shared__ uint64_t dirty_s[4];
   uint64_t plus = 0, minus = 0;
-  auto clean = [&](at64::lds_t* vt, int kv0, bool same) {
+  auto clean = [&](at64::lds_t* vt, const int* sg, int kv0, bool same) {
     const Dirty<D> dirty{dirty_s};
     if (!dirty.find(vt, wave, lane)) return;
 #pragma unroll 1
     for (int r = 0; r < kRows; ++r) {
       if (!__builtin_amdgcn_readfirstlane(dirty.row(r))) continue;
-      const int key = kv0 + r;
-      bool vis = key <= my_last;
-      if (kSeg && !same) vis = vis && seg[(size_t)b * S + min(key, S - 1)] == seg_q;
+      bool vis = kv0 + r <= my_last;
+      if (kSeg && !same) vis = vis && sg[r] == seg_q;
 #pragma unroll 1
       for (int e = 0; e < 16 * DB; ++e) {
         const int col = 32 * (e >> 4) + acc_row(e & 15) + 4 * hl;
@@ -146,18 +181,26 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     dirty.clear(vt, wave, lane);
   };
 
-  // Tile `it` from (kt, vt), the next one, nx, on its way to (nkt, nvt).
-  auto tile = [&](const at64::lds_t* kt, at64::lds_t* vt, at64::lds_t* nkt, at64::lds_t* nvt, int it, int nx,
-                  bool same) __attribute__((always_inline)) {
+  // Tile `it` from (kt, vt, sg), the next one, nx, on its way to (nkt, nvt, nsg).
+  // The halves and the two tiles of the loop below stand in loops without other
+  // exits: acc then has one place (conditional copies of it cost a quarter of the
+  // vector instructions and spilled).
+  auto tile = [&](const at64::lds_t* kt, at64::lds_t* vt, const int* sg, at64::lds_t* nkt, at64::lds_t* nvt, int* nsg,
+                  int it, int nx, bool same) __attribute__((always_inline)) {
     const int kv0 = it * kRows;
-    if (nx < ntiles) {
-      kf(k_rs, nkt, nx * kRows, wave);
-      vf(v_rs, nvt, nx * kRows, wave);
+    int sb = 0, end = 0, docs = 0;
+    if (it < ntiles) {
+      if (nx < ntiles) fill(nkt, nvt, nsg, nx * kRows);
+      if (kv0 + kRows - 1 > max(q0, last_prefix) || (kSeg && !same)) clean(vt, sg, kv0, same);
+      end = kv0 > wave_last ? 0 : kv0 + 32 > wave_last ? 1 : 2;
+      if (kSeg && !same) {
+        const int in = ids.look(sg, lane, docs);
+        sb = in & 1 ? 0 : 1;
+        end = min(end, in & 2 ? 2 : in);
+      }
     }
-    if (kv0 + kRows - 1 > max(q0, last_prefix) || (kSeg && !same)) clean(vt, kv0, same);
-    if (kv0 <= wave_last) half(kt, vt, kv0, 0, same);
-    __builtin_amdgcn_sched_barrier(0);  // keep the halves' live ranges apart
-    if (kv0 + 32 <= wave_last) half(kt, vt, kv0, 1, same);
+#pragma unroll 1
+    for (; sb < end; ++sb) half(kt, vt, sg, kv0, sb, docs >> sb & 1);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   };
@@ -173,19 +216,14 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   };
   bool same = true, same_n = true;
   int it = next(0, same);
-  kf(k_rs, k0s, it * kRows, wave);
-  vf(v_rs, v0s, it * kRows, wave);
+  fill(k0s, v0s, sg0, it * kRows);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  while (true) {  // (A workgroup's own positions hold visible pairs: there is a first tile.)
-    int nx = next(it + 1, same_n);
-    tile(k0s, v0s, k1s, v1s, it, nx, same);
-    if (nx >= ntiles) break;
-    it = nx;
-    nx = next(it + 1, same);
-    tile(k1s, v1s, k0s, v0s, it, nx, same_n);
-    if (nx >= ntiles) break;
-    it = nx;
+  while (it < ntiles) {  // (A workgroup's own positions hold visible pairs: there is a first tile.)
+    const int nx = next(it + 1, same_n);
+    tile(k0s, v0s, sg0, k1s, v1s, sg1, it, nx, same);
+    it = next(nx + 1, same);
+    tile(k1s, v1s, sg1, k0s, v0s, sg0, nx, it, same_n);
   }
 
   const float l_tot = l_run + __shfl_xor(l_run, 32);
@@ -234,11 +272,15 @@ int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const in
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2);
   const MutView O = c.out(3);
-#define SCORED_FWD(D, CAP, BIAS, SEG)                                                                             \
-  scored_fwd_kernel<D, CAP, BIAS, SEG><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, lse2, segment_ids, c.args, batch, \
-                                                                      heads, kv_heads, seq, head_dim)
+#define SCORED_FWD_(D, CAP, BIAS, SEG, MAX)                                                                  \
+  scored_fwd_kernel<D, CAP, BIAS, SEG, MAX><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, lse2, segment_ids, c.args, \
+                                                                           batch, heads, kv_heads, seq, head_dim)
+#define SCORED_FWD(D, CAP, BIAS, SEG)                                                     \
+  if (CAP && !BIAS && score_cap <= kFixedCap) SCORED_FWD_(D, CAP, BIAS, SEG, CAP && !BIAS ? kFixed : kRunning); \
+  else SCORED_FWD_(D, CAP, BIAS, SEG, kRunning)
   SCORED_DISPATCH(SCORED_FWD, c, segment_ids != nullptr);
 #undef SCORED_FWD
+#undef SCORED_FWD_
   GPTRIG_CHECK_LAUNCH();
   return GPTRIG_OK;
 }

@@ -16,10 +16,26 @@ namespace {
 
 constexpr int kOwn = 128;  // queries or keys of a workgroup: 4 waves x 32
 
+// A wave's accumulators in LDS, in the room of one tile, and back.
+template <int DB>
+__device__ __forceinline__ void put(float* at, const f32x16 (&acc)[DB], int lane) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) at[(16 * db + i) * 64 + lane] = acc[db][i];
+}
+template <int DB>
+__device__ __forceinline__ void add(f32x16 (&acc)[DB], const float* at, int lane) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[db][i] += at[(16 * db + i) * 64 + lane];
+}
+
 // The dq pass leaves two numbers a query for the other pass: the constant of its
 // exponents, cap log2 e - L_i (with a bias less slope (i mod 64), the part of the
 // bias that is the query's own in its tile), and -delta_i.
-template <int D, bool kCap, bool kBias, bool kSeg>
+template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, 2)
     scored_dq_kernel(View Q, View K, View V, View O, View dO, const float* __restrict__ lse2,
                      const int32_t* __restrict__ seg, float* __restrict__ shifts, float* __restrict__ minus_delta,
@@ -32,7 +48,8 @@ __global__ void __launch_bounds__(256, 2)
   __shared__ __attribute__((aligned(16))) int sg0[kRows], sg1[kRows];
   __shared__ uint64_t dirty_s[4], scan_s[2];
 
-  const int nq = (S + kOwn - 1) / kOwn;
+  constexpr int kMine = kOwn / kSplit;
+  const int nq = (S + kMine - 1) / kMine;
   int bh, qb;
   xcd_map(blockIdx.x, nq, B * H, bh, qb);
   qb = nq - 1 - qb;
@@ -40,11 +57,12 @@ __global__ void __launch_bounds__(256, 2)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  const int q0 = qb * kOwn, qw0 = q0 + 32 * wave, my_q = qw0 + l32;
+  const int own = wave % (4 / kSplit), part = wave / (4 / kSplit);  // (as in the forward)
+  const int q0 = qb * kMine, qw0 = q0 + 32 * own, my_q = qw0 + l32;
   const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
   const int my_last = min(max(my_q, last_prefix), S - 1);
   const int wave_last = max(qw0 + 31, last_prefix);
-  const int ntiles = max(min(q0 + kOwn, S) - 1, last_prefix) / kRows + 1;
+  const int ntiles = max(min(q0 + kMine, S) - 1, last_prefix) / kRows + 1;
   const float slope2 = kBias ? a.slopes[h] * GPTRIG_LOG2E : 0.f;
   float bias[16], raw = a.raw, twice = -2.0f * a.cap2;
   if constexpr (kBias) {
@@ -67,7 +85,7 @@ __global__ void __launch_bounds__(256, 2)
   delta += __shfl_xor(delta, 32);
   const size_t my_row = (size_t)bh * S + my_q;
   const float shift = my_q < S ? (kCap ? a.cap2 : 0.f) - lse2[my_row] : 0.f;
-  if (my_q < S && hl == 0) {
+  if (my_q < S && hl == 0 && part == 0) {
     shifts[my_row] = kBias ? fmaf(-slope2, (float)(my_q & (kRows - 1)), shift) : shift;
     minus_delta[my_row] = -delta;
   }
@@ -76,7 +94,7 @@ __global__ void __launch_bounds__(256, 2)
   SegScan<4> scan;
   if constexpr (kSeg) {
     ids.init(seg_q);
-    scan.template init<kOwn / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+    scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
   }
 
   f32x16 acc[DB];
@@ -172,6 +190,10 @@ __global__ void __launch_bounds__(256, 2)
         sb = in & 1 ? 0 : 1;
         end = min(end, in & 2 ? 2 : in);
       }
+      if (kSplit == 2) {
+        sb = max(sb, part);
+        end = min(end, part + 1);
+      }
     }
 #pragma unroll 1
     for (; sb < end; ++sb) half(kt, vt, sg, kv0, sb, docs >> sb & 1);
@@ -200,6 +222,13 @@ __global__ void __launch_bounds__(256, 2)
     tile(k1s, v1s, sg1, k0s, v0s, sg0, nx, it, same_n);
   }
 
+  if constexpr (kSplit == 2) {
+    float* const at = reinterpret_cast<float*>(own ? fv0 : fk0);
+    if (part) put<DB>(at, acc, lane);
+    __syncthreads();
+    if (part) return;
+    add<DB>(acc, at, lane);
+  }
   if (my_q < S) {
     const float f = spoilt ? __builtin_nanf("") : kCap ? 4.0f * scale : scale;
     bf16* row = dQ.row(b, h, my_q);
@@ -220,7 +249,7 @@ __global__ void __launch_bounds__(256, 2)
 // dk and dv.  Each wave computes S = Q K^T and dP = do V^T with a lane holding one
 // key, whose k and v stay in registers as operands, and sums dv^T += do^T P and
 // dk^T += Q^T dU over the queries.
-template <int D, bool kCap, bool kBias, bool kSeg>
+template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ shifts,
                       const float* __restrict__ minus_delta, const int32_t* __restrict__ seg, MutView dK, MutView dV,
@@ -236,14 +265,16 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   __shared__ uint64_t dirty_s[4], scan_s[2];
 
   // parts workgroups share the heads of a group where there are few keys to own.
-  const int nkv = (S + kOwn - 1) / kOwn, G = H / Hk / parts;
+  constexpr int kMine = kOwn / kSplit;
+  const int nkv = (S + kMine - 1) / kMine, G = H / Hk / parts;
   int bh, kb;
   xcd_map(blockIdx.x, nkv, B * Hk * parts, bh, kb);
-  const int part = bh % parts, b = bh / parts / Hk, hk = bh / parts % Hk, h0 = hk * (H / Hk) + part * G;
+  const int b = bh / parts / Hk, hk = bh / parts % Hk, h0 = hk * (H / Hk) + bh % parts * G;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  const int k0 = kb * kOwn, kw0 = k0 + 32 * wave, my_k = kw0 + l32;
+  const int group = wave % (4 / kSplit), part = wave / (4 / kSplit);  // (as in the forward)
+  const int k0 = kb * kMine, kw0 = k0 + 32 * group, my_k = kw0 + l32;
   const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
 
   bf16x8 kfr[KC], vfr[KC];
@@ -259,7 +290,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   SegScan<4> scan;
   if constexpr (kSeg) {
     ids.init(seg_k);
-    scan.template init<kOwn / 64>(seg + (size_t)b * S, scan_s, S, k0, lane);
+    scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, k0, lane);
   }
 
   f32x16 dv_acc[DB], dk_acc[DB];
@@ -304,7 +335,6 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
       dp = mfma32(tile_row(gt, 32 * qs + l32, 2 * kc + hl), vfr[kc], dp);
     }
     const int qh0 = qq0 + 32 * qs;
-    __builtin_amdgcn_sched_barrier(0);
     const float off = -slope2 * (float)(qq0 - my_k);
     const bool border = kw0 + 31 > qh0 || qh0 + 32 > S || (kSeg && docs);
     bf16x8 p8[2], ds8[2];
@@ -344,7 +374,6 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     };
     if (border) middle(std::true_type{});
     else middle(std::false_type{});
-    __builtin_amdgcn_sched_barrier(0);
     product<DB>(dv_acc, gt, 32 * qs, p8, lane);
     product<DB>(dk_acc, qt, 32 * qs, ds8, lane);
   };
@@ -369,7 +398,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     const float slope2 = kBias ? a.slopes[h0 + min(g, G - 1)] * GPTRIG_LOG2E : 0.f;
     int qs = 0, end = 0, docs = 0;
     if (g < G) {
-      if (k0 + kOwn - 1 > max(qq0, last_prefix) || (kSeg && !same)) {
+      if (k0 + kMine - 1 > max(qq0, last_prefix) || (kSeg && !same)) {
         clean(qt, sg, qq0, same);
         __syncthreads();  // (the second search reuses the first one's words)
         clean(gt, sg, qq0, same);
@@ -380,6 +409,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
         const int in = ids.look(sg, lane, docs);
         qs = max(qs, in & 1 ? 0 : 1);
         end = min(end, in & 2 ? 2 : in);
+      }
+      if (kSplit == 2) {
+        qs = max(qs, part);
+        end = min(end, part + 1);
       }
     }
 #pragma unroll 1
@@ -427,6 +460,18 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     tile(q1s, g1s, ls1, dl1, sg1, nx, gn, same_n);
   }
 
+  if constexpr (kSplit == 2) {
+    float* const kat = reinterpret_cast<float*>(group ? fq1 : fq0);
+    float* const vat = reinterpret_cast<float*>(group ? fg1 : fg0);
+    if (part) {
+      put<DB>(kat, dk_acc, lane);
+      put<DB>(vat, dv_acc, lane);
+    }
+    __syncthreads();
+    if (part) return;
+    add<DB>(dk_acc, kat, lane);
+    add<DB>(dv_acc, vat, lane);
+  }
   if (my_k < S) {
     const float bad = spoilt ? __builtin_nanf("") : 1.0f;
     const float f = bad * (kCap ? 4.0f * scale : scale);
@@ -530,25 +575,35 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
   if (workspace_bytes < gptrig_scored_attn_bwd_workspace_bytes(batch, heads, kv_heads, seq, head_dim))
     return GPTRIG_E_WORKSPACE;
   if ((uintptr_t)workspace & 15) return GPTRIG_E_SHAPE;
-  const long long grid = (long long)batch * heads * ceil_div(seq, kOwn);
+  const bool split = split_rows((long long)batch * heads, seq, head_dim, false);
+  const long long grid = (long long)batch * heads * ceil_div(seq, split ? kOwn / 2 : kOwn);
   if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
   const int parts = parts_of(batch, heads, kv_heads, seq);
-  const unsigned kv_grid = (unsigned)((long long)batch * kv_heads * parts * ceil_div(seq, kOwn));
+  const bool kv_split = split_rows((long long)batch * kv_heads * parts, seq, head_dim, true);
+  const unsigned kv_grid = (unsigned)((long long)batch * kv_heads * parts * ceil_div(seq, kv_split ? kOwn / 2 : kOwn));
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2), O = c.view(3), dO = c.view(4);
   const MutView dQ = c.out(5), dK = c.out(6), dV = c.out(7);
   float* const shifts = (float*)workspace;
   float* const minus_delta = shifts + row_numbers_bytes(batch, heads, seq) / sizeof(float);
   float* const partial = minus_delta + row_numbers_bytes(batch, heads, seq) / sizeof(float);
-#define SCORED_BWD(D, CAP, BIAS, SEG)                                                                                \
-  scored_dq_kernel<D, CAP, BIAS, SEG><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, dO, lse2, segment_ids, shifts,        \
-                                                                     minus_delta, dQ, c.args, batch, heads, kv_heads,  \
-                                                                     seq, head_dim, softmax_scale);                    \
-  scored_dkv_kernel<D, CAP, BIAS, SEG><<<kv_grid, 256, 0, s>>>(Q, K, V, dO, shifts, minus_delta, segment_ids, dK, dV,  \
-                                                               partial, parts, c.args, batch, heads, kv_heads, seq,    \
-                                                               head_dim, softmax_scale)
+#define SCORED_DQ(D, CAP, BIAS, SEG, SPLIT)                                                                          \
+  scored_dq_kernel<D, CAP, BIAS, SEG, SPLIT><<<(unsigned)grid, 256, 0, s>>>(                                         \
+      Q, K, V, O, dO, lse2, segment_ids, shifts, minus_delta, dQ, c.args, batch, heads, kv_heads, seq, head_dim,     \
+      softmax_scale)
+#define SCORED_DKV(D, CAP, BIAS, SEG, SPLIT)                                                                         \
+  scored_dkv_kernel<D, CAP, BIAS, SEG, SPLIT><<<kv_grid, 256, 0, s>>>(                                               \
+      Q, K, V, dO, shifts, minus_delta, segment_ids, dK, dV, partial, parts, c.args, batch, heads, kv_heads, seq,    \
+      head_dim, softmax_scale)
+#define SCORED_BWD(D, CAP, BIAS, SEG)               \
+  if (split) SCORED_DQ(D, CAP, BIAS, SEG, 2);       \
+  else SCORED_DQ(D, CAP, BIAS, SEG, 1);             \
+  if (kv_split) SCORED_DKV(D, CAP, BIAS, SEG, 2);   \
+  else SCORED_DKV(D, CAP, BIAS, SEG, 1)
   SCORED_DISPATCH(SCORED_BWD, c, segment_ids != nullptr);
 #undef SCORED_BWD
+#undef SCORED_DKV
+#undef SCORED_DQ
   if (parts > 1) {
     const long long threads = 2ll * batch * kv_heads * seq * (head_dim / 8);
     if (threads > 256ll * INT32_MAX) return GPTRIG_E_SHAPE;

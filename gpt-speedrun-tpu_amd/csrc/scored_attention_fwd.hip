@@ -7,7 +7,7 @@
 
 namespace {
 
-constexpr int kQueries = 128;
+constexpr int kQueries = 128;  // of a workgroup; kSplit 2: 64
 
 // With a cap and no bias every score lies within +-cap, so up to kFixedCap a fixed
 // reference in place of the running maximum keeps every P within [2^-100, 1].
@@ -15,7 +15,7 @@ constexpr float kFixedCap = 34.0f;
 
 enum { kRunning = 0, kFixed = 1 };
 
-template <int D, bool kCap, bool kBias, bool kSeg, int kMax>
+template <int D, bool kCap, bool kBias, bool kSeg, int kMax, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     scored_fwd_kernel(View Q, View K, View V, MutView O, float* __restrict__ lse2, const int32_t* __restrict__ seg,
                       ScoreArgs a, int B, int H, int Hk, int S, int dim) {
@@ -27,7 +27,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   __shared__ __attribute__((aligned(16))) bf16 fv1[kRows * D];
   __shared__ __attribute__((aligned(16))) int sg0[kRows], sg1[kRows];
 
-  const int nq = (S + kQueries - 1) / kQueries;
+  constexpr int kMine = kQueries / kSplit;
+  const int nq = (S + kMine - 1) / kMine;
   int bh, qb;
   xcd_map(blockIdx.x, nq, B * H, bh, qb);
   qb = nq - 1 - qb;
@@ -35,11 +36,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  const int q0 = qb * kQueries, qw0 = q0 + 32 * wave, my_q = qw0 + l32;
+  // Two waves share 32 queries where kSplit is 2, each with one half of every tile.
+  const int own = wave % (4 / kSplit), part = wave / (4 / kSplit);
+  const int q0 = qb * kMine, qw0 = q0 + 32 * own, my_q = qw0 + l32;
   const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
   const int my_last = min(max(my_q, last_prefix), S - 1);  // the last key this lane's query may see
   const int wave_last = max(qw0 + 31, last_prefix);
-  const int ntiles = max(min(q0 + kQueries, S) - 1, last_prefix) / kRows + 1;
+  const int ntiles = max(min(q0 + kMine, S) - 1, last_prefix) / kRows + 1;
   const float slope2 = kBias ? a.slopes[h] * GPTRIG_LOG2E : 0.f;
 
   float bias[16];  // of a key acc_row(i) after element 0's
@@ -61,7 +64,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   SegScan<4> scan;
   if constexpr (kSeg) {
     ids.init(seg_q);
-    scan.template init<kQueries / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
+    scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
   }
 
   f32x16 acc[DB];
@@ -198,6 +201,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
         sb = in & 1 ? 0 : 1;
         end = min(end, in & 2 ? 2 : in);
       }
+      if (kSplit == 2) {
+        sb = max(sb, part);
+        end = min(end, part + 1);
+      }
     }
 #pragma unroll 1
     for (; sb < end; ++sb) half(kt, vt, sg, kv0, sb, docs >> sb & 1);
@@ -226,6 +233,28 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     tile(k1s, v1s, sg1, k0s, v0s, sg0, nx, it, same_n);
   }
 
+  if constexpr (kSplit == 2) {  // the second half's sums join the first's
+    __shared__ float ml[2][2][64];
+    float* const at = reinterpret_cast<float*>(own ? fv0 : fk0);  // a tile's room is an accumulator's
+    if (part) {
+      ml[own][0][lane] = m_run;
+      ml[own][1][lane] = l_run;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) at[(16 * db + i) * 64 + lane] = acc[db][i];
+    }
+    __syncthreads();
+    if (part) return;
+    const float m1 = ml[own][0][lane], m = fmaxf(m_run, m1);
+    const float f0 = fast_exp2(m_run - m), f1 = fast_exp2(m1 - m);
+    m_run = m;
+    l_run = l_run * f0 + ml[own][1][lane] * f1;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] = acc[db][i] * f0 + at[(16 * db + i) * 64 + lane] * f1;
+  }
   const float l_tot = l_run + __shfl_xor(l_run, 32);
   if (__ballot((plus | minus) != 0)) {
 #pragma unroll
@@ -267,17 +296,21 @@ int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const in
   const int status = c.init(tensors, 4, 0b0110u, batch, heads, kv_heads, seq, head_dim, strides, softmax_scale,
                             score_cap, distance_slopes, prefix_lengths);
   if (status != GPTRIG_OK) return status;
-  const long long grid = (long long)batch * heads * ceil_div(seq, kQueries);
-  if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2);
   const MutView O = c.out(3);
-#define SCORED_FWD_(D, CAP, BIAS, SEG, MAX)                                                                  \
-  scored_fwd_kernel<D, CAP, BIAS, SEG, MAX><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, lse2, segment_ids, c.args, \
-                                                                           batch, heads, kv_heads, seq, head_dim)
-#define SCORED_FWD(D, CAP, BIAS, SEG)                                                     \
-  if (CAP && !BIAS && score_cap <= kFixedCap) SCORED_FWD_(D, CAP, BIAS, SEG, CAP && !BIAS ? kFixed : kRunning); \
-  else SCORED_FWD_(D, CAP, BIAS, SEG, kRunning)
+  const bool split = split_rows((long long)batch * heads, seq, head_dim, false);
+  const long long grid = (long long)batch * heads * ceil_div(seq, split ? kQueries / 2 : kQueries);
+  if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
+#define SCORED_FWD_(D, CAP, BIAS, SEG, MAX, SPLIT)                                                                  \
+  scored_fwd_kernel<D, CAP, BIAS, SEG, MAX, SPLIT><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, lse2, segment_ids, c.args, \
+                                                                                  batch, heads, kv_heads, seq, head_dim)
+#define SCORED_FWD(D, CAP, BIAS, SEG)                                                                      \
+  constexpr int fixed = CAP && !BIAS ? kFixed : kRunning;                                                  \
+  if (fixed == kFixed && score_cap <= kFixedCap && split) SCORED_FWD_(D, CAP, BIAS, SEG, fixed, 2);        \
+  else if (fixed == kFixed && score_cap <= kFixedCap) SCORED_FWD_(D, CAP, BIAS, SEG, fixed, 1);            \
+  else if (split) SCORED_FWD_(D, CAP, BIAS, SEG, kRunning, 2);                                             \
+  else SCORED_FWD_(D, CAP, BIAS, SEG, kRunning, 1)
   SCORED_DISPATCH(SCORED_FWD, c, segment_ids != nullptr);
 #undef SCORED_FWD
 #undef SCORED_FWD_

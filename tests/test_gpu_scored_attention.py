@@ -200,6 +200,23 @@ def test_long(options):
     compare(*inputs(1, 1, 1, 5000, 128, seed=9), **o)
 
 
+@pytest.mark.parametrize("options", OPTIONS, ids=lambda o: "-".join(o) or "plain")
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_workgroups(options, D):
+    """Enough of them that each owns 128 rows (with fewer, as in the other tests, 64)."""
+
+    print(f"scored attention, many workgroups {options} D={D}", flush=True)
+    B, H, S = 33, 16, 290
+    o = dict(options)
+    if "prefix" in o:
+        o["prefix"] = torch.arange(-3, 10 * B - 3, 10, dtype=torch.int32, device=DEV)
+    if "seg" in o:
+        o["seg"] = documents(B, S, o["seg"])
+    if "slopes" in o:
+        o["slopes"] = slopes_of(H)
+    compare(*inputs(B, H, H if D == 64 else 8, S, D, seed=21), **o)
+
+
 def test_large_scores_and_extreme_caps():
     q, k, v, do = inputs(1, 2, 2, 180, 64, seed=4, size=6.0)
     for cap, scale in ((2.0, None), (0.01, None), (1000.0, None), (40.0, 3.0), (None, 1.0), (None, 0.001)):

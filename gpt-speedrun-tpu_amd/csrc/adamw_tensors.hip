@@ -27,6 +27,9 @@
 #include "common.h"
 
 #include <math.h>
+#include <stdlib.h>
+
+#include <algorithm>
 
 namespace {
 
@@ -54,7 +57,7 @@ struct Items {
   int count;
 };
 struct Scalars {
-  float lr, b1, omb1, b2, omb2, bc1, bc2;
+  float lr, b1, omb1, b2, omb2, ibc1, ibc2;  // ibc: 1 / (1 - beta^step)
   uint32_t seed;  // mix(seed)
 };
 
@@ -66,14 +69,14 @@ __host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-// Four values from a place aligned as one of them.
+// Four values from a place aligned as one of them; kWhole: all four exist.
 template <typename T>
 struct __attribute__((packed)) Four {
   T v[4];
 };
-template <typename T>
+template <bool kWhole, typename T>
 __device__ __forceinline__ void load4(float (&out)[4], const T* __restrict__ at, int left) {
-  if (left >= 4) {
+  if (kWhole || left >= 4) {
     const Four<T> f = *reinterpret_cast<const Four<T>*>(at);
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = (float)f.v[j];
@@ -82,9 +85,9 @@ __device__ __forceinline__ void load4(float (&out)[4], const T* __restrict__ at,
     for (int j = 0; j < 4; ++j) out[j] = j < left ? (float)at[j] : 0.f;
   }
 }
-template <typename T>
+template <bool kWhole, typename T>
 __device__ __forceinline__ void store4(T* __restrict__ at, const float (&v)[4], int left) {
-  if (left >= 4) {
+  if (kWhole || left >= 4) {
     Four<T> f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.v[j] = (T)v[j];
@@ -99,15 +102,17 @@ __device__ __forceinline__ void store4(T* __restrict__ at, const float (&v)[4], 
 struct __attribute__((packed)) Codes {
   uint32_t v;
 };
+template <bool kWhole>
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* __restrict__ at, int left) {
-  if (left >= 4) return reinterpret_cast<const Codes*>(at)->v;
+  if (kWhole || left >= 4) return reinterpret_cast<const Codes*>(at)->v;
   uint32_t c = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) c |= j < left ? (uint32_t)at[j] << (8 * j) : 0u;
   return c;
 }
+template <bool kWhole>
 __device__ __forceinline__ void store_codes(uint8_t* __restrict__ at, uint32_t c, int left) {
-  if (left >= 4) {
+  if (kWhole || left >= 4) {
     reinterpret_cast<Codes*>(at)->v = c;
     return;
   }
@@ -123,35 +128,130 @@ __device__ __forceinline__ void decode(float (&out)[4], uint32_t c, float scale)
   out[3] = b[1] * scale;
 }
 
+// The largest of the wave's values (none negative or NaN), without LDS.
+__device__ __forceinline__ float largest(float v) {
+#define FOLD(ctrl)                                                                                                \
+  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), \
+                                                                     ctrl, 0xF, 0xF, false)));
+  FOLD(0xB1)   // quads, then half rows, rows, and row 15 / 31 on to the rows above
+  FOLD(0x4E)
+  FOLD(0x141)
+  FOLD(0x140)
+  FOLD(0x142)
+  FOLD(0x143)
+#undef FOLD
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // The codes of a lane's four values of a block that the wave holds, and the
-// block's scale.  half: shift of the random half-word.
+// block's scale.  shift: where the random half-words are.
 template <bool kFloor>
 __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&bits)[4], int shift, float& scale) {
   float top = 0.f;
+  bool finite[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = fabsf(x[j]);
-    top = a <= 3.402823466e38f ? fmaxf(top, a) : top;
+    finite[j] = fabsf(x[j]) <= 3.402823466e38f;
+    top = finite[j] ? fmaxf(top, fabsf(x[j])) : top;
   }
-  top = wave_max(top);
+  top = largest(top);
   const bool none = top < kTiny;
   scale = none ? 0.f : top * (1.0f / 448.0f);
   const float inv = none ? 0.f : 1.0f / scale;
   float code[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = fabsf(x[j]);
-    const float y = a <= 3.402823466e38f ? fminf(a * inv, 448.0f) : __builtin_nanf("");
+    const float y = fminf(fabsf(x[j]) * inv, 448.0f);
     uint32_t step = __builtin_bit_cast(uint32_t, y) & 0x7F800000u;
     step = (step < 0x3C800000u ? 0x3C800000u : step) - 0x01800000u;  // at least 2^-6, over 8
-    const float u = ((float)((bits[j] >> shift) & 0xFFFFu) + 0.5f) * (1.0f / 65536.0f);
+    const float u = fmaf((float)((bits[j] >> shift) & 0xFFFFu), 0x1p-16f, 0x1p-17f);
     float c = floorf(fmaf(y, __builtin_bit_cast(float, 0x7F000000u - step), u)) * __builtin_bit_cast(float, step);
-    if (kFloor && a > 0.f && c < 0x1p-9f && !none) c = 0x1p-9f;
-    code[j] = copysignf(c, x[j]);
+    if (kFloor) c = y > 0.f ? fmaxf(c, 0x1p-9f) : c;
+    c = finite[j] ? c : __builtin_nanf("");
+    code[j] = kFloor ? c : copysignf(c, x[j]);
   }
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(code[0], code[1], 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(code[2], code[3], w, true);
   return (uint32_t)w;
+}
+
+// One chunk of a tensor.  Bound by HBM with float32 moments; 8-bit ones also cost
+// about 100 vector operations an element (the hash 10, each encoding 18), a little
+// less than the time of their 16 bytes.  So the square root and the reciprocal are
+// the instructions of one unit in the last place, the root of a small v taken of 2^24
+// times it (the instruction does not take denormals).
+template <typename G, bool k8, bool kWhole>
+__device__ __forceinline__ void update_chunk(const Item& it, const Scalars& k, float lr, float eps, float decay,
+                                             float clip, int64_t base) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = it.n;
+  float* const p = it.p;
+  const G* const g = (const G*)it.g;
+  float pv[kUnroll][4], gv[kUnroll][4], mv[kUnroll][4], vv[kUnroll][4];
+  uint32_t mc[kUnroll], vc[kUnroll];
+  float ms[kUnroll], vs[kUnroll];
+  auto block_of = [&](int u) { return base + (wave + 4 * u) * kBlock; };
+  auto left_of = [&](int64_t at) { return kWhole ? 4 : (int)(n - at < 4 ? (n - at < 0 ? 0 : n - at) : 4); };
+  // Every load of the chunk before the first use.
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t block = block_of(u), at = block + 4 * lane;
+    const int left = left_of(at);
+    load4<kWhole, float>(pv[u], p + at, left);
+    load4<kWhole, G>(gv[u], g + at, left);
+    if constexpr (k8) {
+      mc[u] = load_codes<kWhole>((const uint8_t*)it.m + at, left);
+      vc[u] = load_codes<kWhole>((const uint8_t*)it.v + at, left);
+      ms[u] = kWhole || block < n ? it.ms[block / kBlock] : 0.f;
+      vs[u] = kWhole || block < n ? it.vs[block / kBlock] : 0.f;
+    } else {
+      load4<kWhole, float>(mv[u], (const float*)it.m + at, left);
+      load4<kWhole, float>(vv[u], (const float*)it.v + at, left);
+    }
+  }
+  const uint32_t key = k8 ? mix(k.seed + (uint32_t)it.index * kPhi) + (uint32_t)(base >> 32) * kR3 : 0u;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t block = block_of(u), at = block + 4 * lane;
+    if (!kWhole && block >= n) break;  // (the whole wave)
+    const int left = left_of(at);
+    if constexpr (k8) {
+      decode(mv[u], mc[u], ms[u]);
+      decode(vv[u], vc[u], vs[u]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float gj = gv[u][j] * clip;
+      const float m = k.b1 * mv[u][j] + k.omb1 * gj;
+      const float v = k.b2 * vv[u][j] + k.omb2 * gj * gj;
+      const float vhat = v * k.ibc2;
+      const bool small = vhat < 1.0f;
+      const float root = __builtin_amdgcn_sqrtf(vhat * (small ? 0x1p24f : 1.0f));
+      const float step = (m * k.ibc1) * __builtin_amdgcn_rcpf(fmaf(root, small ? 0x1p-12f : 1.0f, eps));
+      pv[u][j] -= lr * fmaf(decay, pv[u][j], step);
+      // (Past the tensor's end m and v are 0 unless clip is infinite or NaN.)
+      mv[u][j] = kWhole || j < left ? m : 0.f;
+      vv[u][j] = kWhole || j < left ? v : 0.f;
+    }
+    store4<kWhole, float>(p + at, pv[u], left);
+    if (it.shadow) store4<kWhole, bf16>(it.shadow + at, pv[u], left);
+    if constexpr (k8) {
+      uint32_t bits[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bits[j] = mix((uint32_t)(at + j) * kPhi + key);  // (a chunk crosses no 2^32)
+      const uint32_t m8 = encode<false>(mv[u], bits, 0, ms[u]);
+      const uint32_t v8 = encode<true>(vv[u], bits, 16, vs[u]);
+      store_codes<kWhole>((uint8_t*)it.m + at, m8, left);
+      store_codes<kWhole>((uint8_t*)it.v + at, v8, left);
+      if (lane == 0) {
+        it.ms[block / kBlock] = ms[u];
+        it.vs[block / kBlock] = vs[u];
+      }
+    } else {
+      store4<kWhole, float>((float*)it.m + at, mv[u], left);
+      store4<kWhole, float>((float*)it.v + at, vv[u], left);
+    }
+  }
 }
 
 template <typename G, bool k8>
@@ -165,76 +265,44 @@ __global__ void __launch_bounds__(256) adamw_tensors_kernel(Items items, Scalars
     else hi = mid - 1;
   }
   const Item& it = items.item[lo];
-  const int64_t n = it.n;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t base = (int64_t)((int)blockIdx.x - it.first) * kChunk;
   const float lr = k.lr * hparams[3 * it.index], eps = hparams[3 * it.index + 1], decay = hparams[3 * it.index + 2];
   const float clip = clip_scale ? *clip_scale : 1.0f;
-  float* const p = it.p;
-  const G* const g = (const G*)it.g;
-  float pv[kUnroll][4], gv[kUnroll][4], mv[kUnroll][4], vv[kUnroll][4];
-  uint32_t mc[kUnroll], vc[kUnroll];
-  float ms[kUnroll], vs[kUnroll];
-  // Every load of the chunk before the first use.
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int64_t block = base + (wave + 4 * u) * kBlock;
-    const int64_t at = block + 4 * lane;
-    const int left = (int)(n - at < 4 ? (n - at < 0 ? 0 : n - at) : 4);
-    load4<float>(pv[u], p + at, left);
-    load4<G>(gv[u], g + at, left);
-    if constexpr (k8) {
-      mc[u] = load_codes((const uint8_t*)it.m + at, left);
-      vc[u] = load_codes((const uint8_t*)it.v + at, left);
-      ms[u] = block < n ? it.ms[block / kBlock] : 0.f;
-      vs[u] = block < n ? it.vs[block / kBlock] : 0.f;
-    } else {
-      load4<float>(mv[u], (const float*)it.m + at, left);
-      load4<float>(vv[u], (const float*)it.v + at, left);
+  if (base + kChunk <= it.n) update_chunk<G, k8, true>(it, k, lr, eps, decay, clip, base);
+  else update_chunk<G, k8, false>(it, k, lr, eps, decay, clip, base);
+}
+
+// GPTRIG_E_OVERLAP where two of the arrays that the step writes share memory.
+int check_written(const gptrig_adamw_tensor* tensors, int count, bool k8) {
+  struct Range {
+    uintptr_t from, to;
+  };
+  Range few[6 * 64];
+  Range* const r = count <= 64 ? few : (Range*)malloc(sizeof(Range) * 6 * (size_t)count);
+  if (!r) return GPTRIG_E_WORKSPACE;
+  int n = 0;
+  for (int i = 0; i < count; ++i) {
+    const gptrig_adamw_tensor& t = tensors[i];
+    if (t.n == 0) continue;
+    const size_t size = (size_t)t.n, scales = (size_t)((t.n + kBlock - 1) / kBlock) * 4;
+    auto put = [&](const void* p, size_t bytes) {
+      if (p) r[n++] = {(uintptr_t)p, (uintptr_t)p + bytes};
+    };
+    put(t.param, 4 * size);
+    put(t.m, (k8 ? 1 : 4) * size);
+    put(t.v, (k8 ? 1 : 4) * size);
+    put(t.shadow, 2 * size);
+    if (k8) {
+      put(t.m_scale, scales);
+      put(t.v_scale, scales);
     }
   }
-  const uint32_t key = k8 ? mix(k.seed + (uint32_t)it.index * kPhi) : 0u;
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int64_t block = base + (wave + 4 * u) * kBlock;
-    if (block >= n) break;  // (the whole wave)
-    const int64_t at = block + 4 * lane;
-    const int left = (int)(n - at < 4 ? (n - at < 0 ? 0 : n - at) : 4);
-    if constexpr (k8) {
-      decode(mv[u], mc[u], ms[u]);
-      decode(vv[u], vc[u], vs[u]);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float gj = gv[u][j] * clip;
-      const float m = k.b1 * mv[u][j] + k.omb1 * gj;
-      const float v = k.b2 * vv[u][j] + k.omb2 * gj * gj;
-      const float step = (m / k.bc1) / (sqrtf(v / k.bc2) + eps);
-      pv[u][j] -= lr * (step + decay * pv[u][j]);
-      // (Past the tensor's end m and v are 0 unless clip is infinite or NaN.)
-      mv[u][j] = j < left ? m : 0.f;
-      vv[u][j] = j < left ? v : 0.f;
-    }
-    store4<float>(p + at, pv[u], left);
-    if (it.shadow) store4<bf16>(it.shadow + at, pv[u], left);
-    if constexpr (k8) {
-      uint32_t bits[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        bits[j] = mix((uint32_t)(at + j) * kPhi + key + (uint32_t)((at + j) >> 32) * kR3);
-      const uint32_t m8 = encode<false>(mv[u], bits, 0, ms[u]);
-      const uint32_t v8 = encode<true>(vv[u], bits, 16, vs[u]);
-      store_codes((uint8_t*)it.m + at, m8, left);
-      store_codes((uint8_t*)it.v + at, v8, left);
-      if (lane == 0) {
-        it.ms[block / kBlock] = ms[u];
-        it.vs[block / kBlock] = vs[u];
-      }
-    } else {
-      store4<float>((float*)it.m + at, mv[u], left);
-      store4<float>((float*)it.v + at, vv[u], left);
-    }
-  }
+  std::sort(r, r + n, [](const Range& a, const Range& b) { return a.from < b.from; });
+  int status = GPTRIG_OK;
+  for (int i = 1; i < n; ++i)
+    if (r[i].from < r[i - 1].to) status = GPTRIG_E_OVERLAP;
+  if (r != few) free(r);
+  return status;
 }
 
 }  // namespace
@@ -260,14 +328,16 @@ int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad
     if ((words & 3) || ((uintptr_t)t.grad & (grad_type == GPTRIG_TYPE_F32 ? 3 : 1)) || ((uintptr_t)t.shadow & 1))
       return GPTRIG_E_SHAPE;
   }
+  const int written = check_written(tensors, count, k8);
+  if (written != GPTRIG_OK) return written;
   Scalars k;
   k.lr = (float)lr;
   k.b1 = (float)beta1;
   k.omb1 = (float)(1.0 - beta1);
   k.b2 = (float)beta2;
   k.omb2 = (float)(1.0 - beta2);
-  k.bc1 = (float)(1.0 - pow(beta1, (double)step));
-  k.bc2 = (float)(1.0 - pow(beta2, (double)step));
+  k.ibc1 = (float)(1.0 / (1.0 - pow(beta1, (double)step)));
+  k.ibc2 = (float)(1.0 / (1.0 - pow(beta2, (double)step)));
   k.seed = mix(seed);
   hipStream_t s = (hipStream_t)stream;
   int i = 0;

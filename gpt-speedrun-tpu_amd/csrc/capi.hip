@@ -21,6 +21,8 @@ const char* gptrig_status_string(int status) {
       return "HIP kernel launch failed";
     case GPTRIG_E_WORKSPACE:
       return "workspace too small";
+    case GPTRIG_E_OVERLAP:
+      return "buffers that the call writes overlap";
     default:
       return "unknown status";
   }

@@ -61,10 +61,34 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
+// A lane's C pieces of a row held by L lanes, without a branch: the row's last
+// piece ends with the row, so where the width is no multiple of V it repeats some
+// columns of the piece before (skip of them; V for a lane past the row's end).
+// Sums leave those out; stores write the same values to them twice.
+template <typename T, int V, int L, int C, bool kEven>
+struct Row {
+  int at[C], skip[C];
+  __device__ __forceinline__ void init(int lane, int d) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int first = V * (lane + L * c);
+      at[c] = min(first, d - V);
+      skip[c] = min(first - at[c], V);
+    }
+  }
+  // 1 for a column that piece c owns, else 0.
+  __device__ __forceinline__ bool owns(int c, int j) const { return kEven ? skip[c] == 0 : j >= skip[c]; }
+  __device__ __forceinline__ bool some(int c) const { return skip[c] < V; }
+};
+template <typename T, int V>
+__device__ __forceinline__ Piece<T, V> piece(const T* row, int at) {
+  return *reinterpret_cast<const Piece<T, V>*>(row + at);
+}
+
 // ---------------------------------------------------------------------------
 // Forward: L lanes hold a row, C pieces of V = 16 bytes each.
 // ---------------------------------------------------------------------------
-template <typename T, typename P, int L, int C>
+template <typename T, typename P, int L, int C, bool kEven>
 __global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx,
                                                             const P* __restrict__ scale, const P* __restrict__ bias,
                                                             T* __restrict__ y, float* __restrict__ mean,
@@ -75,14 +99,20 @@ __global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict_
   const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (row >= rows) return;  // (with L = 256 the whole workgroup)
   const T* xr = x + row * ldx;
+  Row<T, V, L, C, kEven> my;
+  my.init(lane, d);
+  Piece<T, V> raw[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) raw[c] = piece<T, V>(xr, my.at[c]);
   float v[C][V];
   float sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    load_piece<T, V>(v[c], xr, V * (lane + L * c), d);
+  for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum += v[c][j];
-  }
+    for (int j = 0; j < V; ++j) {
+      v[c][j] = (float)raw[c].v[j];
+      sum += my.owns(c, j) ? v[c][j] : 0.f;
+    }
   const float mu = row_sum<L>(sum, red[0]) / (float)d;
   float sq = 0.f;
 #pragma unroll
@@ -90,7 +120,7 @@ __global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict_
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       v[c][j] -= mu;
-      if (V * (lane + L * c) + j < d) sq += v[c][j] * v[c][j];
+      sq += my.owns(c, j) ? v[c][j] * v[c][j] : 0.f;
     }
   const float r = rsqrtf(row_sum<L>(sq, red[1]) / (float)d + eps);
   if (lane == 0 && mean) {
@@ -99,16 +129,14 @@ __global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict_
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int at = V * (lane + L * c);
-    if (at >= d) break;
-    float s[V], b[V];
-    load_piece<P, V>(s, scale, at, d);
+    if (!my.some(c)) continue;
+    const Piece<P, V> s = piece<P, V>(scale, my.at[c]);
+    Piece<P, V> b;
+    if (bias) b = piece<P, V>(bias, my.at[c]);
+    Piece<T, V> o;
 #pragma unroll
-    for (int j = 0; j < V; ++j) b[j] = 0.f;
-    if (bias) load_piece<P, V>(b, bias, at, d);
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = fmaf(v[c][j] * r, s[j], b[j]);
-    store_piece<T, V>(y + row * d, s, at, d);
+    for (int j = 0; j < V; ++j) o.v[j] = (T)fmaf(v[c][j] * r, (float)s.v[j], bias ? (float)b.v[j] : 0.f);
+    *reinterpret_cast<Piece<T, V>*>(y + row * d + my.at[c]) = o;
   }
 }
 
@@ -164,7 +192,8 @@ __global__ void __launch_bounds__(256) layernorm_fwd_wide_kernel(const T* __rest
 // layernorm_columns_kernel adds the partial rows in a fixed order (no atomics:
 // the gradients are the same on every run).
 // ---------------------------------------------------------------------------
-template <typename T, typename P, int L, int C>
+// The next row's pieces are on their way while this row is summed.
+template <typename T, typename P, int L, int C, bool kEven>
 __global__ void __launch_bounds__(256)
     layernorm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
                          const P* __restrict__ scale, const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -173,49 +202,61 @@ __global__ void __launch_bounds__(256)
   __shared__ float red[2][2][4];
   __shared__ float join[G > 1 ? G : 1][G > 1 ? L * V : 1];
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  Row<T, V, L, C, kEven> my;
+  my.init(lane, d);
   float ds[C][V], db[C][V], s[C][V];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    load_piece<P, V>(s[c], scale, V * (lane + L * c), d);
+    const Piece<P, V> p = piece<P, V>(scale, my.at[c]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) ds[c][j] = db[c][j] = 0.f;
+    for (int j = 0; j < V; ++j) {
+      s[c][j] = (float)p.v[j];
+      ds[c][j] = db[c][j] = 0.f;
+    }
   }
   const float inv_d = 1.f / (float)d;
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * G + group; row < rows; row += (int64_t)gridDim.x * G, turn ^= 1) {
-    const T* gr = dy + row * lddy;
-    const T* xr = x + row * ldx;
-    const float mu = mean[row], r = rstd[row];
-    float g[C][V], h[C][V];
+  const int64_t step = (int64_t)gridDim.x * G;
+  Piece<T, V> gp[C], xp[C];
+  float mu = 0.f, r = 0.f;
+  auto load = [&](int64_t row) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      load_piece<T, V>(g[c], gr, V * (lane + L * c), d);
-      load_piece<T, V>(h[c], xr, V * (lane + L * c), d);
+      gp[c] = piece<T, V>(dy + row * lddy, my.at[c]);
+      xp[c] = piece<T, V>(x + row * ldx, my.at[c]);
     }
+    mu = mean[row];
+    r = rstd[row];
+  };
+  int turn = 0;
+  int64_t row = (int64_t)blockIdx.x * G + group;
+  if (row < rows) load(row);
+  for (; row < rows; row += step, turn ^= 1) {
+    float g[C][V], h[C][V];
     float a = 0.f, b = 0.f;
+    const float my_r = r;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        // (Past the row's end dy is 0 and so is everything summed here.)
-        h[c][j] = (h[c][j] - mu) * r;
-        db[c][j] += g[c][j];
-        ds[c][j] = fmaf(g[c][j], h[c][j], ds[c][j]);
-        g[c][j] *= s[c][j];
-        a += g[c][j];
-        b = fmaf(g[c][j], h[c][j], b);
+        h[c][j] = ((float)xp[c].v[j] - mu) * r;
+        const float u = (float)gp[c].v[j], own = my.owns(c, j) ? u : 0.f;
+        db[c][j] += own;
+        ds[c][j] = fmaf(own, h[c][j], ds[c][j]);
+        g[c][j] = u * s[c][j];
+        a = fmaf(own, s[c][j], a);
+        b = fmaf(my.owns(c, j) ? g[c][j] : 0.f, h[c][j], b);
       }
+    load(row + step < rows ? row + step : row);
     if (dx) {
       a = row_sum<L>(a, red[turn][0]) * inv_d;
       b = row_sum<L>(b, red[turn][1]) * inv_d;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int at = V * (lane + L * c);
-        if (at < d) {
+        if (!my.some(c)) continue;
+        Piece<T, V> o;
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[c][j] = r * (g[c][j] - a - h[c][j] * b);
-          store_piece<T, V>(dx + row * d, g[c], at, d);
-        }
+        for (int j = 0; j < V; ++j) o.v[j] = (T)(my_r * (g[c][j] - a - h[c][j] * b));
+        *reinterpret_cast<Piece<T, V>*>(dx + row * d + my.at[c]) = o;
       }
     }
   }
@@ -226,6 +267,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       if constexpr (G > 1) {
+        // (By the columns that a piece owns: those it repeats are the piece's before.)
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j) join[group][V * lane + j] = which ? db[c][j] : ds[c][j];
@@ -234,14 +276,13 @@ __global__ void __launch_bounds__(256)
           float t = 0.f;
 #pragma unroll
           for (int k = 0; k < G; ++k) t += join[k][i];
-          if (L * V * c + i < d) out[(size_t)which * d + L * V * c + i] = t;
+          const int first = V * (i / V + L * c), at = min(first, d - V), col = at + i % V;
+          if (col >= first) out[(size_t)which * d + col] = t;
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int at = V * (lane + L * c) + j;
-          if (at < d) out[(size_t)which * d + at] = which ? db[c][j] : ds[c][j];
-        }
+        for (int j = 0; j < V; ++j)
+          if (my.owns(c, j)) out[(size_t)which * d + my.at[c] + j] = which ? db[c][j] : ds[c][j];
       }
     }
 }
@@ -337,14 +378,15 @@ __global__ void __launch_bounds__(256) layernorm_columns_kernel(const float* __r
   }
 }
 
-// Lanes a row and pieces a lane for pieces of V values: the fewest idle lanes
-// among 32 lanes of up to 4 pieces, then 64, then a workgroup of up to 4; {0, 0}
-// for wider rows.
+// Lanes a row and pieces a lane for pieces of V values: 32 lanes of up to 4
+// pieces, then 64, then a workgroup of up to 4; {0, 0} for wider rows, and for rows
+// of less than a piece.
 struct Shape {
   int lanes, pieces;
 };
 Shape row_shape(int d, int v) {
   const int pieces = ceil_div(d, v);
+  if (d < v) return {0, 0};
   if (pieces <= 128) return {32, ceil_div(pieces, 32)};
   if (pieces <= 256) return {64, ceil_div(pieces, 64)};
   if (pieces <= 1024) return {256, ceil_div(pieces, 256)};
@@ -382,11 +424,14 @@ void launch_fwd(const void* x, int64_t ldx, const void* scale, const void* bias,
     return;
   }
   const unsigned grid = (unsigned)((rows + 256 / sh.lanes - 1) / (256 / sh.lanes));
-#define LN_FWD(L, C)                                                                                             \
-  layernorm_fwd_kernel<T, P, L, C><<<grid, 256, 0, st>>>((const T*)x, ldx, (const P*)scale, (const P*)bias, (T*)y, \
-                                                         mean, rstd, rows, d, eps)
+  const bool even = d % (16 / sizeof(T)) == 0;
+#define LN_FWD_(L, C, EVEN)                                                                                       \
+  layernorm_fwd_kernel<T, P, L, C, EVEN><<<grid, 256, 0, st>>>((const T*)x, ldx, (const P*)scale, (const P*)bias,  \
+                                                               (T*)y, mean, rstd, rows, d, eps)
+#define LN_FWD(L, C) if (even) LN_FWD_(L, C, true); else LN_FWD_(L, C, false)
   LN_SHAPES(LN_FWD)
 #undef LN_FWD
+#undef LN_FWD_
 }
 
 template <typename T, typename P>
@@ -395,15 +440,18 @@ void launch_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const 
                 hipStream_t st) {
   const Shape sh = row_shape(d, 16 / sizeof(T));
   const int parts = parts_of(rows, d, 16 / sizeof(T));
+  const bool even = d % (16 / sizeof(T)) == 0;
   if (!dscale && !dbias) partial = nullptr;
   if (rows > 0) {
     if (sh.lanes) {
-#define LN_BWD(L, C)                                                                                              \
-  layernorm_bwd_kernel<T, P, L, C><<<dx && !partial ? (unsigned)((rows + 256 / L - 1) / (256 / L)) : (unsigned)parts, \
-                                     256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx, (const P*)scale, mean, rstd, \
-                                                   (T*)dx, partial, rows, d)
+#define LN_BWD_(L, C, EVEN)                                                                                           \
+  layernorm_bwd_kernel<T, P, L, C, EVEN>                                                                              \
+      <<<dx && !partial ? (unsigned)((rows + 256 / L - 1) / (256 / L)) : (unsigned)parts, 256, 0, st>>>(              \
+          (const T*)dy, lddy, (const T*)x, ldx, (const P*)scale, mean, rstd, (T*)dx, partial, rows, d)
+#define LN_BWD(L, C) if (even) LN_BWD_(L, C, true); else LN_BWD_(L, C, false)
       LN_SHAPES(LN_BWD)
 #undef LN_BWD
+#undef LN_BWD_
     } else {
       if (dx)
         layernorm_bwd_wide_kernel<T, P><<<(unsigned)rows, 256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx,

@@ -141,23 +141,33 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+class StatusError(RuntimeError):
+    """An entry point's non-zero status."""
+
+    def __init__(self, text: str, status: int):
+        super().__init__(text)
+        self.status = status
+
+
 def call(name: str, *args) -> None:
-    """Invoke an entry point; a non-zero status raises ``RuntimeError``."""
+    """Invoke an entry point; a non-zero status raises ``StatusError``, a ``RuntimeError``."""
 
     status = getattr(lib(), name)(*args)
     if status != 0:
         text = lib().gptrig_status_string(status).decode()
-        raise RuntimeError(f"{name} failed: {text} (status {status})")
+        raise StatusError(f"{name} failed: {text} (status {status})", status)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call(name, *args, stream)`` on ``device``'s current stream, with that device the current one."""
+def call_on(device: int, name: str, *args) -> None:
+    """``call(name, *args, stream)`` on GPU ``device``'s current stream, with that GPU the current one."""
 
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream())
+    # (The bindings below torch.cuda's functions: those look for a pending
+    # initialisation first, and a call of a small size is bound by the host.)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(device))
         return
-    with torch.cuda.device(device):
-        call(name, *args, stream())
+    call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def query(name: str, *args) -> int:
@@ -182,13 +192,19 @@ def require_device(*tensors: torch.Tensor) -> None:
             raise RuntimeError("gptrig kernels run on the GPU; got a CPU tensor")
 
 
-def require_one_device(*tensors: torch.Tensor | None) -> None:
+def require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
     """All of them on one GPU."""
 
-    require_device(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f"the tensors lie on several devices: {sorted(map(str, devices))}")
+    device = first.get_device()  # (-1: host memory)
+    if device >= 0:
+        for t in others:
+            if t is not None and t.get_device() != device:
+                break
+        else:
+            return
+    require_device(first, *others)
+    devices = sorted({str(t.device) for t in (first, *others) if t is not None})
+    raise RuntimeError(f"the tensors lie on several devices: {devices}")
 
 
 def workspace(nbytes: int, device) -> torch.Tensor:

@@ -92,7 +92,7 @@ class _ScoredAttention(torch.autograd.Function):
         o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
         keep = any(ctx.needs_input_grad)
         lse2 = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if keep else None
-        _lib.call_on(q.device, "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _lib.call_on(q.get_device(), "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
                      _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(lse2),
                      B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
         if keep:
@@ -101,21 +101,28 @@ class _ScoredAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse2, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
-        B, H, S, D = q.shape
-        Hk = k.shape[1]
-        do = _view(do)
-        dq = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
-        dk = torch.empty((B, Hk, S, D), dtype=q.dtype, device=q.device)
-        dv = torch.empty_like(dk)
-        ws = _lib.workspace(_lib.query("gptrig_scored_attn_bwd_workspace_bytes", B, H, Hk, S, D), q.device)
-        _lib.call_on(q.device, "gptrig_scored_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                     do.data_ptr(), lse2.data_ptr(), _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes),
-                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), B, H, Hk, S, D,
-                     _strides(q, k, v, o, do, dq, dk, dv), *ctx.scalars)
-        return dq, dk, dv, None, None, None, None, None
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, do)
+
+
+def _backward(ctx, do):
+    q, k, v, o, lse2, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
+    B, H, S, D = q.shape
+    Hk = k.shape[1]
+    do = _view(do)
+    dq = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((B, Hk, S, D), dtype=q.dtype, device=q.device)
+    dv = torch.empty_like(dk)
+    size = _lib.query("gptrig_scored_attn_bwd_workspace_bytes", B, H, Hk, S, D)
+    ws = _lib.workspace(size, q.device)
+    _lib.call_on(q.get_device(), "gptrig_scored_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                 do.data_ptr(), lse2.data_ptr(), _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes),
+                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size, B, H, Hk, S, D,
+                 _strides(q, k, v, o, do, dq, dk, dv), *ctx.scalars)
+    return dq, dk, dv, None, None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def make_scored_attention(config: ScoredAttentionConfig = ScoredAttentionConfig()) -> Callable:

@@ -107,52 +107,61 @@ _TYPES = {BF16: 0, torch.float32: 1}  # GPTRIG_TYPE_* of include/gptrig.h
 def _strided_rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` as ``[rows, width]`` with unit stride along the width, without a copy where its strides allow it."""
 
-    x2 = x.reshape(-1, x.shape[-1])
-    return x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous()
+    if x.ndim != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, eps):
         x2 = _strided_rows(x)
-        s = scale.contiguous()
-        b = None if bias is None else bias.contiguous()
+        scale = scale.contiguous()
+        bias = None if bias is None else bias.contiguous()
         rows, d = x2.shape
         y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
         keep = any(ctx.needs_input_grad)
         stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-        mean, rstd = (stats.data_ptr(), stats.data_ptr() + 4 * rows) if keep else (None, None)
+        mean = stats.data_ptr() if keep else None
         if rows:
-            _lib.call_on(x.device, "gptrig_layernorm_fwd", x2.data_ptr(), x2.stride(0), _TYPES[x.dtype], s.data_ptr(),
-                         _lib.ptr(b), _TYPES[s.dtype], y.data_ptr(), mean, rstd, rows, d, eps)
+            _lib.call_on(x.get_device(), "gptrig_layernorm_fwd", x2.data_ptr(), x2.stride(0), _TYPES[x.dtype],
+                         scale.data_ptr(), _lib.ptr(bias), _TYPES[scale.dtype], y.data_ptr(), mean,
+                         mean + 4 * rows if keep else None, rows, d, eps)
         if keep:
-            ctx.save_for_backward(x2, s, stats)
+            ctx.save_for_backward(x2, scale, stats)
             ctx.shape = x.shape
-        return y.reshape(x.shape)
+        return y if x.ndim == 2 else y.reshape(x.shape)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x2, s, stats = ctx.saved_tensors
-        rows, d = x2.shape
-        dev = x2.device
-        need_x, need_s, need_b = ctx.needs_input_grad[:3]
-        if not rows:
-            zero = torch.zeros(d, dtype=s.dtype, device=dev)
-            return (dy.reshape(ctx.shape) if need_x else None, zero if need_s else None,
-                    zero.clone() if need_b else None, None)
-        dy2 = _strided_rows(dy)
-        dx = torch.empty((rows, d), dtype=x2.dtype, device=dev) if need_x else None
-        dscale = torch.empty(d, dtype=s.dtype, device=dev) if need_s else None
-        dbias = torch.empty(d, dtype=s.dtype, device=dev) if need_b else None
-        ws = None
-        if need_s or need_b:
-            ws = _lib.workspace(_lib.query("gptrig_layernorm_bwd_workspace_bytes", rows, d, _TYPES[x2.dtype]), dev)
-        _lib.call_on(dev, "gptrig_layernorm_bwd", dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0),
-                     _TYPES[x2.dtype], s.data_ptr(), _TYPES[s.dtype], stats.data_ptr(), stats.data_ptr() + 4 * rows,
-                     _lib.ptr(dx), _lib.ptr(dscale), _lib.ptr(dbias), _lib.ptr(ws), 0 if ws is None else ws.numel(),
-                     rows, d)
-        return None if dx is None else dx.reshape(ctx.shape), dscale, dbias, None
+        return (_layer_norm_backward_once if torch.is_grad_enabled() else _layer_norm_backward)(ctx, dy)
+
+
+def _layer_norm_backward(ctx, dy):
+    x2, scale, stats = ctx.saved_tensors
+    need_x, need_s, need_b, _ = ctx.needs_input_grad
+    rows, d = x2.shape
+    dev = x2.device
+    if not rows:
+        zero = torch.zeros(d, dtype=scale.dtype, device=dev)
+        return (dy.reshape(ctx.shape) if need_x else None, zero if need_s else None, zero.clone() if need_b else None,
+                None)
+    dy2 = _strided_rows(dy)
+    dx = torch.empty((rows, d), dtype=x2.dtype, device=dev) if need_x else None
+    dscale = torch.empty(d, dtype=scale.dtype, device=dev) if need_s else None
+    dbias = torch.empty(d, dtype=scale.dtype, device=dev) if need_b else None
+    kind, ws, size = _TYPES[x2.dtype], None, 0
+    if need_s or need_b:
+        size = _lib.query("gptrig_layernorm_bwd_workspace_bytes", rows, d, kind)
+        ws = _lib.workspace(size, dev)
+    mean = stats.data_ptr()
+    _lib.call_on(x2.get_device(), "gptrig_layernorm_bwd", dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0),
+                 kind, scale.data_ptr(), _TYPES[scale.dtype], mean, mean + 4 * rows, _lib.ptr(dx), _lib.ptr(dscale),
+                 _lib.ptr(dbias), _lib.ptr(ws), size, rows, d)
+    return dx if dx is None or len(ctx.shape) == 2 else dx.reshape(ctx.shape), dscale, dbias, None
+
+
+_layer_norm_backward_once = once_differentiable(_layer_norm_backward)
 
 
 def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -170,18 +179,19 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None =
     if scale.dtype not in _TYPES or (bias is not None and bias.dtype != scale.dtype):
         raise TypeError(f"scale and bias must both be float32 or both bfloat16, got {scale.dtype} and "
                         f"{None if bias is None else bias.dtype}")
-    if x.ndim == 0 or x.shape[-1] == 0:
-        raise ValueError(f"x needs a last dimension to normalise over, got {tuple(x.shape)}")
-    width = x.shape[-1]
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"x needs a last dimension to normalise over, got {tuple(shape)}")
+    width = shape[-1]
     if scale.shape != (width,) or (bias is not None and bias.shape != (width,)):
         raise ValueError(f"scale and bias must be [{width}], got {tuple(scale.shape)} and "
                          f"{None if bias is None else tuple(bias.shape)}")
     if width > 1 << 30 or x.numel() // width >= 1 << 31:
-        raise ValueError(f"at most 2^30 wide and fewer than 2^31 rows, got {tuple(x.shape)}")
-    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"at most 2^30 wide and fewer than 2^31 rows, got {tuple(shape)}")
+    if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     _lib.require_one_device(x, scale, bias)
-    return _LayerNorm.apply(x, scale, bias, float(eps))
+    return _LayerNorm.apply(x, scale, bias, eps)
 
 
 _ROPE_TABLES: dict = {}

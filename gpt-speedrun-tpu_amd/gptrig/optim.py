@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -116,6 +117,9 @@ def tensor_hparams(paths, cfg: OptimizerConfig, parameterization: str, width: fl
 # Consecutive values of a tensor that share a scale of the 8-bit moments.
 STATE_BLOCK = 256
 _STATE_TYPES = {torch.float32: 32, torch.float8_e4m3fn: 8}
+_F32, _BF16 = {torch.float32}, {torch.bfloat16}
+_DTYPE, _SHAPE = operator.attrgetter("dtype"), operator.attrgetter("shape")
+E_OVERLAP = -7  # GPTRIG_E_OVERLAP
 
 
 def adamw_tensors_state(params: Sequence[torch.Tensor], bits: int = 32) -> dict[str, list[torch.Tensor]]:
@@ -134,22 +138,24 @@ def adamw_tensors_state(params: Sequence[torch.Tensor], bits: int = 32) -> dict[
     return state
 
 
-def _list_of(name: str, tensors, like: Sequence[torch.Tensor], sizes: Sequence, dtypes, device) -> torch.dtype | None:
-    """Checks a list of tensors beside ``like``; its type (None for an empty list)."""
+def _list_of(name: str, tensors, shapes: list, dtypes, device: int) -> torch.dtype:
+    """Checks a list of tensors against the shapes and the GPU it must have; its type."""
 
-    if len(tensors) != len(like):
-        raise ValueError(f"{name} has {len(tensors)} tensors, params {len(like)}")
-    types = {t.dtype for t in tensors}
+    # (Maps over bound methods: with many small tensors the host's work is the step's.)
+    if len(tensors) != len(shapes):
+        raise ValueError(f"{name} has {len(tensors)} tensors, params {len(shapes)}")
+    types = set(map(_DTYPE, tensors))
     if len(types) > 1 or not types <= dtypes:
         raise TypeError(f"{name} must all be one of {sorted(map(str, dtypes))}, got {sorted(map(str, types))}")
-    for i, (t, size) in enumerate(zip(tensors, sizes)):
-        if t.shape != size:
-            raise ValueError(f"{name}[{i}] must be {tuple(size)}, got {tuple(t.shape)}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name}[{i}] must be contiguous")
-        if t.device != device:
-            raise RuntimeError(f"{name}[{i}] is on {t.device}, params[0] on {device}")
-    return types.pop() if types else None
+    if list(map(_SHAPE, tensors)) != shapes:
+        i = next(i for i, t in enumerate(tensors) if t.shape != shapes[i])
+        raise ValueError(f"{name}[{i}] must be {tuple(shapes[i])}, got {tuple(tensors[i].shape)}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        i = next(i for i, t in enumerate(tensors) if not t.is_contiguous())
+        raise ValueError(f"{name}[{i}] must be contiguous")
+    if set(map(torch.Tensor.get_device, tensors)) != {device}:
+        raise RuntimeError(f"{name} must all be on the device of params[0]")
+    return types.pop()
 
 
 def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
@@ -175,23 +181,22 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
 
     if not params:
         raise ValueError("adamw_tensors needs at least one tensor")
-    f32 = {torch.float32}
-    device = params[0].device
-    shapes = [p.shape for p in params]
-    _list_of("params", params, params, shapes, f32, device)
-    grad_type = _list_of("grads", grads, params, shapes, {torch.float32, torch.bfloat16}, device)
-    kind = _list_of("exp_avg", exp_avg, params, shapes, set(_STATE_TYPES), device)
-    _list_of("exp_avg_sq", exp_avg_sq, params, shapes, {kind}, device)
+    device = params[0].get_device()
+    shapes = list(map(_SHAPE, params))
+    counts = list(map(torch.Tensor.numel, params))
+    _list_of("params", params, shapes, _F32, device)
+    grad_type = _list_of("grads", grads, shapes, _F32 | _BF16, device)
+    kind = _list_of("exp_avg", exp_avg, shapes, _STATE_TYPES.keys(), device)
+    _list_of("exp_avg_sq", exp_avg_sq, shapes, {kind}, device)
     bits = _STATE_TYPES[kind]
-    counts = [p.numel() for p in params]
     if (exp_avg_scale is None) != (bits == 32) or (exp_avg_sq_scale is None) != (bits == 32):
         raise ValueError("8-bit moments, and only those, come with exp_avg_scale and exp_avg_sq_scale")
     if bits == 8:
         blocks = [(-(-n // STATE_BLOCK),) for n in counts]
-        _list_of("exp_avg_scale", exp_avg_scale, params, blocks, f32, device)
-        _list_of("exp_avg_sq_scale", exp_avg_sq_scale, params, blocks, f32, device)
+        _list_of("exp_avg_scale", exp_avg_scale, blocks, _F32, device)
+        _list_of("exp_avg_sq_scale", exp_avg_sq_scale, blocks, _F32, device)
     if shadow is not None:
-        _list_of("shadow", shadow, params, shapes, {torch.bfloat16}, device)
+        _list_of("shadow", shadow, shapes, _BF16, device)
     if hparams.dtype != torch.float32 or hparams.shape != (len(params), 3) or not hparams.is_contiguous():
         raise ValueError(f"hparams must be contiguous float32 [{len(params)}, 3], got {hparams.dtype} "
                          f"{tuple(hparams.shape)}")
@@ -204,22 +209,19 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     seed = step % 2 ** 32 if seed is None else seed
     if not 0 <= seed < 2 ** 32:
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
-
-    def addresses(tensors):
-        return [0] * len(params) if tensors is None else [t.data_ptr() for t in tensors]
-
-    lists = [addresses(t) for t in (params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, shadow)]
-    sizes = (4, None, bits // 8, bits // 8, 4 / STATE_BLOCK, 4 / STATE_BLOCK, 2)
-    written = sorted((a, a + n * size) for addr, size in zip(lists, sizes) if size
-                     for a, n in zip(addr, counts) if n and a)
-    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
-        raise ValueError("tensors that the step writes overlap")
     _lib.require_one_device(params[0], hparams, clip_scale)
     # One row of gptrig_adamw_tensor a tensor: seven addresses and the count.
     table = [0] * (8 * len(params))
-    for column, values in enumerate((*lists, counts)):
-        table[column::8] = values
-    _lib.call_on(device, "gptrig_adamw_tensors", (ctypes.c_int64 * len(table))(*table), len(params),
-                 1 if grad_type == torch.float32 else 0, bits, hparams.data_ptr(), float(lr), float(beta1), float(beta2),
-                 int(step), _lib.ptr(clip_scale), seed)
+    for column, tensors in enumerate((params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, shadow)):
+        if tensors is not None:
+            table[column::8] = map(torch.Tensor.data_ptr, tensors)
+    table[7::8] = counts
+    try:
+        _lib.call_on(device, "gptrig_adamw_tensors", (ctypes.c_int64 * len(table))(*table), len(params),
+                     1 if grad_type == torch.float32 else 0, bits, hparams.data_ptr(), float(lr), float(beta1),
+                     float(beta2), int(step), _lib.ptr(clip_scale), seed)
+    except _lib.StatusError as error:
+        if error.status == E_OVERLAP:
+            raise ValueError("tensors that the step writes overlap") from error
+        raise
     torch.autograd.graph.increment_version(params)  # (a graph that saved one of them must not run backward now)

@@ -32,6 +32,7 @@ extern "C" {
 #define GPTRIG_E_UNSUPPORTED (-4) /* legal but not implemented (e.g. head_dim) */
 #define GPTRIG_E_LAUNCH (-5)      /* the HIP launch failed */
 #define GPTRIG_E_WORKSPACE (-6)   /* workspace smaller than the query says */
+#define GPTRIG_E_OVERLAP (-7)     /* buffers that a call writes overlap */
 
 /* Element types, where an entry point takes more than one. */
 #define GPTRIG_TYPE_BF16 0
@@ -400,8 +401,9 @@ int gptrig_adamw(float* param, const float* grad, float* m, float* v, void* para
  * list and the element's in the tensor: give every step another seed.  An
  * infinite or NaN moment is kept as a NaN code.  grad_type of all gradients;
  * tensor_hparams f32 [count, 3] = {lr_mult, epsilon, decay} in device memory;
- * clip_scale a nullable device scalar.  Pointers aligned to their element; no
- * two tensors' memory may overlap; at most 2^40 elements a tensor. */
+ * clip_scale a nullable device scalar.  Pointers aligned to their element; at
+ * most 2^40 elements a tensor; GPTRIG_E_OVERLAP where two of the arrays that the
+ * call writes share memory. */
 typedef struct {
   float* param;    /* f32 [n], updated */
   const void* grad;

@@ -277,3 +277,17 @@ def test_backward_through_a_changed_parameter_is_refused():
     L.step(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_the_same_tensor_twice_is_refused():
+    L = Lists([(300,), (300,)], 32)
+    before = L.p[0].clone()
+    L.p[1] = L.p[0]
+    with pytest.raises(ValueError, match="overlap"):
+        L.step(1)
+    M = Lists([(300,), (300,)], 8)
+    M.vs[1] = M.ms[1]
+    with pytest.raises(ValueError, match="overlap"):
+        M.step(1)
+    torch.cuda.synchronize()
+    assert torch.equal(L.p[0], before)

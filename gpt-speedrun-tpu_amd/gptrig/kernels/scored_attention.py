@@ -17,6 +17,7 @@ are handled in-kernel.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 from typing import Callable
@@ -25,7 +26,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .flash_attention import _kernel_view, _strides
 
 MAX_CAP = 1000.0  # float32 tells tanh scores of a larger cap apart less well than bfloat16 operands do
 
@@ -75,30 +75,49 @@ def _validate(q, k, v, segment_ids, prefix_lengths, distance_slopes) -> None:
             raise ValueError("distance_slopes are constants: no gradient is computed for them")
 
 
-def _view(t: torch.Tensor) -> torch.Tensor:
-    """A view the kernels accept: as the causal kernels', and a (batch, head) slice within 32-bit offsets."""
+def _fits(t: torch.Tensor) -> bool:
+    """Unit last stride, 8-element strides, 16-byte base, a (batch, head) slice within 32-bit offsets."""
 
-    t = _kernel_view(t)
-    if t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t if (t.shape[2] + 64) * t.stride(2) < 1 << 30 else t.contiguous()
+    a, b, c, d = t.stride()
+    return d == 1 and not (a | b | c) % 8 and not t.data_ptr() % 16 and (t.shape[2] + 64) * c < 1 << 30
+
+
+def _view(t: torch.Tensor) -> torch.Tensor:
+    """A BHSD view the kernels accept."""
+
+    # (contiguous() returns the tensor itself where only its base or the strides of dimensions of size 1 are odd.)
+    return t if _fits(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+_ARRAYS = {n: ctypes.c_int64 * (3 * n) for n in (4, 8)}
+
+
+def _strides(*tensors: torch.Tensor):
+    """The (batch, head, seq) strides of each tensor as the int64 array the entry points read."""
+
+    return _ARRAYS[len(tensors)](*[s for t in tensors for s in t.stride()[:3]])
+
+
+def _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale: float, cap: float, keep: bool):
+    """``o``, the views read, and the scores' sums for the backward (``None`` unless ``keep``)."""
+
+    q, k, v = _view(q), _view(k), _view(v)
+    B, H, S, D = q.shape
+    o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+    lse2 = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if keep else None
+    _lib.call_on(q.get_device(), "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(lse2),
+                 B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
+    return q, k, v, o, lse2
 
 
 class _ScoredAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, segment_ids, prefix_lengths, slopes, scale, cap):
-        q, k, v = (_view(t) for t in (q, k, v))
-        B, H, S, D = q.shape
-        o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
-        keep = any(ctx.needs_input_grad)
-        lse2 = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if keep else None
-        _lib.call_on(q.get_device(), "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(lse2),
-                     B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
-        if keep:
-            ctx.save_for_backward(q, k, v, o, lse2, segment_ids, prefix_lengths, slopes)
-            ctx.scalars = (scale, cap)
-        return o
+        kept = _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale, cap, True)
+        ctx.save_for_backward(*kept, segment_ids, prefix_lengths, slopes)
+        ctx.scalars = (scale, cap)
+        return kept[3]
 
     @staticmethod
     def backward(ctx, do):
@@ -152,7 +171,9 @@ def make_scored_attention(config: ScoredAttentionConfig = ScoredAttentionConfig(
         if (S + 64) * q.shape[3] >= 1 << 30:
             raise ValueError(f"a head's tensors must stay below 2 GiB, got {tuple(q.shape)}")
         scale = q.shape[3] ** -0.5 if config.softmax_scale is None else config.softmax_scale
-        return _ScoredAttention.apply(q, k, v, segment_ids, prefix_lengths, distance_slopes, float(scale),
-                                      float(config.score_cap or 0.0))
+        call = (q, k, v, segment_ids, prefix_lengths, distance_slopes, float(scale), float(config.score_cap or 0.0))
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _ScoredAttention.apply(*call)
+        return _forward(*call, False)[3]
 
     return attention

@@ -112,25 +112,30 @@ def _strided_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+def _layer_norm_forward(x, scale, bias, eps: float, keep: bool):
+    """``y``, and what the backward needs (``None`` for the statistics unless ``keep``)."""
+
+    x2 = _strided_rows(x)
+    scale = scale.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    rows, d = x2.shape
+    y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+    mean = stats.data_ptr() if keep else None
+    if rows:
+        _lib.call_on(x.get_device(), "gptrig_layernorm_fwd", x2.data_ptr(), x2.stride(0), _TYPES[x.dtype],
+                     scale.data_ptr(), _lib.ptr(bias), _TYPES[scale.dtype], y.data_ptr(), mean,
+                     mean + 4 * rows if keep else None, rows, d, eps)
+    return y if x.ndim == 2 else y.reshape(x.shape), x2, scale, stats
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, eps):
-        x2 = _strided_rows(x)
-        scale = scale.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        rows, d = x2.shape
-        y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
-        keep = any(ctx.needs_input_grad)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-        mean = stats.data_ptr() if keep else None
-        if rows:
-            _lib.call_on(x.get_device(), "gptrig_layernorm_fwd", x2.data_ptr(), x2.stride(0), _TYPES[x.dtype],
-                         scale.data_ptr(), _lib.ptr(bias), _TYPES[scale.dtype], y.data_ptr(), mean,
-                         mean + 4 * rows if keep else None, rows, d, eps)
-        if keep:
-            ctx.save_for_backward(x2, scale, stats)
-            ctx.shape = x.shape
-        return y if x.ndim == 2 else y.reshape(x.shape)
+        y, *kept = _layer_norm_forward(x, scale, bias, eps, True)
+        ctx.save_for_backward(*kept)
+        ctx.shape = x.shape
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -191,7 +196,9 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None =
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     _lib.require_one_device(x, scale, bias)
-    return _LayerNorm.apply(x, scale, bias, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or bias is not None and bias.requires_grad):
+        return _LayerNorm.apply(x, scale, bias, eps)
+    return _layer_norm_forward(x, scale, bias, eps, False)[0]
 
 
 _ROPE_TABLES: dict = {}

@@ -10,7 +10,7 @@ or 8-bit moments.
 
 from __future__ import annotations
 
-import ctypes
+import array
 import math
 import operator
 from dataclasses import dataclass
@@ -216,8 +216,9 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         if tensors is not None:
             table[column::8] = map(torch.Tensor.data_ptr, tensors)
     table[7::8] = counts
+    table = array.array("q", table)
     try:
-        _lib.call_on(device, "gptrig_adamw_tensors", (ctypes.c_int64 * len(table))(*table), len(params),
+        _lib.call_on(device, "gptrig_adamw_tensors", table.buffer_info()[0], len(params),
                      1 if grad_type == torch.float32 else 0, bits, hparams.data_ptr(), float(lr), float(beta1),
                      float(beta2), int(step), _lib.ptr(clip_scale), seed)
     except _lib.StatusError as error:

@@ -37,6 +37,14 @@ __device__ __forceinline__ float cap_w(float r, const ScoreArgs& a) {
   return __builtin_amdgcn_rcpf(1.0f + fast_exp2(r * a.raw));
 }
 
+// The larger of a lane's value and its counterpart's in the other half-wave (an
+// exchange of half-waves between registers; a shuffle goes through LDS).
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
 // The row of accumulator element i (of 16) in the lower half of the wave; the upper half adds 4.
 __host__ __device__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
@@ -70,12 +78,12 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, void* lds, int o
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)lds, 4, offset, 0, 0, 0);
 }
 
-// One tile of 64 rows x D columns, global -> LDS by the DMA path.  Wave w of 4
-// fills 1 KB blocks D/32 w .. of 8 rows each; rows at or past S and columns at
-// or past `dim` read as zeros.
-template <int D>
+// One tile of 64 rows x D columns, global -> LDS by the DMA path.  Wave w of
+// kWaves fills its 1 KB blocks of 8 rows each; rows at or past S and columns at or
+// past `dim` read as zeros.
+template <int D, int kWaves = 4>
 struct Fill {
-  static constexpr int NB = D / 32;
+  static constexpr int NB = D / 8 / kWaves;
   int off[NB];
   int stride;  // bytes a row
   __device__ __forceinline__ void init(int64_t row_stride, int dim, int wave, int lane) {
@@ -140,6 +148,7 @@ struct Dirty {
   __device__ __forceinline__ bool find(const at64::lds_t* tile, int wave, int lane) const {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     u16x2 top = u16x2{};
+    if (wave < 4)  // (a workgroup of 8 waves leaves it to 4)
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       const u32x4 w = __builtin_bit_cast(u32x4, tile_row(tile, 16 * wave + (lane >> 2), (lane & 3) + 4 * j));
@@ -147,7 +156,7 @@ struct Dirty {
       for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[e] & 0x7FFF7FFFu));
     }
     const uint64_t mine = __ballot(top[0] >= 0x7F80u || top[1] >= 0x7F80u);
-    if (lane == 0) found[wave] = mine;
+    if (lane == 0 && wave < 4) found[wave] = mine;
     __syncthreads();
     return __builtin_amdgcn_readfirstlane((found[0] | found[1] | found[2] | found[3]) != 0);
   }
@@ -156,7 +165,7 @@ struct Dirty {
   __device__ __forceinline__ void clear(at64::lds_t* tile, int wave, int lane) const {
     __syncthreads();
     const int r = 16 * wave + (lane >> 2);
-    if (row(r))
+    if (wave < 4 && row(r))
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
         at64::lds_x8* const at = (at64::lds_x8*)(tile + tile_at(r, (lane & 3) + 4 * j));

@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(256, 2)
     for (int kc = 0; kc < KC; ++kc) {
       s = mfma32(tile_row(kt, 32 * sb + l32, 2 * kc + hl), qreg[kc], s);
       dp = mfma32(tile_row(vt, 32 * sb + l32, 2 * kc + hl), greg[kc], dp);
+      if (D == 128 && (kc & 1)) __builtin_amdgcn_sched_barrier(0);
     }
     const int kh0 = kv0 + 32 * sb;
     const float x = (float)(my_q - kh0 - 4 * hl);
@@ -161,6 +162,7 @@ __global__ void __launch_bounds__(256, 2)
     bf16x8 ds8[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) ds8[i >> 3][i & 7] = (bf16)s[i];
+    if (D == 128) __builtin_amdgcn_sched_barrier(0);
     product<DB>(acc, kt, 32 * sb, ds8, lane);
   };
 
@@ -249,13 +251,21 @@ __global__ void __launch_bounds__(256, 2)
 // dk and dv.  Each wave computes S = Q K^T and dP = do V^T with a lane holding one
 // key, whose k and v stay in registers as operands, and sums dv^T += do^T P and
 // dk^T += Q^T dU over the queries.
-template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
-__global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
+//
+// kSplit waves share 32 keys, each with its half of every tile.  At D = 128 the sums
+// of a wave are 128 registers: with k and v in registers too there is room for one
+// wave a SIMD, which waits for every product (B4 H16/4 S2048 capped and biased 265
+// us); so there 8 waves own 128 keys, two waves a SIMD, and k and v are in LDS.
+template <int D, bool kCap, bool kBias, bool kSeg, int kSplit, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ shifts,
                       const float* __restrict__ minus_delta, const int32_t* __restrict__ seg, MutView dK, MutView dV,
                       float* __restrict__ partial, int parts, ScoreArgs a, int B, int H, int Hk, int S, int dim,
                       float scale) {
-  constexpr int KC = D / 16, DB = D / 32;
+  constexpr int KC = D / 16, DB = D / 32, kGroups = kWaves / kSplit, kMine = 32 * kGroups;
+  constexpr bool kKeysInLds = kWaves == 8;
+  __shared__ __attribute__((aligned(16))) bf16 fk[kKeysInLds ? kMine * D : 8];
+  __shared__ __attribute__((aligned(16))) bf16 fv[kKeysInLds ? kMine * D : 8];
   __shared__ __attribute__((aligned(16))) bf16 fq0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fq1[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fg0[kRows * D];
@@ -265,7 +275,6 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   __shared__ uint64_t dirty_s[4], scan_s[2];
 
   // parts workgroups share the heads of a group where there are few keys to own.
-  constexpr int kMine = kOwn / kSplit;
   const int nkv = (S + kMine - 1) / kMine, G = H / Hk / parts;
   int bh, kb;
   xcd_map(blockIdx.x, nkv, B * Hk * parts, bh, kb);
@@ -273,21 +282,36 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  const int group = wave % (4 / kSplit), part = wave / (4 / kSplit);  // (as in the forward)
+  const int group = wave % kGroups, part = wave / kGroups;
   const int k0 = kb * kMine, kw0 = k0 + 32 * group, my_k = kw0 + l32;
   const int last_prefix = __builtin_amdgcn_readfirstlane(prefix_of(a, b, S)) - 1;
 
+  // The keys' operands: in registers, or as tiles of 64 keys in LDS.
+  at64::lds_t* const ks = gemm::lds_cast(fk);
+  at64::lds_t* const vs = gemm::lds_cast(fv);
   bf16x8 kfr[KC], vfr[KC];
+  if constexpr (kKeysInLds) {
+    Fill<D, kWaves> kf, vf;
+    kf.init(K.ss, dim, wave, lane);
+    vf.init(V.ss, dim, wave, lane);
 #pragma unroll
-  for (int kc = 0; kc < KC; ++kc) {
-    const int c = 16 * kc + 8 * hl;
-    const bool ok = my_k < S && c < dim;
-    kfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(K.row(b, hk, my_k) + c) : bf16x8{};
-    vfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(V.row(b, hk, my_k) + c) : bf16x8{};
+    for (int i = 0; i < kMine / kRows; ++i) {  // (waited for with the first queries)
+      kf(slice(K.row(b, hk, 0), S, K.ss, dim), ks + i * kRows * D, k0 + i * kRows, wave);
+      vf(slice(V.row(b, hk, 0), S, V.ss, dim), vs + i * kRows * D, k0 + i * kRows, wave);
+    }
+  } else {
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      const int c = 16 * kc + 8 * hl;
+      const bool ok = my_k < S && c < dim;
+      kfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(K.row(b, hk, my_k) + c) : bf16x8{};
+      vfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(V.row(b, hk, my_k) + c) : bf16x8{};
+    }
   }
+  const int key_tile = (32 * group / kRows) * kRows * D, key_row = 32 * group % kRows + l32;
   const int seg_k = kSeg ? seg[(size_t)b * S + min(my_k, S - 1)] : 0;
   WaveIds ids;
-  SegScan<4> scan;
+  SegScan<kWaves> scan;
   if constexpr (kSeg) {
     ids.init(seg_k);
     scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, k0, lane);
@@ -301,7 +325,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   }
   bool spoilt = false;
 
-  Fill<D> qf, gf;
+  Fill<D, kWaves> qf, gf;
   qf.init(Q.ss, dim, wave, lane);
   gf.init(dO.ss, dim, wave, lane);
   // Rows of head h: past the last one everything reads as zeros.
@@ -331,8 +355,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
     }
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      s = mfma32(tile_row(qt, 32 * qs + l32, 2 * kc + hl), kfr[kc], s);
-      dp = mfma32(tile_row(gt, 32 * qs + l32, 2 * kc + hl), vfr[kc], dp);
+      const bf16x8 k8 = kKeysInLds ? tile_row(ks + key_tile, key_row, 2 * kc + hl) : kfr[kc];
+      const bf16x8 v8 = kKeysInLds ? tile_row(vs + key_tile, key_row, 2 * kc + hl) : vfr[kc];
+      s = mfma32(tile_row(qt, 32 * qs + l32, 2 * kc + hl), k8, s);
+      dp = mfma32(tile_row(gt, 32 * qs + l32, 2 * kc + hl), v8, dp);
+      if (kWaves == 8 && (kc & 1)) __builtin_amdgcn_sched_barrier(0);
     }
     const int qh0 = qq0 + 32 * qs;
     const float off = -slope2 * (float)(qq0 - my_k);
@@ -372,9 +399,12 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
         }
       }
     };
+    if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);  // (registers are short)
     if (border) middle(std::true_type{});
     else middle(std::false_type{});
+    if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);
     product<DB>(dv_acc, gt, 32 * qs, p8, lane);
+    if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);
     product<DB>(dk_acc, qt, 32 * qs, ds8, lane);
   };
 
@@ -461,16 +491,16 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1)
   }
 
   if constexpr (kSplit == 2) {
-    float* const kat = reinterpret_cast<float*>(group ? fq1 : fq0);
-    float* const vat = reinterpret_cast<float*>(group ? fg1 : fg0);
-    if (part) {
-      put<DB>(kat, dk_acc, lane);
-      put<DB>(vat, dv_acc, lane);
-    }
+    // (Each group's sums take a tile's room, dk's and dv's one after the other.)
+    float* const at = reinterpret_cast<float*>(group == 0 ? fq0 : group == 1 ? fq1 : group == 2 ? fg0 : fg1);
+    if (part) put<DB>(at, dk_acc, lane);
+    __syncthreads();
+    if (!part) add<DB>(dk_acc, at, lane);
+    __syncthreads();
+    if (part) put<DB>(at, dv_acc, lane);
     __syncthreads();
     if (part) return;
-    add<DB>(dk_acc, kat, lane);
-    add<DB>(dv_acc, vat, lane);
+    add<DB>(dv_acc, at, lane);
   }
   if (my_k < S) {
     const float bad = spoilt ? __builtin_nanf("") : 1.0f;
@@ -591,15 +621,15 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
   scored_dq_kernel<D, CAP, BIAS, SEG, SPLIT><<<(unsigned)grid, 256, 0, s>>>(                                         \
       Q, K, V, O, dO, lse2, segment_ids, shifts, minus_delta, dQ, c.args, batch, heads, kv_heads, seq, head_dim,     \
       softmax_scale)
-#define SCORED_DKV(D, CAP, BIAS, SEG, SPLIT)                                                                         \
-  scored_dkv_kernel<D, CAP, BIAS, SEG, SPLIT><<<kv_grid, 256, 0, s>>>(                                               \
+#define SCORED_DKV(D, CAP, BIAS, SEG, SPLIT, WAVES)                                                                  \
+  scored_dkv_kernel<D, CAP, BIAS, SEG, SPLIT, WAVES><<<kv_grid, 64 * WAVES, 0, s>>>(                                 \
       Q, K, V, dO, shifts, minus_delta, segment_ids, dK, dV, partial, parts, c.args, batch, heads, kv_heads, seq,    \
       head_dim, softmax_scale)
-#define SCORED_BWD(D, CAP, BIAS, SEG)               \
-  if (split) SCORED_DQ(D, CAP, BIAS, SEG, 2);       \
-  else SCORED_DQ(D, CAP, BIAS, SEG, 1);             \
-  if (kv_split) SCORED_DKV(D, CAP, BIAS, SEG, 2);   \
-  else SCORED_DKV(D, CAP, BIAS, SEG, 1)
+#define SCORED_BWD(D, CAP, BIAS, SEG)                                           \
+  if (split) SCORED_DQ(D, CAP, BIAS, SEG, 2);                                   \
+  else SCORED_DQ(D, CAP, BIAS, SEG, 1);                                         \
+  if (kv_split) SCORED_DKV(D, CAP, BIAS, SEG, 2, 4);                            \
+  else SCORED_DKV(D, CAP, BIAS, SEG, (D == 64 ? 1 : 2), (D == 64 ? 4 : 8))
   SCORED_DISPATCH(SCORED_BWD, c, segment_ids != nullptr);
 #undef SCORED_BWD
 #undef SCORED_DKV

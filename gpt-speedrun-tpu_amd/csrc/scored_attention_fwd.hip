@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
       for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
       if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
       m_tile += off;  // (with a bias each half-wave has its own)
-      m_tile = fmaxf(m_tile, __shfl_xor(m_tile, 32));
+      m_tile = max_halves(m_tile);
       // The running maximum moves only when a row's maximum exceeds it by more
       // than 8 (log2): P stays below 2^8 and most halves rescale nothing.
       const bool grow = m_tile > m_run + 8.0f;

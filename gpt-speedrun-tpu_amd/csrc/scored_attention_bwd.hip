@@ -135,16 +135,23 @@ __global__ void __launch_bounds__(256, 2)
         s[i] = kBias ? fmaf(s[i], raw, bias[i]) + off : fmaf(s[i], raw, off);
       }
     }
-    if (kBias && kh0 + 31 > qw0 && last_prefix > qw0) {  // keys after their query
+    const bool after = kh0 + 31 > qw0;
+    if constexpr (kBias) {  // (as in the forward)
+      if (kh0 > qw0 + 31) {
+        const float twice_off = 2.0f * slope2 * x;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f * slope2, fmaxf((float)acc_row(i) - x, 0.f), s[i]);
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f, bias[i], s[i] + twice_off);
+      } else if (after && last_prefix > qw0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f * slope2, fmaxf((float)acc_row(i) - x, 0.f), s[i]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[i] = fast_exp2(s[i]) * (dp[i] - delta);
       if constexpr (kCap) s[i] *= fmaf(-w[i], w[i], w[i]);  // (1 - tanh^2) / 4
     }
-    if (kh0 + 31 > qw0 || kh0 + 32 > S || (kSeg && docs)) {
+    if ((after && kh0 + 31 > last_prefix) || kh0 + 32 > S || (kSeg && docs)) {
       const int lim = my_last - kh0 - 4 * hl;
       if (kSeg && docs) {
 #pragma unroll
@@ -328,17 +335,22 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
   Fill<D, kWaves> qf, gf;
   qf.init(Q.ss, dim, wave, lane);
   gf.init(dO.ss, dim, wave, lane);
-  // Rows of head h: past the last one everything reads as zeros.
-  auto fill = [&](at64::lds_t* qt, at64::lds_t* gt, float* ls, float* dl, int* sg, int h, int qq0) {
-    qf(slice(Q.row(b, h, 0), S, Q.ss, dim), qt, qq0, wave);
-    gf(slice(dO.row(b, h, 0), S, dO.ss, dim), gt, qq0, wave);
+  // The rows of one head at a time: past the last everything reads as zeros.
+  __amdgpu_buffer_rsrc_t q_rs, g_rs, l_rs, d_rs;
+  auto of_head = [&](int g) {
+    const int h = h0 + min(g, G - 1);
+    q_rs = slice(Q.row(b, h, 0), S, Q.ss, dim);
+    g_rs = slice(dO.row(b, h, 0), S, dO.ss, dim);
     const size_t row = ((size_t)b * H + h) * S;
-    if (wave == 0)
-      dma4(make_rsrc(shifts + row, (uint32_t)S * 4u), ls, (qq0 + lane) * 4);
-    if (wave == 1)
-      dma4(make_rsrc(minus_delta + row, (uint32_t)S * 4u), dl, (qq0 + lane) * 4);
-    if (kSeg && wave == 2)
-      dma4(make_rsrc(seg + (size_t)b * S, (uint32_t)S * 4u), sg, (qq0 + lane) * 4);
+    l_rs = make_rsrc(shifts + row, (uint32_t)S * 4u);
+    d_rs = make_rsrc(minus_delta + row, (uint32_t)S * 4u);
+  };
+  auto fill = [&](at64::lds_t* qt, at64::lds_t* gt, float* ls, float* dl, int* sg, int qq0) {
+    qf(q_rs, qt, qq0, wave);
+    gf(g_rs, gt, qq0, wave);
+    if (wave == 0) dma4(l_rs, ls, (qq0 + lane) * 4);
+    if (wave == 1) dma4(d_rs, dl, (qq0 + lane) * 4);
+    if (kSeg && wave == 2) dma4(make_rsrc(seg + (size_t)b * S, (uint32_t)S * 4u), sg, (qq0 + lane) * 4);
   };
 
   // 32 queries qq0 + 32 qs .. of the tile.
@@ -363,10 +375,14 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     }
     const int qh0 = qq0 + 32 * qs;
     const float off = -slope2 * (float)(qq0 - my_k);
-    const bool border = kw0 + 31 > qh0 || qh0 + 32 > S || (kSeg && docs);
+    const bool after = kw0 + 31 > qh0;  // some key comes after some query
+    const bool masked = (after && kw0 + 31 > last_prefix) || qh0 + 32 > S || (kSeg && docs);
     bf16x8 p8[2], ds8[2];
-    auto middle = [&](auto tag) __attribute__((always_inline)) {
-      constexpr bool kBorder = decltype(tag)::value;
+    // kAll: every key comes after every query and all are visible, so the distance
+    // counts the other way; kBorder: the pairs are looked at one by one.
+    auto middle = [&](auto border, auto all) __attribute__((always_inline)) {
+      constexpr bool kBorder = decltype(border)::value, kAll = decltype(all)::value;
+      const float ahead = kAll ? 2.0f * slope2 * (float)(qh0 + 4 * hl - my_k) : 0.f;
       // Query own + c sees my_k from c = first on, all of them inside the prefix.
       const int first = my_k <= last_prefix ? -64 : my_k - qh0 - 4 * hl, end = S - qh0 - 4 * hl;
 #pragma unroll
@@ -384,6 +400,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
             e = fmaf(s[i], raw, l4[t]);
           }
           if constexpr (kBias) e += off;
+          if constexpr (kAll) e += fmaf(2.0f * slope2, (float)c, ahead);
           if constexpr (kBias && kBorder)  // keys after their query, where a prefix shows them
             e = fmaf(-2.0f * slope2, fmaxf((float)(my_k - qh0 - 4 * hl - c), 0.f), e);
           float p = fast_exp2(e), ds = p * dp[i];
@@ -400,8 +417,9 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
       }
     };
     if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);  // (registers are short)
-    if (border) middle(std::true_type{});
-    else middle(std::false_type{});
+    if (masked || (kBias && after && qh0 + 31 >= kw0)) middle(std::true_type{}, std::false_type{});
+    else if (kBias && after) middle(std::false_type{}, std::bool_constant<kBias>{});
+    else middle(std::false_type{}, std::false_type{});
     if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);
     product<DB>(dv_acc, gt, 32 * qs, p8, lane);
     if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);
@@ -423,9 +441,8 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
   };
 
   auto tile = [&](at64::lds_t* qt, at64::lds_t* gt, const float* ls, const float* dl, const int* sg, int qb, int g,
-                  bool same) __attribute__((always_inline)) {
+                  float slope2, bool same) __attribute__((always_inline)) {
     const int qq0 = qb * kRows;
-    const float slope2 = kBias ? a.slopes[h0 + min(g, G - 1)] * GPTRIG_LOG2E : 0.f;
     int qs = 0, end = 0, docs = 0;
     if (g < G) {
       if (k0 + kMine - 1 > max(qq0, last_prefix) || (kSeg && !same)) {
@@ -476,18 +493,31 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
   int g = 0;
   bool same = true, same_n = true;
   int qb = next(start, g, same);
-  fill(q0s, g0s, ls0, dl0, sg0, h0 + g, qb * kRows);
+  auto slope_of = [&](int g) { return kBias ? a.slopes[h0 + min(g, G - 1)] * GPTRIG_LOG2E : 0.f; };
+  of_head(g);
+  float slope = slope_of(g);
+  fill(q0s, g0s, ls0, dl0, sg0, qb * kRows);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
   while (g < G) {  // (The workgroup's own positions hold visible pairs: every head has a first tile.)
     int gn = g;
     const int nx = next(qb + 1, gn, same_n);
-    if (gn < G) fill(q1s, g1s, ls1, dl1, sg1, h0 + gn, nx * kRows);
-    tile(q0s, g0s, ls0, dl0, sg0, qb, g, same);
+    float slope_n = slope;
+    if (gn != g) {
+      of_head(gn);
+      slope_n = slope_of(gn);
+    }
+    if (gn < G) fill(q1s, g1s, ls1, dl1, sg1, nx * kRows);
+    tile(q0s, g0s, ls0, dl0, sg0, qb, g, slope, same);
     g = gn;
     qb = next(nx + 1, g, same);
-    if (g < G) fill(q0s, g0s, ls0, dl0, sg0, h0 + g, qb * kRows);
-    tile(q1s, g1s, ls1, dl1, sg1, nx, gn, same_n);
+    slope = slope_n;
+    if (g != gn) {
+      of_head(g);
+      slope = slope_of(g);
+    }
+    if (g < G) fill(q0s, g0s, ls0, dl0, sg0, qb * kRows);
+    tile(q1s, g1s, ls1, dl1, sg1, nx, gn, slope_n, same_n);
   }
 
   if constexpr (kSplit == 2) {

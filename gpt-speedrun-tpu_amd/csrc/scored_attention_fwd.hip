@@ -105,13 +105,20 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
       }
       if constexpr (kBias) off = fmaf(-slope2, (float)(my_q - kh0 - 4 * hl), off);  // element 0's
     }
-    // (One branch for everything that the halves behind every query go without.)
-    if (kh0 + 31 > qw0 || kh0 + 32 > S || (kSeg && docs)) {
-      if constexpr (kBias) {  // keys after their query, where a prefix shows them
+    const bool after = kh0 + 31 > qw0;  // some key comes after some query
+    if constexpr (kBias) {
+      // The distance of such a pair counts the other way.
+      if (kh0 > qw0 + 31) {  // all of them
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f, bias[i], s[i]);
+        off = fmaf(2.0f * slope2, (float)(my_q - kh0 - 4 * hl), off);
+      } else if (after && last_prefix > qw0) {
         const float x = (float)(my_q - kh0 - 4 * hl);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = fmaf(-2.0f * slope2, fmaxf((float)acc_row(i) - x, 0.f), s[i]);
       }
+    }
+    if ((after && kh0 + 31 > last_prefix) || kh0 + 32 > S || (kSeg && docs)) {
       const int lim = my_last - kh0 - 4 * hl;
       if (kSeg && docs) {
 #pragma unroll

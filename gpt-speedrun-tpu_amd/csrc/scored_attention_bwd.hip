@@ -596,8 +596,11 @@ __global__ void __launch_bounds__(256) scored_join_kernel(const float* __restric
 }
 
 // Parts of each group of heads: the fewest that divide it and give kWant
-// workgroups (they are of uneven length, so several a CU).
-constexpr long long kWant = 1024;
+// workgroups (they are of uneven length, so several a CU; each part's sums are
+// written and read once more).  us of a backward with kWant 256 / 512 / 1024, 16 query
+// heads on 4: D128 B4 S2048 391 / 331 / 375, B2 S2048 224 / 191 / 194, B4 S2048
+// documents 474 / 363 / 344; D64 B4 S2048 274 / 242 / 252, B8 S2048 382 / 382 / 387.
+constexpr long long kWant = 512;
 int parts_of(int batch, int heads, int kv_heads, int seq) {
   const int G = heads / kv_heads;
   const long long blocks = (long long)batch * kv_heads * ceil_div(seq, kOwn);

@@ -217,6 +217,16 @@ def test_many_workgroups(options, D):
     compare(*inputs(B, H, H if D == 64 else 8, S, D, seed=21), **o)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B, H, Hk", [(8, 32, 8), (10, 24, 8), (2, 12, 3)])
+def test_shared_heads_in_parts(B, H, Hk, D):
+    """Groups of query heads whose key gradients come in several parts, of one head or of two."""
+
+    S = 600 if B > 2 else 1100
+    print(f"scored attention, shared heads in parts B={B} H={H}/{Hk} S={S} D={D}", flush=True)
+    compare(*inputs(B, H, Hk, S, D, seed=23), cap=25.0, seg=documents(B, S, 300), slopes=slopes_of(H))
+
+
 def test_large_scores_and_extreme_caps():
     q, k, v, do = inputs(1, 2, 2, 180, 64, seed=4, size=6.0)
     for cap, scale in ((2.0, None), (0.01, None), (1000.0, None), (40.0, 3.0), (None, 1.0), (None, 0.001)):

@@ -10,6 +10,8 @@
 // few values one by one.
 #include "common.h"
 
+#include <algorithm>
+
 namespace {
 
 enum { kBf16 = GPTRIG_TYPE_BF16, kF32 = GPTRIG_TYPE_F32 };
@@ -414,10 +416,20 @@ int parts_of(int64_t rows, int d, int v) {
     case 256 * 8 + 4: CALL(256, 4); break;                                                          \
   }
 
+// Workgroups of a launch at most (it has fewer than 2^32 threads a dimension).
+constexpr int64_t kGrid = 1 << 22;
+
 template <typename T, typename P>
 void launch_fwd(const void* x, int64_t ldx, const void* scale, const void* bias, void* y, float* mean, float* rstd,
                 int64_t rows, int d, float eps, hipStream_t st) {
   const Shape sh = row_shape(d, 16 / sizeof(T));
+  const int64_t most = kGrid * (sh.lanes ? 256 / sh.lanes : 1);
+  if (rows > most) {
+    launch_fwd<T, P>(x, ldx, scale, bias, y, mean, rstd, most, d, eps, st);
+    launch_fwd<T, P>((const T*)x + most * ldx, ldx, scale, bias, (T*)y + most * d, mean ? mean + most : nullptr,
+                     rstd ? rstd + most : nullptr, rows - most, d, eps, st);
+    return;
+  }
   if (!sh.lanes) {
     layernorm_fwd_wide_kernel<T, P><<<(unsigned)rows, 256, 0, st>>>((const T*)x, ldx, (const P*)scale, (const P*)bias,
                                                                     (T*)y, mean, rstd, d, eps);
@@ -446,16 +458,17 @@ void launch_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const 
     if (sh.lanes) {
 #define LN_BWD_(L, C, EVEN)                                                                                           \
   layernorm_bwd_kernel<T, P, L, C, EVEN>                                                                              \
-      <<<dx && !partial ? (unsigned)((rows + 256 / L - 1) / (256 / L)) : (unsigned)parts, 256, 0, st>>>(              \
+      <<<partial ? (unsigned)parts : (unsigned)std::min((rows + 256 / L - 1) / (256 / L), kGrid), 256, 0, st>>>(      \
           (const T*)dy, lddy, (const T*)x, ldx, (const P*)scale, mean, rstd, (T*)dx, partial, rows, d)
 #define LN_BWD(L, C) if (even) LN_BWD_(L, C, true); else LN_BWD_(L, C, false)
       LN_SHAPES(LN_BWD)
 #undef LN_BWD
 #undef LN_BWD_
     } else {
-      if (dx)
-        layernorm_bwd_wide_kernel<T, P><<<(unsigned)rows, 256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx,
-                                                                        (const P*)scale, mean, rstd, (T*)dx, d);
+      for (int64_t at = 0; dx && at < rows; at += kGrid)
+        layernorm_bwd_wide_kernel<T, P><<<(unsigned)std::min(rows - at, kGrid), 256, 0, st>>>(
+            (const T*)dy + at * lddy, lddy, (const T*)x + at * ldx, ldx, (const P*)scale, mean + at, rstd + at,
+            (T*)dx + at * d, d);
       if (partial)
         layernorm_bwd_wide_columns_kernel<T>
             <<<dim3(ceil_div(d, 256 * (16 / sizeof(T))), parts), 256, 0, st>>>((const T*)dy, lddy, (const T*)x, ldx, mean,

@@ -101,6 +101,25 @@ def test_many_rows(rows, width, dtype):
     compare(*inputs((rows, width), dtype, F32, True, seed=1))
 
 
+@pytest.mark.parametrize("rows,width", [((1 << 25) + 9, 8), ((1 << 22) + 3, 5)])
+def test_more_rows_than_a_launch_has_workgroups_for(rows, width):
+    from gptrig.nn import layer_norm
+
+    print(f"layer_norm rows={rows} width={width}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn((rows, width), generator=g, device=DEV).to(BF16)
+    scale, b = torch.randn(width, generator=g, device=DEV), torch.randn(width, generator=g, device=DEV)
+    leaf = x.requires_grad_()
+    y = layer_norm(leaf, scale, b)
+    dx, = torch.autograd.grad(y, leaf, y.detach())
+    torch.cuda.synchronize()
+    middle = rows - rows % (1 << 22)  # where a launch ends
+    for part in (slice(0, 9), slice(middle - 9, middle + 9), slice(rows - 9, rows)):
+        want, bounds = reference(x.detach()[part], scale, b, y.detach()[part])
+        check("y", y.detach()[part], want["y"], bounds["y"])
+        check("dx", dx[part], want["dx"], bounds["dx"])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 def test_strides_and_alignment(dtype):
     """Rows of a wider buffer, an odd start, a transposed view, a repeated row and an expanded gradient."""

@@ -19,6 +19,10 @@
 // momentum that is not would divide by eps alone.  A value that is infinite or NaN
 // becomes the NaN code and stays out of the scale, so it spoils no neighbour.
 // Blocks whose largest magnitude is below 2^-100 are kept as zeros.
+// Every product, sum and quotient up to a code is rounded to float32 on its own (no
+// fused ones): a value close to a tie goes to either of two codes 12% apart, so the
+// last bit decides a few codes of a million, and anyone who computes the formula in
+// float32 gets the same ones.
 // u comes from 32 bits h(seed, tensor, i), m's from the low half, v's from the
 // high one, (half + 0.5) / 2^16.  h is a multiply and shift mixer over the
 // fractional bits of the golden ratio, sqrt 2 and sqrt 3:
@@ -147,6 +151,7 @@ __device__ __forceinline__ float largest(float v) {
 // block's scale.  shift: where the random half-words are.
 template <bool kFloor>
 __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&bits)[4], int shift, float& scale) {
+#pragma clang fp contract(off)
   float top = 0.f;
   bool finite[4];
 #pragma unroll
@@ -161,7 +166,8 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
   float code[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float y = fminf(fabsf(x[j]) * inv, 448.0f);
+    // |x| / scale, correctly rounded.
+    const float q = fabsf(x[j]) * inv, y = fminf(fmaf(fmaf(-q, scale, fabsf(x[j])), inv, q), 448.0f);
     uint32_t step = __builtin_bit_cast(uint32_t, y) & 0x7F800000u;
     step = (step < 0x3C800000u ? 0x3C800000u : step) - 0x01800000u;  // at least 2^-6, over 8
     const float u = fmaf((float)((bits[j] >> shift) & 0xFFFFu), 0x1p-16f, 0x1p-17f);
@@ -183,6 +189,7 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
 template <typename G, bool k8, bool kWhole>
 __device__ __forceinline__ void update_chunk(const Item& it, const Scalars& k, float lr, float eps, float decay,
                                              float clip, int64_t base) {
+#pragma clang fp contract(off)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n = it.n;
   float* const p = it.p;
@@ -228,7 +235,7 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Scalars& k, f
       const bool small = vhat < 1.0f;
       const float root = __builtin_amdgcn_sqrtf(vhat * (small ? 0x1p24f : 1.0f));
       const float step = (m * k.ibc1) * __builtin_amdgcn_rcpf(fmaf(root, small ? 0x1p-12f : 1.0f, eps));
-      pv[u][j] -= lr * fmaf(decay, pv[u][j], step);
+      pv[u][j] = fmaf(-lr, fmaf(decay, pv[u][j], step), pv[u][j]);
       // (Past the tensor's end m and v are 0 unless clip is infinite or NaN.)
       mv[u][j] = kWhole || j < left ? m : 0.f;
       vv[u][j] = kWhole || j < left ? v : 0.f;
@@ -272,22 +279,24 @@ __global__ void __launch_bounds__(256) adamw_tensors_kernel(Items items, Scalars
   else update_chunk<G, k8, false>(it, k, lr, eps, decay, clip, base);
 }
 
-// GPTRIG_E_OVERLAP where two of the arrays that the step writes share memory.
-int check_written(const gptrig_adamw_tensor* tensors, int count, bool k8) {
+// GPTRIG_E_OVERLAP where an array that the step writes shares memory with another of its arrays.
+int check_written(const gptrig_adamw_tensor* tensors, int count, bool k8, size_t grad_bytes) {
   struct Range {
     uintptr_t from, to;
+    bool written;
   };
-  Range few[6 * 64];
-  Range* const r = count <= 64 ? few : (Range*)malloc(sizeof(Range) * 6 * (size_t)count);
+  Range few[7 * 64];
+  Range* const r = count <= 64 ? few : (Range*)malloc(sizeof(Range) * 7 * (size_t)count);
   if (!r) return GPTRIG_E_WORKSPACE;
   int n = 0;
   for (int i = 0; i < count; ++i) {
     const gptrig_adamw_tensor& t = tensors[i];
     if (t.n == 0) continue;
     const size_t size = (size_t)t.n, scales = (size_t)((t.n + kBlock - 1) / kBlock) * 4;
-    auto put = [&](const void* p, size_t bytes) {
-      if (p) r[n++] = {(uintptr_t)p, (uintptr_t)p + bytes};
+    auto put = [&](const void* p, size_t bytes, bool written = true) {
+      if (p) r[n++] = {(uintptr_t)p, (uintptr_t)p + bytes, written};
     };
+    put(t.grad, grad_bytes * size, false);
     put(t.param, 4 * size);
     put(t.m, (k8 ? 1 : 4) * size);
     put(t.v, (k8 ? 1 : 4) * size);
@@ -299,8 +308,12 @@ int check_written(const gptrig_adamw_tensor* tensors, int count, bool k8) {
   }
   std::sort(r, r + n, [](const Range& a, const Range& b) { return a.from < b.from; });
   int status = GPTRIG_OK;
-  for (int i = 1; i < n; ++i)
-    if (r[i].from < r[i - 1].to) status = GPTRIG_E_OVERLAP;
+  uintptr_t end = 0, written_end = 0;
+  for (int i = 0; i < n; ++i) {
+    if (r[i].from < (r[i].written ? end : written_end)) status = GPTRIG_E_OVERLAP;
+    end = std::max(end, r[i].to);
+    if (r[i].written) written_end = std::max(written_end, r[i].to);
+  }
   if (r != few) free(r);
   return status;
 }
@@ -320,7 +333,7 @@ int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad
   const bool k8 = state_bits == 8;
   for (int i = 0; i < count; ++i) {
     const gptrig_adamw_tensor& t = tensors[i];
-    if (t.n < 0 || t.n > ((int64_t)1 << 40)) return GPTRIG_E_SHAPE;
+    if (t.n < 0 || t.n > ((int64_t)1 << 35)) return GPTRIG_E_SHAPE;
     if (t.n == 0) continue;
     if (!t.param || !t.grad || !t.m || !t.v || (k8 && (!t.m_scale || !t.v_scale))) return GPTRIG_E_NULL;
     const uintptr_t words = (uintptr_t)t.param | (uintptr_t)t.m_scale | (uintptr_t)t.v_scale |
@@ -328,7 +341,7 @@ int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad
     if ((words & 3) || ((uintptr_t)t.grad & (grad_type == GPTRIG_TYPE_F32 ? 3 : 1)) || ((uintptr_t)t.shadow & 1))
       return GPTRIG_E_SHAPE;
   }
-  const int written = check_written(tensors, count, k8);
+  const int written = check_written(tensors, count, k8, grad_type == GPTRIG_TYPE_F32 ? 4 : 2);
   if (written != GPTRIG_OK) return written;
   Scalars k;
   k.lr = (float)lr;
@@ -349,7 +362,7 @@ int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad
       const gptrig_adamw_tensor& t = tensors[i];
       if (t.n == 0) continue;
       const int64_t more = (t.n + kChunk - 1) / kChunk;
-      if (blocks + more > INT32_MAX) break;  // (2^40 values are 2^28 chunks: one tensor always fits)
+      if (blocks + more >= 1 << 24) break;  // (2^32 threads; a tensor of 2^35 values, 2^23 chunks, always fits)
       items.item[items.count++] = {t.param, t.grad, t.m, t.v, t.m_scale, t.v_scale, (bf16*)t.shadow, t.n, (int)blocks, i};
       blocks += more;
     }

@@ -175,7 +175,7 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``step``), which every step needs another of; the same call gives the same
     result.  ``clip_scale``: a float32 scalar on the device that multiplies the
     gradients.  ``shadow``: bfloat16 tensors that receive the rounded parameters.
-    No two of the tensors written may overlap.  ``lr``, ``step`` and ``seed`` are
+    A tensor that is written may overlap no other.  ``lr``, ``step`` and ``seed`` are
     fixed in a captured graph.
     """
 
@@ -204,8 +204,8 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         raise ValueError("clip_scale must be one float32 value")
     if not 0.0 <= beta1 < 1.0 or not 0.0 <= beta2 < 1.0:
         raise ValueError(f"beta1 and beta2 must be in [0, 1), got {beta1} and {beta2}")
-    if step < 1:
-        raise ValueError(f"step counts from 1, got {step}")
+    if not 1 <= step < 2 ** 31:
+        raise ValueError(f"step counts from 1 and stays below 2^31, got {step}")
     seed = step % 2 ** 32 if seed is None else seed
     if not 0 <= seed < 2 ** 32:
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
@@ -223,6 +223,9 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                      float(beta2), int(step), _lib.ptr(clip_scale), seed)
     except _lib.StatusError as error:
         if error.status == E_OVERLAP:
-            raise ValueError("tensors that the step writes overlap") from error
+            raise ValueError("a tensor that the step writes overlaps another") from error
         raise
-    torch.autograd.graph.increment_version(params)  # (a graph that saved one of them must not run backward now)
+    # (A graph that saved one of them must not run backward now.)
+    torch.autograd.graph.increment_version(params)
+    if shadow is not None:
+        torch.autograd.graph.increment_version(shadow)

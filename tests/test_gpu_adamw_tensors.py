@@ -291,3 +291,19 @@ def test_the_same_tensor_twice_is_refused():
         M.step(1)
     torch.cuda.synchronize()
     assert torch.equal(L.p[0], before)
+    N = Lists([(300,), (300,)], 32)
+    N.g[1] = N.p[0]
+    with pytest.raises(ValueError, match="overlap"):
+        N.step(1)
+
+
+def test_a_shared_gradient_and_a_saved_shadow():
+    L, M = Lists([(300,), (300,)], 32, shadow=True), Lists([(300,), (300,)], 32, shadow=True)
+    L.g[1], M.g[1] = L.g[0], M.g[0].clone()
+    w = torch.ones(300, dtype=BF16, device=DEV, requires_grad=True)
+    loss = (w * L.shadow[0]).sum()
+    L.step(1), M.step(1)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(L.p + L.shadow, M.p + M.shadow))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

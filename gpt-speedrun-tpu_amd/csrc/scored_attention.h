@@ -59,6 +59,16 @@ __device__ __forceinline__ int prefix_of(const ScoreArgs& a, int b, int S) {
   return a.prefix ? min(max(a.prefix[b], 0), S) : 0;
 }
 
+// What rounding x to the bf16 `high` cut off, in 8 bits: the difference of the two as
+// float32 bits, which lies in [-2^15, 2^15], over 2^8; and x again, to 16 bits.
+__device__ __forceinline__ uint32_t low_bits(float x, bf16 high) {
+  const int rest = (int)(__builtin_bit_cast(uint32_t, x) - __builtin_bit_cast(uint32_t, (float)high));
+  return (uint32_t)min(max((rest + 128) >> 8, -128), 127) & 0xFFu;
+}
+__device__ __forceinline__ float with_low_bits(bf16 high, uint32_t low) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)high) + (uint32_t)((int)(int8_t)low * 256));
+}
+
 // Element offset of 16-byte chunk c16 of row `row` in a tile of kRows rows: a
 // tile of 128 columns is two swizzled ones of 64.
 __device__ __forceinline__ int tile_at(int row, int c16) { return (c16 >> 3) * kRows * 64 + at64::swz(row, c16 & 7); }
@@ -213,6 +223,8 @@ struct ScoredCall {
     if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq <= 0 || head_dim <= 0 || head_dim % 8)
       return GPTRIG_E_SHAPE;
     if (head_dim > 128) return GPTRIG_E_UNSUPPORTED;
+    // 2^22 workgroups of up to 512 threads (a launch has fewer than 2^32 threads).
+    if ((long long)batch * heads * (((long long)seq + 63) / 64) > 1 << 22) return GPTRIG_E_SHAPE;
     if (!(softmax_scale > 0.f) || !(softmax_scale <= 3.0e38f)) return GPTRIG_E_SHAPE;
     if (!(score_cap >= 0.f) || score_cap > 1000.f) return GPTRIG_E_SHAPE;
     dim = head_dim;

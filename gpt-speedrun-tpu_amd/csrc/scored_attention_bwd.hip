@@ -1,7 +1,10 @@
 // Backward of the attention of scored_attention.h, in two passes that each own
 // what they sum, so no atomics: results do not depend on the order of anything.
 //   dq: a workgroup owns 128 queries of one head, like the forward, and walks the
-//     keys; it also leaves delta_i = o_i . do_i for the other pass.
+//     keys; it also leaves delta_i = o_i . do_i for the other pass, of o and o_low,
+//     which holds what the rounding of o to bf16 cut off: delta is subtracted from
+//     dP values of its own size, so a rounded o would add half as much to the error
+//     of dq and dk as the rounding of dU does (0.9 and 1.7 in 1000 of dq's norm).
 //   dk, dv: a workgroup owns 128 keys of one kv head and walks the queries of
 //     every head of its group.
 // Both compute the scores and dP anew (3 and 4 products of the pair matrix
@@ -37,8 +40,8 @@ __device__ __forceinline__ void add(f32x16 (&acc)[DB], const float* at, int lane
 // bias that is the query's own in its tile), and -delta_i.
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, 2)
-    scored_dq_kernel(View Q, View K, View V, View O, View dO, const float* __restrict__ lse2,
-                     const int32_t* __restrict__ seg, float* __restrict__ shifts, float* __restrict__ minus_delta,
+    scored_dq_kernel(View Q, View K, View V, View O, View dO, const uint8_t* __restrict__ o_low,
+                     const float* __restrict__ lse2, const int32_t* __restrict__ seg, float* __restrict__ shifts, float* __restrict__ minus_delta,
                      MutView dQ, ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
   constexpr int KC = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
@@ -71,6 +74,7 @@ __global__ void __launch_bounds__(256, 2)
   }
 
   bf16x8 qreg[KC], greg[KC];
+  const size_t my_row = (size_t)bh * S + my_q;
   float delta = 0.f;
 #pragma unroll
   for (int kc = 0; kc < KC; ++kc) {
@@ -79,11 +83,12 @@ __global__ void __launch_bounds__(256, 2)
     qreg[kc] = ok ? *reinterpret_cast<const bf16x8*>(Q.row(b, h, my_q) + c) : bf16x8{};
     greg[kc] = ok ? *reinterpret_cast<const bf16x8*>(dO.row(b, h, my_q) + c) : bf16x8{};
     const bf16x8 o = ok ? *reinterpret_cast<const bf16x8*>(O.row(b, h, my_q) + c) : bf16x8{};
+    const uint2 low = ok ? *reinterpret_cast<const uint2*>(o_low + my_row * dim + c) : uint2{};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) delta = fmaf((float)o[j], (float)greg[kc][j], delta);
+    for (int j = 0; j < 8; ++j)
+      delta = fmaf(with_low_bits(o[j], (j < 4 ? low.x : low.y) >> (8 * (j & 3))), (float)greg[kc][j], delta);
   }
   delta += __shfl_xor(delta, 32);
-  const size_t my_row = (size_t)bh * S + my_q;
   const float shift = my_q < S ? (kCap ? a.cap2 : 0.f) - lse2[my_row] : 0.f;
   if (my_q < S && hl == 0 && part == 0) {
     shifts[my_row] = kBias ? fmaf(-slope2, (float)(my_q & (kRows - 1)), shift) : shift;
@@ -625,25 +630,24 @@ size_t gptrig_scored_attn_bwd_workspace_bytes(int batch, int heads, int kv_heads
 }
 
 int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
-                           const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
+                           const void* o_low, const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
                            const float* distance_slopes, void* dq, void* dk, void* dv, void* workspace,
                            size_t workspace_bytes, int batch, int heads, int kv_heads, int seq, int head_dim,
                            const int64_t* strides, float softmax_scale, float score_cap, void* stream) {
   ScoredCall c;
-  if (!lse2 || !workspace) return GPTRIG_E_NULL;
+  if (!lse2 || !o_low || !workspace) return GPTRIG_E_NULL;
   const void* tensors[8] = {q, k, v, o, dout, dq, dk, dv};
   const int status = c.init(tensors, 8, 0b11000110u, batch, heads, kv_heads, seq, head_dim, strides, softmax_scale,
                             score_cap, distance_slopes, prefix_lengths);
   if (status != GPTRIG_OK) return status;
   if (workspace_bytes < gptrig_scored_attn_bwd_workspace_bytes(batch, heads, kv_heads, seq, head_dim))
     return GPTRIG_E_WORKSPACE;
-  if ((uintptr_t)workspace & 15) return GPTRIG_E_SHAPE;
+  if (((uintptr_t)workspace | (uintptr_t)o_low) & 15) return GPTRIG_E_SHAPE;
   const bool split = split_rows((long long)batch * heads, seq, head_dim, false);
-  const long long grid = (long long)batch * heads * ceil_div(seq, split ? kOwn / 2 : kOwn);
-  if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
+  const unsigned grid = (unsigned)(batch * heads * ceil_div(seq, split ? kOwn / 2 : kOwn));
   const int parts = parts_of(batch, heads, kv_heads, seq);
   const bool kv_split = split_rows((long long)batch * kv_heads * parts, seq, head_dim, true);
-  const unsigned kv_grid = (unsigned)((long long)batch * kv_heads * parts * ceil_div(seq, kv_split ? kOwn / 2 : kOwn));
+  const unsigned kv_grid = (unsigned)(batch * kv_heads * parts * ceil_div(seq, kv_split ? kOwn / 2 : kOwn));
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2), O = c.view(3), dO = c.view(4);
   const MutView dQ = c.out(5), dK = c.out(6), dV = c.out(7);
@@ -651,9 +655,9 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
   float* const minus_delta = shifts + row_numbers_bytes(batch, heads, seq) / sizeof(float);
   float* const partial = minus_delta + row_numbers_bytes(batch, heads, seq) / sizeof(float);
 #define SCORED_DQ(D, CAP, BIAS, SEG, SPLIT)                                                                          \
-  scored_dq_kernel<D, CAP, BIAS, SEG, SPLIT><<<(unsigned)grid, 256, 0, s>>>(                                         \
-      Q, K, V, O, dO, lse2, segment_ids, shifts, minus_delta, dQ, c.args, batch, heads, kv_heads, seq, head_dim,     \
-      softmax_scale)
+  scored_dq_kernel<D, CAP, BIAS, SEG, SPLIT><<<grid, 256, 0, s>>>(                                         \
+      Q, K, V, O, dO, (const uint8_t*)o_low, lse2, segment_ids, shifts, minus_delta, dQ, c.args, batch, heads, kv_heads, \
+      seq, head_dim, softmax_scale)
 #define SCORED_DKV(D, CAP, BIAS, SEG, SPLIT, WAVES)                                                                  \
   scored_dkv_kernel<D, CAP, BIAS, SEG, SPLIT, WAVES><<<kv_grid, 64 * WAVES, 0, s>>>(                                 \
       Q, K, V, dO, shifts, minus_delta, segment_ids, dK, dV, partial, parts, c.args, batch, heads, kv_heads, seq,    \
@@ -668,8 +672,7 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
 #undef SCORED_DKV
 #undef SCORED_DQ
   if (parts > 1) {
-    const long long threads = 2ll * batch * kv_heads * seq * (head_dim / 8);
-    if (threads > 256ll * INT32_MAX) return GPTRIG_E_SHAPE;
+    const long long threads = 2ll * batch * kv_heads * seq * (head_dim / 8);  // (of fewer than kWant blocks)
     scored_join_kernel<<<ceil_div(threads, 256), 256, 0, s>>>(partial, parts, dK, dV, batch, kv_heads, seq, head_dim);
   }
   GPTRIG_CHECK_LAUNCH();

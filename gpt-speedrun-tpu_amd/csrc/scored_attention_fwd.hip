@@ -9,16 +9,10 @@ namespace {
 
 constexpr int kQueries = 128;  // of a workgroup; kSplit 2: 64
 
-// With a cap and no bias every score lies within +-cap, so up to kFixedCap a fixed
-// reference in place of the running maximum keeps every P within [2^-100, 1].
-constexpr float kFixedCap = 34.0f;
-
-enum { kRunning = 0, kFixed = 1 };
-
-template <int D, bool kCap, bool kBias, bool kSeg, int kMax, int kSplit>
+template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
-    scored_fwd_kernel(View Q, View K, View V, MutView O, float* __restrict__ lse2, const int32_t* __restrict__ seg,
-                      ScoreArgs a, int B, int H, int Hk, int S, int dim) {
+    scored_fwd_kernel(View Q, View K, View V, MutView O, uint8_t* __restrict__ o_low, float* __restrict__ lse2,
+                      const int32_t* __restrict__ seg, ScoreArgs a, int B, int H, int Hk, int S, int dim) {
   constexpr int KC = D / 16, DB = D / 32;
   constexpr bool kRaw = !kCap && !kBias;  // the softmax scales the raw products itself
   __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
@@ -70,7 +64,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
-  float m_run = kMax == kFixed ? a.cap2 : kMinusBig, l_run = 0.f;
+  float m_run = kMinusBig, l_run = 0.f;
 
   const __amdgpu_buffer_rsrc_t k_rs = slice(K.row(b, hk, 0), S, K.ss, dim);
   const __amdgpu_buffer_rsrc_t v_rs = slice(V.row(b, hk, 0), S, V.ss, dim);
@@ -92,7 +86,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     const int kh0 = kv0 + 32 * sb;
     // Scores less `off`, which is the same for all of a lane's keys: what a score
     // has in common with the others of its query costs no operation here.
-    float off = kCap && kMax == kRunning ? a.cap2 : 0.f;
+    float off = kCap ? a.cap2 : 0.f;
     if constexpr (!kRaw) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -133,34 +127,34 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
         for (int i = 0; i < 16; ++i) s[i] = acc_row(i) <= lim ? s[i] : -INFINITY;
       }
     }
-    float shift = 0.f;  // of the exponents
-    if constexpr (kMax == kRunning) {
-      float m_tile = -INFINITY;
+    float m_tile = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
-      if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
-      m_tile += off;  // (with a bias each half-wave has its own)
-      m_tile = max_halves(m_tile);
-      // The running maximum moves only when a row's maximum exceeds it by more
-      // than 8 (log2): P stays below 2^8 and most halves rescale nothing.
-      const bool grow = m_tile > m_run + 8.0f;
-      const float m_new = grow ? m_tile : m_run;
-      if (__ballot(grow)) {
-        const float alpha = fast_exp2(m_run - m_new);
-        l_run *= alpha;
+    for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
+    if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
+    m_tile += off;  // (with a bias each half-wave has its own)
+    m_tile = max_halves(m_tile);
+    // (With a cap a fixed reference would do, at 1% less time; but the largest P of a
+    // row is then no power of two, and its rounding adds a fifth to the error of o and,
+    // through delta, 4 to 13% to that of dq and dk.)
+    // The running maximum moves only when a row's maximum exceeds it by more
+    // than 8 (log2): P stays below 2^8 and most halves rescale nothing.
+    const bool grow = m_tile > m_run + 8.0f;
+    const float m_new = grow ? m_tile : m_run;
+    if (__ballot(grow)) {
+      const float alpha = fast_exp2(m_run - m_new);
+      l_run *= alpha;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
-      }
-      m_run = m_new;
-      shift = off - m_new;
+        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
     }
+    m_run = m_new;
+    const float shift = off - m_new;
     bf16x8 pb[2];
     float lsum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, shift) : kMax == kFixed ? s[i] : s[i] + shift);
+      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, shift) : s[i] + shift);
       lsum += p;
       pb[i >> 3][i & 7] = (bf16)p;
     }
@@ -275,6 +269,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   if (my_q < S) {
     const float inv = 1.0f / l_tot;
     bf16* orow = O.row(b, h, my_q);
+    uint8_t* const low_row = o_low ? o_low + (((size_t)b * H + h) * S + my_q) * dim : nullptr;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -282,9 +277,15 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
         const int d0 = 32 * db + 8 * r + 4 * hl;
         if (d0 >= dim) continue;
         bf16x4 o4;
+        uint32_t low = 0;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) o4[t] = (bf16)(acc[db][4 * r + t] * inv);
+        for (int t = 0; t < 4; ++t) {
+          const float x = acc[db][4 * r + t] * inv;
+          o4[t] = (bf16)x;
+          low |= low_bits(x, o4[t]) << (8 * t);
+        }
         *reinterpret_cast<bf16x4*>(orow + d0) = o4;
+        if (low_row) *reinterpret_cast<uint32_t*>(low_row + d0) = low;
       }
     if (hl == 0 && lse2) lse2[((size_t)b * H + h) * S + my_q] = m_run + __log2f(l_tot);
   }
@@ -295,10 +296,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
 extern "C" {
 
 int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const int32_t* segment_ids,
-                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, float* lse2,
-                           int batch, int heads, int kv_heads, int seq, int head_dim, const int64_t* strides,
-                           float softmax_scale, float score_cap, void* stream) {
+                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, void* o_low,
+                           float* lse2, int batch, int heads, int kv_heads, int seq, int head_dim,
+                           const int64_t* strides, float softmax_scale, float score_cap, void* stream) {
   ScoredCall c;
+  if ((uintptr_t)o_low & 15) return GPTRIG_E_SHAPE;
   const void* tensors[4] = {q, k, v, o};
   const int status = c.init(tensors, 4, 0b0110u, batch, heads, kv_heads, seq, head_dim, strides, softmax_scale,
                             score_cap, distance_slopes, prefix_lengths);
@@ -307,17 +309,13 @@ int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const in
   const View Q = c.view(0), K = c.view(1), V = c.view(2);
   const MutView O = c.out(3);
   const bool split = split_rows((long long)batch * heads, seq, head_dim, false);
-  const long long grid = (long long)batch * heads * ceil_div(seq, split ? kQueries / 2 : kQueries);
-  if (grid > INT32_MAX) return GPTRIG_E_SHAPE;
-#define SCORED_FWD_(D, CAP, BIAS, SEG, MAX, SPLIT)                                                                  \
-  scored_fwd_kernel<D, CAP, BIAS, SEG, MAX, SPLIT><<<(unsigned)grid, 256, 0, s>>>(Q, K, V, O, lse2, segment_ids, c.args, \
-                                                                                  batch, heads, kv_heads, seq, head_dim)
-#define SCORED_FWD(D, CAP, BIAS, SEG)                                                                      \
-  constexpr int fixed = CAP && !BIAS ? kFixed : kRunning;                                                  \
-  if (fixed == kFixed && score_cap <= kFixedCap && split) SCORED_FWD_(D, CAP, BIAS, SEG, fixed, 2);        \
-  else if (fixed == kFixed && score_cap <= kFixedCap) SCORED_FWD_(D, CAP, BIAS, SEG, fixed, 1);            \
-  else if (split) SCORED_FWD_(D, CAP, BIAS, SEG, kRunning, 2);                                             \
-  else SCORED_FWD_(D, CAP, BIAS, SEG, kRunning, 1)
+  const unsigned grid = (unsigned)(batch * heads * ceil_div(seq, split ? kQueries / 2 : kQueries));
+#define SCORED_FWD_(D, CAP, BIAS, SEG, SPLIT)                                                                       \
+  scored_fwd_kernel<D, CAP, BIAS, SEG, SPLIT><<<grid, 256, 0, s>>>(Q, K, V, O, (uint8_t*)o_low, lse2, segment_ids,  \
+                                                                   c.args, batch, heads, kv_heads, seq, head_dim)
+#define SCORED_FWD(D, CAP, BIAS, SEG)            \
+  if (split) SCORED_FWD_(D, CAP, BIAS, SEG, 2);  \
+  else SCORED_FWD_(D, CAP, BIAS, SEG, 1)
   SCORED_DISPATCH(SCORED_FWD, c, segment_ids != nullptr);
 #undef SCORED_FWD
 #undef SCORED_FWD_

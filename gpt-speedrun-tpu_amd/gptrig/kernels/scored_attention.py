@@ -99,16 +99,18 @@ def _strides(*tensors: torch.Tensor):
 
 
 def _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale: float, cap: float, keep: bool):
-    """``o``, the views read, and the scores' sums for the backward (``None`` unless ``keep``)."""
+    """The views read, ``o``, and for the backward (``None`` unless ``keep``) what its rounding cut off and the
+    logarithms of the scores' sums."""
 
     q, k, v = _view(q), _view(k), _view(v)
     B, H, S, D = q.shape
     o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+    low = torch.empty((B, H, S, D), dtype=torch.uint8, device=q.device) if keep else None
     lse2 = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if keep else None
     _lib.call_on(q.get_device(), "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(lse2),
-                 B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
-    return q, k, v, o, lse2
+                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(low),
+                 _lib.ptr(lse2), B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
+    return q, k, v, o, low, lse2
 
 
 class _ScoredAttention(torch.autograd.Function):
@@ -125,7 +127,7 @@ class _ScoredAttention(torch.autograd.Function):
 
 
 def _backward(ctx, do):
-    q, k, v, o, lse2, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
+    q, k, v, o, low, lse2, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
     B, H, S, D = q.shape
     Hk = k.shape[1]
     do = _view(do)
@@ -135,8 +137,8 @@ def _backward(ctx, do):
     size = _lib.query("gptrig_scored_attn_bwd_workspace_bytes", B, H, Hk, S, D)
     ws = _lib.workspace(size, q.device)
     _lib.call_on(q.get_device(), "gptrig_scored_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                 do.data_ptr(), lse2.data_ptr(), _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes),
-                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size, B, H, Hk, S, D,
+                 do.data_ptr(), low.data_ptr(), lse2.data_ptr(), _lib.ptr(segment_ids), _lib.ptr(prefix_lengths),
+                 _lib.ptr(slopes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size, B, H, Hk, S, D,
                  _strides(q, k, v, o, do, dq, dk, dv), *ctx.scalars)
     return dq, dk, dv, None, None, None, None, None
 
@@ -150,7 +152,7 @@ def make_scored_attention(config: ScoredAttentionConfig = ScoredAttentionConfig(
     ``q`` ``[batch, heads, seq, head_dim]``, ``k`` and ``v`` ``[batch, kv_heads,
     seq, head_dim]`` bfloat16 of any strides, ``heads`` a multiple of ``kv_heads``
     (head h reads kv head ``h // (heads // kv_heads)``).  ``segment_ids``: integers
-    ``[batch, seq]``; ``prefix_lengths``: integers ``[batch]``, the positions that
+    ``[batch, seq]``, compared in their lower 32 bits; ``prefix_lengths``: integers ``[batch]``, the positions that
     every query of the sequence sees; ``distance_slopes``: float32 ``[heads]``,
     constants.  Differentiable once in q, k and v; the same call gives the same
     bits.  Pairs that are not visible add nothing, whatever they hold.
@@ -170,6 +172,8 @@ def make_scored_attention(config: ScoredAttentionConfig = ScoredAttentionConfig(
         _lib.require_one_device(q, k, v, segment_ids, prefix_lengths, distance_slopes)
         if (S + 64) * q.shape[3] >= 1 << 30:
             raise ValueError(f"a head's tensors must stay below 2 GiB, got {tuple(q.shape)}")
+        if q.shape[0] * q.shape[1] * (-(-S // 64)) > 1 << 22:
+            raise ValueError(f"batch x heads x (seq / 64, rounded up) must be at most 2^22, got {tuple(q.shape)}")
         scale = q.shape[3] ** -0.5 if config.softmax_scale is None else config.softmax_scale
         call = (q, k, v, segment_ids, prefix_lengths, distance_slopes, float(scale), float(config.score_cap or 0.0))
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -95,17 +95,19 @@ int gptrig_attn_bwd_rope(const void* q, const void* k, const void* v, const void
  * NULL; values are clamped to [0, seq]) and, with segment_ids (i32 [batch, seq] or
  * NULL), the ids are equal.  `strides` as above (order q, k, v, o; in the backward q,
  * k, v, o, dout, dq, dk, dv); all tensors 16-byte aligned.  lse2 f32 [batch, heads,
- * seq]: log2 of the sum of exponentials (NULL where no backward follows).
+ * seq]: log2 of the sum of exponentials; o_low, 8 bits, contiguous [batch, heads,
+ * seq, head_dim]: what the rounding of o cut off (both NULL where no backward follows).
+ * At most 2^22 blocks of 64 rows over all heads: batch heads ceil(seq / 64).
  * Hidden pairs add nothing even where their values are infinite or NaN.
  * Results do not depend on the order of the workgroups (no atomics).
  * ---------------------------------------------------------------------- */
 int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const int32_t* segment_ids,
-                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, float* lse2,
-                           int batch, int heads, int kv_heads, int seq, int head_dim,
+                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, void* o_low,
+                           float* lse2, int batch, int heads, int kv_heads, int seq, int head_dim,
                            const int64_t* strides /* q,k,v,o */, float softmax_scale, float score_cap, void* stream);
 size_t gptrig_scored_attn_bwd_workspace_bytes(int batch, int heads, int kv_heads, int seq, int head_dim);
 int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
-                           const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
+                           const void* o_low, const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
                            const float* distance_slopes, void* dq, void* dk, void* dv, void* workspace,
                            size_t workspace_bytes, int batch, int heads, int kv_heads, int seq, int head_dim,
                            const int64_t* strides /* q,k,v,o,dout,dq,dk,dv */, float softmax_scale, float score_cap,
@@ -402,8 +404,8 @@ int gptrig_adamw(float* param, const float* grad, float* m, float* v, void* para
  * infinite or NaN moment is kept as a NaN code.  grad_type of all gradients;
  * tensor_hparams f32 [count, 3] = {lr_mult, epsilon, decay} in device memory;
  * clip_scale a nullable device scalar.  Pointers aligned to their element; at
- * most 2^40 elements a tensor; GPTRIG_E_OVERLAP where two of the arrays that the
- * call writes share memory. */
+ * most 2^35 elements a tensor; GPTRIG_E_OVERLAP where an array that the call writes
+ * shares memory with another one of the table's. */
 typedef struct {
   float* param;    /* f32 [n], updated */
   const void* grad;

@@ -217,7 +217,7 @@ def test_many_workgroups(options, D):
     compare(*inputs(B, H, H if D == 64 else 8, S, D, seed=21), **o)
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [40, 64, 72, 128])
 @pytest.mark.parametrize("B, H, Hk", [(8, 32, 8), (10, 24, 8), (2, 12, 3)])
 def test_shared_heads_in_parts(B, H, Hk, D):
     """Groups of query heads whose key gradients come in several parts, of one head or of two."""

@@ -86,8 +86,9 @@ def test_adamw_tensors_refusals():
         for bad in (1.0, -0.1, float("nan")):
             with pytest.raises(ValueError, match="beta1"):
                 step(**{name: bad})
-    with pytest.raises(ValueError, match="counts from 1"):
-        step(step=0)
+    for bad in (0, 2 ** 31, 2 ** 32 + 1):
+        with pytest.raises(ValueError, match="counts from 1"):
+            step(step=bad)
     for bad in (-1, 2 ** 32):
         with pytest.raises(ValueError, match="seed"):
             step(seed=bad)
@@ -131,6 +132,17 @@ def test_entry_points_refuse_on_the_host():
             bad = (ctypes.c_int64 * 16)(*rows)
             bad[second] = bad[first] + shift
             assert adamw(bad, 2, 1, state, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -7, (state, first, second, shift)
+    for state, first, second in ((32, 0, 1), (32, 9, 2), (8, 1, 13), (8, 14, 1)):  # (gradients are read, not written)
+        for shift in (0, 4):
+            bad = (ctypes.c_int64 * 16)(*rows)
+            bad[second] = bad[first] + shift
+            assert adamw(bad, 2, 1, state, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -7, (state, first, second, shift)
+    # A gradient that reaches over several arrays, the written one not next to it by its address.
+    bad = (ctypes.c_int64 * 16)(*rows)
+    bad[1], bad[9], bad[8] = 100 << 20, (100 << 20) + 4, (100 << 20) + 3992
+    assert adamw(bad, 2, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -7
+    rows[7] = (1 << 35) + 1
+    assert adamw(rows, 2, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -2
     many = (ctypes.c_int64 * (8 * 200))(*[v for i in range(200) for v in (*[(i * 8 + k + 1) << 20 for k in range(7)], 10)])
     many[8 * 199] = many[8 * 3 + 2] + 36
     assert adamw(many, 200, 1, 32, at, 0.1, 0.9, 0.95, 1, None, 0, None) == -7
@@ -185,6 +197,9 @@ def test_scored_attention_refusals():
         attention(q, k, k, distance_slopes=torch.zeros(4, requires_grad=True))
     with pytest.raises(RuntimeError, match="GPU"):
         attention(q, k, k)
+    wide = torch.zeros((1, 1, 1, 8), dtype=BF16).expand(1 << 20, 5, 1, 8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        attention(wide, wide, wide)
 
 
 def test_scored_attention_entry_points_refuse_on_the_host():
@@ -192,7 +207,7 @@ def test_scored_attention_entry_points_refuse_on_the_host():
     at, odd = ctypes.c_void_p(1 << 12), ctypes.c_void_p((1 << 12) + 8)
 
     def fwd(q=at, o=at, B=1, H=4, Hk=2, S=16, D=64, strides=None, scale=0.125, cap=0.0):
-        return lib.gptrig_scored_attn_fwd(q, at, at, None, None, None, o, None, B, H, Hk, S, D, strides, scale, cap, None)
+        return lib.gptrig_scored_attn_fwd(q, at, at, None, None, None, o, None, None, B, H, Hk, S, D, strides, scale, cap, None)
 
     assert fwd(q=None) == -1 and fwd(q=odd) == -2
     assert fwd(Hk=3) == -2 and fwd(Hk=0) == -2 and fwd(S=0) == -2 and fwd(B=-1) == -2
@@ -201,6 +216,7 @@ def test_scored_attention_entry_points_refuse_on_the_host():
         assert fwd(scale=scale) == -2
     for cap in (-1.0, 1001.0, float("nan"), 1e-42):
         assert fwd(cap=cap) == -2
+    assert fwd(B=1 << 20, H=5, Hk=5, S=1) == -2 and fwd(B=1 << 30, S=1) == -2 and fwd(B=1 << 14, S=(1 << 14) + 1) == -2
     assert fwd(S=1 << 24) == -2  # a head's slice past 2 GiB
     for change in (4, -64):
         st = (ctypes.c_int64 * 12)(*[4096, 1024, 64] * 4)
@@ -210,9 +226,9 @@ def test_scored_attention_entry_points_refuse_on_the_host():
     need = lib.gptrig_scored_attn_bwd_workspace_bytes(1, 4, 2, 16, 64)
     assert need >= 4 * 16 * 4
 
-    def bwd(ws=at, size=big, lse=at, dv=at):
-        return lib.gptrig_scored_attn_bwd(at, at, at, at, at, lse, None, None, None, at, at, dv, ws, size, 1, 4, 2, 16, 64, None,
+    def bwd(ws=at, size=big, lse=at, dv=at, low=at):
+        return lib.gptrig_scored_attn_bwd(at, at, at, at, at, low, lse, None, None, None, at, at, dv, ws, size, 1, 4, 2, 16, 64, None,
                                           0.125, 0.0, None)
 
-    assert bwd(ws=None) == -1 and bwd(lse=None) == -1 and bwd(dv=None) == -1
+    assert bwd(ws=None) == -1 and bwd(lse=None) == -1 and bwd(low=None) == -1 and bwd(low=odd) == -2 and bwd(dv=None) == -1
     assert bwd(size=need - 1) == -6 and bwd(ws=odd) == -2

@@ -18,6 +18,7 @@ are handled in-kernel.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Callable
@@ -49,7 +50,7 @@ def _validate(q, k, v, segment_ids, prefix_lengths, distance_slopes) -> None:
         raise ValueError(
             f"q, k, and v must use BHSD rank-4 layout; got {tuple(q.shape)}, {tuple(k.shape)}, and {tuple(v.shape)}"
         )
-    if not all(q.shape) or not all(k.shape):
+    if 0 in q.shape or 0 in k.shape:
         raise ValueError(f"q/k/v dimensions must be nonzero, got {tuple(q.shape)} and {tuple(k.shape)}")
     B, H, S, D = q.shape
     if k.shape != v.shape or (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D) or H % k.shape[1]:
@@ -59,6 +60,8 @@ def _validate(q, k, v, segment_ids, prefix_lengths, distance_slopes) -> None:
         raise ValueError(f"the kernel requires head_dim <= 128 and divisible by 8; got {D}")
     if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
         raise TypeError(f"the HIP attention kernels take bfloat16 q/k/v; got {q.dtype}, {k.dtype}, {v.dtype}")
+    if segment_ids is None and prefix_lengths is None and distance_slopes is None:
+        return
     for name, t, shape in (("segment_ids", segment_ids, (B, S)), ("prefix_lengths", prefix_lengths, (B,))):
         if t is None:
             continue
@@ -98,25 +101,44 @@ def _strides(*tensors: torch.Tensor):
     return _ARRAYS[len(tensors)](*[s for t in tensors for s in t.stride()[:3]])
 
 
-def _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale: float, cap: float, keep: bool):
-    """The views read, ``o``, and for the backward (``None`` unless ``keep``) what its rounding cut off and the
-    logarithms of the scores' sums."""
+# (The host's work is most of a small call's time, and backwards run on a thread of
+# their own, at half the speed: so contiguous tensors take the shorter ways below.)
+def _plain(*tensors: torch.Tensor) -> bool:
+    """Whether the kernels take them as they are, with default strides."""
 
-    q, k, v = _view(q), _view(k), _view(v)
+    for t in tensors:
+        if not t.is_contiguous() or t.data_ptr() & 15:
+            return False
+    return True
+
+
+def _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale: float, cap: float, keep: bool):
+    """The views read, ``o``, for the backward (``None`` unless ``keep``) what its rounding cut off and then the
+    logarithms of the scores' sums, in one buffer, and whether the views are plain."""
+
     B, H, S, D = q.shape
-    o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
-    low = torch.empty((B, H, S, D), dtype=torch.uint8, device=q.device) if keep else None
-    lse2 = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if keep else None
+    if _plain(q, k, v):
+        o, strides = torch.empty_like(q), None
+    else:
+        q, k, v = _view(q), _view(k), _view(v)
+        o = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+        strides = _strides(q, k, v, o)
+    kept = low = lse2 = None
+    if keep:
+        rows = B * H * S
+        kept = torch.empty(rows * (D + 4), dtype=torch.uint8, device=q.device)
+        low = kept.data_ptr()
+        lse2 = low + rows * D
     _lib.call_on(q.get_device(), "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), _lib.ptr(low),
-                 _lib.ptr(lse2), B, H, k.shape[1], S, D, _strides(q, k, v, o), scale, cap)
-    return q, k, v, o, low, lse2
+                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), low, lse2,
+                 B, H, k.shape[1], S, D, strides, scale, cap)
+    return q, k, v, o, kept, strides is None
 
 
 class _ScoredAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, segment_ids, prefix_lengths, slopes, scale, cap):
-        kept = _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale, cap, True)
+        *kept, ctx.plain = _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale, cap, True)
         ctx.save_for_backward(*kept, segment_ids, prefix_lengths, slopes)
         ctx.scalars = (scale, cap)
         return kept[3]
@@ -126,20 +148,30 @@ class _ScoredAttention(torch.autograd.Function):
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, do)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(*sizes: int) -> int:
+    return _lib.query("gptrig_scored_attn_bwd_workspace_bytes", *sizes)
+
+
 def _backward(ctx, do):
-    q, k, v, o, low, lse2, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
+    q, k, v, o, kept, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
     B, H, S, D = q.shape
     Hk = k.shape[1]
-    do = _view(do)
-    dq = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty((B, Hk, S, D), dtype=q.dtype, device=q.device)
-    dv = torch.empty_like(dk)
-    size = _lib.query("gptrig_scored_attn_bwd_workspace_bytes", B, H, Hk, S, D)
-    ws = _lib.workspace(size, q.device)
+    if ctx.plain and _plain(do):
+        dq, dk, dv, strides = torch.empty_like(q), torch.empty_like(k), torch.empty_like(k), None
+    else:
+        do = _view(do)
+        dq = torch.empty((B, H, S, D), dtype=q.dtype, device=q.device)
+        dk = torch.empty((B, Hk, S, D), dtype=q.dtype, device=q.device)
+        dv = torch.empty_like(dk)
+        strides = _strides(q, k, v, o, do, dq, dk, dv)
+    size = _workspace_bytes(B, H, Hk, S, D)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    low = kept.data_ptr()
     _lib.call_on(q.get_device(), "gptrig_scored_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                 do.data_ptr(), low.data_ptr(), lse2.data_ptr(), _lib.ptr(segment_ids), _lib.ptr(prefix_lengths),
+                 do.data_ptr(), low, low + B * H * S * D, _lib.ptr(segment_ids), _lib.ptr(prefix_lengths),
                  _lib.ptr(slopes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size, B, H, Hk, S, D,
-                 _strides(q, k, v, o, do, dq, dk, dv), *ctx.scalars)
+                 strides, *ctx.scalars)
     return dq, dk, dv, None, None, None, None, None
 
 

@@ -9,6 +9,7 @@ rounding points.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Any, Mapping
 
@@ -112,6 +113,11 @@ def _strided_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _layer_norm_workspace_bytes(rows: int, width: int, kind: int) -> int:
+    return _lib.query("gptrig_layernorm_bwd_workspace_bytes", rows, width, kind)
+
+
 def _layer_norm_forward(x, scale, bias, eps: float, keep: bool):
     """``y``, and what the backward needs (``None`` for the statistics unless ``keep``)."""
 
@@ -119,7 +125,7 @@ def _layer_norm_forward(x, scale, bias, eps: float, keep: bool):
     scale = scale.contiguous()
     bias = None if bias is None else bias.contiguous()
     rows, d = x2.shape
-    y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x2) if x2.is_contiguous() else torch.empty((rows, d), dtype=x.dtype, device=x.device)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
     mean = stats.data_ptr() if keep else None
     if rows:
@@ -152,12 +158,14 @@ def _layer_norm_backward(ctx, dy):
         return (dy.reshape(ctx.shape) if need_x else None, zero if need_s else None, zero.clone() if need_b else None,
                 None)
     dy2 = _strided_rows(dy)
-    dx = torch.empty((rows, d), dtype=x2.dtype, device=dev) if need_x else None
-    dscale = torch.empty(d, dtype=scale.dtype, device=dev) if need_s else None
-    dbias = torch.empty(d, dtype=scale.dtype, device=dev) if need_b else None
+    dx = None
+    if need_x:
+        dx = torch.empty_like(x2) if x2.is_contiguous() else torch.empty((rows, d), dtype=x2.dtype, device=dev)
+    dscale = torch.empty_like(scale) if need_s else None
+    dbias = torch.empty_like(scale) if need_b else None
     kind, ws, size = _TYPES[x2.dtype], None, 0
     if need_s or need_b:
-        size = _lib.query("gptrig_layernorm_bwd_workspace_bytes", rows, d, kind)
+        size = _layer_norm_workspace_bytes(rows, d, kind)
         ws = _lib.workspace(size, dev)
     mean = stats.data_ptr()
     _lib.call_on(x2.get_device(), "gptrig_layernorm_bwd", dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0),

@@ -75,9 +75,42 @@ __device__ __forceinline__ int tile_at(int row, int c16) { return (c16 >> 3) * k
 __device__ __forceinline__ bf16x8 tile_row(const at64::lds_t* t, int row, int c16) {
   return *(const at64::lds_x8*)(t + tile_at(row, c16));
 }
-// Transposed operand of columns 32 db .. +31, rows in accumulator order from r0.
-__device__ __forceinline__ bf16x8 tile_col(const at64::lds_t* t, int db, int r0, int lane) {
-  return at64::trfrag<true>(t + (db >> 1) * kRows * 64, 32 * (db & 1), r0, lane);
+
+// Byte offsets in a tile of what a lane reads for the matrix instructions.  The
+// swizzle of a row depends on it modulo 16, so these few stand for every row block,
+// column block and tile, which are constants of the instructions.  (Computed where
+// they are used they were a fifth of the loops' vector operations.)
+struct Lanes {
+  uint32_t row[4];           // chunk 2 kc + half-wave of row lane % 32
+  uint32_t low[2], high[2];  // transposed: the slots' first and second four rows, column blocks 0 and 1
+  __device__ __forceinline__ void init(int lane) {
+    const int hl = lane >> 5, cq = lane & 15;
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc) row[kc] = 2 * at64::swz(lane & 31, 2 * kc + hl);
+#pragma unroll
+    for (int db = 0; db < 2; ++db) {
+      const int m = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (cq & 3), r = 4 * hl + (cq >> 2);
+      low[db] = 2 * (at64::swz(r, m >> 3) + (m & 4));
+      high[db] = 2 * (at64::swz(r + 8, m >> 3) + (m & 4));
+    }
+  }
+};
+constexpr uint32_t kRowBytes = 128;                    // of one of a tile's halves of 64 columns
+constexpr uint32_t kColumns64 = kRows * kRowBytes;     // from one of them to the next
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __forceinline__ const at64::lds_t* byte_at(const at64::lds_t* t, uint32_t offset) {
+  return (const at64::lds_t*)((const lds_char*)t + offset);
+}
+// Operand kc of 32 rows; at: byte offset of the first, a multiple of 16 rows.
+__device__ __forceinline__ bf16x8 row_operand(const at64::lds_t* t, const Lanes& l, uint32_t at, int kc) {
+  return *(const at64::lds_x8*)byte_at(t, (l.row[kc & 3] + at) + (kc >> 2) * kColumns64);
+}
+// Transposed operand of columns 32 db .. +31 and 16 rows, in accumulator order.
+__device__ __forceinline__ bf16x8 column_operand(const at64::lds_t* t, const Lanes& l, uint32_t at, int c, int db) {
+  const uint32_t constant = (db >> 1) * kColumns64 + 16 * c * kRowBytes;
+  const bf16x4 lo = at64::read_tr(byte_at(t, (l.low[db & 1] + at) + constant));
+  const bf16x4 hi = at64::read_tr(byte_at(t, (l.high[db & 1] + at) + constant));
+  return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
 // 16 bytes a lane, or 4, global -> LDS: lane l's land at lds + 16 l (4 l).
@@ -188,16 +221,25 @@ struct Dirty {
   }
 };
 
-// acc[db] += (columns of `tile`, rows r0 .. r0 + 31)^T x, x the wave's 32 x 32
-// operand in accumulator order (16 rows of this lane's column as bf16).
+// acc[db] += (columns of a tile, 32 rows)^T x, x the wave's 32 x 32 operand in
+// accumulator order (16 rows of this lane's column as bf16).  The tile's operands are
+// loaded ahead, so that their way from LDS is behind other work.
 template <int DB>
-__device__ __forceinline__ void product(f32x16 (&acc)[DB], const at64::lds_t* tile, int r0, const bf16x8 (&x)[2],
-                                        int lane) {
+struct Columns {
+  bf16x8 v[2][DB];
+  __device__ __forceinline__ void load(const at64::lds_t* t, const Lanes& l, uint32_t at) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int db = 0; db < DB; ++db) acc[db] = mfma32(tile_col(tile, db, r0 + 16 * c, lane), x[c], acc[db]);
-}
+      for (int db = 0; db < DB; ++db) v[c][db] = column_operand(t, l, at, c, db);
+  }
+  __device__ __forceinline__ void product(f32x16 (&acc)[DB], const bf16x8 (&x)[2]) const {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = mfma32(v[c][db], x[c], acc[db]);
+  }
+};
 
 // ---------------------------------------------------------------------------
 // Host side: what every entry point checks, and the choice of a kernel

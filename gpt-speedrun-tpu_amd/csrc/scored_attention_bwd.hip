@@ -39,7 +39,7 @@ __device__ __forceinline__ void add(f32x16 (&acc)[DB], const float* at, int lane
 // exponents, cap log2 e - L_i (with a bias less slope (i mod 64), the part of the
 // bias that is the query's own in its tile), and -delta_i.
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
     scored_dq_kernel(View Q, View K, View V, View O, View dO, const uint8_t* __restrict__ o_low,
                      const float* __restrict__ lse2, const int32_t* __restrict__ seg, float* __restrict__ shifts, float* __restrict__ minus_delta,
                      MutView dQ, ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
@@ -102,6 +102,8 @@ __global__ void __launch_bounds__(256, 2)
     scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
   }
 
+  Lanes lanes;
+  lanes.init(lane);
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
@@ -120,13 +122,27 @@ __global__ void __launch_bounds__(256, 2)
 
   auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, const int* sg, int kv0, int sb,
                   int docs) __attribute__((always_inline)) {
+    const uint32_t at = 32 * kRowBytes * sb;
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      s = mfma32(tile_row(kt, 32 * sb + l32, 2 * kc + hl), qreg[kc], s);
-      dp = mfma32(tile_row(vt, 32 * sb + l32, 2 * kc + hl), greg[kc], dp);
-      if (D == 128 && (kc & 1)) __builtin_amdgcn_sched_barrier(0);
+    for (int k0 = 0; k0 < KC; k0 += 4) {
+      bf16x8 kr[4], vr[4];
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc) {
+        kr[kc] = row_operand(kt, lanes, at, k0 + kc);
+        vr[kc] = row_operand(vt, lanes, at, k0 + kc);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kc = 0; kc < 4; ++kc) {
+        s = mfma32(kr[kc], qreg[k0 + kc], s);
+        dp = mfma32(vr[kc], greg[k0 + kc], dp);
+      }
     }
+    constexpr bool kAhead = D == 64 && kBias;  // (elsewhere registers are short)
+    Columns<DB> kcol;
+    if (kAhead) kcol.load(kt, lanes, at);
+    __builtin_amdgcn_sched_barrier(0);
     const int kh0 = kv0 + 32 * sb;
     const float x = (float)(my_q - kh0 - 4 * hl);
     const float off = kBias ? fmaf(-slope2, x, shift) : shift;
@@ -174,8 +190,9 @@ __global__ void __launch_bounds__(256, 2)
     bf16x8 ds8[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) ds8[i >> 3][i & 7] = (bf16)s[i];
-    if (D == 128) __builtin_amdgcn_sched_barrier(0);
-    product<DB>(acc, kt, 32 * sb, ds8, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!kAhead) kcol.load(kt, lanes, at);
+    kcol.product(acc, ds8);
   };
 
   auto clean = [&](at64::lds_t* kt, const int* sg, int kv0, bool same) {
@@ -320,7 +337,8 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
       vfr[kc] = ok ? *reinterpret_cast<const bf16x8*>(V.row(b, hk, my_k) + c) : bf16x8{};
     }
   }
-  const int key_tile = (32 * group / kRows) * kRows * D, key_row = 32 * group % kRows + l32;
+  // (Byte offset of the wave's keys in LDS.)
+  const uint32_t key_at = (32 * group / kRows) * kRows * D * 2 + (32 * group % kRows) * kRowBytes;
   const int seg_k = kSeg ? seg[(size_t)b * S + min(my_k, S - 1)] : 0;
   WaveIds ids;
   SegScan<kWaves> scan;
@@ -329,6 +347,8 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, k0, lane);
   }
 
+  Lanes lanes;
+  lanes.init(lane);
   f32x16 dv_acc[DB], dk_acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) {
@@ -370,14 +390,28 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
 #pragma unroll
       for (int t = 0; t < 4; ++t) dp[4 * r + t] = d4[t];
     }
+    const uint32_t at = 32 * kRowBytes * qs;
+    constexpr int kStep = kKeysInLds ? 2 : 4;  // operands in flight
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      const bf16x8 k8 = kKeysInLds ? tile_row(ks + key_tile, key_row, 2 * kc + hl) : kfr[kc];
-      const bf16x8 v8 = kKeysInLds ? tile_row(vs + key_tile, key_row, 2 * kc + hl) : vfr[kc];
-      s = mfma32(tile_row(qt, 32 * qs + l32, 2 * kc + hl), k8, s);
-      dp = mfma32(tile_row(gt, 32 * qs + l32, 2 * kc + hl), v8, dp);
-      if (kWaves == 8 && (kc & 1)) __builtin_amdgcn_sched_barrier(0);
+    for (int k0 = 0; k0 < KC; k0 += kStep) {
+      bf16x8 qr[kStep], gr[kStep], kr[kStep], vr[kStep];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        qr[i] = row_operand(qt, lanes, at, k0 + i);
+        kr[i] = kKeysInLds ? row_operand(ks, lanes, key_at, k0 + i) : kfr[k0 + i];
+        gr[i] = row_operand(gt, lanes, at, k0 + i);
+        vr[i] = kKeysInLds ? row_operand(vs, lanes, key_at, k0 + i) : vfr[k0 + i];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        s = mfma32(qr[i], kr[i], s);
+        dp = mfma32(gr[i], vr[i], dp);
+      }
     }
+    Columns<DB> gc, qc;
+    if (kWaves == 4) gc.load(gt, lanes, at);
+    __builtin_amdgcn_sched_barrier(0);
     const int qh0 = qq0 + 32 * qs;
     const float off = -slope2 * (float)(qq0 - my_k);
     const bool after = kw0 + 31 > qh0;  // some key comes after some query
@@ -421,14 +455,15 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
         }
       }
     };
-    if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);  // (registers are short)
     if (masked || (kBias && after && qh0 + 31 >= kw0)) middle(std::true_type{}, std::false_type{});
     else if (kBias && after) middle(std::false_type{}, std::bool_constant<kBias>{});
     else middle(std::false_type{}, std::false_type{});
-    if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);
-    product<DB>(dv_acc, gt, 32 * qs, p8, lane);
-    if (kWaves == 8) __builtin_amdgcn_sched_barrier(0);
-    product<DB>(dk_acc, qt, 32 * qs, ds8, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    if (kWaves == 8) gc.load(gt, lanes, at);
+    else qc.load(qt, lanes, at);
+    gc.product(dv_acc, p8);
+    if (kWaves == 8) qc.load(qt, lanes, at);
+    qc.product(dk_acc, ds8);
   };
 
   auto clean = [&](at64::lds_t* t, const int* sg, int qq0, bool same) {

@@ -61,6 +61,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     scan.template init<kMine / 64>(seg + (size_t)b * S, scan_s, S, q0, lane);
   }
 
+  Lanes lanes;
+  lanes.init(lane);
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
@@ -80,9 +82,17 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   // One half of a tile, keys kh0 .. kh0 + 31.  docs: ids have to be compared.
   auto half = [&](const at64::lds_t* kt, const at64::lds_t* vt, const int* sg, int kv0, int sb,
                   int docs) __attribute__((always_inline)) {
+    const uint32_t at = 32 * kRowBytes * sb;
+    bf16x8 kr[KC];
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) kr[kc] = row_operand(kt, lanes, at, kc);
+    __builtin_amdgcn_sched_barrier(0);
     f32x16 s = f32x16{};
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc) s = mfma32(tile_row(kt, 32 * sb + l32, 2 * kc + hl), qreg[kc], s);
+    for (int kc = 0; kc < KC; ++kc) s = mfma32(kr[kc], qreg[kc], s);
+    Columns<DB> vc;
+    vc.load(vt, lanes, at);
+    __builtin_amdgcn_sched_barrier(0);
     const int kh0 = kv0 + 32 * sb;
     // Scores less `off`, which is the same for all of a lane's keys: what a score
     // has in common with the others of its query costs no operation here.
@@ -159,7 +169,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
       pb[i >> 3][i & 7] = (bf16)p;
     }
     l_run += lsum;
-    product<DB>(acc, vt, 32 * sb, pb, lane);
+    vc.product(acc, pb);
   };
 
   // Infinities and NaN of visible v rows in tiles that clear() changed: a bit per

@@ -411,6 +411,10 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     }
     Columns<DB> gc, qc;
     if (kWaves == 4) gc.load(gt, lanes, at);
+    f32x4 l16[4];
+    if (kWaves == 4)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) l16[r] = *reinterpret_cast<const f32x4*>(ls + own + 8 * r);
     __builtin_amdgcn_sched_barrier(0);
     const int qh0 = qq0 + 32 * qs;
     const float off = -slope2 * (float)(qq0 - my_k);
@@ -426,7 +430,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
       const int first = my_k <= last_prefix ? -64 : my_k - qh0 - 4 * hl, end = S - qh0 - 4 * hl;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + own + 8 * r);
+        const f32x4 l4 = kWaves == 4 ? l16[r] : *reinterpret_cast<const f32x4*>(ls + own + 8 * r);
         const i32x4 id = kBorder && kSeg ? *reinterpret_cast<const i32x4*>(sg + own + 8 * r) : i32x4{};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {

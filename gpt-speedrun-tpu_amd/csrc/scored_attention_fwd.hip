@@ -14,7 +14,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     scored_fwd_kernel(View Q, View K, View V, MutView O, uint8_t* __restrict__ o_low, float* __restrict__ lse2,
                       const int32_t* __restrict__ seg, ScoreArgs a, int B, int H, int Hk, int S, int dim) {
   constexpr int KC = D / 16, DB = D / 32;
-  constexpr bool kRaw = !kCap && !kBias;  // the softmax scales the raw products itself
+  // Without a bias s stays the raw product or, with a cap, its w: the softmax scales it.
+  constexpr bool kRaw = !kCap && !kBias, kW = kCap && !kBias;
+  constexpr float kHidden = kW ? INFINITY : -INFINITY;  // (a score falls with w)
   __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fk1[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fv0[kRows * D];
@@ -102,7 +104,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
       for (int i = 0; i < 16; ++i) {
         if constexpr (kCap) {
           const float w = cap_w(s[i], a);
-          s[i] = kBias ? fmaf(twice, w, bias[i]) : twice * w;
+          s[i] = kBias ? fmaf(twice, w, bias[i]) : w;
         } else {
           s[i] = fmaf(s[i], raw, bias[i]);
         }
@@ -130,17 +132,18 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
           const i32x4 id = *reinterpret_cast<const i32x4*>(sg + 32 * sb + 8 * r + 4 * hl);
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            s[4 * r + t] = acc_row(4 * r + t) <= lim && id[t] == seg_q ? s[4 * r + t] : -INFINITY;
+            s[4 * r + t] = acc_row(4 * r + t) <= lim && id[t] == seg_q ? s[4 * r + t] : kHidden;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = acc_row(i) <= lim ? s[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[i] = acc_row(i) <= lim ? s[i] : kHidden;
       }
     }
-    float m_tile = -INFINITY;
+    float m_tile = kHidden;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m_tile = fmaxf(m_tile, s[i]);
+    for (int i = 0; i < 16; ++i) m_tile = kW ? fminf(m_tile, s[i]) : fmaxf(m_tile, s[i]);
     if constexpr (kRaw) m_tile *= a.raw;  // (raw > 0)
+    if constexpr (kW) m_tile *= twice;
     m_tile += off;  // (with a bias each half-wave has its own)
     m_tile = max_halves(m_tile);
     // (With a cap a fixed reference would do, at 1% less time; but the largest P of a
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     float lsum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, shift) : s[i] + shift);
+      const float p = fast_exp2(kRaw ? fmaf(s[i], a.raw, shift) : kW ? fmaf(s[i], twice, shift) : s[i] + shift);
       lsum += p;
       pb[i >> 3][i & 7] = (bf16)p;
     }

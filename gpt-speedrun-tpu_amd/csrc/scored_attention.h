@@ -308,6 +308,48 @@ inline bool split_rows(long long batch_heads, int seq, int dim, bool keys) {
   return batch_heads * ceil_div(seq, 128) <= most;
 }
 
+// Rows of a workgroup of the forward and of dq, keys of one of dk and dv, and the
+// parts that the heads of a group are divided into for the latter: the fewest that
+// divide it and give kWant workgroups (they are of uneven length, so several a CU;
+// each part's sums are written and read once more).  us of a backward with kWant
+// 256 / 512 / 1024, 16 query heads on 4: D128 B4 S2048 391 / 331 / 375, B2 S2048 224 /
+// 191 / 194, B4 S2048 documents 474 / 363 / 344; D64 B4 S2048 274 / 242 / 252, B8 S2048
+// 382 / 382 / 387.
+constexpr long long kWant = 512;
+struct Blocks {
+  bool row_split, key_split;
+  int rows, keys, parts;  // rows and keys of a block
+  Blocks(int batch, int heads, int kv_heads, int seq, int dim) {
+    const int G = heads / kv_heads;
+    const long long blocks = (long long)batch * kv_heads * ceil_div(seq, 128);
+    parts = G;
+    for (int p = 1; p < G; ++p)
+      if (G % p == 0 && blocks * p >= kWant) {
+        parts = p;
+        break;
+      }
+    row_split = split_rows((long long)batch * heads, seq, dim, false);
+    key_split = split_rows((long long)batch * kv_heads * parts, seq, dim, true);
+    rows = row_split ? 64 : 128;
+    keys = key_split ? 64 : 128;
+  }
+};
+
+// Which block a workgroup has: by a plan (see scored_plan_kernel) that lists
+// batch x blocks, the longest first, each for all its heads; or by rank, the last
+// block first where `last_first` (longest first, without a prefix or documents).
+__device__ __forceinline__ void block_of(const int* plan, int id, int blocks, int batch, int heads, bool last_first,
+                                         int& bh, int& block) {
+  if (plan) {
+    const int item = min(max(plan[id / heads], 0), batch * blocks - 1);
+    bh = item / blocks * heads + id % heads;
+    block = item % blocks;
+  } else {
+    xcd_map(id, blocks, batch * heads, bh, block);
+    if (last_first) block = blocks - 1 - block;
+  }
+}
+
 // CALL(head dim of the kernel, cap, bias, segment ids) for a call c.
 #define SCORED_BIAS_SEG(CALL, c, D, CAP, seg)                                                          \
   do {                                                                                                 \

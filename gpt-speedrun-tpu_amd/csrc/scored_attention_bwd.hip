@@ -41,7 +41,7 @@ __device__ __forceinline__ void add(f32x16 (&acc)[DB], const float* at, int lane
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
     scored_dq_kernel(View Q, View K, View V, View O, View dO, const uint8_t* __restrict__ o_low,
-                     const float* __restrict__ lse2, const int32_t* __restrict__ seg, float* __restrict__ shifts, float* __restrict__ minus_delta,
+                     const float* __restrict__ lse2, const int32_t* __restrict__ seg, const int* __restrict__ plan, float* __restrict__ shifts, float* __restrict__ minus_delta,
                      MutView dQ, ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
   constexpr int KC = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
@@ -54,8 +54,7 @@ __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
   constexpr int kMine = kOwn / kSplit;
   const int nq = (S + kMine - 1) / kMine;
   int bh, qb;
-  xcd_map(blockIdx.x, nq, B * H, bh, qb);
-  qb = nq - 1 - qb;
+  block_of(plan, blockIdx.x, nq, B, H, true, bh, qb);
   const int b = bh / H, h = bh % H, hk = h / (H / Hk);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -288,7 +287,7 @@ __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ shifts,
-                      const float* __restrict__ minus_delta, const int32_t* __restrict__ seg, MutView dK, MutView dV,
+                      const float* __restrict__ minus_delta, const int32_t* __restrict__ seg, const int* __restrict__ plan, MutView dK, MutView dV,
                       float* __restrict__ partial, int parts, ScoreArgs a, int B, int H, int Hk, int S, int dim,
                       float scale) {
   constexpr int KC = D / 16, DB = D / 32, kGroups = kWaves / kSplit, kMine = 32 * kGroups;
@@ -306,7 +305,7 @@ __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
   // parts workgroups share the heads of a group where there are few keys to own.
   const int nkv = (S + kMine - 1) / kMine, G = H / Hk / parts;
   int bh, kb;
-  xcd_map(blockIdx.x, nkv, B * Hk * parts, bh, kb);
+  block_of(plan, blockIdx.x, nkv, B, Hk * parts, false, bh, kb);
   const int b = bh / parts / Hk, hk = bh / parts % Hk, h0 = hk * (H / Hk) + bh % parts * G;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -639,20 +638,6 @@ __global__ void __launch_bounds__(256) scored_join_kernel(const float* __restric
   *reinterpret_cast<bf16x8*>((values ? dV : dK).row(bh / Hk, bh % Hk, s) + c) = o;
 }
 
-// Parts of each group of heads: the fewest that divide it and give kWant
-// workgroups (they are of uneven length, so several a CU; each part's sums are
-// written and read once more).  us of a backward with kWant 256 / 512 / 1024, 16 query
-// heads on 4: D128 B4 S2048 391 / 331 / 375, B2 S2048 224 / 191 / 194, B4 S2048
-// documents 474 / 363 / 344; D64 B4 S2048 274 / 242 / 252, B8 S2048 382 / 382 / 387.
-constexpr long long kWant = 512;
-int parts_of(int batch, int heads, int kv_heads, int seq) {
-  const int G = heads / kv_heads;
-  const long long blocks = (long long)batch * kv_heads * ceil_div(seq, kOwn);
-  for (int p = 1; p < G; ++p)
-    if (G % p == 0 && blocks * p >= kWant) return p;
-  return G;
-}
-
 size_t row_numbers_bytes(int batch, int heads, int seq) {
   return ((size_t)batch * heads * seq * sizeof(float) + 255) & ~(size_t)255;
 }
@@ -663,14 +648,14 @@ extern "C" {
 
 size_t gptrig_scored_attn_bwd_workspace_bytes(int batch, int heads, int kv_heads, int seq, int head_dim) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq <= 0 || head_dim <= 0) return 0;
-  const int parts = parts_of(batch, heads, kv_heads, seq);
+  const int parts = Blocks(batch, heads, kv_heads, seq, head_dim).parts;
   const size_t sums = parts > 1 ? (size_t)2 * batch * kv_heads * parts * seq * head_dim * sizeof(float) : 0;
   return 2 * row_numbers_bytes(batch, heads, seq) + sums;
 }
 
 int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
                            const void* o_low, const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
-                           const float* distance_slopes, void* dq, void* dk, void* dv, void* workspace,
+                           const float* distance_slopes, const void* plan, void* dq, void* dk, void* dv, void* workspace,
                            size_t workspace_bytes, int batch, int heads, int kv_heads, int seq, int head_dim,
                            const int64_t* strides, float softmax_scale, float score_cap, void* stream) {
   ScoredCall c;
@@ -681,12 +666,15 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
   if (status != GPTRIG_OK) return status;
   if (workspace_bytes < gptrig_scored_attn_bwd_workspace_bytes(batch, heads, kv_heads, seq, head_dim))
     return GPTRIG_E_WORKSPACE;
-  if (((uintptr_t)workspace | (uintptr_t)o_low) & 15) return GPTRIG_E_SHAPE;
-  const bool split = split_rows((long long)batch * heads, seq, head_dim, false);
-  const unsigned grid = (unsigned)(batch * heads * ceil_div(seq, split ? kOwn / 2 : kOwn));
-  const int parts = parts_of(batch, heads, kv_heads, seq);
-  const bool kv_split = split_rows((long long)batch * kv_heads * parts, seq, head_dim, true);
-  const unsigned kv_grid = (unsigned)(batch * kv_heads * parts * ceil_div(seq, kv_split ? kOwn / 2 : kOwn));
+  if (((uintptr_t)workspace | (uintptr_t)o_low | (uintptr_t)plan) & 15) return GPTRIG_E_SHAPE;
+  const Blocks blocks(batch, heads, kv_heads, seq, head_dim);
+  const bool split = blocks.row_split, kv_split = blocks.key_split;
+  const int parts = blocks.parts, row_blocks = ceil_div(seq, blocks.rows);
+  const unsigned grid = (unsigned)(batch * heads * row_blocks);
+  const unsigned kv_grid = (unsigned)(batch * kv_heads * parts * ceil_div(seq, blocks.keys));
+  if (!gptrig_scored_attn_plan_bytes(batch, heads, kv_heads, seq, head_dim)) plan = nullptr;
+  const int* const row_plan = (const int*)plan;
+  const int* const key_plan = plan ? row_plan + batch * row_blocks : nullptr;
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2), O = c.view(3), dO = c.view(4);
   const MutView dQ = c.out(5), dK = c.out(6), dV = c.out(7);
@@ -695,11 +683,11 @@ int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const vo
   float* const partial = minus_delta + row_numbers_bytes(batch, heads, seq) / sizeof(float);
 #define SCORED_DQ(D, CAP, BIAS, SEG, SPLIT)                                                                          \
   scored_dq_kernel<D, CAP, BIAS, SEG, SPLIT><<<grid, 256, 0, s>>>(                                         \
-      Q, K, V, O, dO, (const uint8_t*)o_low, lse2, segment_ids, shifts, minus_delta, dQ, c.args, batch, heads, kv_heads, \
-      seq, head_dim, softmax_scale)
+      Q, K, V, O, dO, (const uint8_t*)o_low, lse2, segment_ids, row_plan, shifts, minus_delta, dQ, c.args, batch, heads, \
+      kv_heads, seq, head_dim, softmax_scale)
 #define SCORED_DKV(D, CAP, BIAS, SEG, SPLIT, WAVES)                                                                  \
   scored_dkv_kernel<D, CAP, BIAS, SEG, SPLIT, WAVES><<<kv_grid, 64 * WAVES, 0, s>>>(                                 \
-      Q, K, V, dO, shifts, minus_delta, segment_ids, dK, dV, partial, parts, c.args, batch, heads, kv_heads, seq,    \
+      Q, K, V, dO, shifts, minus_delta, segment_ids, key_plan, dK, dV, partial, parts, c.args, batch, heads, kv_heads, seq,    \
       head_dim, softmax_scale)
 #define SCORED_BWD(D, CAP, BIAS, SEG)                                           \
   if (split) SCORED_DQ(D, CAP, BIAS, SEG, 2);                                   \

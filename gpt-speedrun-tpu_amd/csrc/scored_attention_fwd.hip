@@ -9,10 +9,92 @@ namespace {
 
 constexpr int kQueries = 128;  // of a workgroup; kSplit 2: 64
 
+// With a prefix or documents the blocks of a call are of very uneven length, and
+// long ones that start last keep a few CUs busy alone: so their order is planned,
+// the longest first, in a launch of its own.  Blocks of the same 1/512 of the longest
+// possible are in any order; nothing but the time depends on it.
+constexpr int kPlanItems = 2048, kPlanBuckets = 512;
+struct Plan {
+  int blocks[2], size[2];  // rows (0) and keys (1): blocks of a sequence, positions of one
+};
+// Workgroup 0 orders the blocks of rows, workgroup 1 those of keys: their lengths in
+// tiles, counted from the lowest and highest id of each tile where there are
+// documents, sorted by counting.
+__global__ void __launch_bounds__(1024) scored_plan_kernel(const int32_t* __restrict__ seg,
+                                                           const int32_t* __restrict__ prefix, int* __restrict__ plan,
+                                                           Plan sizes, int B, int S) {
+  __shared__ int lowest[kPlanItems], highest[kPlanItems], length[kPlanItems], count[kPlanBuckets];
+  const int which = blockIdx.x, tid = threadIdx.x;
+  const int tiles = (S + kRows - 1) / kRows, blocks = sizes.blocks[which], size = sizes.size[which];
+  const int items = B * blocks;
+  if (which) plan += B * sizes.blocks[0];
+  for (int i = tid; i < kPlanBuckets; i += 1024) count[i] = 0;
+  const int l16 = tid & 15;  // 16 lanes a tile, and then a block
+  if (seg)
+    for (int i = tid >> 4; i < B * tiles; i += 64) {
+      const int32_t* const ids = seg + (size_t)(i / tiles) * S;
+      int id[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) id[j] = ids[min(i % tiles * kRows + 16 * j + l16, S - 1)];
+      int lo = min(min(id[0], id[1]), min(id[2], id[3])), hi = max(max(id[0], id[1]), max(id[2], id[3]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+      }
+      if (l16 == 0) {
+        lowest[i] = lo;
+        highest[i] = hi;
+      }
+    }
+  __syncthreads();
+  for (int i = tid >> 4; i < items; i += 64) {
+    const int b = i / blocks, at = i % blocks * size, own = at / kRows, after = min(at + size, S);
+    const int p = prefix ? min(max(prefix[b], 0), S) : 0;
+    const int from = which == 0 || at < p ? 0 : own;
+    const int to = which ? tiles : (max(after, p) + kRows - 1) / kRows;
+    int n = to - from;
+    if (seg) {
+      const int* const lo = lowest + b * tiles;
+      const int* const hi = highest + b * tiles;
+      const int last = (after - 1) / kRows, low = min(lo[own], lo[last]), high = max(hi[own], hi[last]);
+      n = 0;
+#pragma unroll 4
+      for (int t = from + l16; t < to; t += 16) n += lo[t] <= high && hi[t] >= low;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    }
+    if (l16 == 0) {
+      length[i] = (int)((long long)(tiles - n) * (kPlanBuckets - 1) / tiles);
+      atomicAdd(&count[length[i]], 1);
+    }
+  }
+  __syncthreads();
+  if (tid < 64) {  // the first place of each bucket
+    int sum = 0;
+    for (int i = 0; i < kPlanBuckets / 64; ++i) sum += count[tid * (kPlanBuckets / 64) + i];
+    int place = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int below = __shfl_up(place, o);
+      if (tid >= o) place += below;
+    }
+    place -= sum;
+    for (int i = 0; i < kPlanBuckets / 64; ++i) {
+      const int n = count[tid * (kPlanBuckets / 64) + i];
+      count[tid * (kPlanBuckets / 64) + i] = place;
+      place += n;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < items; i += 1024) plan[atomicAdd(&count[length[i]], 1)] = i;
+}
+
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     scored_fwd_kernel(View Q, View K, View V, MutView O, uint8_t* __restrict__ o_low, float* __restrict__ lse2,
-                      const int32_t* __restrict__ seg, ScoreArgs a, int B, int H, int Hk, int S, int dim) {
+                      const int32_t* __restrict__ seg, const int* __restrict__ plan, ScoreArgs a, int B, int H, int Hk,
+                      int S, int dim) {
   constexpr int KC = D / 16, DB = D / 32;
   // Without a bias s stays the raw product or, with a cap, its w: the softmax scales it.
   constexpr bool kRaw = !kCap && !kBias, kW = kCap && !kBias;
@@ -26,8 +108,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   constexpr int kMine = kQueries / kSplit;
   const int nq = (S + kMine - 1) / kMine;
   int bh, qb;
-  xcd_map(blockIdx.x, nq, B * H, bh, qb);
-  qb = nq - 1 - qb;
+  block_of(plan, blockIdx.x, nq, B, H, true, bh, qb);
   const int b = bh / H, h = bh % H, hk = h / (H / Hk);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -308,12 +389,38 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
 
 extern "C" {
 
+size_t gptrig_scored_attn_plan_bytes(int batch, int heads, int kv_heads, int seq, int head_dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq <= 0 || head_dim <= 0) return 0;
+  const Blocks k(batch, heads, kv_heads, seq, head_dim);
+  const long long rows = (long long)batch * ceil_div(seq, k.rows), keys = (long long)batch * ceil_div(seq, k.keys);
+  // (Where every workgroup starts at once their order matters little.)  The plan costs 4
+  // to 8 us a call.  us forward and backward with / without, H12 D64 biased: documents
+  // of 1500 B1 S8192 403 / 421, B2 493 / 572; of 700 B8 S4096 674 / 773; of 200 B16 S1024
+  // 251 / 247; prefixes B2 S2000 169 / 180, B4 247 / 290.
+  if ((long long)batch * ceil_div(seq, kRows) > kPlanItems || rows * heads <= 512) return 0;
+  return (size_t)(rows + keys) * sizeof(int);
+}
+
+int gptrig_scored_attn_plan(const int32_t* segment_ids, const int32_t* prefix_lengths, void* plan, size_t plan_bytes,
+                            int batch, int heads, int kv_heads, int seq, int head_dim, void* stream) {
+  const size_t need = gptrig_scored_attn_plan_bytes(batch, heads, kv_heads, seq, head_dim);
+  if (!need) return GPTRIG_E_SHAPE;
+  if (!plan) return GPTRIG_E_NULL;
+  if (plan_bytes < need) return GPTRIG_E_WORKSPACE;
+  if ((uintptr_t)plan & 15) return GPTRIG_E_SHAPE;
+  const Blocks k(batch, heads, kv_heads, seq, head_dim);
+  const Plan sizes = {{ceil_div(seq, k.rows), ceil_div(seq, k.keys)}, {k.rows, k.keys}};
+  scored_plan_kernel<<<2, 1024, 0, (hipStream_t)stream>>>(segment_ids, prefix_lengths, (int*)plan, sizes, batch, seq);
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
+}
+
 int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const int32_t* segment_ids,
-                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, void* o_low,
-                           float* lse2, int batch, int heads, int kv_heads, int seq, int head_dim,
+                           const int32_t* prefix_lengths, const float* distance_slopes, const void* plan,
+                           void* o, void* o_low, float* lse2, int batch, int heads, int kv_heads, int seq, int head_dim,
                            const int64_t* strides, float softmax_scale, float score_cap, void* stream) {
   ScoredCall c;
-  if ((uintptr_t)o_low & 15) return GPTRIG_E_SHAPE;
+  if (((uintptr_t)o_low | (uintptr_t)plan) & 15) return GPTRIG_E_SHAPE;
   const void* tensors[4] = {q, k, v, o};
   const int status = c.init(tensors, 4, 0b0110u, batch, heads, kv_heads, seq, head_dim, strides, softmax_scale,
                             score_cap, distance_slopes, prefix_lengths);
@@ -321,13 +428,14 @@ int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const in
   hipStream_t s = (hipStream_t)stream;
   const View Q = c.view(0), K = c.view(1), V = c.view(2);
   const MutView O = c.out(3);
-  const bool split = split_rows((long long)batch * heads, seq, head_dim, false);
-  const unsigned grid = (unsigned)(batch * heads * ceil_div(seq, split ? kQueries / 2 : kQueries));
+  const Blocks blocks(batch, heads, kv_heads, seq, head_dim);
+  if (!gptrig_scored_attn_plan_bytes(batch, heads, kv_heads, seq, head_dim)) plan = nullptr;
+  const unsigned grid = (unsigned)(batch * heads * ceil_div(seq, blocks.rows));
 #define SCORED_FWD_(D, CAP, BIAS, SEG, SPLIT)                                                                       \
   scored_fwd_kernel<D, CAP, BIAS, SEG, SPLIT><<<grid, 256, 0, s>>>(Q, K, V, O, (uint8_t*)o_low, lse2, segment_ids,  \
-                                                                   c.args, batch, heads, kv_heads, seq, head_dim)
+                                                                   (const int*)plan, c.args, batch, heads, kv_heads, seq, head_dim)
 #define SCORED_FWD(D, CAP, BIAS, SEG)            \
-  if (split) SCORED_FWD_(D, CAP, BIAS, SEG, 2);  \
+  if (blocks.row_split) SCORED_FWD_(D, CAP, BIAS, SEG, 2); \
   else SCORED_FWD_(D, CAP, BIAS, SEG, 1)
   SCORED_DISPATCH(SCORED_FWD, c, segment_ids != nullptr);
 #undef SCORED_FWD

@@ -44,9 +44,11 @@ SIGNATURES: dict[str, tuple] = {
     "gptrig_attn_bwd_workspace_bytes": (Z, [I, I, I, I]),
     "gptrig_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, P, F, P]),
     "gptrig_attn_bwd_rope": (I, [P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, P, F, P, P, P]),
-    "gptrig_scored_attn_fwd": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, F, F, P]),
+    "gptrig_scored_attn_plan_bytes": (Z, [I, I, I, I, I]),
+    "gptrig_scored_attn_plan": (I, [P, P, P, Z, I, I, I, I, I, P]),
+    "gptrig_scored_attn_fwd": (I, [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, F, F, P]),
     "gptrig_scored_attn_bwd_workspace_bytes": (Z, [I, I, I, I, I]),
-    "gptrig_scored_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P, F, F, P]),
+    "gptrig_scored_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, Z, I, I, I, I, I, P, F, F, P]),
     "gptrig_flce_fwd_workspace_bytes": (Z, [I, I, I]),
     "gptrig_flce_fwd": (I, [P, P, P, P, P, P, Z, I, I, I, I, P]),
     "gptrig_flce_fwd_noalloc": (I, [P, P, P, P, P, I, I, I, I, P]),

@@ -112,9 +112,14 @@ def _plain(*tensors: torch.Tensor) -> bool:
     return True
 
 
+@functools.lru_cache(maxsize=512)
+def _sizes(query: str, *sizes: int) -> int:
+    return _lib.query(query, *sizes)
+
+
 def _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale: float, cap: float, keep: bool):
     """The views read, ``o``, for the backward (``None`` unless ``keep``) what its rounding cut off and then the
-    logarithms of the scores' sums, in one buffer, and whether the views are plain."""
+    logarithms of the scores' sums, in one buffer, the plan if the call has one, and whether the views are plain."""
 
     B, H, S, D = q.shape
     if _plain(q, k, v):
@@ -129,10 +134,18 @@ def _forward(q, k, v, segment_ids, prefix_lengths, slopes, scale: float, cap: fl
         kept = torch.empty(rows * (D + 4), dtype=torch.uint8, device=q.device)
         low = kept.data_ptr()
         lse2 = low + rows * D
+    plan = None
+    if segment_ids is not None or prefix_lengths is not None:
+        sizes = (B, H, k.shape[1], S, D)
+        need = _sizes("gptrig_scored_attn_plan_bytes", *sizes)
+        if need:
+            plan = torch.empty(need, dtype=torch.uint8, device=q.device)
+            _lib.call_on(q.get_device(), "gptrig_scored_attn_plan", _lib.ptr(segment_ids), _lib.ptr(prefix_lengths),
+                         plan.data_ptr(), need, *sizes)
     _lib.call_on(q.get_device(), "gptrig_scored_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), o.data_ptr(), low, lse2,
-                 B, H, k.shape[1], S, D, strides, scale, cap)
-    return q, k, v, o, kept, strides is None
+                 _lib.ptr(segment_ids), _lib.ptr(prefix_lengths), _lib.ptr(slopes), _lib.ptr(plan), o.data_ptr(),
+                 low, lse2, B, H, k.shape[1], S, D, strides, scale, cap)
+    return q, k, v, o, kept, plan, strides is None
 
 
 class _ScoredAttention(torch.autograd.Function):
@@ -148,13 +161,8 @@ class _ScoredAttention(torch.autograd.Function):
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, do)
 
 
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(*sizes: int) -> int:
-    return _lib.query("gptrig_scored_attn_bwd_workspace_bytes", *sizes)
-
-
 def _backward(ctx, do):
-    q, k, v, o, kept, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
+    q, k, v, o, kept, plan, segment_ids, prefix_lengths, slopes = ctx.saved_tensors
     B, H, S, D = q.shape
     Hk = k.shape[1]
     if ctx.plain and _plain(do):
@@ -165,13 +173,13 @@ def _backward(ctx, do):
         dk = torch.empty((B, Hk, S, D), dtype=q.dtype, device=q.device)
         dv = torch.empty_like(dk)
         strides = _strides(q, k, v, o, do, dq, dk, dv)
-    size = _workspace_bytes(B, H, Hk, S, D)
+    size = _sizes("gptrig_scored_attn_bwd_workspace_bytes", B, H, Hk, S, D)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device)
     low = kept.data_ptr()
     _lib.call_on(q.get_device(), "gptrig_scored_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                  do.data_ptr(), low, low + B * H * S * D, _lib.ptr(segment_ids), _lib.ptr(prefix_lengths),
-                 _lib.ptr(slopes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size, B, H, Hk, S, D,
-                 strides, *ctx.scalars)
+                 _lib.ptr(slopes), _lib.ptr(plan), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size,
+                 B, H, Hk, S, D, strides, *ctx.scalars)
     return dq, dk, dv, None, None, None, None, None
 
 

@@ -101,16 +101,22 @@ int gptrig_attn_bwd_rope(const void* q, const void* k, const void* v, const void
  * Hidden pairs add nothing even where their values are infinite or NaN.
  * Results do not depend on the order of the workgroups (no atomics).
  * ---------------------------------------------------------------------- */
+/* The order of a call's blocks, the longest first, for calls with a prefix or segment
+ * ids; NULL as `plan` is the plain order, with the same results.  The forward and the
+ * backward of one call take the same plan.  plan_bytes 0: these sizes take none. */
+size_t gptrig_scored_attn_plan_bytes(int batch, int heads, int kv_heads, int seq, int head_dim);
+int gptrig_scored_attn_plan(const int32_t* segment_ids, const int32_t* prefix_lengths, void* plan, size_t plan_bytes,
+                            int batch, int heads, int kv_heads, int seq, int head_dim, void* stream);
 int gptrig_scored_attn_fwd(const void* q, const void* k, const void* v, const int32_t* segment_ids,
-                           const int32_t* prefix_lengths, const float* distance_slopes, void* o, void* o_low,
-                           float* lse2, int batch, int heads, int kv_heads, int seq, int head_dim,
+                           const int32_t* prefix_lengths, const float* distance_slopes, const void* plan,
+                           void* o, void* o_low, float* lse2, int batch, int heads, int kv_heads, int seq, int head_dim,
                            const int64_t* strides /* q,k,v,o */, float softmax_scale, float score_cap, void* stream);
 size_t gptrig_scored_attn_bwd_workspace_bytes(int batch, int heads, int kv_heads, int seq, int head_dim);
 int gptrig_scored_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
                            const void* o_low, const float* lse2, const int32_t* segment_ids, const int32_t* prefix_lengths,
-                           const float* distance_slopes, void* dq, void* dk, void* dv, void* workspace,
-                           size_t workspace_bytes, int batch, int heads, int kv_heads, int seq, int head_dim,
-                           const int64_t* strides /* q,k,v,o,dout,dq,dk,dv */, float softmax_scale, float score_cap,
+                           const float* distance_slopes, const void* plan, void* dq, void* dk, void* dv,
+                           void* workspace, size_t workspace_bytes, int batch, int heads, int kv_heads, int seq,
+                           int head_dim, const int64_t* strides /* q,k,v,o,dout,dq,dk,dv */, float softmax_scale, float score_cap,
                            void* stream);
 
 /* ------------------------------------------------------------------------

@@ -389,3 +389,37 @@ def test_partial_gradients_and_no_grad():
     with torch.no_grad():
         assert torch.equal(attend(20.0)(q, k, v), want["o"])
     assert torch.equal(attend(20.0)(q, k, v, torch.zeros((1, 130), dtype=torch.int64, device=DEV)), want["o"])
+
+
+@pytest.mark.parametrize("options", [dict(prefix=True), dict(seg=90, cap=20.0), dict(prefix=True, seg=150, slopes=True)],
+                         ids=lambda o: "-".join(o))
+def test_the_order_of_blocks_changes_nothing(options, monkeypatch):
+    from gptrig.kernels import scored_attention as module
+
+    print(f"scored attention, planned order {options}", flush=True)
+    B, H, S = 5, 12, 1000
+    o = resolve(options, B, H, S)
+    if "seg" in o:
+        o["seg"][1] = torch.randint(0, 4, (S,), device=DEV)  # (ids in no order)
+    tensors = inputs(B, H, 4, S, 64, seed=31)
+    assert module._sizes("gptrig_scored_attn_plan_bytes", B, H, 4, S, 64) > 0
+    got = compare(*tensors, **o)
+    leaves = [t.detach().clone().requires_grad_() for t in tensors[:3]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend(o.get("cap"))(*leaves, o.get("seg"), prefix_lengths=o.get("prefix"),
+                                   distance_slopes=o.get("slopes"))
+        again = dict(zip(("o", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, tensors[3]))))
+    for shift in range(3):
+        if "prefix" in o:
+            o["prefix"].copy_(torch.roll(o["prefix"], shift))
+        if "seg" in o:
+            o["seg"].copy_(torch.roll(o["seg"], shift, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        with monkeypatch.context() as m:
+            m.setattr(module, "_sizes", lambda name, *sizes: 0 if "plan" in name else module._lib.query(name, *sizes))
+            plain = run(*tensors, **o)
+        assert all(torch.equal(again[n].detach(), plain[n]) for n in plain), shift
+        if not shift:
+            assert all(torch.equal(got[n], plain[n]) for n in plain)

@@ -207,7 +207,7 @@ def test_scored_attention_entry_points_refuse_on_the_host():
     at, odd = ctypes.c_void_p(1 << 12), ctypes.c_void_p((1 << 12) + 8)
 
     def fwd(q=at, o=at, B=1, H=4, Hk=2, S=16, D=64, strides=None, scale=0.125, cap=0.0):
-        return lib.gptrig_scored_attn_fwd(q, at, at, None, None, None, o, None, None, B, H, Hk, S, D, strides, scale, cap, None)
+        return lib.gptrig_scored_attn_fwd(q, at, at, None, None, None, None, o, None, None, B, H, Hk, S, D, strides, scale, cap, None)
 
     assert fwd(q=None) == -1 and fwd(q=odd) == -2
     assert fwd(Hk=3) == -2 and fwd(Hk=0) == -2 and fwd(S=0) == -2 and fwd(B=-1) == -2
@@ -222,12 +222,18 @@ def test_scored_attention_entry_points_refuse_on_the_host():
         st = (ctypes.c_int64 * 12)(*[4096, 1024, 64] * 4)
         st[2] = change
         assert fwd(strides=st) == -2
+    assert lib.gptrig_scored_attn_plan_bytes(1, 4, 2, 16, 64) == 0
+    need = lib.gptrig_scored_attn_plan_bytes(4, 12, 12, 2000, 64)
+    assert need >= 2 * 4 * 16 * 4
+    plan = lib.gptrig_scored_attn_plan
+    assert plan(at, at, at, need, 1, 4, 2, 16, 64, None) == -2 and plan(at, at, None, need, 4, 12, 12, 2000, 64, None) == -1
+    assert plan(at, at, at, need - 1, 4, 12, 12, 2000, 64, None) == -6 and plan(at, at, odd, need, 4, 12, 12, 2000, 64, None) == -2
     big = ctypes.c_size_t(1 << 40)
     need = lib.gptrig_scored_attn_bwd_workspace_bytes(1, 4, 2, 16, 64)
     assert need >= 4 * 16 * 4
 
     def bwd(ws=at, size=big, lse=at, dv=at, low=at):
-        return lib.gptrig_scored_attn_bwd(at, at, at, at, at, low, lse, None, None, None, at, at, dv, ws, size, 1, 4, 2, 16, 64, None,
+        return lib.gptrig_scored_attn_bwd(at, at, at, at, at, low, lse, None, None, None, None, at, at, dv, ws, size, 1, 4, 2, 16, 64, None,
                                           0.125, 0.0, None)
 
     assert bwd(ws=None) == -1 and bwd(lse=None) == -1 and bwd(low=None) == -1 and bwd(low=odd) == -2 and bwd(dv=None) == -1

@@ -7,9 +7,15 @@
 //     of dq and dk as the rounding of dU does (0.9 and 1.7 in 1000 of dq's norm).
 //   dk, dv: a workgroup owns 128 keys of one kv head and walks the queries of
 //     every head of its group.
-// Both compute the scores and dP anew (3 and 4 products of the pair matrix
-// instead of 5 in one pass), which costs less than carrying dq across
-// workgroups through float32 atomics.
+// Both compute the scores and dP anew: 3 and 4 products of the pair matrix instead
+// of 5 in one pass that adds dq up in float32 atomics.  The causal attention of
+// attention.hip is such a pass: plain scores, B16 H12 S1024 D64 161 us against 168 for
+// the two here, B4 H16 S2048 D128 494 against 300, of other bits on every run.
+//
+// Bound by the issue of vector and matrix instructions, which overlap little at two
+// waves a SIMD.  B16 H12 S1024 D64, cap 30: dq 88 us (of a CU's busy time 73% vector,
+// 23% matrix instructions), dk and dv 104 us (56%, 25%; all of them 79%).  B4 H16/4
+// S2048 D128, cap and bias: 155 us (57%, 34%) and 200 us (43%, 34%; all of them 67%).
 //
 // A visible infinity or NaN in a tile that also holds hidden pairs makes the rows
 // of dq, or of dk and dv, that it reaches NaN throughout.
@@ -38,11 +44,15 @@ __device__ __forceinline__ void add(f32x16 (&acc)[DB], const float* at, int lane
 // The dq pass leaves two numbers a query for the other pass: the constant of its
 // exponents, cap log2 e - L_i (with a bias less slope (i mod 64), the part of the
 // bias that is the query's own in its tile), and -delta_i.
+//
+// At D = 64 without a bias the loop fits the 168 registers of three waves a SIMD, with
+// kt's transposed operands loaded only after the vector work: 89 us (B16 H12 S1024,
+// cap 30; ahead of it, at two waves, 104).  With a bias, two waves and the loads ahead.
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
     scored_dq_kernel(View Q, View K, View V, View O, View dO, const uint8_t* __restrict__ o_low,
-                     const float* __restrict__ lse2, const int32_t* __restrict__ seg, const int* __restrict__ plan, float* __restrict__ shifts, float* __restrict__ minus_delta,
-                     MutView dQ, ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
+                     const float* __restrict__ lse2, const int32_t* __restrict__ seg, const int* __restrict__ plan,
+                     float* __restrict__ shifts, float* __restrict__ minus_delta, MutView dQ, ScoreArgs a, int B, int H, int Hk, int S, int dim, float scale) {
   constexpr int KC = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(16))) bf16 fk0[kRows * D];
   __shared__ __attribute__((aligned(16))) bf16 fk1[kRows * D];
@@ -282,13 +292,14 @@ __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
 //
 // kSplit waves share 32 keys, each with its half of every tile.  At D = 128 the sums
 // of a wave are 128 registers: with k and v in registers too there is room for one
-// wave a SIMD, which waits for every product (B4 H16/4 S2048 capped and biased 265
-// us); so there 8 waves own 128 keys, two waves a SIMD, and k and v are in LDS.
+// wave a SIMD, which waits for every product; so where there are enough of them 8
+// waves own 128 keys, two waves a SIMD, and k and v are in LDS (B4 H16/4 S2048 capped
+// and biased, forward and backward: 535 us with one wave a SIMD, 497 with two).
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ shifts,
-                      const float* __restrict__ minus_delta, const int32_t* __restrict__ seg, const int* __restrict__ plan, MutView dK, MutView dV,
-                      float* __restrict__ partial, int parts, ScoreArgs a, int B, int H, int Hk, int S, int dim,
+                      const float* __restrict__ minus_delta, const int32_t* __restrict__ seg,
+                      const int* __restrict__ plan, MutView dK, MutView dV, float* __restrict__ partial, int parts, ScoreArgs a, int B, int H, int Hk, int S, int dim,
                       float scale) {
   constexpr int KC = D / 16, DB = D / 32, kGroups = kWaves / kSplit, kMine = 32 * kGroups;
   constexpr bool kKeysInLds = kWaves == 8;

@@ -300,7 +300,7 @@ struct ScoredCall {
 // slots, of uneven length at that, since it halves the longest.  us with 128 / 64
 // rows, capped, forward and backward: B1 H12 S1024 D64 (96 workgroups of 128) 24 / 15
 // and 67 / 43, B4 S2048 (768) 61 / 50 and 171 / 158, B16 S1024 (1536) 56 / 56 and 185 /
-// 188, B2 S8192 documents (1536) 171 / 151 and 516 / 480, B8 S4096 documents (3072) 193
+// 188, B2 S8192 documents (1536) 171 / 151 and 516 / 480, B8 S4096 documents (twice that) 193
 // / 227 and 644 / 792; D128 forward B2 S2048 (384) 60 / 45, B4 S2048 (768) 81 / 79, B16
 // S1024 (1536) 87 / 104.  D128 backward with the keys in 128 / 64: B1 S1024 (96) 69 / 63,
 // B2 S1024 (192) 75 / 71, B4 S1024 (384) 98 / 118, B4 S2048 (768) 264 / 327.

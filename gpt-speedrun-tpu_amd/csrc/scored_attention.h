@@ -298,14 +298,15 @@ struct ScoredCall {
 // Whether workgroups own 64 rows instead of 128, two waves to every 32 of them
 // (each with one half of every tile): where there are few workgroups for the CUs'
 // slots, of uneven length at that, since it halves the longest.  us with 128 / 64
-// rows, capped, forward and backward: B1 H12 S1024 D64 (96 workgroups of 128) 24 / 15
-// and 67 / 43, B4 S2048 (768) 61 / 50 and 171 / 158, B16 S1024 (1536) 56 / 56 and 185 /
-// 188, B2 S8192 documents (1536) 171 / 151 and 516 / 480, B8 S4096 documents (twice that) 193
-// / 227 and 644 / 792; D128 forward B2 S2048 (384) 60 / 45, B4 S2048 (768) 81 / 79, B16
-// S1024 (1536) 87 / 104.  D128 backward with the keys in 128 / 64: B1 S1024 (96) 69 / 63,
-// B2 S1024 (192) 75 / 71, B4 S1024 (384) 98 / 118, B4 S2048 (768) 264 / 327.
+// rows, 12 heads, capped, in brackets the workgroups of 128.  Rows of the forward and
+// of dq, forward and backward: D64 B4 S1024 (384) 29 / 23 and 84 / 81, B4 S2048 (768) 63
+// / 54 and 168 / 160, B8 S2048 (1536) 94 / 97 and 277 / 290, B2 S8192 documents (1536)
+// 157 / 163 and 366 / 390; D128 B4 S1024 35 / 32, B4 S2048 83 / 83, B8 S2048 142 / 156.
+// Keys of the backward: D64 B4 S1024 83 / 79, B4 S2048 166 / 160, B8 S2048 290 / 305;
+// D128 B1 S1024 (96) 69 / 63, B2 S1024 (192) 75 / 71, B4 S1024 102 / 119, B4 S2048 263 /
+// 312.
 inline bool split_rows(long long batch_heads, int seq, int dim, bool keys) {
-  const int most = dim <= 64 ? (keys ? 1024 : 1536) : (keys ? 192 : 768);
+  const int most = dim <= 64 ? 1024 : keys ? 192 : 768;
   return batch_heads * ceil_div(seq, 128) <= most;
 }
 

@@ -13,8 +13,8 @@
 // the two here, B4 H16 S2048 D128 494 against 300, of other bits on every run.
 //
 // Bound by the issue of vector and matrix instructions, which overlap little at two
-// waves a SIMD.  B16 H12 S1024 D64, cap 30: dq 88 us (of a CU's busy time 73% vector,
-// 23% matrix instructions), dk and dv 104 us (56%, 25%; all of them 79%).  B4 H16/4
+// waves a SIMD.  B16 H12 S1024 D64, cap 30: dq 88 us (of a CU's busy time 70% vector,
+// 24% matrix instructions), dk and dv 104 us (56%, 25%; all of them 79%).  B4 H16/4
 // S2048 D128, cap and bias: 155 us (57%, 34%) and 200 us (43%, 34%; all of them 67%).
 //
 // A visible infinity or NaN in a tile that also holds hidden pairs makes the rows

@@ -242,6 +242,15 @@ struct Columns {
   }
 };
 
+// c + the sum of x, two values an instruction.
+__device__ __forceinline__ float sum_of(const bf16x8 (&x)[2], float c) {
+  const bf16x2 ones = {(bf16)1.0f, (bf16)1.0f};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[i >> 2][2 * (i & 3)], x[i >> 2][2 * (i & 3) + 1]}, ones, c, false);
+  return c;
+}
+
 // ---------------------------------------------------------------------------
 // Host side: what every entry point checks, and the choice of a kernel
 // ---------------------------------------------------------------------------

@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
-  float m_run = kMinusBig, l_run = 0.f;
+  float m_run = kMinusBig, l_run = 0.f, r_run = 0.f;  // r: the sum of the rounded P
 
   const __amdgpu_buffer_rsrc_t k_rs = slice(K.row(b, hk, 0), S, K.ss, dim);
   const __amdgpu_buffer_rsrc_t v_rs = slice(V.row(b, hk, 0), S, V.ss, dim);
@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     if (__ballot(grow)) {
       const float alpha = fast_exp2(m_run - m_new);
       l_run *= alpha;
+      r_run *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
       pb[i >> 3][i & 7] = (bf16)p;
     }
     l_run += lsum;
+    r_run = sum_of(pb, r_run);
     vc.product(acc, pb);
   };
 
@@ -337,11 +339,12 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
   }
 
   if constexpr (kSplit == 2) {  // the second half's sums join the first's
-    __shared__ float ml[2][2][64];
+    __shared__ float ml[2][3][64];
     float* const at = reinterpret_cast<float*>(own ? fv0 : fk0);  // a tile's room is an accumulator's
     if (part) {
       ml[own][0][lane] = m_run;
       ml[own][1][lane] = l_run;
+      ml[own][2][lane] = r_run;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -353,12 +356,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
     const float f0 = fast_exp2(m_run - m), f1 = fast_exp2(m1 - m);
     m_run = m;
     l_run = l_run * f0 + ml[own][1][lane] * f1;
+    r_run = r_run * f0 + ml[own][2][lane] * f1;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[db][i] = acc[db][i] * f0 + at[(16 * db + i) * 64 + lane] * f1;
   }
-  const float l_tot = l_run + __shfl_xor(l_run, 32);
+  const float l_tot = l_run + __shfl_xor(l_run, 32), r_tot = r_run + __shfl_xor(r_run, 32);
   if (__ballot((plus | minus) != 0)) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -369,7 +373,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2)
       }
   }
   if (my_q < S) {
-    const float inv = 1.0f / l_tot;
+    // Over the sum of the P that the product took: their roundings weigh against each
+    // other instead of scaling o (of few visible keys one rounding is all of it).
+    const float inv = 1.0f / r_tot;
     bf16* orow = O.row(b, h, my_q);
     uint8_t* const low_row = o_low ? o_low + (((size_t)b * H + h) * S + my_q) * dim : nullptr;
 #pragma unroll

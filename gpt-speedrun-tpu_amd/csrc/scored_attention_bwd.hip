@@ -14,8 +14,8 @@
 //
 // Bound by the issue of vector and matrix instructions, which overlap little at two
 // waves a SIMD.  B16 H12 S1024 D64, cap 30: dq 88 us (of a CU's busy time 70% vector,
-// 24% matrix instructions), dk and dv 104 us (56%, 25%; all of them 79%).  B4 H16/4
-// S2048 D128, cap and bias: 155 us (57%, 34%) and 200 us (43%, 34%; all of them 67%).
+// 24% matrix instructions), dk and dv 109 us (56%, 25%; all of them 79%).  B4 H16/4
+// S2048 D128, cap and bias: 165 us (57%, 34%) and 209 us (43%, 34%; all of them 67%).
 //
 // A visible infinity or NaN in a tile that also holds hidden pairs makes the rows
 // of dq, or of dk and dv, that it reaches NaN throughout.

@@ -12,6 +12,7 @@ import os
 from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p, c_char_p
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgptrig.so")
 
@@ -207,6 +208,19 @@ def require_one_device(first: torch.Tensor, *others: torch.Tensor | None) -> Non
     require_device(first, *others)
     devices = sorted({str(t.device) for t in (first, *others) if t is not None})
     raise RuntimeError(f"the tensors lie on several devices: {devices}")
+
+
+def needs_autograd(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call has to go through its autograd function: an input asks for a gradient, or forward-mode
+    derivatives are on (``requires_grad`` does not show a tangent, and the function refuses one)."""
+
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def workspace(nbytes: int, device) -> torch.Tensor:

@@ -216,7 +216,7 @@ def make_scored_attention(config: ScoredAttentionConfig = ScoredAttentionConfig(
             raise ValueError(f"batch x heads x (seq / 64, rounded up) must be at most 2^22, got {tuple(q.shape)}")
         scale = q.shape[3] ** -0.5 if config.softmax_scale is None else config.softmax_scale
         call = (q, k, v, segment_ids, prefix_lengths, distance_slopes, float(scale), float(config.score_cap or 0.0))
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        if _lib.needs_autograd(q, k, v):
             return _ScoredAttention.apply(*call)
         return _forward(*call, False)[3]
 

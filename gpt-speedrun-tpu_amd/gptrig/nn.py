@@ -204,7 +204,7 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None =
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     _lib.require_one_device(x, scale, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or bias is not None and bias.requires_grad):
+    if _lib.needs_autograd(x, scale, bias):
         return _LayerNorm.apply(x, scale, bias, eps)
     return _layer_norm_forward(x, scale, bias, eps, False)[0]
 

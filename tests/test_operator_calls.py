@@ -1,0 +1,52 @@
+"""How ``layer_norm``, ``adamw_tensors`` and the scored attention treat a call before anything is launched: the
+launches are replaced by stand-ins on the CPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from gptrig import _lib, nn
+from gptrig.kernels import make_scored_attention, scored_attention
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    """Both operators on CPU tensors, their outputs copies of an input."""
+
+    monkeypatch.setattr(_lib, "require_one_device", lambda *tensors: None)
+    monkeypatch.setattr(nn, "_layer_norm_forward",
+                        lambda x, scale, bias, eps, keep: (x.clone(), x.clone(), scale.clone(), torch.zeros((2, 3))))
+    monkeypatch.setattr(scored_attention, "_forward",
+                        lambda q, k, v, *rest: (q, k, v, q.clone(), torch.zeros(8), None, True))
+
+
+def calls():
+    x, scale = torch.randn((3, 8)), torch.ones(8)
+    q = torch.randn((1, 2, 4, 8)).to(BF16)
+    return [(nn.layer_norm, [x, scale]), (nn.layer_norm, [x, scale, scale.clone()]),
+            (make_scored_attention(), [q, q.clone(), q.clone()])]
+
+
+@pytest.mark.parametrize("gradients", [True, False])
+def test_forward_derivatives_are_refused(no_launch, gradients):
+    """A tangent does not show in ``requires_grad``: without autograd's node the result would have none, a derivative
+    of zero.  ``rms_norm`` and the causal attention refuse it in the same way."""
+
+    for operator, tensors in calls():
+        for i in range(len(tensors)):
+            with forward_ad.dual_level(), torch.set_grad_enabled(gradients):
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    operator(*dual)
+
+
+def test_a_dual_level_without_tangents_changes_nothing(no_launch):
+    for operator, tensors in calls():
+        with forward_ad.dual_level():
+            assert torch.equal(operator(*tensors), tensors[0])
+        assert torch.equal(operator(*tensors), tensors[0])
+        assert operator(*(t.clone().requires_grad_() for t in tensors)).requires_grad

@@ -18,7 +18,10 @@
 // A v above zero keeps at least the smallest code, 2^-9: a v of zero beside a
 // momentum that is not would divide by eps alone.  A value that is infinite or NaN
 // becomes the NaN code and stays out of the scale, so it spoils no neighbour.
-// Blocks whose largest magnitude is below 2^-100 are kept as zeros.
+// Blocks of m whose largest magnitude is below 2^-100 are kept as zeros, and blocks of
+// v from 2^-117 down (v is a square; a scale below that is no normal float32).  So that
+// no step divides by eps alone, a v of such a block with a momentum counts as 2^-117
+// in the next step, and a new v of 0 as 2^-149: the most that was cut off.
 // Every product, sum and quotient up to a code is rounded to float32 on its own (no
 // fused ones): a value close to a tie goes to either of two codes 12% apart, so the
 // last bit decides a few codes of a million, and anyone who computes the formula in
@@ -42,7 +45,7 @@ constexpr int kMost = 48;      // tensors a launch: their table travels as a ker
 constexpr int kBlock = 256;    // values a scale
 constexpr int kUnroll = 4;     // blocks a wave has in flight (2: the same time, 8: 2% more, 12% with 8 bits)
 constexpr int kChunk = 4 * kUnroll * kBlock;  // values a workgroup
-constexpr float kTiny = 0x1p-100f;
+constexpr float kTinyM = 0x1p-100f, kTinyV = 0x1p-117f;
 
 struct Item {
   float* p;
@@ -160,13 +163,13 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
     top = finite[j] ? fmaxf(top, fabsf(x[j])) : top;
   }
   top = largest(top);
-  const bool none = top < kTiny;
+  const bool none = top < (kFloor ? kTinyV : kTinyM);
   scale = none ? 0.f : top * (1.0f / 448.0f);
   const float inv = none ? 0.f : 1.0f / scale;
   float code[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    // |x| / scale, correctly rounded.
+    // |x| / scale, correctly rounded (for a v below 2^-100 to the last bit or two).
     const float q = fabsf(x[j]) * inv, y = fminf(fmaf(fmaf(-q, scale, fabsf(x[j])), inv, q), 448.0f);
     uint32_t step = __builtin_bit_cast(uint32_t, y) & 0x7F800000u;
     step = (step < 0x3C800000u ? 0x3C800000u : step) - 0x01800000u;  // at least 2^-6, over 8
@@ -227,13 +230,16 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Scalars& k, f
     if constexpr (k8) {
       decode(mv[u], mc[u], ms[u]);
       decode(vv[u], vc[u], vs[u]);
+      if (vs[u] == 0.f)  // (the whole wave)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vv[u][j] = vv[u][j] == 0.f && mv[u][j] != 0.f ? kTinyV : vv[u][j];
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float gj = gv[u][j] * clip;
       const float m = k.b1 * mv[u][j] + k.omb1 * gj;
       const float v = k.b2 * vv[u][j] + k.omb2 * gj * gj;
-      const float vhat = v * k.ibc2;
+      const float vhat = (k8 && v == 0.f ? 0x1p-149f : v) * k.ibc2;
       const bool small = vhat < 1.0f;
       const float root = __builtin_amdgcn_sqrtf(vhat * (small ? 0x1p24f : 1.0f));
       const float step = (m * k.ibc1) * __builtin_amdgcn_rcpf(fmaf(root, small ? 0x1p-12f : 1.0f, eps));

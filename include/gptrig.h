@@ -407,7 +407,10 @@ int gptrig_adamw(float* param, const float* grad, float* m, float* v, void* para
  * [ceil(n / 256)]; a moment is code x scale, zeros to begin with).  8-bit moments
  * are rounded stochastically, from a hash of seed, the tensor's place in the
  * list and the element's in the tensor: give every step another seed.  An
- * infinite or NaN moment is kept as a NaN code.  grad_type of all gradients;
+ * infinite or NaN moment is kept as a NaN code; a block of m below 2^-100, or of v
+ * below 2^-117, as zeros, and such a v counts as 2^-117 beside a momentum (a new v
+ * that is 0 in float32 as 2^-149), so that no step divides by epsilon alone.
+ * grad_type of all gradients;
  * tensor_hparams f32 [count, 3] = {lr_mult, epsilon, decay} in device memory;
  * clip_scale a nullable device scalar.  Pointers aligned to their element; at
  * most 2^35 elements a tensor; GPTRIG_E_OVERLAP where an array that the call writes

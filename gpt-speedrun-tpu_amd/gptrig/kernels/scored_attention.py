@@ -29,6 +29,7 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 
 MAX_CAP = 1000.0  # float32 tells tanh scores of a larger cap apart less well than bfloat16 operands do
+MIN_CAP = 2.0 ** -126  # the kernels take the cap as a float32; one that this rounds to 0 would be none
 
 
 @dataclass(frozen=True)
@@ -41,8 +42,8 @@ class ScoredAttentionConfig:
     def __post_init__(self) -> None:
         if self.softmax_scale is not None and not 0.0 < self.softmax_scale < math.inf:
             raise ValueError(f"softmax_scale must be positive and finite, got {self.softmax_scale}")
-        if self.score_cap is not None and not 0.0 < self.score_cap <= MAX_CAP:
-            raise ValueError(f"score_cap must be in (0, {MAX_CAP:g}], got {self.score_cap}")
+        if self.score_cap is not None and not MIN_CAP <= self.score_cap <= MAX_CAP:
+            raise ValueError(f"score_cap must be in [2^-126, {MAX_CAP:g}], got {self.score_cap}")
 
 
 def _validate(q, k, v, segment_ids, prefix_lengths, distance_slopes) -> None:

@@ -50,3 +50,15 @@ def test_a_dual_level_without_tangents_changes_nothing(no_launch):
             assert torch.equal(operator(*tensors), tensors[0])
         assert torch.equal(operator(*tensors), tensors[0])
         assert operator(*(t.clone().requires_grad_() for t in tensors)).requires_grad
+
+
+def test_caps_that_float32_does_not_hold_are_refused():
+    """A cap reaches the kernels as float32, where 0 is no cap at all; below 2^-126 it loses bits, from 2^-150 down all."""
+
+    from gptrig.kernels import ScoredAttentionConfig
+
+    for bad in (5e-324, 1e-300, 2.0 ** -150, 7e-46, 1e-42, 2.0 ** -127):
+        with pytest.raises(ValueError, match="score_cap"):
+            ScoredAttentionConfig(score_cap=bad)
+    for cap in (2.0 ** -126, 1e-30, 0.01, 1000.0):
+        assert ScoredAttentionConfig(score_cap=cap).score_cap == cap

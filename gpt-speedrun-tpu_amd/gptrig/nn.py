@@ -10,7 +10,6 @@ rounding points.
 from __future__ import annotations
 
 import functools
-import math
 from typing import Any, Mapping
 
 import numpy as np
@@ -103,6 +102,7 @@ def rms_norm(x: torch.Tensor, scale: torch.Tensor, dtype: Any = BF16) -> torch.T
 
 
 _TYPES = {BF16: 0, torch.float32: 1}  # GPTRIG_TYPE_* of include/gptrig.h
+_LEAST_F32, _MOST_F32 = 2.0 ** -149, (2.0 - 2.0 ** -23) * 2.0 ** 127
 
 
 def _strided_rows(x: torch.Tensor) -> torch.Tensor:
@@ -201,8 +201,8 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None =
                          f"{None if bias is None else tuple(bias.shape)}")
     if width > 1 << 30 or x.numel() // width >= 1 << 31:
         raise ValueError(f"at most 2^30 wide and fewer than 2^31 rows, got {tuple(shape)}")
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if not (eps == 0 or _LEAST_F32 <= eps <= _MOST_F32):
+        raise ValueError(f"eps must be 0 or a positive float32, got {eps}")
     _lib.require_one_device(x, scale, bias)
     if _lib.needs_autograd(x, scale, bias):
         return _LayerNorm.apply(x, scale, bias, eps)

@@ -62,3 +62,15 @@ def test_caps_that_float32_does_not_hold_are_refused():
             ScoredAttentionConfig(score_cap=bad)
     for cap in (2.0 ** -126, 1e-30, 0.01, 1000.0):
         assert ScoredAttentionConfig(score_cap=cap).score_cap == cap
+
+
+def test_an_eps_that_float32_does_not_hold_is_refused(no_launch):
+    """It reaches the kernels as float32: one that this rounds to 0 would make a constant row 0 / 0, one that it
+    rounds to infinity every row 0."""
+
+    x, scale = torch.randn((3, 8)), torch.ones(8)
+    for bad in (1e-46, 5e-324, 2.0 ** -150, 3.5e38, 1e300):
+        with pytest.raises(ValueError, match="eps"):
+            nn.layer_norm(x, scale, eps=bad)
+    for eps in (0, 0.0, 2.0 ** -149, 1e-12, 1.0, 3e38):
+        assert torch.equal(nn.layer_norm(x, scale, eps=eps), x)

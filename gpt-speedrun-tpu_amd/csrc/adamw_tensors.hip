@@ -31,6 +31,9 @@
 // fractional bits of the golden ratio, sqrt 2 and sqrt 3:
 //   mix(x): x ^= x >> 16; x *= R2; x ^= x >> 15; x *= R3; x ^= x >> 16
 //   h = mix(i PHI + mix(mix(seed) + tensor PHI) + (i >> 32) R3)
+// A captured graph replays the same scalars, so a seed among them would give every
+// replay the same u: an element would then stand still or decay for good, as without
+// any.  There the seed is read from device memory.
 #include "common.h"
 
 #include <math.h>
@@ -271,7 +274,9 @@ __device__ __forceinline__ void update_chunk(const Item& it, const Scalars& k, f
 
 template <typename G, bool k8>
 __global__ void __launch_bounds__(256) adamw_tensors_kernel(Items items, Scalars k, const float* __restrict__ hparams,
-                                                            const float* __restrict__ clip_scale) {
+                                                            const float* __restrict__ clip_scale,
+                                                            const int64_t* __restrict__ seed) {
+  if (k8 && seed) k.seed = mix((uint32_t)*seed);
   // The tensor of this workgroup: the last whose first workgroup is not after it.
   int lo = 0, hi = items.count - 1;
   while (lo < hi) {
@@ -326,13 +331,10 @@ int check_written(const gptrig_adamw_tensor* tensors, int count, bool k8, size_t
   return status;
 }
 
-}  // namespace
-
-extern "C" {
-
-int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
-                         const float* tensor_hparams, double lr, double beta1, double beta2, int step,
-                         const float* clip_scale, uint32_t seed, void* stream) {
+// seed_at: the seed in device memory, or null for `seed`.
+int update(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits, const float* tensor_hparams,
+           double lr, double beta1, double beta2, int step, const float* clip_scale, uint32_t seed,
+           const int64_t* seed_at, void* stream) {
   if (count < 0 || step <= 0 || !(beta1 >= 0. && beta1 < 1.) || !(beta2 >= 0. && beta2 < 1.)) return GPTRIG_E_SHAPE;
   if (grad_type != GPTRIG_TYPE_BF16 && grad_type != GPTRIG_TYPE_F32) return GPTRIG_E_DTYPE;
   if (state_bits != 8 && state_bits != 32) return GPTRIG_E_UNSUPPORTED;
@@ -377,15 +379,35 @@ int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad
     if (blocks == 0) continue;
     const unsigned grid = (unsigned)blocks;
     if (grad_type == GPTRIG_TYPE_F32) {
-      if (k8) adamw_tensors_kernel<float, true><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale);
-      else adamw_tensors_kernel<float, false><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale);
+      if (k8) adamw_tensors_kernel<float, true><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale, seed_at);
+      else adamw_tensors_kernel<float, false><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale, seed_at);
     } else {
-      if (k8) adamw_tensors_kernel<bf16, true><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale);
-      else adamw_tensors_kernel<bf16, false><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale);
+      if (k8) adamw_tensors_kernel<bf16, true><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale, seed_at);
+      else adamw_tensors_kernel<bf16, false><<<grid, 256, 0, s>>>(items, k, tensor_hparams, clip_scale, seed_at);
     }
     GPTRIG_CHECK_LAUNCH();
   }
   return GPTRIG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
+                         const float* tensor_hparams, double lr, double beta1, double beta2, int step,
+                         const float* clip_scale, uint32_t seed, void* stream) {
+  return update(tensors, count, grad_type, state_bits, tensor_hparams, lr, beta1, beta2, step, clip_scale, seed, nullptr,
+                stream);
+}
+
+int gptrig_adamw_tensors_device_seed(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
+                                     const float* tensor_hparams, double lr, double beta1, double beta2, int step,
+                                     const float* clip_scale, const int64_t* seed, void* stream) {
+  if (!seed) return GPTRIG_E_NULL;
+  if ((uintptr_t)seed & 7) return GPTRIG_E_SHAPE;
+  return update(tensors, count, grad_type, state_bits, tensor_hparams, lr, beta1, beta2, step, clip_scale, 0, seed,
+                stream);
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@ from __future__ import annotations
 import array
 import math
 import operator
+import warnings
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -162,7 +163,7 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                   exp_avg_sq: Sequence[torch.Tensor], hparams: torch.Tensor, *, lr: float, beta1: float, beta2: float,
                   step: int, exp_avg_scale: Sequence[torch.Tensor] | None = None,
                   exp_avg_sq_scale: Sequence[torch.Tensor] | None = None, clip_scale: torch.Tensor | None = None,
-                  shadow: Sequence[torch.Tensor] | None = None, seed: int | None = None) -> None:
+                  shadow: Sequence[torch.Tensor] | None = None, seed: int | torch.Tensor | None = None) -> None:
     """One AdamW step, in place, over a list of contiguous float32 tensors.
 
     The update of ``GPTTrainer`` (``recipes/reference/train.py:1386-1445``), in a
@@ -175,8 +176,11 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``step``), which every step needs another of; the same call gives the same
     result.  ``clip_scale``: a float32 scalar on the device that multiplies the
     gradients.  ``shadow``: bfloat16 tensors that receive the rounded parameters.
-    A tensor that is written may overlap no other.  ``lr``, ``step`` and ``seed`` are
-    fixed in a captured graph.
+    A tensor that is written may overlap no other.  ``lr``, ``step`` and a ``seed``
+    that is a number are fixed in a captured graph: its replays would round 8-bit moments
+    the same way each time, so that some elements stand still and others decay for good.
+    For a graph give ``seed`` as an int64 scalar on the device (its lower 32 bits count)
+    that every replay finds changed, by ``seed.add_(1)`` in the graph or between replays.
     """
 
     if not params:
@@ -206,10 +210,18 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         raise ValueError(f"beta1 and beta2 must be in [0, 1), got {beta1} and {beta2}")
     if not 1 <= step < 2 ** 31:
         raise ValueError(f"step counts from 1 and stays below 2^31, got {step}")
-    seed = step % 2 ** 32 if seed is None else seed
-    if not 0 <= seed < 2 ** 32:
-        raise ValueError(f"seed must be in [0, 2^32), got {seed}")
-    _lib.require_one_device(params[0], hparams, clip_scale)
+    on_device = isinstance(seed, torch.Tensor)
+    if on_device:
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError("a seed on the device must be one int64 value")
+    else:
+        seed = step % 2 ** 32 if seed is None else seed
+        if not 0 <= seed < 2 ** 32:
+            raise ValueError(f"seed must be in [0, 2^32), got {seed}")
+    _lib.require_one_device(params[0], hparams, clip_scale, seed if on_device else None)
+    if bits == 8 and not on_device and torch.cuda.is_current_stream_capturing():
+        warnings.warn("adamw_tensors captured with 8-bit moments and a seed that is a number: every replay rounds them "
+                      "the same way; give the seed as an int64 tensor that changes between replays", stacklevel=2)
     # One row of gptrig_adamw_tensor a tensor: seven addresses and the count.
     table = [0] * (8 * len(params))
     for column, tensors in enumerate((params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, shadow)):
@@ -218,9 +230,10 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     table[7::8] = counts
     table = array.array("q", table)
     try:
-        _lib.call_on(device, "gptrig_adamw_tensors", table.buffer_info()[0], len(params),
-                     1 if grad_type == torch.float32 else 0, bits, hparams.data_ptr(), float(lr), float(beta1),
-                     float(beta2), int(step), _lib.ptr(clip_scale), seed)
+        _lib.call_on(device, "gptrig_adamw_tensors_device_seed" if on_device else "gptrig_adamw_tensors",
+                     table.buffer_info()[0], len(params), 1 if grad_type == torch.float32 else 0, bits,
+                     hparams.data_ptr(), float(lr), float(beta1), float(beta2), int(step), _lib.ptr(clip_scale),
+                     seed.data_ptr() if on_device else seed)
     except _lib.StatusError as error:
         if error.status == E_OVERLAP:
             raise ValueError("a tensor that the step writes overlaps another") from error

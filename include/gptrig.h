@@ -428,6 +428,11 @@ typedef struct {
 int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
                          const float* tensor_hparams, double lr, double beta1, double beta2, int step,
                          const float* clip_scale, uint32_t seed, void* stream);
+/* The same with the seed in device memory (its lower 32 bits), read by the kernels: for
+ * captured graphs, whose replays repeat a host seed, and with it the same roundings. */
+int gptrig_adamw_tensors_device_seed(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
+                                     const float* tensor_hparams, double lr, double beta1, double beta2, int step,
+                                     const float* clip_scale, const int64_t* seed, void* stream);
 /* Per-chunk sums of squares of an f32 arena (for clipping before the update). */
 int gptrig_sq_norm_partials(const float* x, int64_t n_chunks, int chunk, float* partials, void* stream);
 /* norm = sqrt(sum partials); clip = min(1, grad_clip/(norm+1e-6)) (1 if grad_clip <= 0);

@@ -74,3 +74,25 @@ def test_an_eps_that_float32_does_not_hold_is_refused(no_launch):
             nn.layer_norm(x, scale, eps=bad)
     for eps in (0, 0.0, 2.0 ** -149, 1e-12, 1.0, 3e38):
         assert torch.equal(nn.layer_norm(x, scale, eps=eps), x)
+
+
+def test_a_seed_on_the_device_is_checked():
+    import ctypes
+
+    from gptrig.optim import adamw_tensors, adamw_tensors_state
+
+    p = [torch.zeros(300)]
+    call = dict(params=p, grads=[torch.zeros(300)], hparams=torch.zeros((1, 3)), lr=0.1, beta1=0.9, beta2=0.95, step=1,
+                **adamw_tensors_state(p, 8))
+    for bad in (torch.zeros((), dtype=torch.int32), torch.zeros(2, dtype=torch.int64), torch.zeros(()),
+                torch.zeros(0, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="one int64"):
+            adamw_tensors(**call, seed=bad)
+    with pytest.raises(RuntimeError, match="GPU"):
+        adamw_tensors(**call, seed=torch.zeros((), dtype=torch.int64))
+    entry, at = _lib.lib().gptrig_adamw_tensors_device_seed, ctypes.c_void_p(1 << 12)
+    row = (ctypes.c_int64 * 8)(*[k << 20 for k in range(1, 8)], 100)
+    assert entry(row, 1, 1, 8, at, 0.1, 0.9, 0.95, 1, None, None, None) == -1
+    assert entry(row, 1, 1, 8, at, 0.1, 0.9, 0.95, 1, None, ctypes.c_void_p((1 << 12) + 4), None) == -2
+    assert entry(row, 1, 1, 16, at, 0.1, 0.9, 0.95, 1, None, at, None) == -4
+    assert entry(row, 0, 1, 8, at, 0.1, 0.9, 0.95, 1, None, at, None) == 0

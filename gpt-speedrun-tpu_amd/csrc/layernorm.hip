@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict_
   }
 }
 
-// Rows wider than the registers of a workgroup: three passes over the row, the
-// later two from the caches.
+// Rows of more than 1024 pieces (bf16 from 8193 columns on, float32 from 4097: a
+// workgroup of 4 pieces a lane, though 8 of float32 would be no more values than 4 of
+// bf16): three passes over the row, the later two from the caches.
 template <typename T, typename P>
 __global__ void __launch_bounds__(256) layernorm_fwd_wide_kernel(const T* __restrict__ x, int64_t ldx,
                                                                  const P* __restrict__ scale,

@@ -89,8 +89,8 @@ __device__ __forceinline__ Piece<T, V> piece(const T* row, int at) {
 
 // ---------------------------------------------------------------------------
 // Forward: L lanes hold a row, C pieces of V = 16 bytes each, so x is read once.
-// Bound by HBM: 65536 x 768 bf16 (201 MB in and out) 38 us, 5.3 TB/s, the rate of a
-// large copy.
+// Bound by HBM: 65536 x 768 bf16 (201 MB in and out) on inputs that change between
+// launches 38 us, 5.3 TB/s, the rate of a large copy.
 // ---------------------------------------------------------------------------
 template <typename T, typename P, int L, int C, bool kEven>
 __global__ void __launch_bounds__(256) layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx,
@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(256) layernorm_fwd_wide_kernel(const T* __rest
 // the gradients are the same on every run).
 // ---------------------------------------------------------------------------
 // The next row's pieces are on their way while this row is summed.  Bound by HBM:
-// 65536 x 768 bf16 (302 MB) 54 us, 5.6 TB/s (without the row ahead 88 us); the columns
-// kernel 4 us.
+// 65536 x 768 bf16 (302 MB), as above, 54 us, 5.6 TB/s (without the row ahead 88 us);
+// the columns kernel 4 us.
 template <typename T, typename P, int L, int C, bool kEven>
 __global__ void __launch_bounds__(256)
     layernorm_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
@@ -389,6 +389,12 @@ __global__ void __launch_bounds__(256) layernorm_columns_kernel(const float* __r
 // pieces, then 64, then a workgroup of up to 4; {0, 0} for wider rows, and for rows
 // of less than a piece.  (Width 768 bf16, forward: 3 pieces of 32 lanes 38 us, 2 of
 // 64, a quarter of which are idle, 43; the backward 54 with either.)
+// Never fewer than 32 lanes, so most of them idle on rows of a few pieces.  TB/s of
+// forward / backward at 2^25 values in a loop on the same inputs (part of them in the
+// last cache): bf16 16 columns 0.6 / 0.5, 64 2.3 / 2.0, 128 3.9 / 3.6, 256 to 2048 5.6 to
+// 6.1 / 4.6 to 5.6, 4096 5.5 / 4.7, 8192 5.2 / 3.6, wider (bytes that the backward's
+// second reading adds not counted) 3.5 / 2.1; float32 64 3.4 / 3.4, 256 to 4096 5.2 to 5.9
+// / 4.6 to 5.2, 8192 3.6 / 2.6.
 struct Shape {
   int lanes, pieces;
 };
@@ -402,7 +408,7 @@ Shape row_shape(int d, int v) {
 }
 
 // Partial rows at most: two workgroups a CU.  Backward and columns of 65536 x 768 with
-// 256 / 512 / 1024: 59 / 58 / 65 us.
+// 256 / 512 / 1024: 59 / 58 / 65 us (other counts were timed at this width only).
 constexpr int kParts = 512;
 
 int parts_of(int64_t rows, int d, int v) {

@@ -80,7 +80,8 @@ __device__ __forceinline__ bf16x8 tile_row(const at64::lds_t* t, int row, int c1
 // swizzle of a row depends on it modulo 16, so these few stand for every row block,
 // column block and tile, which are constants of the instructions.  (Computed where
 // they were used, 25 to 45 vector operations for 32 x 32 pairs: dk and dv 112 us
-// instead of 104 at B16 H12 S1024 D64 with a cap, with the loads ahead of their use.)
+// instead of 104 at B16 H12 S1024 D64 with a cap, with the loads ahead of their use; the
+// two in one run, on inputs that change between launches.)
 struct Lanes {
   uint32_t row[4];           // chunk 2 kc + half-wave of row lane % 32
   uint32_t low[2], high[2];  // transposed: the slots' first and second four rows, column blocks 0 and 1

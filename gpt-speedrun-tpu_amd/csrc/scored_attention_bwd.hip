@@ -9,13 +9,14 @@
 //     every head of its group.
 // Both compute the scores and dP anew: 3 and 4 products of the pair matrix instead
 // of 5 in one pass that adds dq up in float32 atomics.  The causal attention of
-// attention.hip is such a pass: plain scores, B16 H12 S1024 D64 161 us against 168 for
-// the two here, B4 H16 S2048 D128 494 against 300, of other bits on every run.
+// attention.hip is such a pass: plain scores, B16 H12 S1024 D64 148 us against 136 for
+// the two here, B4 H16 S2048 D128 495 against 293, of other bits on every run.
 //
 // Bound by the issue of vector and matrix instructions, which overlap little at two
-// waves a SIMD.  B16 H12 S1024 D64, cap 30: dq 88 us (of a CU's busy time 70% vector,
-// 24% matrix instructions), dk and dv 109 us (56%, 25%; all of them 79%).  B4 H16/4
-// S2048 D128, cap and bias: 165 us (57%, 34%) and 209 us (43%, 34%; all of them 67%).
+// waves a SIMD.  In a loop of passes on the same inputs, B16 H12 S1024 D64, cap 30: dq
+// 75 us (of a CU's busy time 70% vector, 24% matrix instructions), dk and dv 93 us (56%,
+// 25%; all of them 79%).  B4 H16/4 S2048 D128, cap and bias: 140 us (57%, 34%) and 174
+// us (43%, 34%; all of them 67%), and 14 for the join.
 //
 // A visible infinity or NaN in a tile that also holds hidden pairs makes the rows
 // of dq, or of dk and dv, that it reaches NaN throughout.
@@ -46,8 +47,9 @@ __device__ __forceinline__ void add(f32x16 (&acc)[DB], const float* at, int lane
 // bias that is the query's own in its tile), and -delta_i.
 //
 // At D = 64 without a bias the loop fits the 168 registers of three waves a SIMD, with
-// kt's transposed operands loaded only after the vector work: 89 us (B16 H12 S1024,
-// cap 30; ahead of it, at two waves, 104).  With a bias, two waves and the loads ahead.
+// kt's transposed operands loaded only after the vector work: B16 H12 S1024, cap 30, 89
+// us against 104 with the loads ahead of it at two waves (the two in one run, on inputs
+// that change between launches).  With a bias, two waves and the loads ahead.
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit>
 __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
     scored_dq_kernel(View Q, View K, View V, View O, View dO, const uint8_t* __restrict__ o_low,
@@ -294,7 +296,8 @@ __global__ void __launch_bounds__(256, D == 64 && !kBias ? 3 : 2)
 // of a wave are 128 registers: with k and v in registers too there is room for one
 // wave a SIMD, which waits for every product; so where there are enough of them 8
 // waves own 128 keys, two waves a SIMD, and k and v are in LDS (B4 H16/4 S2048 capped
-// and biased, forward and backward: 535 us with one wave a SIMD, 497 with two).
+// and biased, forward and backward: 535 us with one wave a SIMD, 497 with two, when
+// this was chosen; 451 with the later steps).
 template <int D, bool kCap, bool kBias, bool kSeg, int kSplit, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves, D == 64 || kWaves == 8 ? 2 : 1)
     scored_dkv_kernel(View Q, View K, View V, View dO, const float* __restrict__ shifts,

@@ -6,11 +6,11 @@
 //
 // Bound by vector operations, not by the products: a pair of the capped score costs
 // two exponentials, a reciprocal and six or seven others against 4 D operations of the matrix
-// cores.  B16 H12 S1024 D64, cap 30: 75 us, of a CU's busy time 76% vector and 19%
-// matrix instructions, and 18% of the time without work at the start and the end (four
-// waves a SIMD instead of three take as long);
-// B4 H16/4 S2048 D128, cap and bias: 148 us (65% and 24%; two waves a SIMD).  At D =
-// 64 three workgroups share a CU (168 registers).
+// cores.  Times of the kernel alone, in a loop of passes on the same inputs: B16 H12
+// S1024 D64, cap 30: 63 us, of a CU's busy time 76% vector and 19% matrix
+// instructions, and 18% of the time without work at the start and the end (four waves a
+// SIMD instead of three take as long); B4 H16/4 S2048 D128, cap and bias: 123 us (65%
+// and 24%; two waves a SIMD).  At D = 64 three workgroups share a CU (168 registers).
 #include "scored_attention.h"
 
 namespace {

@@ -92,6 +92,9 @@ SIGNATURES: dict[str, tuple] = {
     "gptrig_bias_rope_fwd": (I, [P, L, I, I, P, I, I, I, P, P, P]),
     "gptrig_embedding_fwd": (I, [P, P, P, I, I, I, P]),
     "gptrig_embedding_bwd": (I, [P, P, P, I, I, I, P]),
+    "gptrig_scaled_embedding_fwd": (I, [P, I, P, L, I, P, I, L, I, I, F, P]),
+    "gptrig_scaled_embedding_bwd_workspace_bytes": (Z, [L, I, I]),
+    "gptrig_scaled_embedding_bwd": (I, [P, I, P, L, I, P, I, L, I, I, F, P, Z, P]),
     "gptrig_adamw": (I, [P, P, P, P, P, P, P, L, I, F, F, F, I, P, P, P]),
     "gptrig_adamw_tensors": (I, [P, I, I, I, P, N, N, N, I, P, U, P]),
     "gptrig_adamw_tensors_device_seed": (I, [P, I, I, I, P, N, N, N, I, P, P, P]),

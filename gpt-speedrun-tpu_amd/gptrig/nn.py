@@ -209,6 +209,84 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None =
     return _layer_norm_forward(x, scale, bias, eps, False)[0]
 
 
+@functools.lru_cache(maxsize=256)
+def _embedding_workspace_bytes(tokens: int, width: int, vocab: int) -> int:
+    return _lib.query("gptrig_scaled_embedding_bwd_workspace_bytes", tokens, width, vocab)
+
+
+def _embedding_forward(tokens, table, scale: float, dtype):
+    """``y``, and the tokens as the kernels read them."""
+
+    tokens = tokens.contiguous()
+    if table.stride(1) != 1 and table.shape[1] != 1:
+        table = table.contiguous()
+    vocab, width = table.shape
+    y = torch.empty((*tokens.shape, width), dtype=dtype, device=table.device)
+    if tokens.numel():
+        _lib.call_on(table.get_device(), "gptrig_scaled_embedding_fwd", tokens.data_ptr(),
+                     int(tokens.dtype == torch.int64), table.data_ptr(), table.stride(0), _TYPES[table.dtype],
+                     y.data_ptr(), _TYPES[dtype], tokens.numel(), width, vocab, scale)
+    return y, tokens
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens, scale, dtype):
+        y, tokens = _embedding_forward(tokens, table, scale, dtype)
+        ctx.save_for_backward(tokens)
+        ctx.meta = (table.shape, table.dtype, scale)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        return (_embedding_backward_once if torch.is_grad_enabled() else _embedding_backward)(ctx, dy)
+
+
+def _embedding_backward(ctx, dy):
+    (tokens,) = ctx.saved_tensors
+    (vocab, width), kind, scale = ctx.meta
+    n, dev = tokens.numel(), dy.device
+    dtable = torch.empty((vocab, width), dtype=kind, device=dev)
+    dy2 = _strided_rows(dy) if n else dy
+    size = _embedding_workspace_bytes(n, width, vocab)
+    ws = _lib.workspace(size, dev)
+    _lib.call_on(dev.index, "gptrig_scaled_embedding_bwd", tokens.data_ptr(), int(tokens.dtype == torch.int64),
+                 dy2.data_ptr(), dy2.stride(0) if n else width, _TYPES[dy.dtype], dtable.data_ptr(), _TYPES[kind], n,
+                 width, vocab, scale, ws.data_ptr(), size)
+    return dtable, None, None, None
+
+
+_embedding_backward_once = once_differentiable(_embedding_backward)
+
+
+def embedding(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, dtype: Any = BF16) -> torch.Tensor:
+    """``scale * table[tokens]`` in ``dtype``: the product in float32, rounded once.
+
+    ``tokens``: int32 or int64 of any shape; a token outside ``[0, vocab)``, such
+    as -1 for padding, gives a row of zeros and takes no part in the gradient.
+    ``table``: float32 or bfloat16 ``[vocab, width]``, any row stride; ``dtype``:
+    bfloat16 or float32.  Differentiable once in ``table``: the gradient has its
+    shape and type, each row the float32 sum of its tokens' gradients in a fixed
+    order, so that the same call gives the same bits.
+    """
+
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    if table.dtype not in _TYPES or dtype not in _TYPES:
+        raise TypeError(f"the HIP embedding takes and gives bfloat16 or float32, got {table.dtype} and {dtype}")
+    if table.ndim != 2 or not table.shape[0] or not table.shape[1]:
+        raise ValueError(f"table must be [vocab, width], got {tuple(table.shape)}")
+    if table.shape[0] >= 2 ** 31 - 1 or table.shape[1] > 1 << 24 or tokens.numel() >= 2 ** 31 - 65536:
+        raise ValueError(f"at most 2^31 - 2 rows of 2^24 columns and fewer than 2^31 - 65536 tokens, got "
+                         f"{tuple(table.shape)} and {tuple(tokens.shape)}")
+    if not -_MOST_F32 <= scale <= _MOST_F32:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
+    _lib.require_one_device(table, tokens)
+    if _lib.needs_autograd(table):
+        return _Embedding.apply(table, tokens, scale, dtype)
+    return _embedding_forward(tokens, table, scale, dtype)[0]
+
+
 _ROPE_TABLES: dict = {}
 
 

@@ -387,6 +387,27 @@ int gptrig_embedding_bwd(const int32_t* tokens, const void* dout, float* dtable,
                          void* stream);
 
 /* ------------------------------------------------------------------------
+ * Token embedding with a scale, and its gradient in a fixed order (no counterpart
+ * in the reference, whose scatter is the pair above): y[i] = scale *
+ * table[tokens[i]], a row of zeros where the token is outside [0, vocab);
+ * dtable[v] = scale * sum of dy[i] over the i with tokens[i] = v, in float32 and
+ * in an order that the arguments fix, rows without a token zeros.  All of dtable
+ * is written.  tokens i32 or i64 [n]; table, y, dy, dtable of the types given,
+ * [vocab, d] and [n, d]; table with row stride ldt and dy with lddy (any; 0
+ * repeats a row), y and dtable contiguous.  Pointers aligned to their element, n
+ * below 2^31 - 65536 (0 allowed), d at most 2^24, vocab below 2^31 - 1.  The
+ * backward takes gptrig_scaled_embedding_bwd_workspace_bytes of workspace, 16-byte
+ * aligned.
+ * ---------------------------------------------------------------------- */
+int gptrig_scaled_embedding_fwd(const void* tokens, int tokens_are_int64, const void* table, int64_t ldt,
+                                int table_type, void* y, int y_type, int64_t n, int d, int vocab, float scale,
+                                void* stream);
+size_t gptrig_scaled_embedding_bwd_workspace_bytes(int64_t n, int d, int vocab);
+int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const void* dy, int64_t lddy, int dy_type,
+                                void* dtable, int table_type, int64_t n, int d, int vocab, float scale,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * AdamW over one flat f32 arena: recipes/reference/train.py:1386-1445
  * (_apply_training_update), with the per-tensor multipliers of
  * optimizer_hyperparameter_trees (:1274-1333) and the decay mask of

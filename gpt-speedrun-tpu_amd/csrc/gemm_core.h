@@ -69,10 +69,15 @@ typedef const __attribute__((address_space(1))) bf16x8 gbl_x8;
 // column blocks of 32 stored one after another, each as blk rows of 64 bytes
 // (so a 32-deep K-major stage, or the rows of an MN-major stage, read whole
 // contiguous runs instead of 64-byte pieces of longer rows).
+// pair (read by the kPair forms only): the operand is two matrices side by side,
+// the second `pair` elements after the first, whose rows (K-major) or columns
+// (MN-major) take turns in the tile in blocks of 32: row m of the operand is row
+// 32 (m / 64) + m % 32 of the first (m / 32 even) or the second matrix.
 struct Operand {
   const bf16* p;
   int64_t ld;
   int64_t blk = 0;
+  int64_t pair = 0;
 };
 
 __device__ __forceinline__ lds_t* lds_cast(bf16* p) { return (lds_t*)p; }
@@ -113,8 +118,13 @@ constexpr uint32_t kOffZero = 0xFFFFFFF0u;    // past the range: the copy reads 
 // lane's offset reaches 448 blk bytes and the rows of one stage.
 constexpr int kMaxBlk = (int)((kRsrcRange - 4096u) / 448u);
 
-template <bool KMAJOR>
+template <bool KMAJOR, bool kPair = false>
 __device__ __forceinline__ Src make_src(Operand op, int mn0, int k_begin, int MN, int k_end, int wave, int lane) {
+  static_assert(!(KMAJOR && kPair), "paired operands are MN-major");
+  if (kPair) {  // rows of one of the two matrices
+    mn0 >>= 1;
+    MN >>= 1;
+  }
   Src s;
   // (k_begin is a multiple of BK = 32 and mn0 of 256, so blocked stages and
   // tiles start on a 32-block.)
@@ -137,9 +147,13 @@ __device__ __forceinline__ Src make_src(Operand op, int mn0, int k_begin, int MN
     } else {
       const int row = blk * 2 + (lane >> 5);
       const int c = (lane & 31) ^ (4 * (row & 3));
-      const int m = mn0 + 8 * c;
-      s.off[j] = 2u * (uint32_t)(op.blk ? ((int64_t)(c >> 2) * op.blk + row) * 32 + 8 * (c & 3)
-                                        : (int64_t)row * op.ld + 8 * c);
+      const int at = kPair ? 32 * (c >> 3) + 8 * (c & 3) : 8 * c;  // column of the matrix the chunk comes from
+      const int m = mn0 + at;
+      if (kPair)
+        s.off[j] = 2u * (uint32_t)((int64_t)row * op.ld + at + ((c >> 2) & 1 ? op.pair : 0));
+      else
+        s.off[j] = 2u * (uint32_t)(op.blk ? ((int64_t)(c >> 2) * op.blk + row) * 32 + 8 * (c & 3)
+                                          : (int64_t)row * op.ld + 8 * c);
       const int rem = k_end - k_begin - row;
       s.nvalid[j] = (m < MN && rem > 0) ? (rem + BK - 1) / BK : 0;
     }
@@ -161,8 +175,9 @@ __device__ __forceinline__ void issue(lds_t* slab, const Src& s, int kt, int wav
 // MFMA operand (8 k-values) for rows r0 .. r0+31 at k-chunk kc (0 or 1) of a slab.
 // K-major slabs: the lane reads row r0 + lrow (lrow = lane & 31 unless the
 // caller permutes the rows of the block; accumulator row m then belongs to the
-// slab row that lane m read).
-template <bool KMAJOR>
+// slab row that lane m read).  MN-major slabs: kContiguous takes the block's
+// columns four at a time in contiguous_row's order.
+template <bool KMAJOR, bool kContiguous = false>
 __device__ __forceinline__ bf16x8 frag(const lds_t* slab, int r0, int kc, int lane, int lrow) {
   const int hl = lane >> 5;
   if (KMAJOR) {
@@ -171,7 +186,9 @@ __device__ __forceinline__ bf16x8 frag(const lds_t* slab, int r0, int kc, int la
     return *(const lds_x8*)(slab + row * BK + 8 * (c ^ ((row >> 2) & 3)));
   } else {
     const int cq = lane & 15;
-    const int m = r0 + 16 * ((lane >> 4) & 1) + 4 * (cq & 3);
+    // The lane supplies the address of four columns: quad q of the block's eight.
+    const int q = 4 * ((lane >> 4) & 1) + (cq & 3);
+    const int m = r0 + (kContiguous ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
     const int k = 16 * kc + 8 * hl + (cq >> 2);
     const int off = 8 * ((m >> 3) ^ (4 * (k & 3))) + 4 * ((m >> 2) & 1);
     bf16x4 lo = read_tr(slab + k * 256 + off), hi = read_tr(slab + (k + 4) * 256 + off);
@@ -218,10 +235,10 @@ struct Ctx {
 // slab row 16h + 4a + b.
 __device__ __forceinline__ int contiguous_row(int l32) { return 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3); }
 
-template <bool AK, bool BKM>
+template <bool AK, bool BKM, bool kContiguous = false>
 __device__ __forceinline__ void read_half(bf16x8 (&a)[4], bf16x8 (&b)[2], const lds_t* st, int kc, const Ctx& c) {
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb) a[mb] = frag<AK>(st, c.wm0 + 32 * mb, kc, c.lane, c.arow);
+  for (int mb = 0; mb < 4; ++mb) a[mb] = frag<AK, kContiguous>(st, c.wm0 + 32 * mb, kc, c.lane, c.arow);
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb) b[nb] = frag<BKM>(st + OPE, c.wn0 + 32 * nb, kc, c.lane, c.lane & 31);
 }
@@ -243,25 +260,25 @@ __device__ __forceinline__ void fill(lds_t* st, const Ctx& c, int kt) {
 // the barrier (every wave is done with buffer S), refills S from `fc` at
 // stage fkt (the current tile's stage kt+4, or one of the next tile's first
 // stages), reads chunk 0 of stage kt+1, runs chunk 1's MFMAs.
-template <bool AK, bool BKM, int S, bool kReadNext = true>
+template <bool AK, bool BKM, bool kContiguous, int S, bool kReadNext = true>
 __device__ __forceinline__ void step_fill(f32x16 (&acc)[4][2], const Ctx& c, const Ctx& fc, int fkt, bf16x8 (&a0)[4],
                                           bf16x8 (&b0)[2]) {
   bf16x8 a1[4], b1[2];
-  read_half<AK, BKM>(a1, b1, stage_ptr<S>(), 1, c);
+  read_half<AK, BKM, kContiguous>(a1, b1, stage_ptr<S>(), 1, c);
   GEMM_SCHED_FENCE();
   mma_half(acc, a0, b0);
   GEMM_SCHED_FENCE();
   GEMM_WAIT_VM8_LGKM0();
   wg_barrier();
   fill(stage_ptr<S>(), fc, fkt);
-  if (kReadNext) read_half<AK, BKM>(a0, b0, stage_ptr<(S + 1) % 4>(), 0, c);
+  if (kReadNext) read_half<AK, BKM, kContiguous>(a0, b0, stage_ptr<(S + 1) % 4>(), 0, c);
   GEMM_SCHED_FENCE();
   mma_half(acc, a1, b1);
   GEMM_SCHED_FENCE();
 }
 
-// Persistent main loop for K a multiple of 4*BK (every tile then
-// starts at stage buffer 0): the workgroup runs tiles blockIdx.x,
+// Persistent main loop: whole groups of four stages (every tile then starts at
+// stage buffer 0; the stages past K read zeros).  The workgroup runs tiles blockIdx.x,
 // blockIdx.x + gridDim.x, ... over the full K range, and the first four
 // stages of its next tile are copied during the last four stages of the
 // current one, so the epilogue runs while the next operands are in flight.
@@ -269,20 +286,21 @@ __device__ __forceinline__ void step_fill(f32x16 (&acc)[4][2], const Ctx& c, con
 // before each tile's stages (after the previous tile's epilogue), e.g. to
 // prefetch per-tile epilogue inputs far ahead of their use; epi(acc, tm, tn)
 // must not touch the stage arrays (its own LDS and barriers are fine).
-// kContiguousRows (K-major A only): A rows are read in the contiguous_row
-// order, so each lane's accumulator elements 0 .. 15 are 16 consecutive rows.
-template <bool AK, bool BKM, bool kContiguousRows = false, class Coords, class Pre, class Epi>
+// kContiguousRows: A rows are read in the contiguous_row order, so each lane's
+// accumulator elements 0 .. 15 of a 32-row block are 16 consecutive rows.
+// kPairA: A is a paired operand (MN-major), M the rows of both matrices.
+template <bool AK, bool BKM, bool kContiguousRows = false, bool kPairA = false, class Coords, class Pre, class Epi>
 __device__ __forceinline__ void persistent(Operand A, Operand B, int M, int N, int K, int ntiles, Coords coords,
                                            Pre pre, Epi epi) {
-  static_assert(AK || !kContiguousRows, "row permutation needs a K-major A operand");
+  constexpr bool kContig = kContiguousRows && !AK;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int arow = kContiguousRows ? contiguous_row(lane & 31) : (lane & 31);
   int t = blockIdx.x;
   if (t >= ntiles) return;  // uniform
-  const int nk = K / BK;
+  const int nk = ((K + BK - 1) / BK + 3) & ~3;
   int tm, tn;
   coords(t, tm, tn);
-  Ctx c{make_src<AK>(A, tm * BM, 0, M, K, wave, lane), make_src<BKM>(B, tn * BN, 0, N, K, wave, lane),
+  Ctx c{make_src<AK, kPairA>(A, tm * BM, 0, M, K, wave, lane), make_src<BKM>(B, tn * BN, 0, N, K, wave, lane),
         128 * (wave & 1), 64 * (wave >> 1), wave, lane, tid, arow};
   fill(stage_ptr<0>(), c, 0);
   fill(stage_ptr<1>(), c, 1);
@@ -292,7 +310,7 @@ __device__ __forceinline__ void persistent(Operand A, Operand B, int M, int N, i
   GEMM_WAIT_VM12_LGKM0();
   wg_barrier();
   bf16x8 a0[4], b0[2];
-  read_half<AK, BKM>(a0, b0, stage_ptr<0>(), 0, c);
+  read_half<AK, BKM, kContig>(a0, b0, stage_ptr<0>(), 0, c);
   f32x16 acc[4][2];
   while (true) {
 #pragma unroll
@@ -300,25 +318,25 @@ __device__ __forceinline__ void persistent(Operand A, Operand B, int M, int N, i
 #pragma unroll
       for (int b = 0; b < 2; ++b) acc[a][b] = f32x16{};
     for (int kt = 0; kt < nk - 4; kt += 4) {
-      step_fill<AK, BKM, 0>(acc, c, c, kt + 4, a0, b0);
-      step_fill<AK, BKM, 1>(acc, c, c, kt + 5, a0, b0);
-      step_fill<AK, BKM, 2>(acc, c, c, kt + 6, a0, b0);
-      step_fill<AK, BKM, 3>(acc, c, c, kt + 7, a0, b0);
+      step_fill<AK, BKM, kContig, 0>(acc, c, c, kt + 4, a0, b0);
+      step_fill<AK, BKM, kContig, 1>(acc, c, c, kt + 5, a0, b0);
+      step_fill<AK, BKM, kContig, 2>(acc, c, c, kt + 6, a0, b0);
+      step_fill<AK, BKM, kContig, 3>(acc, c, c, kt + 7, a0, b0);
     }
     const int t_next = t + (int)gridDim.x;
     const bool has_next = t_next < ntiles;
     int tm_n = 0, tn_n = 0;
     if (has_next) coords(t_next, tm_n, tn_n);
     // Sources of the next tile; with none, extents of 0 make every copy read zeros.
-    const Ctx cn{make_src<AK>(A, tm_n * BM, 0, has_next ? M : 0, K, wave, lane),
+    const Ctx cn{make_src<AK, kPairA>(A, tm_n * BM, 0, has_next ? M : 0, K, wave, lane),
                  make_src<BKM>(B, tn_n * BN, 0, has_next ? N : 0, K, wave, lane), c.wm0, c.wn0, wave, lane, tid,
                  arow};
-    step_fill<AK, BKM, 0>(acc, c, cn, 0, a0, b0);
-    step_fill<AK, BKM, 1>(acc, c, cn, 1, a0, b0);
-    step_fill<AK, BKM, 2>(acc, c, cn, 2, a0, b0);
+    step_fill<AK, BKM, kContig, 0>(acc, c, cn, 0, a0, b0);
+    step_fill<AK, BKM, kContig, 1>(acc, c, cn, 1, a0, b0);
+    step_fill<AK, BKM, kContig, 2>(acc, c, cn, 2, a0, b0);
     // (The next tile's first fragments are read after the epilogue, so they
     // are not live across it.)
-    step_fill<AK, BKM, 3, false>(acc, c, cn, 3, a0, b0);
+    step_fill<AK, BKM, kContig, 3, false>(acc, c, cn, 3, a0, b0);
     epi(acc, tm, tn);
     if (!has_next) break;
     pre(tm_n, tn_n);
@@ -326,7 +344,7 @@ __device__ __forceinline__ void persistent(Operand A, Operand B, int M, int N, i
     tm = tm_n;
     tn = tn_n;
     c = cn;
-    read_half<AK, BKM>(a0, b0, stage_ptr<0>(), 0, c);
+    read_half<AK, BKM, kContig>(a0, b0, stage_ptr<0>(), 0, c);
   }
   GEMM_WAIT_VM0_LGKM0();  // no copy may land in LDS after the workgroup ends
 }

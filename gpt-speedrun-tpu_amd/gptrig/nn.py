@@ -287,6 +287,117 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, 
     return _embedding_forward(tokens, table, scale, dtype)[0]
 
 
+_ACTIVATIONS = {"silu": 0, "gelu": 1}  # GPTRIG_SILU, GPTRIG_GELU
+_MOST_WIDTH, _MOST_STRIDE = 1 << 20, 1 << 22
+
+
+def _operand(x: torch.Tensor) -> torch.Tensor:
+    """``x`` as ``[rows, width]`` in the layout that the matrix products read (unit stride along the width, rows that do
+    not overlap, 16-byte alignment), without a copy where it has that."""
+
+    if x.ndim != 2:
+        x = x.reshape(-1, x.shape[-1])
+    rows, width = x.shape
+    if x.stride(1) == 1 and x.data_ptr() % 16 == 0:
+        ld = x.stride(0)
+        if ld == width or rows > 1 and ld > width and ld % 8 == 0 and ld <= _MOST_STRIDE:
+            return x
+    return torch.empty((rows, width), dtype=x.dtype, device=x.device).copy_(x)
+
+
+@functools.lru_cache(maxsize=256)
+def _gated_workspace_bytes(n: int, d: int, f: int, d_out: int) -> int:
+    return _lib.query("gptrig_gated_mlp_bwd_workspace_bytes", n, d, f, d_out)
+
+
+def _gated_forward(x, gate_up_w, down_w, activation: int, keep: bool):
+    """``y``, and what the backward needs (``None`` for the projection's output unless ``keep``)."""
+
+    x2, w, v = _operand(x), _operand(gate_up_w), _operand(down_w)
+    n, d = x2.shape
+    f, d_out = v.shape
+    dev = x2.device
+    h = torch.empty((n, f), dtype=BF16, device=dev)
+    gate_up = torch.empty((n, 2 * f), dtype=BF16, device=dev) if keep else None
+    y = torch.empty((n, d_out), dtype=BF16, device=dev)
+    if n:
+        _lib.call_on(x2.get_device(), "gptrig_gated_mlp_fwd", x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0),
+                     v.data_ptr(), v.stride(0), activation, _lib.ptr(gate_up), h.data_ptr(), y.data_ptr(), n, d, f,
+                     d_out)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], d_out), x2, w, v, gate_up, h
+
+
+class _GatedMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_up_w, down_w, activation):
+        y, *kept = _gated_forward(x, gate_up_w, down_w, activation, True)
+        ctx.save_for_backward(*kept)
+        ctx.meta = (x.shape, activation)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        return (_gated_backward_once if torch.is_grad_enabled() else _gated_backward)(ctx, dy)
+
+
+def _gated_backward(ctx, dy):
+    x, w, v, gate_up, h = ctx.saved_tensors
+    shape, activation = ctx.meta
+    need_x, need_w, need_v, _ = ctx.needs_input_grad
+    n, d = x.shape
+    f, d_out = v.shape
+    dev = x.device
+    if not n:
+        return (torch.zeros(shape, dtype=BF16, device=dev) if need_x else None,
+                torch.zeros((d, 2 * f), dtype=BF16, device=dev) if need_w else None,
+                torch.zeros((f, d_out), dtype=BF16, device=dev) if need_v else None, None)
+    dy = _operand(dy)
+    dx = torch.empty((n, d), dtype=BF16, device=dev) if need_x else None
+    dw = torch.empty((d, 2 * f), dtype=BF16, device=dev) if need_w else None
+    dv = torch.empty((f, d_out), dtype=BF16, device=dev) if need_v else None
+    size = _gated_workspace_bytes(n, d, f, d_out)
+    ws = _lib.workspace(size, dev)
+    _lib.call_on(x.get_device(), "gptrig_gated_mlp_bwd", dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
+                 w.data_ptr(), w.stride(0), v.data_ptr(), v.stride(0), activation, gate_up.data_ptr(), h.data_ptr(),
+                 _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(dv), n, d, f, d_out, ws.data_ptr(), size)
+    return None if dx is None else dx.view(shape), dw, dv, None
+
+
+_gated_backward_once = once_differentiable(_gated_backward)
+
+
+def gated_mlp(x: torch.Tensor, gate_up_w: torch.Tensor, down_w: torch.Tensor, *,
+              activation: str = "silu") -> torch.Tensor:
+    """A gated feed-forward block: ``(act(x @ gate) * (x @ up)) @ down_w`` with
+    ``gate_up_w = [gate | up]``, ``act`` ``"silu"`` or ``"gelu"`` (tanh form).
+
+    ``x``: bfloat16 ``[..., d]`` of any strides; ``gate_up_w`` ``[d, 2 * hidden]``
+    and ``down_w`` ``[hidden, d_out]`` in bfloat16; widths are multiples of 8.  The
+    sums are float32; the hidden values, and for the backward both halves of the
+    projection, are held in bfloat16.  Differentiable once in all three, the
+    gradients in bfloat16 and the same at every call.
+    """
+
+    for name, t in (("x", x), ("gate_up_w", gate_up_w), ("down_w", down_w)):
+        if t.dtype != BF16:
+            raise TypeError(f"the HIP gated_mlp computes bfloat16, got {name} of {t.dtype}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    if not x.ndim or gate_up_w.ndim != 2 or down_w.ndim != 2 or gate_up_w.shape[0] != x.shape[-1] or (
+            gate_up_w.shape[1] != 2 * down_w.shape[0]):
+        raise ValueError(f"x, gate_up_w and down_w must be [..., d], [d, 2 * hidden] and [hidden, d_out], got "
+                         f"{tuple(x.shape)}, {tuple(gate_up_w.shape)} and {tuple(down_w.shape)}")
+    widths = (x.shape[-1], *down_w.shape)
+    if any(w == 0 or w % 8 for w in widths) or max(widths[0], 2 * widths[1], widths[2]) > _MOST_WIDTH:
+        raise ValueError(f"widths must be multiples of 8, and d, 2 * hidden and d_out at most 2^20, got {widths}")
+    if x.numel() // widths[0] > 1 << 26:
+        raise ValueError(f"at most 2^26 tokens, got {x.numel() // widths[0]}")
+    _lib.require_one_device(x, gate_up_w, down_w)
+    if _lib.needs_autograd(x, gate_up_w, down_w):
+        return _GatedMLP.apply(x, gate_up_w, down_w, _ACTIVATIONS[activation])
+    return _gated_forward(x, gate_up_w, down_w, _ACTIVATIONS[activation], False)[0]
+
+
 _ROPE_TABLES: dict = {}
 
 

@@ -408,6 +408,31 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated feed-forward block (no counterpart in the reference, whose block has one
+ * up-projection): with [g | u] = x gate_up_w the two halves of a projection,
+ * h = act(g) * u and y = h down_w; act is GPTRIG_SILU or GPTRIG_GELU (tanh form).
+ * All bf16: x [n, d], gate_up_w [d, 2f] (the gate's columns first), down_w
+ * [f, d_out] with row strides ldx, ldw and ldv, gate_up [n, 2f] (nullable: what the
+ * backward needs of g and u), h [n, f] (for the backward, or scratch) and y
+ * [n, d_out] contiguous.  Sums are float32; h is rounded from the unrounded g, u.
+ * The backward writes dx [n, d], d_gate_up_w and d_down_w (contiguous, each
+ * nullable) in an order of additions that the sizes fix;
+ * gptrig_gated_mlp_bwd_workspace_bytes of workspace.
+ * Widths and row strides are multiples of 8, strides at most 2^22, d, 2f and d_out
+ * at most 2^20, pointers 16-byte aligned; n may be 0 in the forward.
+ * ---------------------------------------------------------------------- */
+#define GPTRIG_SILU 0
+#define GPTRIG_GELU 1
+int gptrig_gated_mlp_fwd(const void* x, int64_t ldx, const void* gate_up_w, int64_t ldw, const void* down_w,
+                         int64_t ldv, int activation, void* gate_up, void* h, void* y, int n, int d, int f, int d_out,
+                         void* stream);
+size_t gptrig_gated_mlp_bwd_workspace_bytes(int n, int d, int f, int d_out);
+int gptrig_gated_mlp_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* gate_up_w, int64_t ldw,
+                         const void* down_w, int64_t ldv, int activation, const void* gate_up, const void* h, void* dx,
+                         void* d_gate_up_w, void* d_down_w, int n, int d, int f, int d_out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * AdamW over one flat f32 arena: recipes/reference/train.py:1386-1445
  * (_apply_training_update), with the per-tensor multipliers of
  * optimizer_hyperparameter_trees (:1274-1333) and the decay mask of

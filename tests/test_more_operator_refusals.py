@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from gptrig import _lib
-from gptrig.nn import embedding
+from gptrig.nn import embedding, gated_mlp
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -64,3 +64,60 @@ def test_embedding_workspace(n):
     size = _lib.query("gptrig_scaled_embedding_bwd_workspace_bytes", n, 16, 1000)
     chunks = [-(-n // c) for c in (4, 32)]
     assert 16 * n + 128 * chunks[1] <= size <= 16 * n + 128 * chunks[0] + 256 * 1024 + 6 * 256
+
+
+def test_gated_mlp_refusals():
+    x, w, v = (torch.zeros(s, dtype=BF16) for s in ((3, 16), (16, 48), (24, 8)))
+    for bad in (x.float(), x.half()):
+        with pytest.raises(TypeError, match="bfloat16, got x"):
+            gated_mlp(bad, w, v)
+    with pytest.raises(TypeError, match="gate_up_w"):
+        gated_mlp(x, w.float(), v)
+    with pytest.raises(TypeError, match="down_w"):
+        gated_mlp(x, w, v.float())
+    with pytest.raises(ValueError, match="activation"):
+        gated_mlp(x, w, v, activation="relu")
+    for args in ((x[:, :8], w, v), (x, w[:, :40], v), (x, w, v[:16]), (x, w[0], v), (x, w, v[0]), (x[0, 0], w, v),
+                 (x, w[None], v)):
+        with pytest.raises(ValueError, match="must be"):
+            gated_mlp(*args)
+    for shapes in (((3, 12), (12, 48), (24, 8)), ((3, 16), (16, 40), (20, 8)), ((3, 16), (16, 48), (24, 7)),
+                   ((3, 0), (0, 48), (24, 8)), ((3, 16), (16, 0), (0, 8))):
+        with pytest.raises(ValueError, match="multiples of 8"):
+            gated_mlp(*(torch.zeros(s, dtype=BF16) for s in shapes))
+    with pytest.raises(RuntimeError, match="GPU"):
+        gated_mlp(x, w, v)
+
+
+def test_gated_entry_points_check_their_arguments():
+    lib = _lib.lib()
+    at, odd = ctypes.c_void_p(1 << 12), ctypes.c_void_p((1 << 12) + 8)
+    fwd = lib.gptrig_gated_mlp_fwd
+    good = [at, 16, at, 48, at, 8, 0, at, at, at, 3, 16, 24, 8, None]
+
+    def changed(**by):
+        return [by.get(f"a{i}", a) for i, a in enumerate(good)]
+
+    for i in (0, 2, 4, 8, 9):
+        assert fwd(*changed(**{f"a{i}": None})) == -1
+        assert fwd(*changed(**{f"a{i}": odd})) == -2
+    assert fwd(*changed(a7=odd)) == -2
+    assert fwd(*changed(a6=2)) == -4
+    for i, bad in ((1, 8), (1, 20), (1, 1 << 23), (3, 40), (5, 0), (10, -1), (11, 12), (12, 20), (13, 4), (11, 0),
+                   (12, 1 << 20), (13, 1 << 21)):
+        assert fwd(*changed(**{f"a{i}": bad})) == -2, (i, bad)
+    assert fwd(*changed(a10=0)) == 0
+    size = _lib.query("gptrig_gated_mlp_bwd_workspace_bytes", 3, 16, 24, 8)
+    bwd = lib.gptrig_gated_mlp_bwd
+    call = [at, 8, at, 16, at, 48, at, 8, 0, at, at, at, at, at, 3, 16, 24, 8, at, size, None]
+    for i in (0, 2, 4, 6, 9, 10, 18):
+        assert bwd(*(None if j == i else a for j, a in enumerate(call))) == -1, i
+    for i in (0, 2, 4, 6, 9, 10, 11, 12, 13, 18):
+        assert bwd(*(odd if j == i else a for j, a in enumerate(call))) == -2, i
+    assert bwd(*(size - 1 if j == 19 else a for j, a in enumerate(call))) == -6
+    assert bwd(*(0 if j == 14 else a for j, a in enumerate(call))) == -2
+    assert bwd(*(7 if j == 8 else a for j, a in enumerate(call))) == -4
+    # Inside: the gradient of the projection's output, and float32 parts of at most 32 slices.
+    for n, d, f in ((1, 64, 64), (65536, 768, 2048), (5001, 1000, 2664)):
+        size = _lib.query("gptrig_gated_mlp_bwd_workspace_bytes", n, d, f, d)
+        assert 4 * n * f <= size <= 4 * n * f + 32 * 12 * d * f + 1024

@@ -20,7 +20,7 @@ LIB = os.path.join(OUT_DIR, "libgptrig.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 SOURCES = ("capi.hip", "elementwise.hip", "attention.hip", "flce.hip", "flce32.hip", "moe.hip", "linear.hip",
            "layernorm.hip", "adamw_tensors.hip", "scored_attention_fwd.hip", "scored_attention_bwd.hip", "embedding.hip",
-           "gated_mlp.hip")
+           "gated_mlp.hip", "orthogonalize.hip")
 
 FLAGS = [
     "--offload-arch=gfx950",

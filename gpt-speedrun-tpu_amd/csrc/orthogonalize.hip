@@ -1,0 +1,500 @@
+// Orthogonalised updates by Newton-Schulz products (as the Muon optimiser uses them).
+//
+// For a matrix u [rows][cols], with m the shorter and n the longer side and X [m][n]
+// the matrix u / (|u| + eps) (|u| the root of its squares' sum) or its transpose:
+//   steps times   A = X X^T,   B = b A + c A A,   X <- a X + B X
+// and the result X, transposed back, in bfloat16.  It drives the singular values
+// towards 1 and leaves the directions as they are.
+//
+// Bound: the matrix cores.  A step has 6 m m n operations less the symmetric halves:
+// A and A A are symmetric, and only their tiles on and below the diagonal are
+// computed, each written twice (3 m m n + m m m instead of 4 m m n + 2 m m m).
+//
+// What is held in fewer than 32 bits.  The products take float16 operands (11 bits;
+// every value here is below 2 in size, the normalised X's around (m n)^-1/2, and
+// what float16 flushes near 2^-25 is far below the sums' own rounding) and add in
+// float32.  X itself is held in two float16, the operand `hi` and the rest `lo`,
+// scaled by 2^11 so that it keeps its bits: 22 bits.  That is what the result needs:
+// an error of X in the directions of small singular values grows by a each step (485
+// times in five), but only through the term a X, which is computed from all 22 bits;
+// in B X the rounding of X meets B, which is small in those directions, and the
+// rounding of B multiplies what is there.  In simulations over spectra from flat to
+// falling by 10^6 the result differs from the exact one by 0.1 to 0.9 times the
+// rounding to bfloat16 that follows; with X in one float16 by up to 24 times, in
+// one bfloat16 by up to 200 times.
+//
+// One launch does a product for every matrix of a list (48 matrices of a model of 12
+// layers fill the chip where one would not); matrices of one shape are a group, laid
+// out at a stride, and the groups' table travels as a kernel argument.
+#include "tile_core.h"
+
+namespace {
+
+using tile::f16;
+using tile::f16x8;
+
+constexpr int kMostGroups = 16;   // shapes of a launch
+constexpr int kMostTensors = 64;  // tensors of a launch
+constexpr int kPart = 16384;      // elements of a partial sum of squares
+constexpr float kLow = 2048.0f;   // scale of X's lower part
+constexpr int64_t kMostBytes = 2ll << 30;  // workspace of a launch, where a matrix alone does not need more
+
+struct Group {
+  int m, n;      // the shorter and the longer side
+  int tall;      // the tensors have more rows than columns: X is the transpose
+  int count;     // matrices
+  int parts;     // partial sums of squares a matrix
+  int sum0;      // the first one's index
+  int64_t x0;    // first element in hi and lo
+  int64_t a0;    // in A and B
+  __host__ __device__ int ldx() const { return (n + 7) & ~7; }
+  __host__ __device__ int lda() const { return (m + 7) & ~7; }
+};
+
+struct Tensor {
+  const void* in;
+  bf16* out;
+  int group, first;  // its matrices are first, first + 1, ... of the group
+};
+
+struct Args {
+  Group g[kMostGroups];
+  Tensor t[kMostTensors];
+  int first[kMostGroups + 1];  // each group's first workgroup of this launch, and the end
+  int groups, tensors;
+  double* sums;
+  f16 *hi, *hi_next, *lo, *A, *B;
+  float a, b, c, eps;
+};
+
+// Workgroup -> group, and its index within it.
+__device__ __forceinline__ int find_group(const Args& s, int pid, int& local) {
+  int g = 0;
+  while (g + 1 < s.groups && pid >= s.first[g + 1]) ++g;  // uniform
+  local = pid - s.first[g];
+  return g;
+}
+
+__device__ __forceinline__ const Tensor& find_tensor(const Args& s, int group, int matrix) {
+  int at = 0;
+  for (int i = 0; i < s.tensors; ++i)
+    if (s.t[i].group == group && s.t[i].first <= matrix) at = i;  // (ascending within a group)
+  return s.t[at];
+}
+
+__device__ __forceinline__ double block_sum(double v, double* shared) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return ((shared[0] + shared[1]) + shared[2]) + shared[3];
+}
+
+// Sums of squares in 64 bits: no overflow for any float32, whatever the scale.
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_norm_kernel(Args s) {
+  __shared__ double shared[4];
+  int local;
+  const int gi = find_group(s, blockIdx.x, local);
+  const Group& g = s.g[gi];
+  const int matrix = local / g.parts, part = local % g.parts;
+  const Tensor& t = find_tensor(s, gi, matrix);
+  const int64_t size = (int64_t)g.m * g.n;
+  const T* in = (const T*)t.in + (matrix - t.first) * size;
+  const int64_t begin = (int64_t)part * kPart, end = begin + kPart < size ? begin + kPart : size;
+  double sum = 0.0;
+#pragma unroll 4
+  for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
+    const double v = (double)(float)in[i];
+    sum = __builtin_fma(v, v, sum);
+  }
+  sum = block_sum(sum, shared);
+  if (threadIdx.x == 0) s.sums[g.sum0 + (int64_t)matrix * g.parts + part] = sum;
+}
+
+// X of a matrix, 64 x 64 of it a workgroup: normalised, turned where the matrix is
+// tall, cut in two float16, with zeros up to the row length.
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_load_kernel(Args s) {
+  __shared__ double shared[4];
+  __shared__ float turned[64][65];
+  int local;
+  const int gi = find_group(s, blockIdx.x, local);
+  const Group& g = s.g[gi];
+  const int ld = g.ldx();
+  const int across = (ld + 63) / 64, down = (g.m + 63) / 64;
+  const int matrix = local / (across * down), at = local % (across * down);
+  const int i0 = at / across * 64, j0 = at % across * 64;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < g.parts; i += 256) sum += s.sums[g.sum0 + (int64_t)matrix * g.parts + i];
+  sum = block_sum(sum, shared);
+  const float scale = (float)(1.0 / (sqrt(sum) + (double)s.eps));
+  const Tensor& t = find_tensor(s, gi, matrix);
+  const int64_t size = (int64_t)g.m * g.n;
+  const T* in = (const T*)t.in + (matrix - t.first) * size;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (g.tall) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {  // row j0 + r of the tensor, column i0 + lane
+      const int r = 4 * k + wave, j = j0 + r, i = i0 + lane;
+      turned[r][lane] = j < g.n && i < g.m ? (float)in[(int64_t)j * g.m + i] : 0.f;
+    }
+    __syncthreads();
+  }
+  f16* const hi = s.hi + g.x0 + (int64_t)matrix * g.m * ld;
+  f16* const lo = s.lo + g.x0 + (int64_t)matrix * g.m * ld;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = 4 * k + wave, i = i0 + r, j = j0 + lane;
+    if (i >= g.m || j >= ld) continue;
+    float x = 0.f;
+    if (g.tall)
+      x = turned[lane][r];
+    else if (j < g.n)
+      x = (float)in[(int64_t)i * g.n + j];
+    x *= scale;
+    const f16 h = (f16)x;
+    hi[(int64_t)i * ld + j] = h;
+    lo[(int64_t)i * ld + j] = (f16)((x - (float)h) * kLow);
+  }
+}
+
+// Rows of a lower triangle's tile: t -> (i, j), j <= i.
+__device__ __forceinline__ void triangle(int t, int& i, int& j) {
+  i = (int)((__builtin_sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+  while (i * (i + 1) / 2 > t) --i;
+  while ((i + 1) * (i + 2) / 2 <= t) ++i;
+  j = t - i * (i + 1) / 2;
+}
+
+__device__ __forceinline__ f16x8 to_f16(const float* v) {
+  f16x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (f16)v[e];
+  return r;
+}
+
+enum { kGram = 0, kSquare = 1, kUpdate = 2, kLast = 3 };
+
+// One product of a step for every matrix.  The tile is computed as [feature][row]:
+// the lane holds 16 consecutive features of a row of the result.
+template <int kKind, int MB, int NB, int kSlabs>
+__global__ void __launch_bounds__(256) ortho_product_kernel(Args s) {
+  constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
+  typedef tile::Product<f16, MB, NB, kSymmetric, true, true, kSlabs> P;
+  int local;
+  const int gi = find_group(s, gemm::xcd_swizzle(blockIdx.x, gridDim.x), local);
+  const Group& g = s.g[gi];
+  const int m = g.m, lda = g.lda(), ldx = g.ldx();
+  const int down = (m + P::TN - 1) / P::TN;
+  int matrix, ti, tj;
+  if (kSymmetric) {
+    static_assert(!kSymmetric || MB == NB, "a triangle of square tiles");
+    const int tiles = down * (down + 1) / 2;
+    matrix = local / tiles;
+    triangle(local % tiles, ti, tj);
+  } else {
+    const int tiles = down * ((ldx + P::TM - 1) / P::TM);
+    matrix = local / tiles;
+    const int at = local % tiles;
+    ti = at % down;
+    tj = at / down;
+  }
+  const f16* const hi = s.hi + g.x0 + (int64_t)matrix * m * ldx;
+  f16* const A = s.A + g.a0 + (int64_t)matrix * m * lda;
+  f16* const B = s.B + g.a0 + (int64_t)matrix * m * lda;
+  const auto at = P::place();
+  f32x16 acc[MB][NB];
+  if constexpr (kKind == kGram)
+    P::run(acc, {hi, ldx}, {hi, ldx}, m, m, ldx, tj * P::TM, ti * P::TN, at);
+  else if constexpr (kKind == kSquare)
+    P::run(acc, {A, lda}, {A, lda}, m, m, m, tj * P::TM, ti * P::TN, at);
+  else
+    P::run(acc, {hi, ldx}, {B, lda}, ldx, m, m, tj * P::TM, ti * P::TN, at);
+  const int l32 = at.lane & 31, hl = at.lane >> 5;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = ti * P::TN + 32 * (NB * at.wn + nb) + l32;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const int f0 = tj * P::TM + 32 * (MB * at.wm + mb) + 16 * hl;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[mb][nb][e];
+      if constexpr (kSymmetric) {
+        f16* const out = kKind == kGram ? A : B;
+        if constexpr (kKind == kSquare) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            f16x8 old{};
+            if (row < m && f0 + 8 * h < lda) old = *(const f16x8*)(A + (int64_t)row * lda + f0 + 8 * h);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[8 * h + e] = __builtin_fmaf(s.c, v[8 * h + e], s.b * (float)old[e]);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (row < m && f0 + 8 * h < lda) *(f16x8*)(out + (int64_t)row * lda + f0 + 8 * h) = to_f16(v + 8 * h);
+        // (Past the last row and column both operands read zeros: so the rows' ends are zeros.)
+        if (ti != tj && row < lda) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (f0 + e < m) out[(int64_t)(f0 + e) * lda + row] = (f16)v[e];
+        }
+      } else if (row < m) {
+        const int64_t at0 = g.x0 + ((int64_t)matrix * m + row) * ldx + f0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (f0 + 8 * h >= ldx) continue;
+          const f16x8 high = *(const f16x8*)(s.hi + at0 + 8 * h), low = *(const f16x8*)(s.lo + at0 + 8 * h);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = __builtin_fmaf((float)low[e], 1.0f / kLow, (float)high[e]);
+            v[8 * h + e] = __builtin_fmaf(s.a, x, v[8 * h + e]);
+          }
+          if constexpr (kKind == kUpdate) {
+            const f16x8 next = to_f16(v + 8 * h);
+            float rest[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rest[e] = (v[8 * h + e] - (float)next[e]) * kLow;
+            *(f16x8*)(s.hi_next + at0 + 8 * h) = next;
+            *(f16x8*)(s.lo + at0 + 8 * h) = to_f16(rest);  // (this lane's own, read above)
+          }
+        }
+        if constexpr (kKind == kLast) {
+          const Tensor& t = find_tensor(s, gi, matrix);
+          bf16* const out = t.out + (int64_t)(matrix - t.first) * m * g.n;
+          if (g.tall) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (f0 + e < g.n) out[(int64_t)(f0 + e) * m + row] = (bf16)v[e];
+          } else if (g.n % 8 == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (f0 + 8 * h < g.n) *(bf16x8*)(out + (int64_t)row * g.n + f0 + 8 * h) = pack8(v + 8 * h);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (f0 + e < g.n) out[(int64_t)row * g.n + f0 + e] = (bf16)v[e];
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---- host side ----
+
+size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct Sizes {
+  int64_t x = 0, a = 0, sums = 0;  // elements of hi (and lo, hi_next), of A (and B), of the sums
+  size_t bytes() const {
+    return 3 * round_up((size_t)x * 2) + 2 * round_up((size_t)a * 2) + round_up((size_t)sums * 8);
+  }
+};
+
+Group group_of(const gptrig_matrices& t) {
+  Group g{};
+  g.tall = t.rows > t.cols;
+  g.m = g.tall ? t.cols : t.rows;
+  g.n = g.tall ? t.rows : t.cols;
+  g.parts = ceil_div((int64_t)g.m * g.n, kPart);
+  return g;
+}
+
+Sizes size_of(const Group& g, int64_t count) {
+  Sizes s;
+  s.x = count * g.m * g.ldx();
+  s.a = count * g.m * g.lda();
+  s.sums = count * g.parts;
+  return s;
+}
+
+// Walks a list in launches' worth: at most kMostTensors tensors of kMostGroups shapes
+// and kMostBytes of workspace each; a tensor's matrices may be spread over several.
+struct Walk {
+  const gptrig_matrices* list;
+  int count;
+  int at = 0;          // the tensor that is next
+  int64_t inside = 0;  // and its matrices that are done
+
+  // The next launch's table and sizes; false at the end.
+  bool next(Args& s, Sizes& total, size_t item) {
+    s.groups = s.tensors = 0;
+    total = Sizes{};
+    while (at < count && s.tensors < kMostTensors) {
+      const gptrig_matrices& t = list[at];
+      const Group shape = group_of(t);
+      if (t.count == 0 || shape.m == 0) {
+        ++at;
+        continue;
+      }
+      int gi = 0;
+      while (gi < s.groups && (s.g[gi].m != shape.m || s.g[gi].n != shape.n || s.g[gi].tall != shape.tall)) ++gi;
+      if (gi == kMostGroups) break;
+      const Sizes one = size_of(shape, 1);
+      const int64_t left = kMostBytes - (int64_t)total.bytes();
+      int64_t take = left / (6 * one.x + 4 * one.a + 8 * one.sums);
+      if (take <= 0) {
+        if (s.tensors) break;
+        take = 1;
+      }
+      if (take > t.count - inside) take = t.count - inside;
+      if (take > 65536) take = 65536;
+      if (gi == s.groups) s.g[s.groups++] = shape;
+      Group& g = s.g[gi];
+      const int64_t size = (int64_t)t.rows * t.cols;
+      s.t[s.tensors++] =
+          Tensor{(const char*)t.in + inside * size * item, (bf16*)t.out + inside * size, gi, g.count};
+      g.count += (int)take;
+      const Sizes more = size_of(shape, take);
+      total.x += more.x;
+      total.a += more.a;
+      total.sums += more.sums;
+      inside += take;
+      if (inside < t.count) break;
+      inside = 0;
+      ++at;
+    }
+    Sizes from;
+    for (int i = 0; i < s.groups; ++i) {
+      Group& g = s.g[i];
+      g.x0 = from.x;
+      g.a0 = from.a;
+      g.sum0 = (int)from.sums;
+      const Sizes more = size_of(g, g.count);
+      from.x += more.x;
+      from.a += more.a;
+      from.sums += more.sums;
+    }
+    return s.groups > 0;
+  }
+};
+
+int check_list(const gptrig_matrices* list, int count) {
+  if (count < 0) return GPTRIG_E_SHAPE;
+  if (count && !list) return GPTRIG_E_NULL;
+  for (int i = 0; i < count; ++i) {
+    const gptrig_matrices& t = list[i];
+    if (t.count < 0 || t.rows < 0 || t.cols < 0 || t.rows > 65536 || t.cols > 65536) return GPTRIG_E_SHAPE;
+  }
+  return GPTRIG_OK;
+}
+
+// Workgroups of a launch, `each` a matrix of a group; fills s.first.  (At most some
+// millions: kMostTensors of 65536 matrices, or what kMostBytes or one matrix hold.)
+template <class F>
+int64_t count_groups(Args& s, F each) {
+  int64_t total = 0;
+  for (int i = 0; i < s.groups; ++i) {
+    s.first[i] = (int)total;
+    total += each(s.g[i]) * s.g[i].count;
+  }
+  s.first[s.groups] = (int)total;
+  return total;
+}
+
+template <int kTile>
+int64_t symmetric_tiles(const Group& g) {
+  const int64_t down = ceil_div(g.m, kTile);
+  return down * (down + 1) / 2;
+}
+template <int kTile>
+int64_t update_tiles(const Group& g) {
+  return (int64_t)ceil_div(g.m, kTile) * ceil_div(g.ldx(), kTile);
+}
+
+template <int kKind, int MB, int kSlabs>
+int launch_product(Args& s, hipStream_t stream) {
+  constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
+  const int64_t total = count_groups(s, kSymmetric ? symmetric_tiles<64 * MB> : update_tiles<64 * MB>);
+  ortho_product_kernel<kKind, MB, MB, kSlabs><<<(unsigned)total, 256, 0, stream>>>(s);
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
+}
+
+template <int kKind>
+int product(Args& s, hipStream_t stream) {
+  constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
+  // The wider tile needs fewer reads an operation; the narrower one fills the chip with fewer matrices.
+  const int64_t wide = count_groups(s, kSymmetric ? symmetric_tiles<128> : update_tiles<128>);
+  return wide >= gemm::device_cus() ? launch_product<kKind, 2, 1>(s, stream) : launch_product<kKind, 1, 2>(s, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gptrig_orthogonalize_workspace_bytes(const gptrig_matrices* list, int count) {
+  if (check_list(list, count) != GPTRIG_OK) return 0;
+  Walk walk{list, count};
+  Args s;
+  Sizes total;
+  size_t most = 0;
+  while (walk.next(s, total, 2)) most = total.bytes() > most ? total.bytes() : most;
+  return most;
+}
+
+int gptrig_orthogonalize(const gptrig_matrices* list, int count, int type, int steps, float a, float b, float c,
+                         float eps, void* workspace, size_t workspace_bytes, void* stream) {
+  const int checked = check_list(list, count);
+  if (checked != GPTRIG_OK) return checked;
+  if (type != GPTRIG_TYPE_BF16 && type != GPTRIG_TYPE_F32) return GPTRIG_E_DTYPE;
+  if (steps < 1 || !(eps >= 0.f)) return GPTRIG_E_SHAPE;
+  const size_t item = type == GPTRIG_TYPE_F32 ? 4 : 2;
+  for (int i = 0; i < count; ++i) {
+    if (list[i].count == 0 || list[i].rows == 0 || list[i].cols == 0) continue;
+    if (!list[i].in || !list[i].out) return GPTRIG_E_NULL;
+    if ((uintptr_t)list[i].in % item || (uintptr_t)list[i].out % 16) return GPTRIG_E_SHAPE;
+  }
+  const size_t need = gptrig_orthogonalize_workspace_bytes(list, count);
+  if (need && !workspace) return GPTRIG_E_NULL;
+  if ((uintptr_t)workspace % 16) return GPTRIG_E_SHAPE;
+  if (workspace_bytes < need) return GPTRIG_E_WORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  Walk walk{list, count};
+  Args s;
+  s.a = a;
+  s.b = b;
+  s.c = c;
+  s.eps = eps;
+  Sizes total;
+  while (walk.next(s, total, item)) {
+    const size_t x = round_up((size_t)total.x * 2), sq = round_up((size_t)total.a * 2);
+    char* at = (char*)workspace;
+    s.hi = (f16*)at;
+    s.hi_next = (f16*)(at + x);
+    s.lo = (f16*)(at + 2 * x);
+    s.A = (f16*)(at + 3 * x);
+    s.B = (f16*)(at + 3 * x + sq);
+    s.sums = (double*)(at + 3 * x + 2 * sq);
+    int64_t grid = count_groups(s, [](const Group& g) -> int64_t { return g.parts; });
+    if (type == GPTRIG_TYPE_F32)
+      ortho_norm_kernel<float><<<(unsigned)grid, 256, 0, st>>>(s);
+    else
+      ortho_norm_kernel<bf16><<<(unsigned)grid, 256, 0, st>>>(s);
+    GPTRIG_CHECK_LAUNCH();
+    grid = count_groups(s, [](const Group& g) -> int64_t {
+      return (int64_t)ceil_div(g.ldx(), 64) * ceil_div(g.m, 64);
+    });
+    if (type == GPTRIG_TYPE_F32)
+      ortho_load_kernel<float><<<(unsigned)grid, 256, 0, st>>>(s);
+    else
+      ortho_load_kernel<bf16><<<(unsigned)grid, 256, 0, st>>>(s);
+    GPTRIG_CHECK_LAUNCH();
+    for (int step = 0; step < steps; ++step) {
+      int status = product<kGram>(s, st);
+      if (status == GPTRIG_OK) status = product<kSquare>(s, st);
+      if (status == GPTRIG_OK) status = step + 1 < steps ? product<kUpdate>(s, st) : product<kLast>(s, st);
+      if (status != GPTRIG_OK) return status;
+      f16* const last = s.hi;
+      s.hi = s.hi_next;
+      s.hi_next = last;
+    }
+  }
+  return GPTRIG_OK;
+}
+
+}  // extern "C"

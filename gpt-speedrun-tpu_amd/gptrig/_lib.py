@@ -101,6 +101,8 @@ SIGNATURES: dict[str, tuple] = {
     "gptrig_adamw": (I, [P, P, P, P, P, P, P, L, I, F, F, F, I, P, P, P]),
     "gptrig_adamw_tensors": (I, [P, I, I, I, P, N, N, N, I, P, U, P]),
     "gptrig_adamw_tensors_device_seed": (I, [P, I, I, I, P, N, N, N, I, P, P, P]),
+    "gptrig_orthogonalize_workspace_bytes": (Z, [P, I]),
+    "gptrig_orthogonalize": (I, [P, I, I, I, F, F, F, F, P, Z, P]),
     "gptrig_sq_norm_partials": (I, [P, L, I, P, P]),
     "gptrig_finalize_norm": (I, [P, I, F, P, P, P, F, P, P]),
     "gptrig_transpose_bf16": (I, [P, P, I, I, P]),

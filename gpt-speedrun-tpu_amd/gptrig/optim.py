@@ -5,12 +5,14 @@ The update itself is the fused ``gptrig_adamw`` kernel over one arena; this
 module resolves the host-side scalars (learning rate per step, bias corrections)
 and the per-tensor table ``{lr_mult, epsilon, decay}`` the kernel reads.
 ``adamw_tensors`` is the same update over tensors that lie anywhere, with float32
-or 8-bit moments.
+or 8-bit moments; ``orthogonalize_tensors`` turns matrices' updates into
+orthogonal ones.
 """
 
 from __future__ import annotations
 
 import array
+import functools
 import math
 import operator
 import warnings
@@ -19,6 +21,7 @@ from typing import Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -242,3 +245,72 @@ def adamw_tensors(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     torch.autograd.graph.increment_version(params)
     if shadow is not None:
         torch.autograd.graph.increment_version(shadow)
+
+
+_MATRIX_TYPES = {torch.bfloat16: 0, torch.float32: 1}  # GPTRIG_TYPE_* of include/gptrig.h
+_MOST_SIDE, _MOST_F32 = 65536, (2.0 - 2.0 ** -23) * 2.0 ** 127
+
+
+def _matrices(shapes) -> list[int]:
+    """A row of gptrig_matrices a tensor, as int64: two addresses (left 0), the count, rows and columns in one."""
+
+    table = [0] * (4 * len(shapes))
+    table[2::4] = [math.prod(s[:-2]) for s in shapes]
+    table[3::4] = [s[-2] | s[-1] << 32 for s in shapes]
+    return table
+
+
+@functools.lru_cache(maxsize=64)
+def _orthogonalize_workspace_bytes(shapes: tuple) -> int:
+    table = array.array("q", _matrices(shapes))
+    return _lib.query("gptrig_orthogonalize_workspace_bytes", table.buffer_info()[0], len(shapes))
+
+
+def orthogonalize_tensors(updates: Sequence[torch.Tensor], *, steps: int = 5,
+                          coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315),
+                          eps: float = 1.0e-7) -> list[torch.Tensor]:
+    """Orthogonalised updates, as the Muon optimiser takes its steps: a bfloat16
+    tensor for each of ``updates``, in a few launches however many there are.
+
+    Every matrix u of a tensor (its last two dimensions; leading ones, such as a
+    routed layer's experts, count matrices) becomes ``x = u / (|u| + eps)`` with the
+    Frobenius norm, then ``steps`` times ``x = a x + (b A + c A A) x`` with ``A = x
+    x^T`` and ``coefficients = (a, b, c)``, on the transpose where it has more rows
+    than columns.  That moves its singular values towards 1.  The default
+    coefficients move them fast, to between 0.7 and 1.2.  The products take float16
+    operands: coefficients that make a value pass 65504 give infinities.  ``updates``:
+    all float32 or all bfloat16, of two dimensions or more, sides at most 65536.
+    The results hold no gradient: updates that ask for one are refused.
+    """
+
+    if not updates:
+        return []
+    kind = updates[0].dtype
+    if kind not in _MATRIX_TYPES or any(t.dtype != kind for t in updates):
+        raise TypeError(f"updates must all be float32 or all bfloat16, got {sorted({str(t.dtype) for t in updates})}")
+    shapes = tuple(map(_SHAPE, updates))
+    for i, shape in enumerate(shapes):
+        if len(shape) < 2 or max(shape[-2:]) > _MOST_SIDE:
+            raise ValueError(f"updates[{i}] must be matrices of at most 65536 rows and columns, got {tuple(shape)}")
+    if not 1 <= steps <= 1000:
+        raise ValueError(f"steps must be between 1 and 1000, got {steps}")
+    if len(coefficients) != 3 or not all(-_MOST_F32 <= c <= _MOST_F32 for c in coefficients):
+        raise ValueError(f"coefficients must be three finite float32, got {coefficients}")
+    if not 0.0 <= eps <= _MOST_F32:
+        raise ValueError(f"eps must be 0 or a positive float32, got {eps}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in updates):
+        raise RuntimeError("orthogonalize_tensors has no derivative: give it detached updates")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in updates):
+        raise NotImplementedError("orthogonalize_tensors has no derivative (jvp)")
+    _lib.require_one_device(*updates)
+    updates = [t.contiguous() for t in updates]
+    out = [torch.empty(s, dtype=torch.bfloat16, device=updates[0].device) for s in shapes]
+    size = _orthogonalize_workspace_bytes(shapes)
+    ws = _lib.workspace(size, updates[0].device)
+    table = _matrices(shapes)
+    table[0::4] = map(torch.Tensor.data_ptr, updates)
+    table[1::4] = map(torch.Tensor.data_ptr, out)
+    table = array.array("q", table)
+    _lib.call_on(updates[0].get_device(), "gptrig_orthogonalize", table.buffer_info()[0], len(out),
+                 _MATRIX_TYPES[kind], int(steps), *map(float, coefficients), float(eps), ws.data_ptr(), size)
+    return out

@@ -479,6 +479,28 @@ int gptrig_adamw_tensors(const gptrig_adamw_tensor* tensors, int count, int grad
 int gptrig_adamw_tensors_device_seed(const gptrig_adamw_tensor* tensors, int count, int grad_type, int state_bits,
                                      const float* tensor_hparams, double lr, double beta1, double beta2, int step,
                                      const float* clip_scale, const int64_t* seed, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Orthogonalised updates by Newton-Schulz products (no counterpart in the
+ * reference), over a list (host memory, copied by the call) of tensors of `count`
+ * matrices each: every matrix u [rows, cols] becomes X = u / (|u| + eps), |u| the
+ * root of its squares' sum, then `steps` times X <- a X + (b A + c A A) X with A =
+ * X X^T (of the transpose where rows > cols).  Inputs of type `type`, outputs bf16,
+ * contiguous, outputs 16-byte aligned; an output may overlap nothing else.  Rows and
+ * cols at most 65536; empty tensors are passed over.
+ * gptrig_orthogonalize_workspace_bytes (which reads counts and sizes only) of
+ * workspace, 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t count;
+  int rows, cols;
+} gptrig_matrices;
+size_t gptrig_orthogonalize_workspace_bytes(const gptrig_matrices* list, int count);
+int gptrig_orthogonalize(const gptrig_matrices* list, int count, int type, int steps, float a, float b, float c,
+                         float eps, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Per-chunk sums of squares of an f32 arena (for clipping before the update). */
 int gptrig_sq_norm_partials(const float* x, int64_t n_chunks, int chunk, float* partials, void* stream);
 /* norm = sqrt(sum partials); clip = min(1, grad_clip/(norm+1e-6)) (1 if grad_clip <= 0);

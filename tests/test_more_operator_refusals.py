@@ -6,9 +6,11 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from gptrig import _lib
 from gptrig.nn import embedding, gated_mlp
+from gptrig.optim import orthogonalize_tensors
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -121,3 +123,77 @@ def test_gated_entry_points_check_their_arguments():
     for n, d, f in ((1, 64, 64), (65536, 768, 2048), (5001, 1000, 2664)):
         size = _lib.query("gptrig_gated_mlp_bwd_workspace_bytes", n, d, f, d)
         assert 4 * n * f <= size <= 4 * n * f + 32 * 12 * d * f + 1024
+
+
+def test_orthogonalize_refusals():
+    u = torch.zeros((4, 8))
+    for bad in ([u.half()], [u.double()], [u, u.to(BF16)], [u.int()]):
+        with pytest.raises(TypeError, match="all be float32 or all bfloat16"):
+            orthogonalize_tensors(bad)
+    for bad in (u[0], u[0, 0], torch.empty((65537, 1)), torch.empty((1, 65537))):
+        with pytest.raises(ValueError, match=r"updates\[1\] must be matrices"):
+            orthogonalize_tensors([u, bad])
+    for steps in (0, -1, 1001):
+        with pytest.raises(ValueError, match="steps"):
+            orthogonalize_tensors([u], steps=steps)
+    for c in ((1.0, 2.0), (1.0, 2.0, float("nan")), (1.0, 2.0, 3.0, 4.0), (float("inf"), 0.0, 0.0), (1e39, 0, 0)):
+        with pytest.raises(ValueError, match="coefficients"):
+            orthogonalize_tensors([u], coefficients=c)
+    for eps in (-1e-7, float("nan"), float("inf"), 1e39):
+        with pytest.raises(ValueError, match="eps"):
+            orthogonalize_tensors([u], eps=eps)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        orthogonalize_tensors([u, u.clone().requires_grad_()])
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="jvp"):
+            orthogonalize_tensors([u, forward_ad.make_dual(u.clone(), u)])
+        with pytest.raises(RuntimeError, match="GPU"):
+            orthogonalize_tensors([u])
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+        orthogonalize_tensors([u.clone().requires_grad_()])
+    with pytest.raises(RuntimeError, match="GPU"):
+        orthogonalize_tensors([u])
+
+
+def matrices(*rows):
+    """Rows of gptrig_matrices: input, output, count, rows, columns."""
+
+    return (ctypes.c_int64 * (4 * len(rows)))(*(v for a, b, n, r, c in rows for v in (a, b, n, r | c << 32)))
+
+
+def test_orthogonalize_entry_points_check_their_arguments():
+    lib = _lib.lib()
+    at, f = 1 << 12, ctypes.c_float
+    size = lib.gptrig_orthogonalize_workspace_bytes
+
+    def call(table, count=1, type=1, steps=5, eps=1e-7, ws=at, nbytes=1 << 40):
+        return lib.gptrig_orthogonalize(table, count, type, steps, f(1.0), f(1.0), f(1.0), f(eps), ws, nbytes, None)
+
+    good = matrices((at, at, 2, 30, 50))
+    assert call(None) == -1 and call(good, count=-1) == -2 and call(good, type=2) == -3
+    assert call(good, steps=0) == -2 and call(good, eps=-1.0) == -2 and call(good, eps=float("nan")) == -2
+    assert call(matrices((0, at, 2, 30, 50))) == -1 and call(matrices((at, 0, 2, 30, 50))) == -1
+    assert call(matrices((at + 2, at, 2, 30, 50))) == -2 and call(matrices((at, at + 8, 2, 30, 50))) == -2
+    for row in ((at, at, -1, 30, 50), (at, at, 2, 65537, 50), (at, at, 2, 30, 65537)):
+        assert call(matrices(row)) == -2 and size(matrices(row), 1) == 0
+    assert call(good, ws=None) == -1 and call(good, ws=at + 8) == -2
+    assert call(good, nbytes=size(good, 1) - 1) == -6
+    assert call(matrices((0, 0, 0, 30, 50), (0, 0, 3, 0, 50)), count=2, ws=None, nbytes=0) == 0
+    assert call(None, count=0, ws=None, nbytes=0) == 0
+
+
+def test_orthogonalize_workspace():
+    """Three times X, A and B in 16 bits, rows padded to 8, and the sums: of one launch's tensors, which more matrices
+    than fit 2 GiB do not make larger."""
+
+    size = lambda *rows: _lib.lib().gptrig_orthogonalize_workspace_bytes(matrices(*rows), len(rows))  # noqa: E731
+    assert size() == 0 and size((0, 0, 0, 5, 5)) == 0
+    one = 3 * 2 * 30 * 56 + 2 * 2 * 30 * 32 + 8
+    assert one <= size((0, 0, 1, 30, 50)) <= one + 6 * 255
+    assert size((0, 0, 1, 30, 50)) == size((0, 0, 1, 50, 30))
+    assert 7 * one <= size((0, 0, 3, 30, 50), (0, 0, 4, 50, 30)) <= 7 * one + 6 * 255
+    assert 64 * one <= size(*[(0, 0, 1, 30, 50)] * 100) <= 64 * one + 6 * 255
+    for rows in ([(0, 0, 1000, 2048, 2048)], [(0, 0, 1, 4096, 4096)] * 60, [(0, 0, 10 ** 9, 100, 100)]):
+        assert (1 << 30) < size(*rows) <= (1 << 31) + 4096
+    big = size((0, 0, 3, 65536, 65536))
+    assert 10 * 2 ** 32 <= big <= 10 * 2 ** 32 + 2 ** 23

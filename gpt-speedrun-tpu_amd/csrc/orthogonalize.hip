@@ -47,9 +47,13 @@ struct Group {
   int sum0;      // the first one's index
   int64_t x0;    // first element in hi and lo
   int64_t a0;    // in A and B
-  __host__ __device__ int ldx() const { return (n + 7) & ~7; }
-  __host__ __device__ int lda() const { return (m + 7) & ~7; }
+  // Columns of X and of A with their padding: whole blocks of 32.
+  __host__ __device__ int ldx() const { return (n + 31) & ~31; }
+  __host__ __device__ int lda() const { return (m + 31) & ~31; }
 };
+
+// X, A and B lie 32-blocked with m rows (tile_core.h): element (r, c).
+__device__ __forceinline__ int64_t blocked(int m, int r, int c) { return ((int64_t)(c >> 5) * m + r) * 32 + (c & 31); }
 
 struct Tensor {
   const void* in;
@@ -60,18 +64,25 @@ struct Tensor {
 struct Args {
   Group g[kMostGroups];
   Tensor t[kMostTensors];
-  int first[kMostGroups + 1];  // each group's first workgroup of this launch, and the end
+  int first[kMostGroups + 1];  // each group's first workgroup of this launch, and the end in the others
   int groups, tensors;
   double* sums;
   f16 *hi, *hi_next, *lo, *A, *B;
   float a, b, c, eps;
 };
 
-// Workgroup -> group, and its index within it.
+// Workgroup -> group, and its index within it.  kSpread: each XCD takes a
+// contiguous share of every group, so that tiles that read the same rows meet in
+// one L2 and no XCD gets the matrices with the longest rows (the gram products of a
+// model's 48 matrices: 163 us with a contiguous share of the whole launch).
+template <bool kSpread>
 __device__ __forceinline__ int find_group(const Args& s, int pid, int& local) {
+  // (All of s.first in one load: a search would wait for each of its own.)
   int g = 0;
-  while (g + 1 < s.groups && pid >= s.first[g + 1]) ++g;  // uniform
+#pragma unroll
+  for (int i = 1; i < kMostGroups; ++i) g += pid >= s.first[i];
   local = pid - s.first[g];
+  if (kSpread) local = gemm::xcd_swizzle(local, s.first[g + 1] - s.first[g]);
   return g;
 }
 
@@ -96,7 +107,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(Args s) {
   __shared__ double shared[4];
   int local;
-  const int gi = find_group(s, blockIdx.x, local);
+  const int gi = find_group<false>(s, blockIdx.x, local);
   const Group& g = s.g[gi];
   const int matrix = local / g.parts, part = local % g.parts;
   const Tensor& t = find_tensor(s, gi, matrix);
@@ -120,7 +131,7 @@ __global__ void __launch_bounds__(256) ortho_load_kernel(Args s) {
   __shared__ double shared[4];
   __shared__ float turned[64][65];
   int local;
-  const int gi = find_group(s, blockIdx.x, local);
+  const int gi = find_group<false>(s, blockIdx.x, local);
   const Group& g = s.g[gi];
   const int ld = g.ldx();
   const int across = (ld + 63) / 64, down = (g.m + 63) / 64;
@@ -155,17 +166,38 @@ __global__ void __launch_bounds__(256) ortho_load_kernel(Args s) {
       x = (float)in[(int64_t)i * g.n + j];
     x *= scale;
     const f16 h = (f16)x;
-    hi[(int64_t)i * ld + j] = h;
-    lo[(int64_t)i * ld + j] = (f16)((x - (float)h) * kLow);
+    hi[blocked(g.m, i, j)] = h;
+    lo[blocked(g.m, i, j)] = (f16)((x - (float)h) * kLow);
   }
 }
 
-// Rows of a lower triangle's tile: t -> (i, j), j <= i.
-__device__ __forceinline__ void triangle(int t, int& i, int& j) {
-  i = (int)((__builtin_sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-  while (i * (i + 1) / 2 > t) --i;
-  while ((i + 1) * (i + 2) / 2 <= t) ++i;
-  j = t - i * (i + 1) / 2;
+// Tiles of a product: 64 MB features x 64 NB rows.
+struct Wide {
+  static constexpr int MB = 4, NB = 2, kSlabs = 1, kRing = 3;
+};
+struct Narrow {
+  static constexpr int MB = 1, NB = 1, kSlabs = 2, kRing = 4;
+};
+
+// The tiles of a symmetric result with features at or before a row, `down` rows of
+// tiles: a tile is 1 or 2 rows of tiles wide, row ti of them has ti / kWide + 1.
+template <class Shape>
+__host__ __device__ inline int triangle_tiles(int down) {
+  constexpr int kWide = Shape::MB / Shape::NB;
+  const int pairs = down / kWide;
+  return kWide * pairs * (pairs + 1) / 2 + (down % kWide) * (pairs + 1);
+}
+template <class Shape>
+__device__ __forceinline__ void triangle(int t, int& ti, int& tj) {
+  constexpr int kWide = Shape::MB / Shape::NB;
+  static_assert(kWide == 1 || kWide == 2, "see above");
+  // p: the last number of whole (pairs of) rows with at most t tiles.
+  int p = (int)((__builtin_sqrtf(1.0f + (8.0f / kWide) * t) - 1.0f) * 0.5f);
+  while (kWide * p * (p + 1) / 2 > t) --p;
+  while (kWide * (p + 1) * (p + 2) / 2 <= t) ++p;
+  const int rest = t - kWide * p * (p + 1) / 2;
+  ti = kWide * p + rest / (p + 1);
+  tj = rest % (p + 1);
 }
 
 __device__ __forceinline__ f16x8 to_f16(const float* v) {
@@ -179,21 +211,21 @@ enum { kGram = 0, kSquare = 1, kUpdate = 2, kLast = 3 };
 
 // One product of a step for every matrix.  The tile is computed as [feature][row]:
 // the lane holds 16 consecutive features of a row of the result.
-template <int kKind, int MB, int NB, int kSlabs>
-__global__ void __launch_bounds__(256) ortho_product_kernel(Args s) {
+template <int kKind, class Shape>
+__global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
   constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
-  typedef tile::Product<f16, MB, NB, kSymmetric, true, true, kSlabs> P;
+  constexpr int MB = Shape::MB, NB = Shape::NB;
+  typedef tile::Product<f16, MB, NB, kSymmetric, true, true, Shape::kSlabs, 1, Shape::kRing> P;
   int local;
-  const int gi = find_group(s, gemm::xcd_swizzle(blockIdx.x, gridDim.x), local);
+  const int gi = find_group<true>(s, blockIdx.x, local);
   const Group& g = s.g[gi];
   const int m = g.m, lda = g.lda(), ldx = g.ldx();
   const int down = (m + P::TN - 1) / P::TN;
   int matrix, ti, tj;
   if (kSymmetric) {
-    static_assert(!kSymmetric || MB == NB, "a triangle of square tiles");
-    const int tiles = down * (down + 1) / 2;
+    const int tiles = triangle_tiles<Shape>(down);
     matrix = local / tiles;
-    triangle(local % tiles, ti, tj);
+    triangle<Shape>(local % tiles, ti, tj);
   } else {
     const int tiles = down * ((ldx + P::TM - 1) / P::TM);
     matrix = local / tiles;
@@ -207,77 +239,87 @@ __global__ void __launch_bounds__(256) ortho_product_kernel(Args s) {
   const auto at = P::place();
   f32x16 acc[MB][NB];
   if constexpr (kKind == kGram)
-    P::run(acc, {hi, ldx}, {hi, ldx}, m, m, ldx, tj * P::TM, ti * P::TN, at);
+    P::run(acc, {hi, 0, m}, {hi, 0, m}, m, m, ldx, tj * P::TM, ti * P::TN, at);
   else if constexpr (kKind == kSquare)
-    P::run(acc, {A, lda}, {A, lda}, m, m, m, tj * P::TM, ti * P::TN, at);
+    P::run(acc, {A, 0, m}, {A, 0, m}, m, m, m, tj * P::TM, ti * P::TN, at);
   else
-    P::run(acc, {hi, ldx}, {B, lda}, ldx, m, m, tj * P::TM, ti * P::TN, at);
+    P::run(acc, {hi, 0, m}, {B, 0, m}, ldx, m, m, tj * P::TM, ti * P::TN, at);
   const int l32 = at.lane & 31, hl = at.lane >> 5;
+  // A symmetric result: where the wave's features lie against the tile's rows, in
+  // rows of tiles.  What lies past them is another tile's mirror image.
+  const int past = kSymmetric ? tj * (MB / NB) + at.wm * MB / (2 * NB) - ti : 0;
+  if (kSymmetric && past > 0) return;
+  bf16* out = nullptr;
+  if constexpr (kKind == kLast) {
+    const Tensor& t = find_tensor(s, gi, matrix);
+    out = t.out + (int64_t)(matrix - t.first) * m * g.n;
+  }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int row = ti * P::TN + 32 * (NB * at.wn + nb) + l32;
+    const int j_first = tj * P::TM + 32 * MB * at.wm + 16 * hl;  // block mb adds 32 mb
+    // What the rows hold already, all of it asked for before the first store: behind a
+    // store the loads could not be moved, and each would cost a trip to memory.
+    f16x8 old[MB][2], rest[MB][2];
+    const f16* const from = kSymmetric ? A : hi;
+    const f16* const from_low = s.lo + g.x0 + (int64_t)matrix * m * ldx;
+    if constexpr (kKind != kGram) {
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      const int f0 = tj * P::TM + 32 * (MB * at.wm + mb) + 16 * hl;
-      float v[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = acc[mb][nb][e];
-      if constexpr (kSymmetric) {
-        f16* const out = kKind == kGram ? A : B;
-        if constexpr (kKind == kSquare) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            f16x8 old{};
-            if (row < m && f0 + 8 * h < lda) old = *(const f16x8*)(A + (int64_t)row * lda + f0 + 8 * h);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[8 * h + e] = __builtin_fmaf(s.c, v[8 * h + e], s.b * (float)old[e]);
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (row < m && f0 + 8 * h < lda) *(f16x8*)(out + (int64_t)row * lda + f0 + 8 * h) = to_f16(v + 8 * h);
-        // (Past the last row and column both operands read zeros: so the rows' ends are zeros.)
-        if (ti != tj && row < lda) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (f0 + e < m) out[(int64_t)(f0 + e) * lda + row] = (f16)v[e];
-        }
-      } else if (row < m) {
-        const int64_t at0 = g.x0 + ((int64_t)matrix * m + row) * ldx + f0;
+      for (int mb = 0; mb < MB; ++mb) {
+        // (Of the last ones again where there are none: those are not used.)
+        const int64_t own = blocked(m, min(row, m - 1), min(j_first + 32 * mb, (kSymmetric ? lda : ldx) - 16));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (f0 + 8 * h >= ldx) continue;
-          const f16x8 high = *(const f16x8*)(s.hi + at0 + 8 * h), low = *(const f16x8*)(s.lo + at0 + 8 * h);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = __builtin_fmaf((float)low[e], 1.0f / kLow, (float)high[e]);
-            v[8 * h + e] = __builtin_fmaf(s.a, x, v[8 * h + e]);
-          }
-          if constexpr (kKind == kUpdate) {
-            const f16x8 next = to_f16(v + 8 * h);
-            float rest[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) rest[e] = (v[8 * h + e] - (float)next[e]) * kLow;
-            *(f16x8*)(s.hi_next + at0 + 8 * h) = next;
-            *(f16x8*)(s.lo + at0 + 8 * h) = to_f16(rest);  // (this lane's own, read above)
-          }
+          old[mb][h] = *(const f16x8*)(from + own + 8 * h);
+          if constexpr (!kSymmetric) rest[mb][h] = *(const f16x8*)(from_low + own + 8 * h);
         }
-        if constexpr (kKind == kLast) {
-          const Tensor& t = find_tensor(s, gi, matrix);
-          bf16* const out = t.out + (int64_t)(matrix - t.first) * m * g.n;
-          if (g.tall) {
+      }
+    }
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (f0 + e < g.n) out[(int64_t)(f0 + e) * m + row] = (bf16)v[e];
-          } else if (g.n % 8 == 0) {
+    for (int mb = 0; mb < MB; ++mb) {
+      const int j0 = j_first + 32 * mb;
+      float v[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (f0 + 8 * h < g.n) *(bf16x8*)(out + (int64_t)row * g.n + f0 + 8 * h) = pack8(v + 8 * h);
-          } else {
+      for (int e = 0; e < 16; ++e) {
+        v[e] = acc[mb][nb][e];
+        if constexpr (kKind == kSquare) v[e] = __builtin_fmaf(s.c, v[e], s.b * (float)old[mb][e / 8][e % 8]);
+        if constexpr (!kSymmetric)
+          v[e] = __builtin_fmaf(s.a, __builtin_fmaf((float)rest[mb][e / 8][e % 8], 1.0f / kLow, (float)old[mb][e / 8][e % 8]),
+                                v[e]);
+      }
+      if (row < m && j0 < (kSymmetric ? lda : ldx) && kKind != kLast) {
+        const int64_t own = blocked(m, row, j0);
+        f16* const to = kKind == kGram ? A + own : kKind == kSquare ? B + own : s.hi_next + (hi - s.hi) + own;
+        const f16x8 low = to_f16(v), high = to_f16(v + 8);
+        *(f16x8*)to = low;
+        *(f16x8*)(to + 8) = high;
+        if constexpr (kKind == kUpdate) {  // (this lane's own, read above)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (f0 + e < g.n) out[(int64_t)row * g.n + f0 + e] = (bf16)v[e];
-          }
+          for (int e = 0; e < 16; ++e) v[e] = (v[e] - (float)(e < 8 ? low[e & 7] : high[e & 7])) * kLow;
+          *(f16x8*)(s.lo + (hi - s.hi) + own) = to_f16(v);
+          *(f16x8*)(s.lo + (hi - s.hi) + own + 8) = to_f16(v + 8);
+        }
+      }
+      // The mirrored tile.  (Past the last row and column both operands read zeros, and so are the rows' ends.)
+      if (kSymmetric && past < 0 && row < lda) {
+        f16* const result = kKind == kGram ? A : B;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (j0 + e < m) result[blocked(m, j0 + e, row)] = (f16)v[e];
+      }
+      if (kKind == kLast && row < m) {
+        if (g.tall) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (j0 + e < g.n) out[(int64_t)(j0 + e) * m + row] = (bf16)v[e];
+        } else if (g.n % 8 == 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (j0 + 8 * h < g.n) *(bf16x8*)(out + (int64_t)row * g.n + j0 + 8 * h) = pack8(v + 8 * h);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (j0 + e < g.n) out[(int64_t)row * g.n + j0 + e] = (bf16)v[e];
         }
       }
     }
@@ -343,7 +385,12 @@ struct Walk {
       }
       if (take > t.count - inside) take = t.count - inside;
       if (take > 65536) take = 65536;
-      if (gi == s.groups) s.g[s.groups++] = shape;
+      if (gi == s.groups) {
+        // Longest rows first: their workgroups take longest in the gram products.
+        for (gi = s.groups++; gi > 0 && s.g[gi - 1].n < shape.n; --gi) s.g[gi] = s.g[gi - 1];
+        s.g[gi] = shape;
+        for (int i = 0; i < s.tensors; ++i) s.t[i].group += s.t[i].group >= gi;
+      }
       Group& g = s.g[gi];
       const int64_t size = (int64_t)t.rows * t.cols;
       s.t[s.tensors++] =
@@ -392,35 +439,31 @@ int64_t count_groups(Args& s, F each) {
     s.first[i] = (int)total;
     total += each(s.g[i]) * s.g[i].count;
   }
-  s.first[s.groups] = (int)total;
+  for (int i = s.groups; i <= kMostGroups; ++i) s.first[i] = (int)total;
   return total;
 }
 
-template <int kTile>
-int64_t symmetric_tiles(const Group& g) {
-  const int64_t down = ceil_div(g.m, kTile);
-  return down * (down + 1) / 2;
-}
-template <int kTile>
-int64_t update_tiles(const Group& g) {
-  return (int64_t)ceil_div(g.m, kTile) * ceil_div(g.ldx(), kTile);
-}
-
-template <int kKind, int MB, int kSlabs>
-int launch_product(Args& s, hipStream_t stream) {
-  constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
-  const int64_t total = count_groups(s, kSymmetric ? symmetric_tiles<64 * MB> : update_tiles<64 * MB>);
-  ortho_product_kernel<kKind, MB, MB, kSlabs><<<(unsigned)total, 256, 0, stream>>>(s);
-  GPTRIG_CHECK_LAUNCH();
-  return GPTRIG_OK;
+template <int kKind, class Shape>
+int64_t count_tiles(Args& s) {
+  return count_groups(s, [](const Group& g) -> int64_t {
+    const int64_t down = ceil_div(g.m, 64 * Shape::NB);
+    return kKind == kGram || kKind == kSquare ? triangle_tiles<Shape>(down)
+                                              : down * ceil_div(g.ldx(), 64 * Shape::MB);
+  });
 }
 
 template <int kKind>
 int product(Args& s, hipStream_t stream) {
-  constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
-  // The wider tile needs fewer reads an operation; the narrower one fills the chip with fewer matrices.
-  const int64_t wide = count_groups(s, kSymmetric ? symmetric_tiles<128> : update_tiles<128>);
-  return wide >= gemm::device_cus() ? launch_product<kKind, 2, 1>(s, stream) : launch_product<kKind, 1, 2>(s, stream);
+  // The wide tile needs fewer reads an operation; the narrow one fills the chip with fewer matrices.
+  const int64_t wide = count_tiles<kKind, Wide>(s);
+  if (wide >= gemm::device_cus()) {
+    ortho_product_kernel<kKind, Wide><<<(unsigned)wide, 256, 0, stream>>>(s);
+  } else {
+    const int64_t narrow = count_tiles<kKind, Narrow>(s);
+    ortho_product_kernel<kKind, Narrow><<<(unsigned)narrow, 256, 0, stream>>>(s);
+  }
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
 }
 
 }  // namespace

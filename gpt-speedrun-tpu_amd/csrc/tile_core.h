@@ -8,8 +8,8 @@
 // shortens a product that has many k and few tiles.
 //
 // Staging is the GEMM core's (gemm_core.h): buffer loads copy 16-byte chunks from
-// global memory into LDS through a ring of four stages, each stage waited for with
-// an exact vmcnt and one barrier; operands lie K-major ([mn][k]) or MN-major
+// global memory into LDS through a ring of three or four stages, each stage waited
+// for with an exact vmcnt and one barrier; operands lie K-major ([mn][k]) or MN-major
 // ([k][mn]) as they are in memory, swizzled so that a quarter-wave's reads meet
 // different banks, MN-major fragments read with ds_read_b64_tr_b16.  A stage is
 // 32 kSlabs deep.  K is any multiple of 8 (K-major) or any number (MN-major); what
@@ -35,10 +35,16 @@ __device__ __forceinline__ f32x16 mma(i16x8 a, i16x8 b, f32x16 c, f16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A matrix operand of 16-bit elements with leading dimension ld.
+// A matrix operand of 16-bit elements: row-major with leading dimension ld, or (blk >
+// 0) "32-blocked": element (r, c) at ((c / 32) * blk + r) * 32 + c % 32, column blocks
+// of 32 one after another, each of blk rows of 64 bytes.  The copies of either kind
+// of slab then read whole 128-byte lines; 64-byte pieces of a K-major operand's rows
+// take the address unit as long as whole lines would, twice the time a byte (gram
+// products of 48 matrices of 768 rows: 117 us, 85% of it with the address unit busy).
 struct Operand {
   const void* p;
   int64_t ld;
+  int64_t blk = 0;
 };
 
 template <int kBytes, int kStage>
@@ -63,8 +69,14 @@ struct Source {
 
   // mn0: the tile's first row, MN: the operand's rows; K range [k_begin, k_end).
   __device__ __forceinline__ void init(Operand op, int mn0, int MN, int k_begin, int k_end, int wave, int lane) {
-    base = (const char*)op.p + 2 * (KMAJOR ? (int64_t)mn0 * op.ld + k_begin : (int64_t)k_begin * op.ld + mn0);
-    step = 2 * (KMAJOR ? (int64_t)kDepth : (int64_t)kDepth * op.ld);
+    // (k_begin is a multiple of 32 and mn0 of 64: blocked stages and tiles start on a block.)
+    if (op.blk) {
+      base = (const char*)op.p + (KMAJOR ? (int64_t)(k_begin >> 5) * op.blk + mn0 : (int64_t)(mn0 >> 5) * op.blk + k_begin) * 64;
+      step = KMAJOR ? op.blk * kSlabs * 64 : (int64_t)kDepth * 64;
+    } else {
+      base = (const char*)op.p + 2 * (KMAJOR ? (int64_t)mn0 * op.ld + k_begin : (int64_t)k_begin * op.ld + mn0);
+      step = 2 * (KMAJOR ? (int64_t)kDepth : (int64_t)kDepth * op.ld);
+    }
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const int b = wave * P + j, slab = b / (TM / 16), blk = b % (TM / 16);
@@ -73,62 +85,71 @@ struct Source {
         const int row = blk * 16 + (lane >> 2);
         k = 32 * slab + 8 * ((lane & 3) ^ ((row >> 2) & 3));
         m = row;
-        off[j] = 2u * (uint32_t)((int64_t)row * op.ld + k);
+        off[j] = 2u * (uint32_t)(op.blk ? ((int64_t)slab * op.blk + row) * 32 + (k & 31) : (int64_t)row * op.ld + k);
       } else {
         constexpr int kChunks = TM / 8;
         const int row = blk * (512 / TM) + lane / kChunks;
         k = 32 * slab + row;
         m = 8 * ((lane % kChunks) ^ swizzle(row));
-        off[j] = 2u * (uint32_t)((int64_t)k * op.ld + m);
+        off[j] = 2u * (uint32_t)(op.blk ? ((int64_t)(m >> 5) * op.blk + k) * 32 + (m & 31) : (int64_t)k * op.ld + m);
       }
       const int rem = k_end - k_begin - k;
       nvalid[j] = (mn0 + m < MN && rem > 0) ? (rem + kDepth - 1) / kDepth : 0;
     }
   }
 
-  __device__ __forceinline__ void issue(lds16* slabs, int kt, int wave) const {
+  // Stage kt into the slabs at element `offset` of a stage array.
+  __device__ __forceinline__ void issue(lds16* array, int offset, int kt, int wave) const {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(base + kt * step, gemm::kRsrcRange);
 #pragma unroll
     for (int j = 0; j < P; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (gemm::lds_void*)(slabs + (wave * P + j) * 512), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (gemm::lds_void*)(array + (offset + (wave * P + j) * 512)), 16,
                                                kt < nvalid[j] ? off[j] : gemm::kOffZero, 0, 0, 0);
   }
 };
 
-// Fragment of rows r0 .. r0 + 31 at k-chunk kc (16 deep) of a stage's slabs.
+// Fragment of rows r0 + 32 block .. + 31 at k-chunk kc (16 deep) of the slabs at
+// element `offset` + kOffset of a stage array.
 // kContiguous: in gemm::contiguous_row's order, so that a lane's accumulator
 // elements 0 .. 15 are 16 consecutive rows.
-template <int TM, bool KMAJOR, bool kContiguous>
-__device__ __forceinline__ i16x8 frag(const lds16* slabs, int r0, int kc, int lane) {
-  const lds16* slab = slabs + (kc >> 1) * TM * 32;
+// The lane's part of an address passes through an empty asm: the compiler finds an
+// access's array through a few additions only, would make more of one sum, and takes
+// an access without an array to meet every copy in flight, for which it then waits.
+template <int TM, bool KMAJOR, bool kContiguous, int kOffset>
+__device__ __forceinline__ i16x8 frag(const lds16* array, int offset, int r0, int block, int kc, int lane) {
   const int hl = lane >> 5;
   if (KMAJOR) {
     const int row = r0 + (kContiguous ? gemm::contiguous_row(lane & 31) : (lane & 31));
     const int c = 2 * (kc & 1) + hl;
-    return *(const lds16x8*)(slab + row * 32 + 8 * (c ^ ((row >> 2) & 3)));
+    int at = offset + row * 32 + 8 * (c ^ ((row >> 2) & 3));  // (the same for row + 32)
+    asm("" : "+v"(at));
+    return *(const lds16x8*)(array + at + (kOffset + 1024 * block + (kc >> 1) * TM * 32));
   } else {
     const int cq = lane & 15, q = 4 * ((lane >> 4) & 1) + (cq & 3);
-    const int m = r0 + (kContiguous ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
-    const int k = 16 * (kc & 1) + 8 * hl + (cq >> 2);
-    typedef Source<TM, false, 1> S;
-    const lds16* lo = slab + k * TM + 8 * ((m >> 3) ^ S::swizzle(k)) + 4 * ((m >> 2) & 1);
-    const lds16* hi = slab + (k + 4) * TM + 8 * ((m >> 3) ^ S::swizzle(k + 4)) + 4 * ((m >> 2) & 1);
+    const int m = r0 + 32 * block + (kContiguous ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
+    const int k = 8 * hl + (cq >> 2);
+    typedef Source<TM, false, 1> S;  // (its swizzle is the same for k, k + 4 and k + 16)
+    int at = offset + k * TM + 8 * ((m >> 3) ^ S::swizzle(k)) + 4 * ((m >> 2) & 1);
+    asm("" : "+v"(at));
+    const lds16* const lo = array + at + (kOffset + (kc >> 1) * TM * 32 + (kc & 1) * 16 * TM);
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)lo);
-    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)hi);
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(lo + 4 * TM));
     return i16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 }
 
 // T: bf16 or f16.  MB, NB: the tile in units of 64.  AK, BKM: K-major operands.
 // kContiguous: rows of A in contiguous_row's order.
-template <class T, int MB, int NB, bool AK, bool BKM, bool kContiguous, int kSlabs = 1, int kGroups = 1>
+template <class T, int MB, int NB, bool AK, bool BKM, bool kContiguous, int kSlabs = 1, int kGroups = 1,
+          int kRing = 4>
 struct Product {
   static constexpr int TM = 64 * MB, TN = 64 * NB, kThreads = 256 * kGroups;
   static constexpr int kStageA = TM * 32 * kSlabs, kStageB = TN * 32 * kSlabs;  // elements
   static constexpr int kStageBytes = 2 * kGroups * (kStageA + kStageB);
   static constexpr int kChunks = 2 * kSlabs, kDepth = 32 * kSlabs;
   static constexpr int kLoads = (TM + TN) / 64 * kSlabs;  // a wave's copies of a stage
-  static_assert(4 * kStageBytes <= 160 * 1024, "the ring does not fit LDS");
+  static_assert(kRing * kStageBytes <= 160 * 1024, "the ring does not fit LDS");
+  static_assert(kRing == 3 || kRing == 4, "stages in flight");
   static_assert(kGroups <= 4 && (kGroups == 1 || TM * TN * 4 <= kStageBytes), "parts are joined in the stage arrays");
 
   // Position of a wave: its set, and within it 2 x 2.
@@ -140,11 +161,6 @@ struct Product {
     return Place{(int)threadIdx.x & 63, w & 3, w >> 2, w & 1, (w >> 1) & 1};
   }
 
-  template <int S>
-  static __device__ __forceinline__ lds16* stage(int group) {
-    return stage_array<kStageBytes, S>() + group * (kStageA + kStageB);
-  }
-
   struct State {
     Source<TM, AK, kSlabs> a;
     Source<TN, BKM, kSlabs> b;
@@ -153,19 +169,22 @@ struct Product {
 
   template <int S>
   static __device__ __forceinline__ void fill(const State& s, int kt) {
-    lds16* st = stage<S>(s.at.group);
-    s.a.issue(st, kt, s.at.wave);
-    s.b.issue(st + kStageA, kt, s.at.wave);
+    lds16* const array = stage_array<kStageBytes, S>();
+    const int offset = s.at.group * (kStageA + kStageB);
+    s.a.issue(array, offset, kt, s.at.wave);
+    s.b.issue(array, offset + kStageA, kt, s.at.wave);
   }
 
   template <int S>
   static __device__ __forceinline__ void read(i16x8 (&a)[MB], i16x8 (&b)[NB], const State& s, int kc) {
-    const lds16* st = stage<S>(s.at.group);
+    const lds16* const array = stage_array<kStageBytes, S>();
+    const int offset = s.at.group * (kStageA + kStageB);
 #pragma unroll
     for (int i = 0; i < MB; ++i)
-      a[i] = frag<TM, AK, kContiguous>(st, 32 * (MB * s.at.wm + i), kc, s.at.lane);
+      a[i] = frag<TM, AK, kContiguous, 0>(array, offset, 32 * MB * s.at.wm, i, kc, s.at.lane);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) b[i] = frag<TN, BKM, false>(st + kStageA, 32 * (NB * s.at.wn + i), kc, s.at.lane);
+    for (int i = 0; i < NB; ++i)
+      b[i] = frag<TN, BKM, false, kStageA>(array, offset, 32 * NB * s.at.wn, i, kc, s.at.lane);
   }
 
   template <int S>
@@ -178,10 +197,10 @@ struct Product {
         read<S>(a[next], b[next], s, kc + 1);
       } else {
         // The next stage is there; every wave has read this one, which is refilled.
-        __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(2 * kLoads));
+        __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((kRing - 2) * kLoads));
         wg_barrier();
-        fill<S>(s, kt + 4);
-        read<(S + 1) % 4>(a[next], b[next], s, 0);
+        fill<S>(s, kt + kRing);
+        read<(S + 1) % kRing>(a[next], b[next], s, 0);
       }
       GEMM_SCHED_FENCE();
 #pragma unroll
@@ -206,7 +225,7 @@ struct Product {
     // Whole stages a group, whole rounds of the ring.
     const int share = ((K + kGroups - 1) / kGroups + kDepth - 1) / kDepth * kDepth;
     const int begin = min(K, at.group * share), end = min(K, begin + share);
-    const int nk = (share / kDepth + 3) & ~3;
+    const int nk = (share / kDepth + kRing - 1) / kRing * kRing;
     State s;
     s.at = at;
     s.a.init(A, tm0, M, begin, end, at.wave, at.lane);
@@ -214,16 +233,16 @@ struct Product {
     fill<0>(s, 0);
     fill<1>(s, 1);
     fill<2>(s, 2);
-    fill<3>(s, 3);
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(3 * kLoads));
+    if constexpr (kRing == 4) fill<3>(s, 3);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((kRing - 1) * kLoads));
     wg_barrier();
     i16x8 a[2][MB], b[2][NB];
     read<0>(a[0], b[0], s, 0);
-    for (int kt = 0; kt < nk; kt += 4) {
+    for (int kt = 0; kt < nk; kt += kRing) {
       step<0>(acc, a, b, s, kt);
       step<1>(acc, a, b, s, kt + 1);
       step<2>(acc, a, b, s, kt + 2);
-      step<3>(acc, a, b, s, kt + 3);
+      if constexpr (kRing == 4) step<3>(acc, a, b, s, kt + 3);
     }
     GEMM_WAIT_VM0_LGKM0();
     wg_barrier();

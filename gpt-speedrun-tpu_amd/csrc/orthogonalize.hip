@@ -102,6 +102,38 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
   return ((shared[0] + shared[1]) + shared[2]) + shared[3];
 }
 
+// A float32 that stays one: without it the compiler may round a product or a sum to
+// float16 from its exact value where the float16 is stored and from its float32 value
+// where the rest is taken from it, and in one of some thousand the two differ by a
+// step.
+__device__ __forceinline__ float settled(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ f16x8 to_f16(const float* v) {
+  f16x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (f16)v[e];
+  return r;
+}
+
+// Four consecutive elements of a row, as many as there are.
+template <typename T>
+__device__ __forceinline__ f32x4 load_four(const T* from, int left, bool whole) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  f32x4 v{};
+  if (whole && left >= 4) {
+    const T4 x = *reinterpret_cast<const T4*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)x[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) v[e] = (float)from[e];
+  }
+  return v;
+}
+
 // Sums of squares in 64 bits: no overflow for any float32, whatever the scale.
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(Args s) {
@@ -114,11 +146,13 @@ __global__ void __launch_bounds__(256) ortho_norm_kernel(Args s) {
   const int64_t size = (int64_t)g.m * g.n;
   const T* in = (const T*)t.in + (matrix - t.first) * size;
   const int64_t begin = (int64_t)part * kPart, end = begin + kPart < size ? begin + kPart : size;
+  const bool whole = (uintptr_t)(in + begin) % (4 * sizeof(T)) == 0;
   double sum = 0.0;
 #pragma unroll 4
-  for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-    const double v = (double)(float)in[i];
-    sum = __builtin_fma(v, v, sum);
+  for (int64_t i = begin + 4 * threadIdx.x; i < end; i += 4 * 256) {
+    const f32x4 v = load_four(in + i, end - i < 4 ? (int)(end - i) : 4, whole);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __builtin_fma((double)v[e], (double)v[e], sum);
   }
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) s.sums[g.sum0 + (int64_t)matrix * g.parts + part] = sum;
@@ -137,37 +171,50 @@ __global__ void __launch_bounds__(256) ortho_load_kernel(Args s) {
   const int across = (ld + 63) / 64, down = (g.m + 63) / 64;
   const int matrix = local / (across * down), at = local % (across * down);
   const int i0 = at / across * 64, j0 = at % across * 64;
+  const Tensor& t = find_tensor(s, gi, matrix);
+  const int64_t size = (int64_t)g.m * g.n;
+  const T* in = (const T*)t.in + (matrix - t.first) * size;
+  const int quad = 4 * (threadIdx.x & 15), line = threadIdx.x >> 4;  // of 64 elements, of 16 lines four times
+  // Rows of four elements are aligned where the row length and the tensor are.
+  const bool whole = (g.tall ? g.m : g.n) % 4 == 0 && (uintptr_t)in % (4 * sizeof(T)) == 0;
+  f32x4 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = 16 * k + line;
+    const int row = (g.tall ? j0 : i0) + r, col = (g.tall ? i0 : j0) + quad;  // of the tensor
+    const int rows = g.tall ? g.n : g.m, cols = g.tall ? g.m : g.n;
+    v[k] = row < rows ? load_four(in + (int64_t)row * cols + col, cols - col, whole) : f32x4{};
+  }
   double sum = 0.0;
   for (int i = threadIdx.x; i < g.parts; i += 256) sum += s.sums[g.sum0 + (int64_t)matrix * g.parts + i];
   sum = block_sum(sum, shared);
   const float scale = (float)(1.0 / (sqrt(sum) + (double)s.eps));
-  const Tensor& t = find_tensor(s, gi, matrix);
-  const int64_t size = (int64_t)g.m * g.n;
-  const T* in = (const T*)t.in + (matrix - t.first) * size;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (g.tall) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {  // row j0 + r of the tensor, column i0 + lane
-      const int r = 4 * k + wave, j = j0 + r, i = i0 + lane;
-      turned[r][lane] = j < g.n && i < g.m ? (float)in[(int64_t)j * g.m + i] : 0.f;
-    }
-    __syncthreads();
-  }
-  f16* const hi = s.hi + g.x0 + (int64_t)matrix * g.m * ld;
-  f16* const lo = s.lo + g.x0 + (int64_t)matrix * g.m * ld;
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const int r = 4 * k + wave, i = i0 + r, j = j0 + lane;
+      for (int e = 0; e < 4; ++e) turned[16 * k + line][quad + e] = v[k][e];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = turned[quad + e][16 * k + line];
+  }
+  typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+  const int64_t x0 = g.x0 + (int64_t)matrix * g.m * ld;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = i0 + 16 * k + line, j = j0 + quad;
     if (i >= g.m || j >= ld) continue;
-    float x = 0.f;
-    if (g.tall)
-      x = turned[lane][r];
-    else if (j < g.n)
-      x = (float)in[(int64_t)i * g.n + j];
-    x *= scale;
-    const f16 h = (f16)x;
-    hi[blocked(g.m, i, j)] = h;
-    lo[blocked(g.m, i, j)] = (f16)((x - (float)h) * kLow);
+    f16x4 high, low;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = settled(v[k][e] * scale);
+      high[e] = (f16)x;
+      low[e] = (f16)((x - (float)high[e]) * kLow);
+    }
+    *(f16x4*)(s.hi + x0 + blocked(g.m, i, j)) = high;
+    *(f16x4*)(s.lo + x0 + blocked(g.m, i, j)) = low;
   }
 }
 
@@ -200,12 +247,6 @@ __device__ __forceinline__ void triangle(int t, int& ti, int& tj) {
   tj = rest % (p + 1);
 }
 
-__device__ __forceinline__ f16x8 to_f16(const float* v) {
-  f16x8 r;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = (f16)v[e];
-  return r;
-}
 
 enum { kGram = 0, kSquare = 1, kUpdate = 2, kLast = 3 };
 
@@ -217,7 +258,9 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
   constexpr int MB = Shape::MB, NB = Shape::NB;
   typedef tile::Product<f16, MB, NB, kSymmetric, true, true, Shape::kSlabs, 1, Shape::kRing> P;
   int local;
-  const int gi = find_group<true>(s, blockIdx.x, local);
+  // Every other product walks the matrices backwards: it begins with those that the
+  // one before ended with and that the caches still hold.
+  const int gi = find_group<true>(s, kSymmetric ? blockIdx.x : gridDim.x - 1 - blockIdx.x, local);
   const Group& g = s.g[gi];
   const int m = g.m, lda = g.lda(), ldx = g.ldx();
   const int down = (m + P::TN - 1) / P::TN;
@@ -284,8 +327,8 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
         v[e] = acc[mb][nb][e];
         if constexpr (kKind == kSquare) v[e] = __builtin_fmaf(s.c, v[e], s.b * (float)old[mb][e / 8][e % 8]);
         if constexpr (!kSymmetric)
-          v[e] = __builtin_fmaf(s.a, __builtin_fmaf((float)rest[mb][e / 8][e % 8], 1.0f / kLow, (float)old[mb][e / 8][e % 8]),
-                                v[e]);
+          v[e] = settled(__builtin_fmaf(
+              s.a, __builtin_fmaf((float)rest[mb][e / 8][e % 8], 1.0f / kLow, (float)old[mb][e / 8][e % 8]), v[e]));
       }
       if (row < m && j0 < (kSymmetric ? lda : ldx) && kKind != kLast) {
         const int64_t own = blocked(m, row, j0);

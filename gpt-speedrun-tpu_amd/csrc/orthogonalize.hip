@@ -32,6 +32,7 @@ namespace {
 
 using tile::f16;
 using tile::f16x8;
+using tile::i16x8;
 
 constexpr int kMostGroups = 16;   // shapes of a launch
 constexpr int kMostTensors = 64;  // tensors of a launch
@@ -287,82 +288,108 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
     P::run(acc, {A, 0, m}, {A, 0, m}, m, m, m, tj * P::TM, ti * P::TN, at);
   else
     P::run(acc, {hi, 0, m}, {B, 0, m}, ldx, m, m, tj * P::TM, ti * P::TN, at);
-  const int l32 = at.lane & 31, hl = at.lane >> 5;
   // A symmetric result: where the wave's features lie against the tile's rows, in
   // rows of tiles.  What lies past them is another tile's mirror image.
   const int past = kSymmetric ? tj * (MB / NB) + at.wm * MB / (2 * NB) - ti : 0;
   if (kSymmetric && past > 0) return;
+  const int lane = at.lane, ld = kSymmetric ? lda : ldx;
+  const tile::Block block = P::block(at, 0), block_low = P::block(at, 1);
+  f16* const lo = s.lo + (hi - s.hi);
   bf16* out = nullptr;
   if constexpr (kKind == kLast) {
     const Tensor& t = find_tensor(s, gi, matrix);
     out = t.out + (int64_t)(matrix - t.first) * m * g.n;
   }
+  // A block's two lines of the lane, in 16 bits: `to` its place in a blocked matrix.
+  auto store = [&](const tile::Block& b, f16* to, int rows) {
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      const i16x8 v = b.get_line(it, lane);
+      if (tile::Block::line_row(it, lane) < rows) *(i16x8*)(to + 512 * it + 8 * lane) = v;
+    }
+  };
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int row = ti * P::TN + 32 * (NB * at.wn + nb) + l32;
-    const int j_first = tj * P::TM + 32 * MB * at.wm + 16 * hl;  // block mb adds 32 mb
-    // What the rows hold already, all of it asked for before the first store: behind a
-    // store the loads could not be moved, and each would cost a trip to memory.
-    f16x8 old[MB][2], rest[MB][2];
-    const f16* const from = kSymmetric ? A : hi;
-    const f16* const from_low = s.lo + g.x0 + (int64_t)matrix * m * ldx;
+    const int row0 = ti * P::TN + 32 * (NB * at.wn + nb), f0 = tj * P::TM + 32 * MB * at.wm;
+    if (row0 >= m) break;  // (uniform, as every condition on row0 and f0)
+    // What the blocks hold already, all of it asked for before the first store: behind
+    // a store the loads could not be moved, and each would cost a trip to memory.
+    i16x8 old[MB][2], rest[MB][2];
     if constexpr (kKind != kGram) {
+      const f16* const from = kSymmetric ? A : hi;
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        // (Of the last ones again where there are none: those are not used.)
-        const int64_t own = blocked(m, min(row, m - 1), min(j_first + 32 * mb, (kSymmetric ? lda : ldx) - 16));
+      for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          old[mb][h] = *(const f16x8*)(from + own + 8 * h);
-          if constexpr (!kSymmetric) rest[mb][h] = *(const f16x8*)(from_low + own + 8 * h);
+        for (int it = 0; it < 2; ++it) {
+          // (Of the last row and block again where there are none: those are not used.)
+          const int row = min(row0 + tile::Block::line_row(it, lane), m - 1);
+          const int64_t own = blocked(m, row, min(f0 + 32 * mb, ld - 32) + tile::Block::line_feature(lane));
+          old[mb][it] = *(const i16x8*)(from + own);
+          if constexpr (!kSymmetric) rest[mb][it] = *(const i16x8*)(lo + own);
         }
-      }
     }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      const int j0 = j_first + 32 * mb;
+      const int j0 = f0 + 32 * mb;
+      if (j0 >= ld) break;
+      const int64_t own = blocked(m, row0, j0);
+      if constexpr (kKind != kGram) block.put_lines(lane, old[mb][0], old[mb][1]);
+      if constexpr (!kSymmetric) block_low.put_lines(lane, rest[mb][0], rest[mb][1]);
       float v[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        v[e] = acc[mb][nb][e];
-        if constexpr (kKind == kSquare) v[e] = __builtin_fmaf(s.c, v[e], s.b * (float)old[mb][e / 8][e % 8]);
-        if constexpr (!kSymmetric)
-          v[e] = settled(__builtin_fmaf(
-              s.a, __builtin_fmaf((float)rest[mb][e / 8][e % 8], 1.0f / kLow, (float)old[mb][e / 8][e % 8]), v[e]));
-      }
-      if (row < m && j0 < (kSymmetric ? lda : ldx) && kKind != kLast) {
-        const int64_t own = blocked(m, row, j0);
-        f16* const to = kKind == kGram ? A + own : kKind == kSquare ? B + own : s.hi_next + (hi - s.hi) + own;
-        const f16x8 low = to_f16(v), high = to_f16(v + 8);
-        *(f16x8*)to = low;
-        *(f16x8*)(to + 8) = high;
-        if constexpr (kKind == kUpdate) {  // (this lane's own, read above)
+      for (int h = 0; h < 2; ++h) {
+        f16x8 x{}, x_low{};
+        if constexpr (kKind != kGram) x = __builtin_bit_cast(f16x8, block.get_run(lane, h));
+        if constexpr (!kSymmetric) x_low = __builtin_bit_cast(f16x8, block_low.get_run(lane, h));
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = (v[e] - (float)(e < 8 ? low[e & 7] : high[e & 7])) * kLow;
-          *(f16x8*)(s.lo + (hi - s.hi) + own) = to_f16(v);
-          *(f16x8*)(s.lo + (hi - s.hi) + own + 8) = to_f16(v + 8);
+        for (int e = 0; e < 8; ++e) {
+          float& r = v[8 * h + e];
+          r = acc[mb][nb][8 * h + e];
+          if constexpr (kKind == kSquare) r = __builtin_fmaf(s.c, r, s.b * (float)x[e]);
+          if constexpr (!kSymmetric)
+            r = settled(__builtin_fmaf(s.a, __builtin_fmaf((float)x_low[e], 1.0f / kLow, (float)x[e]), r));
         }
       }
-      // The mirrored tile.  (Past the last row and column both operands read zeros, and so are the rows' ends.)
-      if (kSymmetric && past < 0 && row < lda) {
-        f16* const result = kKind == kGram ? A : B;
+      const int rows = m - row0;
+      if constexpr (kKind != kLast) {
+        f16* const result = kKind == kGram ? A : kKind == kSquare ? B : s.hi_next + (hi - s.hi);
+        const i16x8 low = __builtin_bit_cast(i16x8, to_f16(v)), high = __builtin_bit_cast(i16x8, to_f16(v + 8));
+        block.put_run(lane, low, high);
+        store(block, result + own, rows);
+        if constexpr (kKind == kUpdate) {  // (the lines that this lane has read)
+          const f16x8 l = __builtin_bit_cast(f16x8, low), u = __builtin_bit_cast(f16x8, high);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (j0 + e < m) result[blocked(m, j0 + e, row)] = (f16)v[e];
-      }
-      if (kKind == kLast && row < m) {
-        if (g.tall) {
+          for (int e = 0; e < 16; ++e) v[e] = (v[e] - (float)(e < 8 ? l[e & 7] : u[e & 7])) * kLow;
+          block_low.put_run(lane, __builtin_bit_cast(i16x8, to_f16(v)), __builtin_bit_cast(i16x8, to_f16(v + 8)));
+          store(block_low, lo + own, rows);
+        }
+        // The mirrored tile.  (Past the last row and column both operands read zeros, and so are the rows' ends.)
+        if (kSymmetric && past < 0) {
+          block.put_turned(lane, low, high);
+          store(block, result + blocked(m, j0, row0), m - j0);
+        }
+      } else {
+        // Rows of the result, or of its transpose.
+        const i16x8 low = __builtin_bit_cast(i16x8, pack8(v)), high = __builtin_bit_cast(i16x8, pack8(v + 8));
+        if (g.tall)
+          block.put_turned(lane, low, high);
+        else
+          block.put_run(lane, low, high);
+        const int across = g.tall ? m : g.n, lines = g.tall ? g.n - j0 : rows;
+        const int first = (g.tall ? row0 : j0) + tile::Block::line_feature(lane);
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (j0 + e < g.n) out[(int64_t)(j0 + e) * m + row] = (bf16)v[e];
-        } else if (g.n % 8 == 0) {
+        for (int it = 0; it < 2; ++it) {
+          const i16x8 x = block.get_line(it, lane);
+          const int line = tile::Block::line_row(it, lane);
+          if (line >= lines) continue;
+          short* const to = (short*)out + (int64_t)((g.tall ? j0 : row0) + line) * across + first;
+          if (across % 8 == 0 && first < across) {
+            *(i16x8*)to = x;
+          } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (j0 + 8 * h < g.n) *(bf16x8*)(out + (int64_t)row * g.n + j0 + 8 * h) = pack8(v + 8 * h);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (j0 + e < g.n) out[(int64_t)row * g.n + j0 + e] = (bf16)v[e];
+            for (int e = 0; e < 8; ++e)
+              if (first + e < across) to[e] = x[e];
+          }
         }
       }
     }

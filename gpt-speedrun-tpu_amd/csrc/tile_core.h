@@ -138,6 +138,54 @@ __device__ __forceinline__ i16x8 frag(const lds16* array, int offset, int r0, in
   }
 }
 
+// A wave's block of 32 rows x 32 features of 16 bits in LDS (2 KB, of its own), on the
+// way between its accumulators' layout (a lane holds a run: 16 consecutive features
+// of one row) and lines (four lanes hold a row's 64 bytes, so that an access to
+// global memory takes 1 KB of whole lines).  The address unit takes some 16 cycles
+// for such an access, 85 for 16-byte pieces that lie 64 bytes apart from lane to
+// lane and 170 where each has a line of its own: kept as runs, the result of a
+// product over 768 took longer to write than to compute.  LDS serves a wave in
+// order, so nothing is waited for but the data.
+struct Block {
+  lds16* base;
+  static constexpr int kElements = 1024;
+  // Chunks of 8 features are moved so that 16 lanes' accesses meet all banks once.
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * 32 + 8 * (chunk ^ ((row >> 2) & 3)); }
+  static __device__ __forceinline__ void order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+  __device__ __forceinline__ void put_run(int lane, i16x8 low, i16x8 high) const {
+    order();
+    *(lds16x8*)(base + at(lane & 31, 2 * (lane >> 5))) = low;
+    *(lds16x8*)(base + at(lane & 31, 2 * (lane >> 5) + 1)) = high;
+    order();
+  }
+  __device__ __forceinline__ i16x8 get_run(int lane, int half) const {
+    return *(const lds16x8*)(base + at(lane & 31, 2 * (lane >> 5) + half));
+  }
+  // The run as a column of the turned block: rows are features then.
+  __device__ __forceinline__ void put_turned(int lane, i16x8 low, i16x8 high) const {
+    order();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = 16 * (lane >> 5) + e, col = lane & 31;
+      base[at(row, col >> 3) + (col & 7)] = e < 8 ? low[e & 7] : high[e & 7];
+    }
+    order();
+  }
+  // A lane's piece of turn `it` (0, 1): row and first feature.
+  static __device__ __forceinline__ int line_row(int it, int lane) { return 16 * it + (lane >> 2); }
+  static __device__ __forceinline__ int line_feature(int lane) { return 8 * (lane & 3); }
+  __device__ __forceinline__ void put_lines(int lane, i16x8 first, i16x8 second) const {
+    order();
+    *(lds16x8*)(base + at(lane >> 2, lane & 3)) = first;
+    *(lds16x8*)(base + at(16 + (lane >> 2), lane & 3)) = second;
+    order();
+  }
+  __device__ __forceinline__ i16x8 get_line(int it, int lane) const {
+    return *(const lds16x8*)(base + at(line_row(it, lane), lane & 3));
+  }
+};
+
 // T: bf16 or f16.  MB, NB: the tile in units of 64.  AK, BKM: K-major operands.
 // kContiguous: rows of A in contiguous_row's order.
 template <class T, int MB, int NB, bool AK, bool BKM, bool kContiguous, int kSlabs = 1, int kGroups = 1,
@@ -159,6 +207,12 @@ struct Product {
   static __device__ __forceinline__ Place place() {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     return Place{(int)threadIdx.x & 63, w & 3, w >> 2, w & 1, (w >> 1) & 1};
+  }
+
+  // After run(): a wave's blocks 0 and 1, in the first stage's memory.
+  static __device__ __forceinline__ Block block(const Place& at, int which) {
+    static_assert(4 * 2 * 2 * Block::kElements <= kStageBytes, "two blocks a wave");
+    return Block{stage_array<kStageBytes, 0>() + (2 * at.wave + which) * Block::kElements};
   }
 
   struct State {

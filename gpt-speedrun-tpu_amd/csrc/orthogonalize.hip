@@ -257,7 +257,9 @@ template <int kKind, class Shape>
 __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
   constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
   constexpr int MB = Shape::MB, NB = Shape::NB;
-  typedef tile::Product<f16, MB, NB, kSymmetric, true, true, Shape::kSlabs, 1, Shape::kRing> P;
+  typedef tile::Product<f16, MB, NB, kSymmetric ? tile::kBlockedK : tile::kBlockedMN, tile::kBlockedK, true,
+                        Shape::kSlabs, 1, Shape::kRing>
+      P;
   int local;
   // Every other product walks the matrices backwards: it begins with those that the
   // one before ended with and that the caches still hold.
@@ -283,11 +285,11 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
   const auto at = P::place();
   f32x16 acc[MB][NB];
   if constexpr (kKind == kGram)
-    P::run(acc, {hi, 0, m}, {hi, 0, m}, m, m, ldx, tj * P::TM, ti * P::TN, at);
+    P::run(acc, {hi, m}, {hi, m}, m, m, ldx, tj * P::TM, ti * P::TN, at);
   else if constexpr (kKind == kSquare)
-    P::run(acc, {A, 0, m}, {A, 0, m}, m, m, m, tj * P::TM, ti * P::TN, at);
+    P::run(acc, {A, m}, {A, m}, m, m, m, tj * P::TM, ti * P::TN, at);
   else
-    P::run(acc, {hi, 0, m}, {B, 0, m}, ldx, m, m, tj * P::TM, ti * P::TN, at);
+    P::run(acc, {hi, m}, {B, m}, ldx, m, m, tj * P::TM, ti * P::TN, at);
   // A symmetric result: where the wave's features lie against the tile's rows, in
   // rows of tiles.  What lies past them is another tile's mirror image.
   const int past = kSymmetric ? tj * (MB / NB) + at.wm * MB / (2 * NB) - ti : 0;

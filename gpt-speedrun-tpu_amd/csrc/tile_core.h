@@ -9,9 +9,9 @@
 //
 // Staging is the GEMM core's (gemm_core.h): buffer loads copy 16-byte chunks from
 // global memory into LDS through a ring of three or four stages, each stage waited
-// for with an exact vmcnt and one barrier; operands lie K-major ([mn][k]) or MN-major
-// ([k][mn]) as they are in memory, swizzled so that a quarter-wave's reads meet
-// different banks, MN-major fragments read with ds_read_b64_tr_b16.  A stage is
+// for with an exact vmcnt and one barrier; operands lie there K-major or MN-major, as they
+// do in memory, so that a quarter-wave's reads meet different banks, MN-major
+// fragments read with ds_read_b64_tr_b16.  A stage is
 // 32 kSlabs deep.  K is any multiple of 8 (K-major) or any number (MN-major); what
 // lies past K or past the operand's rows reads zeros.
 #pragma once
@@ -35,16 +35,17 @@ __device__ __forceinline__ f32x16 mma(i16x8 a, i16x8 b, f32x16 c, f16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A matrix operand of 16-bit elements: row-major with leading dimension ld, or (blk >
-// 0) "32-blocked": element (r, c) at ((c / 32) * blk + r) * 32 + c % 32, column blocks
-// of 32 one after another, each of blk rows of 64 bytes.  The copies of either kind
-// of slab then read whole 128-byte lines; 64-byte pieces of a K-major operand's rows
-// take the address unit as long as whole lines would, twice the time a byte (gram
-// products of 48 matrices of 768 rows: 117 us, 85% of it with the address unit busy).
+// How a matrix operand of 16-bit elements lies in memory: K along the rows or the
+// other way, rows with leading dimension ld, or "32-blocked": element (r, c) at
+// ((c / 32) * ld + r) * 32 + c % 32, column blocks of 32 one after another, each of ld
+// rows of 64 bytes.  A copy takes 1 KB: of a blocked operand 16 rows of a block, one
+// run of whole lines, for which the address unit needs some 20 cycles; 64-byte pieces
+// of lines (K-major rows) take it 40 to 50.
+enum Layout { kRowsK, kRowsMN, kBlockedK, kBlockedMN };
+
 struct Operand {
   const void* p;
   int64_t ld;
-  int64_t blk = 0;
 };
 
 template <int kBytes, int kStage>
@@ -55,11 +56,15 @@ __device__ __forceinline__ lds16* stage_array() {
 
 constexpr int wait_vm_lgkm0(int vm) { return (vm & 15) | 0x70 | ((vm >> 4) << 14); }
 
-// Copy sources of one operand for one wave: P blocks of 1 KB a stage.
-template <int TM, bool KMAJOR, int kSlabs>
+// Copy sources of one operand for one wave: P blocks of 1 KB a stage.  In LDS a slab
+// of 32 k is K-major ([row][32 k], chunks of 8 swizzled), MN-major ([k][row],
+// swizzled) or, of a kBlockedMN operand, the blocks as they are ([block][k][32 rows]).
+template <int TM, Layout kLayout, int kSlabs>
 struct Source {
   static constexpr int P = TM / 64 * kSlabs;
   static constexpr int kDepth = 32 * kSlabs;
+  static constexpr bool kBlocked = kLayout == kBlockedK || kLayout == kBlockedMN;
+  static constexpr bool kK = kLayout == kRowsK || kLayout == kBlockedK;
   const char* base;
   int64_t step;
   uint32_t off[P];
@@ -68,31 +73,34 @@ struct Source {
   static __device__ __forceinline__ int swizzle(int k) { return TM == 64 ? 4 * ((k >> 1) & 1) : 4 * (k & 3); }
 
   // mn0: the tile's first row, MN: the operand's rows; K range [k_begin, k_end).
+  // (k_begin is a multiple of 32 and mn0 of 64: blocked stages and tiles start on a block.)
   __device__ __forceinline__ void init(Operand op, int mn0, int MN, int k_begin, int k_end, int wave, int lane) {
-    // (k_begin is a multiple of 32 and mn0 of 64: blocked stages and tiles start on a block.)
-    if (op.blk) {
-      base = (const char*)op.p + (KMAJOR ? (int64_t)(k_begin >> 5) * op.blk + mn0 : (int64_t)(mn0 >> 5) * op.blk + k_begin) * 64;
-      step = KMAJOR ? op.blk * kSlabs * 64 : (int64_t)kDepth * 64;
+    const int r0 = kK ? mn0 : k_begin, c0 = kK ? k_begin : mn0;  // as the memory has rows and columns
+    if (kBlocked) {
+      base = (const char*)op.p + ((int64_t)(c0 >> 5) * op.ld + r0) * 64;
+      step = 64 * (kK ? op.ld * kSlabs : (int64_t)kDepth);
     } else {
-      base = (const char*)op.p + 2 * (KMAJOR ? (int64_t)mn0 * op.ld + k_begin : (int64_t)k_begin * op.ld + mn0);
-      step = 2 * (KMAJOR ? (int64_t)kDepth : (int64_t)kDepth * op.ld);
+      base = (const char*)op.p + 2 * ((int64_t)r0 * op.ld + c0);
+      step = 2 * (kK ? (int64_t)kDepth : kDepth * op.ld);
     }
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const int b = wave * P + j, slab = b / (TM / 16), blk = b % (TM / 16);
       int k, m;
-      if (KMAJOR) {
-        const int row = blk * 16 + (lane >> 2);
-        k = 32 * slab + 8 * ((lane & 3) ^ ((row >> 2) & 3));
-        m = row;
-        off[j] = 2u * (uint32_t)(op.blk ? ((int64_t)slab * op.blk + row) * 32 + (k & 31) : (int64_t)row * op.ld + k);
-      } else {
+      if (kK) {
+        m = blk * 16 + (lane >> 2);
+        k = 32 * slab + 8 * ((lane & 3) ^ ((m >> 2) & 3));
+      } else if (kLayout == kRowsMN) {
         constexpr int kChunks = TM / 8;
         const int row = blk * (512 / TM) + lane / kChunks;
         k = 32 * slab + row;
         m = 8 * ((lane % kChunks) ^ swizzle(row));
-        off[j] = 2u * (uint32_t)(op.blk ? ((int64_t)(m >> 5) * op.blk + k) * 32 + (m & 31) : (int64_t)k * op.ld + m);
+      } else {
+        k = 32 * slab + 16 * (blk & 1) + (lane >> 2);
+        m = 32 * (blk >> 1) + 8 * (lane & 3);
       }
+      const int r = kK ? m : k, c = kK ? k : m;
+      off[j] = 2u * (uint32_t)(kBlocked ? ((int64_t)(c >> 5) * op.ld + r) * 32 + (c & 31) : (int64_t)r * op.ld + c);
       const int rem = k_end - k_begin - k;
       nvalid[j] = (mn0 + m < MN && rem > 0) ? (rem + kDepth - 1) / kDepth : 0;
     }
@@ -115,25 +123,35 @@ struct Source {
 // The lane's part of an address passes through an empty asm: the compiler finds an
 // access's array through a few additions only, would make more of one sum, and takes
 // an access without an array to meet every copy in flight, for which it then waits.
-template <int TM, bool KMAJOR, bool kContiguous, int kOffset>
+template <int TM, Layout kLayout, bool kContiguous, int kOffset>
 __device__ __forceinline__ i16x8 frag(const lds16* array, int offset, int r0, int block, int kc, int lane) {
+  typedef Source<TM, kLayout, 1> S;
   const int hl = lane >> 5;
-  if (KMAJOR) {
+  if (S::kK) {
     const int row = r0 + (kContiguous ? gemm::contiguous_row(lane & 31) : (lane & 31));
     const int c = 2 * (kc & 1) + hl;
     int at = offset + row * 32 + 8 * (c ^ ((row >> 2) & 3));  // (the same for row + 32)
     asm("" : "+v"(at));
     return *(const lds16x8*)(array + at + (kOffset + 1024 * block + (kc >> 1) * TM * 32));
   } else {
+    // The lane supplies the address of four rows: quad q of the block's eight.
     const int cq = lane & 15, q = 4 * ((lane >> 4) & 1) + (cq & 3);
-    const int m = r0 + 32 * block + (kContiguous ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
+    const int quad = kContiguous ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q;
     const int k = 8 * hl + (cq >> 2);
-    typedef Source<TM, false, 1> S;  // (its swizzle is the same for k, k + 4 and k + 16)
-    int at = offset + k * TM + 8 * ((m >> 3) ^ S::swizzle(k)) + 4 * ((m >> 2) & 1);
+    constexpr bool kBlocks = kLayout == kBlockedMN;  // (a half-wave's reads are 256 bytes in a row there)
+    constexpr int kRow = kBlocks ? 32 : TM;          // elements from one k to the next
+    int at;
+    if (kBlocks) {
+      at = offset + r0 * 32 + k * 32 + quad;
+    } else {  // (the swizzle is the same for k, k + 4 and k + 16)
+      const int m = r0 + 32 * block + quad;
+      at = offset + k * TM + 8 * ((m >> 3) ^ S::swizzle(k)) + 4 * ((m >> 2) & 1);
+    }
     asm("" : "+v"(at));
-    const lds16* const lo = array + at + (kOffset + (kc >> 1) * TM * 32 + (kc & 1) * 16 * TM);
+    const lds16* const lo =
+        array + at + (kOffset + (kBlocks ? 1024 * block : 0) + (kc >> 1) * TM * 32 + (kc & 1) * 16 * kRow);
     const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)lo);
-    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(lo + 4 * TM));
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds16x4*)(lo + 4 * kRow));
     return i16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 }
@@ -186,9 +204,9 @@ struct Block {
   }
 };
 
-// T: bf16 or f16.  MB, NB: the tile in units of 64.  AK, BKM: K-major operands.
+// T: bf16 or f16.  MB, NB: the tile in units of 64.  LA, LB: the operands' layouts.
 // kContiguous: rows of A in contiguous_row's order.
-template <class T, int MB, int NB, bool AK, bool BKM, bool kContiguous, int kSlabs = 1, int kGroups = 1,
+template <class T, int MB, int NB, Layout LA, Layout LB, bool kContiguous, int kSlabs = 1, int kGroups = 1,
           int kRing = 4>
 struct Product {
   static constexpr int TM = 64 * MB, TN = 64 * NB, kThreads = 256 * kGroups;
@@ -216,8 +234,8 @@ struct Product {
   }
 
   struct State {
-    Source<TM, AK, kSlabs> a;
-    Source<TN, BKM, kSlabs> b;
+    Source<TM, LA, kSlabs> a;
+    Source<TN, LB, kSlabs> b;
     Place at;
   };
 
@@ -235,10 +253,10 @@ struct Product {
     const int offset = s.at.group * (kStageA + kStageB);
 #pragma unroll
     for (int i = 0; i < MB; ++i)
-      a[i] = frag<TM, AK, kContiguous, 0>(array, offset, 32 * MB * s.at.wm, i, kc, s.at.lane);
+      a[i] = frag<TM, LA, kContiguous, 0>(array, offset, 32 * MB * s.at.wm, i, kc, s.at.lane);
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      b[i] = frag<TN, BKM, false, kStageA>(array, offset, 32 * NB * s.at.wn, i, kc, s.at.lane);
+      b[i] = frag<TN, LB, false, kStageA>(array, offset, 32 * NB * s.at.wn, i, kc, s.at.lane);
   }
 
   template <int S>

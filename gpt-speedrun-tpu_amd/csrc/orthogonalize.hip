@@ -310,33 +310,39 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
       if (tile::Block::line_row(it, lane) < rows) *(i16x8*)(to + 512 * it + 8 * lane) = v;
     }
   };
+  const int row_first = ti * P::TN + 32 * NB * at.wn, f_first = tj * P::TM + 32 * MB * at.wm;
+  // What the blocks hold already, asked for some blocks ahead and so ahead of the
+  // stores between: behind those, a block's loads would cost a trip to memory each.
+  constexpr int kBlocks = MB * NB, kAhead = kBlocks < 4 ? kBlocks : 4;
+  i16x8 old[kAhead][2], rest[kAhead][2];
+  auto fetch = [&](int b) {
+    const f16* const from = kSymmetric ? A : hi;
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      // (Of the last row and block again where there are none: those are not used.)
+      const int row = min(row_first + 32 * (b / MB) + tile::Block::line_row(it, lane), m - 1);
+      const int64_t own = blocked(m, row, min(f_first + 32 * (b % MB), ld - 32) + tile::Block::line_feature(lane));
+      old[b % kAhead][it] = *(const i16x8*)(from + own);
+      if constexpr (!kSymmetric) rest[b % kAhead][it] = *(const i16x8*)(lo + own);
+    }
+  };
+  if constexpr (kKind != kGram) {
+#pragma unroll
+    for (int b = 0; b < kAhead; ++b) fetch(b);
+  }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int row0 = ti * P::TN + 32 * (NB * at.wn + nb), f0 = tj * P::TM + 32 * MB * at.wm;
-    if (row0 >= m) break;  // (uniform, as every condition on row0 and f0)
-    // What the blocks hold already, all of it asked for before the first store: behind
-    // a store the loads could not be moved, and each would cost a trip to memory.
-    i16x8 old[MB][2], rest[MB][2];
-    if constexpr (kKind != kGram) {
-      const f16* const from = kSymmetric ? A : hi;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          // (Of the last row and block again where there are none: those are not used.)
-          const int row = min(row0 + tile::Block::line_row(it, lane), m - 1);
-          const int64_t own = blocked(m, row, min(f0 + 32 * mb, ld - 32) + tile::Block::line_feature(lane));
-          old[mb][it] = *(const i16x8*)(from + own);
-          if constexpr (!kSymmetric) rest[mb][it] = *(const i16x8*)(lo + own);
-        }
-    }
+    const int row0 = row_first + 32 * nb;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      const int j0 = f0 + 32 * mb;
-      if (j0 >= ld) break;
+      const int b = nb * MB + mb, j0 = f_first + 32 * mb;
+      const bool inside = row0 < m && j0 < ld;  // (uniform)
       const int64_t own = blocked(m, row0, j0);
-      if constexpr (kKind != kGram) block.put_lines(lane, old[mb][0], old[mb][1]);
-      if constexpr (!kSymmetric) block_low.put_lines(lane, rest[mb][0], rest[mb][1]);
+      if constexpr (kKind != kGram) block.put_lines(lane, old[b % kAhead][0], old[b % kAhead][1]);
+      if constexpr (!kSymmetric) block_low.put_lines(lane, rest[b % kAhead][0], rest[b % kAhead][1]);
+      if constexpr (kKind != kGram)
+        if (b + kAhead < kBlocks) fetch(b + kAhead);
+      if (!inside) continue;
       float v[16];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {

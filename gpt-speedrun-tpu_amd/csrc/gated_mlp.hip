@@ -10,19 +10,22 @@
 // stands beside the products is therefore kept inside them:
 //   - gate and up columns of W take turns in a tile in blocks of 32 (a paired
 //     operand of the core), so a lane holds g and u of the same 16 features of one
-//     token and writes h, and for the backward g and u, straight from its
-//     accumulators;
+//     token and makes h of them;
 //   - the product dy V^T reads g and u in its epilogue and writes dg and du.
-// Roundings to bfloat16: h, dg and du, which the next product takes in that type,
-// and g and u where the backward is to find them (h itself comes from the
-// unrounded ones).  Everything else is float32.
+// Roundings: h, dg and du to bfloat16, in which the next product takes them, g and u
+// to 11 bits where the backward is to find them (h itself comes from the unrounded
+// ones).  Everything else is float32.
 //
 // The weight gradients cut the tokens into slices where the tiles alone do not
 // fill the chip; each slice writes its float32 sums to the workspace and a small
 // pass adds them in order, so the result does not depend on timing.
-#include "gemm_core.h"
+#include "tile_core.h"
 
 namespace {
+
+using tile::f16;
+using tile::f16x8;
+using tile::i16x8;
 
 using gemm::BM;
 using gemm::BN;
@@ -48,46 +51,159 @@ __device__ __forceinline__ void act_both(float x, float& a, float& slope) {
   }
 }
 
+// What the backward finds of g and u: float16 [n][2f], each run of 16 features (the
+// last may be shorter) scaled by a power of two that brings its largest to 2^14 ..
+// 2^15, and those powers, a byte each, [2][runs][n].  11 bits where bfloat16 has 8,
+// in the same space: with bfloat16 the gradients of x and W were 1.76 times as far
+// off as their own rounding alone, which is 1.41 times now.  (What is 2^-25 of its
+// run's largest or less is lost.)
+__host__ __device__ inline int runs_of(int f) { return (f + 15) / 16; }
+
+struct Kept {
+  f16* values;
+  uint8_t* powers;
+
+  // Of the lane's token and of its run in block `block` of 32 features from f0 (a
+  // multiple of 64) on.
+  static __device__ __forceinline__ uint32_t power_at(int block, int f0, int first, int n, int f, int lane) {
+    const bool inside = f0 + 32 * block + 16 * (lane >> 5) < f && first + (lane & 31) < n;
+    return inside ? (lane >> 5) * (uint32_t)n + (lane & 31) : gemm::kOffZero;
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t power_rows(int half, int block, int f0, int first, int n, int f) const {
+    return make_rsrc(powers + ((int64_t)half * runs_of(f) + (f0 >> 4) + 2 * block) * n + first, gemm::kRsrcRange);
+  }
+  __device__ __forceinline__ void put_power(int half, int block, int power, int f0, int first, int n, int f,
+                                            int lane) const {
+    __builtin_amdgcn_raw_buffer_store_b8((uint8_t)power, power_rows(half, block, f0, first, n, f),
+                                         power_at(block, f0, first, n, f, lane), 0, 0);
+  }
+  __device__ __forceinline__ int get_power(int half, int block, int f0, int first, int n, int f, int lane) const {
+    return __builtin_amdgcn_raw_buffer_load_b8(power_rows(half, block, f0, first, n, f),
+                                               power_at(block, f0, first, n, f, lane), 0, 0);
+  }
+};
+
+// The float32 exponent field of a run's largest value, and the factor that goes with it.
+__device__ __forceinline__ int power_of(const float (&v)[16]) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+  return max(14, __builtin_bit_cast(int, most) >> 23);
+}
+__device__ __forceinline__ float scale_down(int power) { return __builtin_bit_cast(float, (268 - power) << 23); }
+__device__ __forceinline__ float scale_up(int power) {  // its reciprocal; in two steps where that is no normal number
+  return __builtin_bit_cast(float, max(power - 14, 1) << 23);
+}
+
+// A wave's 32 rows of 64 features of 16 bits in LDS, on the way between its
+// accumulators' layout (runs of 16 features of a row) and lines: eight lanes hold 128
+// bytes of a row.  (tile::Block's reasons; here the rows lie in row-major matrices,
+// where 64 features make a whole line.)  The memory is beside the stage ring, which
+// fills for the next tile meanwhile.
+__shared__ __attribute__((aligned(1024))) short g_band[8 * 2048];
+
+struct Band {
+  int lane, offset;
+  static __device__ __forceinline__ void order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+  // (An opaque sum, see tile::frag; volatile, or all of them would wait in registers
+  // through the main loop.)
+  __device__ __forceinline__ tile::lds16x8* slot(int row, int chunk) const {
+    int at = offset + row * 64 + 8 * (chunk ^ ((row >> 1) & 7));
+    asm volatile("" : "+v"(at));
+    return (tile::lds16x8*)((tile::lds16*)g_band + at);
+  }
+  __device__ __forceinline__ void put_run(int block, i16x8 low, i16x8 high) const {
+    *slot(lane & 31, 4 * block + 2 * (lane >> 5)) = low;
+    *slot(lane & 31, 4 * block + 2 * (lane >> 5) + 1) = high;
+  }
+  __device__ __forceinline__ i16x8 get_run(int block, int half) const {
+    return *slot(lane & 31, 4 * block + 2 * (lane >> 5) + half);
+  }
+  // Offsets of the lane's pieces of rows 8 it .. from a uniform place (first row, first
+  // feature) of a matrix, as many as there are; past them one that reads zeros and
+  // writes nothing.
+  __device__ __forceinline__ uint32_t line(int it, uint32_t ld, int rows, int features) const {
+    const int row = 8 * it + (lane >> 3);
+    return row < rows && 8 * (lane & 7) < features ? 2 * (row * ld + 8 * (lane & 7)) : gemm::kOffZero;
+  }
+  // (All of the offset in the vector register: with a part in a scalar one the compiler
+  // let the store's first data register be written anew before the last lanes of every
+  // 16 had been read, here on gfx950.)
+  __device__ __forceinline__ void store(void* place, uint32_t ld, int rows, int features) const {
+    order();
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(place, gemm::kRsrcRange);
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, *slot(8 * it + (lane >> 3), lane & 7)), r,
+                                             line(it, ld, rows, features), 0, 0);
+    order();
+  }
+  __device__ __forceinline__ void fetch(i16x8 (&v)[4], const void* place, uint32_t ld, int rows, int features) const {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(place, gemm::kRsrcRange);
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+      v[it] = __builtin_bit_cast(
+          i16x8, __builtin_amdgcn_raw_buffer_load_b128(r, line(it, ld, rows, features), 0, 0));
+  }
+  __device__ __forceinline__ void put_lines(const i16x8 (&v)[4]) const {
+    order();
+#pragma unroll
+    for (int it = 0; it < 4; ++it) *slot(8 * it + (lane >> 3), lane & 7) = v[it];
+    order();
+  }
+};
+
+__device__ __forceinline__ i16x8 bf16_run(const float* v) { return __builtin_bit_cast(i16x8, pack8(v)); }
+__device__ __forceinline__ i16x8 f16_run(const float* v, float scale) {
+  f16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (f16)(v[i] * scale);
+  return __builtin_bit_cast(i16x8, r);
+}
+
 struct UpArgs {
-  bf16* gate_up;  // [n][2f], NULL: not kept
-  bf16* h;        // [n][f]
+  Kept kept;
+  bf16* h;  // [n][f]
   int n, k, f, group;
 };
 
-// The lane's 16 consecutive features of a token, 8 at a time.
-__device__ __forceinline__ void store_run(bf16* dst, const float (&v)[16], int left) {
-  if (left > 0) *reinterpret_cast<bf16x8*>(dst) = pack8(v);
-  if (left > 8) *reinterpret_cast<bf16x8*>(dst + 8) = pack8(v + 8);
-}
-
 template <int kAct, bool kKeep>
 __global__ void __launch_bounds__(gemm::THREADS) gated_up_kernel(Operand W, Operand X, UpArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int hl = lane >> 5, l32 = lane & 31, wm = wave & 1, wn = wave >> 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
   const int ntiles = ((2 * a.f + BM - 1) / BM) * ((a.n + BN - 1) / BN);
+  const Band band{lane, wave * 2048};
   auto coords = [&](int t, int& tm, int& tn) { gemm::tile_coords(t, 2 * a.f, a.n, tm, tn, a.group); };
   auto pre = [](int, int) {};
   auto epi = [&](f32x16(&acc)[4][2], int tm, int tn) {
+    const int f0 = tm * (BM / 2) + 64 * wm;
+    if (f0 >= a.f) return;  // (uniform; no barrier below)
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
-      const int token = tn * BN + 64 * wn + 32 * nb + l32;
-      if (token >= a.n) continue;
+      const int first = tn * BN + 64 * wn + 32 * nb;
+      Band::order();
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int feature = tm * (BM / 2) + 64 * wm + 32 * p + 16 * hl;
-        const int left = a.f - feature;  // a multiple of 8
-        float g[16], u[16], h[16];
+        float h[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          g[i] = acc[2 * p][nb][i];
-          u[i] = acc[2 * p + 1][nb][i];
-          h[i] = act_f<kAct>(g[i]) * u[i];
-        }
-        store_run(a.h + (int64_t)token * a.f + feature, h, left);
-        if constexpr (kKeep) {
-          bf16* const row = a.gate_up + (int64_t)token * 2 * a.f + feature;
-          store_run(row, g, left);
-          store_run(row + a.f, u, left);
+        for (int i = 0; i < 16; ++i) h[i] = act_f<kAct>(acc[2 * p][nb][i]) * acc[2 * p + 1][nb][i];
+        band.put_run(p, bf16_run(h), bf16_run(h + 8));
+      }
+      band.store(a.h + (int64_t)first * a.f + f0, a.f, a.n - first, a.f - f0);
+      if constexpr (kKeep) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // gate, up
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = acc[2 * p + half][nb][i];
+            const int power = power_of(v);
+            const float scale = scale_down(power);
+            band.put_run(p, f16_run(v, scale), f16_run(v + 8, scale));
+            a.kept.put_power(half, p, power, f0, first, a.n, a.f, lane);
+          }
+          band.store(a.kept.values + (int64_t)first * 2 * a.f + (int64_t)half * a.f + f0, 2 * a.f, a.n - first, a.f - f0);
         }
       }
     }
@@ -96,46 +212,74 @@ __global__ void __launch_bounds__(gemm::THREADS) gated_up_kernel(Operand W, Oper
 }
 
 struct DownBwdArgs {
-  const bf16* gate_up;  // [n][2f]
-  bf16* d_gate_up;      // [n][2f]
+  Kept kept;
+  bf16* d_gate_up;  // [n][2f]
   int n, k, f, group;
 };
 
 template <int kAct>
 __global__ void __launch_bounds__(gemm::THREADS) gated_down_bwd_kernel(Operand V, Operand DY, DownBwdArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int hl = lane >> 5, l32 = lane & 31, wm = wave & 1, wn = wave >> 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
   const int ntiles = ((a.f + BM - 1) / BM) * ((a.n + BN - 1) / BN);
+  const Band band{lane, wave * 2048};
   auto coords = [&](int t, int& tm, int& tn) { gemm::tile_coords(t, a.f, a.n, tm, tn, a.group); };
   auto pre = [](int, int) {};
   auto epi = [&](f32x16(&acc)[4][2], int tm, int tn) {
+    // 32 tokens x 64 features at a time, the next ones asked for before the stores.
+    i16x8 lines[2][4];
+    int powers[2][2];
+    auto fetch = [&](int step) {
+      const int f0 = tm * BM + 128 * wm + 64 * (step & 1), first = tn * BN + 64 * wn + 32 * (step >> 1);
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const int token = tn * BN + 64 * wn + 32 * nb + l32;
-      if (token >= a.n) continue;
+      for (int half = 0; half < 2; ++half) {
+        band.fetch(lines[half], a.kept.values + (int64_t)first * 2 * a.f + (int64_t)half * a.f + f0, 2 * a.f,
+                   a.n - first, a.f - f0);
 #pragma unroll
-      for (int mb = 0; mb < 4; ++mb) {
-        const int feature = tm * BM + 128 * wm + 32 * mb + 16 * hl;
-        const int left = a.f - feature;
-        const int64_t at = (int64_t)token * 2 * a.f + feature;
+        for (int p = 0; p < 2; ++p) powers[half][p] = a.kept.get_power(half, p, f0, first, a.n, a.f, lane);
+      }
+    };
+    fetch(0);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (left <= 8 * half) continue;
-          const bf16x8 g = *reinterpret_cast<const bf16x8*>(a.gate_up + at + 8 * half);
-          const bf16x8 u = *reinterpret_cast<const bf16x8*>(a.gate_up + at + a.f + 8 * half);
-          float dg[8], du[8];
+    for (int step = 0; step < 4; ++step) {
+      const int f0 = tm * BM + 128 * wm + 64 * (step & 1), first = tn * BN + 64 * wn + 32 * (step >> 1);
+      const int nb = step >> 1;
+      const int now[2][2] = {{powers[0][0], powers[0][1]}, {powers[1][0], powers[1][1]}};
+      i16x8 g[2][2], dg[2][2], du[2][2];
+      band.put_lines(lines[0]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) g[p][h] = band.get_run(p, h);
+      band.put_lines(lines[1]);
+      if (step < 3) fetch(step + 1);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const float scale_g = scale_up(now[0][p]), scale_u = scale_up(now[1][p]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f16x8 gates = __builtin_bit_cast(f16x8, g[p][h]), ups = __builtin_bit_cast(f16x8, band.get_run(p, h));
+          float vg[8], vu[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float dh = acc[mb][nb][8 * half + i];
+            const float dh = acc[2 * (step & 1) + p][nb][8 * h + i];
             float value, slope;
-            act_both<kAct>((float)g[i], value, slope);
-            dg[i] = dh * (float)u[i] * slope;
-            du[i] = dh * value;
+            act_both<kAct>((float)gates[i] * scale_g, value, slope);
+            vg[i] = dh * ((float)ups[i] * scale_u) * slope;
+            vu[i] = dh * value;
           }
-          *reinterpret_cast<bf16x8*>(a.d_gate_up + at + 8 * half) = pack8(dg);
-          *reinterpret_cast<bf16x8*>(a.d_gate_up + at + a.f + 8 * half) = pack8(du);
+          dg[p][h] = bf16_run(vg);
+          du[p][h] = bf16_run(vu);
         }
       }
+      Band::order();
+#pragma unroll
+      for (int p = 0; p < 2; ++p) band.put_run(p, dg[p][0], dg[p][1]);
+      bf16* const place = a.d_gate_up + (int64_t)first * 2 * a.f + f0;
+      band.store(place, 2 * a.f, a.n - first, a.f - f0);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) band.put_run(p, du[p][0], du[p][1]);
+      band.store(place + a.f, 2 * a.f, a.n - first, a.f - f0);
     }
   };
   gemm::persistent<true, true, true>(V, DY, a.f, a.n, a.k, ntiles, coords, pre, epi);
@@ -241,6 +385,10 @@ Bwd plan_bwd(int n, int d, int f, int d_out) {
   return b;
 }
 
+Kept kept_at(void* p, int n, int f) {
+  return Kept{(f16*)p, p ? (uint8_t*)p + (size_t)n * 2 * f * 2 : nullptr};
+}
+
 constexpr int kMostWidth = 1 << 20;
 constexpr int64_t kMostStride = 1 << 22;  // a tile's rows stay within the core's 32-bit byte offsets
 
@@ -268,28 +416,33 @@ int tile_group(int m_tiles) { return m_tiles <= 16 ? m_tiles : gemm::kGroupM; }
 extern "C" {
 
 int gptrig_gated_mlp_fwd(const void* x, int64_t ldx, const void* gate_up_w, int64_t ldw, const void* down_w,
-                         int64_t ldv, int activation, void* gate_up, void* h, void* y, int n, int d, int f, int d_out,
+                         int64_t ldv, int activation, void* kept, void* h, void* y, int n, int d, int f, int d_out,
                          void* stream) {
   if (!x || !gate_up_w || !down_w || !h || !y) return GPTRIG_E_NULL;
   if (activation != kSilu && activation != kGelu) return GPTRIG_E_UNSUPPORTED;
   if (check_sizes(n, d, f, d_out) != GPTRIG_OK) return GPTRIG_E_SHAPE;
   if (!rows_ok(x, ldx, d) || !rows_ok(gate_up_w, ldw, 2 * f) || !rows_ok(down_w, ldv, d_out)) return GPTRIG_E_SHAPE;
-  if (((uintptr_t)gate_up | (uintptr_t)h | (uintptr_t)y) & 15) return GPTRIG_E_SHAPE;
+  if (((uintptr_t)kept | (uintptr_t)h | (uintptr_t)y) & 15) return GPTRIG_E_SHAPE;
   if (n == 0) return GPTRIG_OK;
   const hipStream_t s = (hipStream_t)stream;
   const Operand W{(const bf16*)gate_up_w, ldw, 0, f}, X{(const bf16*)x, ldx};
-  const UpArgs a{(bf16*)gate_up, (bf16*)h, n, d, f, tile_group(ceil_div(2 * f, BM))};
+  const UpArgs a{kept_at(kept, n, f), (bf16*)h, n, d, f, tile_group(ceil_div(2 * f, BM))};
   const unsigned grid = persistent_grid(tiles_of(2 * f, n));
-  if (activation == kSilu && gate_up)
+  if (activation == kSilu && kept)
     gated_up_kernel<kSilu, true><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
   else if (activation == kSilu)
     gated_up_kernel<kSilu, false><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
-  else if (gate_up)
+  else if (kept)
     gated_up_kernel<kGelu, true><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
   else
     gated_up_kernel<kGelu, false><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
   GPTRIG_CHECK_LAUNCH();
   return gptrig_linear(h, f, down_w, ldv, 0, nullptr, y, d_out, n, f, d_out, stream);
+}
+
+size_t gptrig_gated_mlp_kept_bytes(int n, int f) {
+  if (check_sizes(n, 8, f, 8) != GPTRIG_OK) return 0;
+  return (size_t)n * 2 * f * 2 + (size_t)n * 2 * runs_of(f);
 }
 
 size_t gptrig_gated_mlp_bwd_workspace_bytes(int n, int d, int f, int d_out) {
@@ -298,16 +451,16 @@ size_t gptrig_gated_mlp_bwd_workspace_bytes(int n, int d, int f, int d_out) {
 }
 
 int gptrig_gated_mlp_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* gate_up_w, int64_t ldw,
-                         const void* down_w, int64_t ldv, int activation, const void* gate_up, const void* h, void* dx,
+                         const void* down_w, int64_t ldv, int activation, const void* kept, const void* h, void* dx,
                          void* d_gate_up_w, void* d_down_w, int n, int d, int f, int d_out, void* workspace,
                          size_t workspace_bytes, void* stream) {
-  if (!dy || !x || !gate_up_w || !down_w || !gate_up || !h || !workspace) return GPTRIG_E_NULL;
+  if (!dy || !x || !gate_up_w || !down_w || !kept || !h || !workspace) return GPTRIG_E_NULL;
   if (activation != kSilu && activation != kGelu) return GPTRIG_E_UNSUPPORTED;
   if (check_sizes(n, d, f, d_out) != GPTRIG_OK || n == 0) return GPTRIG_E_SHAPE;
   if (!rows_ok(x, ldx, d) || !rows_ok(dy, lddy, d_out) || !rows_ok(gate_up_w, ldw, 2 * f) ||
       !rows_ok(down_w, ldv, d_out))
     return GPTRIG_E_SHAPE;
-  if (((uintptr_t)gate_up | (uintptr_t)h | (uintptr_t)dx | (uintptr_t)d_gate_up_w | (uintptr_t)d_down_w |
+  if (((uintptr_t)kept | (uintptr_t)h | (uintptr_t)dx | (uintptr_t)d_gate_up_w | (uintptr_t)d_down_w |
        (uintptr_t)workspace) & 15)
     return GPTRIG_E_SHAPE;
   const Bwd b = plan_bwd(n, d, f, d_out);
@@ -316,7 +469,7 @@ int gptrig_gated_mlp_bwd(const void* dy, int64_t lddy, const void* x, int64_t ld
   bf16* const dgu = (bf16*)workspace;
   if (dx || d_gate_up_w) {
     const Operand V{(const bf16*)down_w, ldv}, DY{(const bf16*)dy, lddy};
-    const DownBwdArgs a{(const bf16*)gate_up, dgu, n, d_out, f, tile_group(ceil_div(f, BM))};
+    const DownBwdArgs a{kept_at(const_cast<void*>(kept), n, f), dgu, n, d_out, f, tile_group(ceil_div(f, BM))};
     const unsigned grid = persistent_grid(tiles_of(f, n));
     if (activation == kSilu)
       gated_down_bwd_kernel<kSilu><<<grid, gemm::THREADS, 0, s>>>(V, DY, a);

@@ -96,6 +96,7 @@ SIGNATURES: dict[str, tuple] = {
     "gptrig_scaled_embedding_bwd_workspace_bytes": (Z, [L, I, I]),
     "gptrig_scaled_embedding_bwd": (I, [P, I, P, L, I, P, I, L, I, I, F, P, Z, P]),
     "gptrig_gated_mlp_fwd": (I, [P, L, P, L, P, L, I, P, P, P, I, I, I, I, P]),
+    "gptrig_gated_mlp_kept_bytes": (Z, [I, I]),
     "gptrig_gated_mlp_bwd_workspace_bytes": (Z, [I, I, I, I]),
     "gptrig_gated_mlp_bwd": (I, [P, L, P, L, P, L, P, L, I, P, P, P, P, P, I, I, I, I, P, Z, P]),
     "gptrig_adamw": (I, [P, P, P, P, P, P, P, L, I, F, F, F, I, P, P, P]),

@@ -306,6 +306,11 @@ def _operand(x: torch.Tensor) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=256)
+def _gated_kept_bytes(n: int, f: int) -> int:
+    return _lib.query("gptrig_gated_mlp_kept_bytes", n, f)
+
+
+@functools.lru_cache(maxsize=256)
 def _gated_workspace_bytes(n: int, d: int, f: int, d_out: int) -> int:
     return _lib.query("gptrig_gated_mlp_bwd_workspace_bytes", n, d, f, d_out)
 
@@ -318,13 +323,13 @@ def _gated_forward(x, gate_up_w, down_w, activation: int, keep: bool):
     f, d_out = v.shape
     dev = x2.device
     h = torch.empty((n, f), dtype=BF16, device=dev)
-    gate_up = torch.empty((n, 2 * f), dtype=BF16, device=dev) if keep else None
+    kept = _lib.workspace(_gated_kept_bytes(n, f), dev) if keep else None
     y = torch.empty((n, d_out), dtype=BF16, device=dev)
     if n:
         _lib.call_on(x2.get_device(), "gptrig_gated_mlp_fwd", x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0),
-                     v.data_ptr(), v.stride(0), activation, _lib.ptr(gate_up), h.data_ptr(), y.data_ptr(), n, d, f,
+                     v.data_ptr(), v.stride(0), activation, _lib.ptr(kept), h.data_ptr(), y.data_ptr(), n, d, f,
                      d_out)
-    return y if x.ndim == 2 else y.view(*x.shape[:-1], d_out), x2, w, v, gate_up, h
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], d_out), x2, w, v, kept, h
 
 
 class _GatedMLP(torch.autograd.Function):
@@ -341,7 +346,7 @@ class _GatedMLP(torch.autograd.Function):
 
 
 def _gated_backward(ctx, dy):
-    x, w, v, gate_up, h = ctx.saved_tensors
+    x, w, v, kept, h = ctx.saved_tensors
     shape, activation = ctx.meta
     need_x, need_w, need_v, _ = ctx.needs_input_grad
     n, d = x.shape
@@ -358,7 +363,7 @@ def _gated_backward(ctx, dy):
     size = _gated_workspace_bytes(n, d, f, d_out)
     ws = _lib.workspace(size, dev)
     _lib.call_on(x.get_device(), "gptrig_gated_mlp_bwd", dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0),
-                 w.data_ptr(), w.stride(0), v.data_ptr(), v.stride(0), activation, gate_up.data_ptr(), h.data_ptr(),
+                 w.data_ptr(), w.stride(0), v.data_ptr(), v.stride(0), activation, kept.data_ptr(), h.data_ptr(),
                  _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(dv), n, d, f, d_out, ws.data_ptr(), size)
     return None if dx is None else dx.view(shape), dw, dv, None
 
@@ -373,8 +378,8 @@ def gated_mlp(x: torch.Tensor, gate_up_w: torch.Tensor, down_w: torch.Tensor, *,
 
     ``x``: bfloat16 ``[..., d]`` of any strides; ``gate_up_w`` ``[d, 2 * hidden]``
     and ``down_w`` ``[hidden, d_out]`` in bfloat16; widths are multiples of 8.  The
-    sums are float32; the hidden values, and for the backward both halves of the
-    projection, are held in bfloat16.  Differentiable once in all three, the
+    sums are float32; the hidden values are held in bfloat16, for the backward both
+    halves of the projection in 11 bits.  Differentiable once in all three, the
     gradients in bfloat16 and the same at every call.
     """
 

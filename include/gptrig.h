@@ -412,9 +412,10 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
  * up-projection): with [g | u] = x gate_up_w the two halves of a projection,
  * h = act(g) * u and y = h down_w; act is GPTRIG_SILU or GPTRIG_GELU (tanh form).
  * All bf16: x [n, d], gate_up_w [d, 2f] (the gate's columns first), down_w
- * [f, d_out] with row strides ldx, ldw and ldv, gate_up [n, 2f] (nullable: what the
- * backward needs of g and u), h [n, f] (for the backward, or scratch) and y
- * [n, d_out] contiguous.  Sums are float32; h is rounded from the unrounded g, u.
+ * [f, d_out] with row strides ldx, ldw and ldv, h [n, f] (for the backward, or
+ * scratch) and y [n, d_out] contiguous; kept (nullable) takes
+ * gptrig_gated_mlp_kept_bytes of what the backward needs of g and u (11 bits of each).
+ * Sums are float32; h is rounded from the unrounded g, u.
  * The backward writes dx [n, d], d_gate_up_w and d_down_w (contiguous, each
  * nullable) in an order of additions that the sizes fix;
  * gptrig_gated_mlp_bwd_workspace_bytes of workspace.
@@ -424,11 +425,12 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
 #define GPTRIG_SILU 0
 #define GPTRIG_GELU 1
 int gptrig_gated_mlp_fwd(const void* x, int64_t ldx, const void* gate_up_w, int64_t ldw, const void* down_w,
-                         int64_t ldv, int activation, void* gate_up, void* h, void* y, int n, int d, int f, int d_out,
+                         int64_t ldv, int activation, void* kept, void* h, void* y, int n, int d, int f, int d_out,
                          void* stream);
+size_t gptrig_gated_mlp_kept_bytes(int n, int f);
 size_t gptrig_gated_mlp_bwd_workspace_bytes(int n, int d, int f, int d_out);
 int gptrig_gated_mlp_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* gate_up_w, int64_t ldw,
-                         const void* down_w, int64_t ldv, int activation, const void* gate_up, const void* h, void* dx,
+                         const void* down_w, int64_t ldv, int activation, const void* kept, const void* h, void* dx,
                          void* d_gate_up_w, void* d_down_w, int n, int d, int f, int d_out, void* workspace,
                          size_t workspace_bytes, void* stream);
 

@@ -102,6 +102,14 @@ __device__ __forceinline__ float scale_up(int power) {  // its reciprocal; in tw
 // fills for the next tile meanwhile.
 __shared__ __attribute__((aligned(1024))) short g_band[8 * 2048];
 
+// A thread's lane, worked out anew: what a tile's end derives from it does not wait in
+// registers through the main loop.
+__device__ __forceinline__ int fresh_lane() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid & 63;
+}
+
 struct Band {
   int lane, offset;
   static __device__ __forceinline__ void order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
@@ -169,15 +177,16 @@ struct UpArgs {
 
 template <int kAct, bool kKeep>
 __global__ void __launch_bounds__(gemm::THREADS) gated_up_kernel(Operand W, Operand X, UpArgs a) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
   const int ntiles = ((2 * a.f + BM - 1) / BM) * ((a.n + BN - 1) / BN);
-  const Band band{lane, wave * 2048};
   auto coords = [&](int t, int& tm, int& tn) { gemm::tile_coords(t, 2 * a.f, a.n, tm, tn, a.group); };
   auto pre = [](int, int) {};
   auto epi = [&](f32x16(&acc)[4][2], int tm, int tn) {
     const int f0 = tm * (BM / 2) + 64 * wm;
     if (f0 >= a.f) return;  // (uniform; no barrier below)
+    const int lane = fresh_lane();
+    const Band band{lane, wave * 2048};
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
       const int first = tn * BN + 64 * wn + 32 * nb;
@@ -219,13 +228,14 @@ struct DownBwdArgs {
 
 template <int kAct>
 __global__ void __launch_bounds__(gemm::THREADS) gated_down_bwd_kernel(Operand V, Operand DY, DownBwdArgs a) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
   const int ntiles = ((a.f + BM - 1) / BM) * ((a.n + BN - 1) / BN);
-  const Band band{lane, wave * 2048};
   auto coords = [&](int t, int& tm, int& tn) { gemm::tile_coords(t, a.f, a.n, tm, tn, a.group); };
   auto pre = [](int, int) {};
   auto epi = [&](f32x16(&acc)[4][2], int tm, int tn) {
+    const int lane = threadIdx.x & 63;
+    const Band band{lane, wave * 2048};
     // 32 tokens x 64 features at a time, the next ones asked for before the stores.
     i16x8 lines[2][4];
     int powers[2][2];
@@ -244,21 +254,22 @@ __global__ void __launch_bounds__(gemm::THREADS) gated_down_bwd_kernel(Operand V
     for (int step = 0; step < 4; ++step) {
       const int f0 = tm * BM + 128 * wm + 64 * (step & 1), first = tn * BN + 64 * wn + 32 * (step >> 1);
       const int nb = step >> 1;
-      const int now[2][2] = {{powers[0][0], powers[0][1]}, {powers[1][0], powers[1][1]}};
-      i16x8 g[2][2], dg[2][2], du[2][2];
+      i16x8 g[2][2];
       band.put_lines(lines[0]);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int h = 0; h < 2; ++h) g[p][h] = band.get_run(p, h);
       band.put_lines(lines[1]);
-      if (step < 3) fetch(step + 1);
+      GEMM_SCHED_FENCE();
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const float scale_g = scale_up(now[0][p]), scale_u = scale_up(now[1][p]);
+        const float scale_g = scale_up(powers[0][p]), scale_u = scale_up(powers[1][p]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f16x8 gates = __builtin_bit_cast(f16x8, g[p][h]), ups = __builtin_bit_cast(f16x8, band.get_run(p, h));
+          // dg takes u's place in the band, du that of g in registers.
+          tile::lds16x8* const at = band.slot(lane & 31, 4 * p + 2 * (lane >> 5) + h);
+          const f16x8 gates = __builtin_bit_cast(f16x8, g[p][h]), ups = __builtin_bit_cast(f16x8, *at);
           float vg[8], vu[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -268,17 +279,16 @@ __global__ void __launch_bounds__(gemm::THREADS) gated_down_bwd_kernel(Operand V
             vg[i] = dh * ((float)ups[i] * scale_u) * slope;
             vu[i] = dh * value;
           }
-          dg[p][h] = bf16_run(vg);
-          du[p][h] = bf16_run(vu);
+          *at = bf16_run(vg);
+          g[p][h] = bf16_run(vu);
+          GEMM_SCHED_FENCE();  // (the eights one after another: together they pass the registers)
         }
       }
-      Band::order();
-#pragma unroll
-      for (int p = 0; p < 2; ++p) band.put_run(p, dg[p][0], dg[p][1]);
+      if (step < 3) fetch(step + 1);
       bf16* const place = a.d_gate_up + (int64_t)first * 2 * a.f + f0;
       band.store(place, 2 * a.f, a.n - first, a.f - f0);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) band.put_run(p, du[p][0], du[p][1]);
+      for (int p = 0; p < 2; ++p) band.put_run(p, g[p][0], g[p][1]);
       band.store(place + a.f, 2 * a.f, a.n - first, a.f - f0);
     }
   };

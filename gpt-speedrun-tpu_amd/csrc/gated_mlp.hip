@@ -295,6 +295,111 @@ __global__ void __launch_bounds__(gemm::THREADS) gated_down_bwd_kernel(Operand V
   gemm::persistent<true, true, true>(V, DY, a.f, a.n, a.k, ntiles, coords, pre, epi);
 }
 
+// ---- few tokens ----
+//
+// The same three products in tiles of 64 tokens, where those of 256 x 256 would leave
+// most of the chip idle.  Four sets of waves share a tile's K and add their parts
+// through LDS: a workgroup's time is that of its loads, one after the other.
+
+// A lane's run of 16 features of a row.
+__device__ __forceinline__ void store_run(bf16* row, int feature, int features, const float* v) {
+  if (feature < features) *reinterpret_cast<bf16x8*>(row + feature) = pack8(v);
+  if (feature + 8 < features) *reinterpret_cast<bf16x8*>(row + feature + 8) = pack8(v + 8);
+}
+
+template <int kAct, bool kKeep>
+__global__ void __launch_bounds__(1024) gated_up_few_kernel(tile::Operand W, tile::Operand X, UpArgs a) {
+  typedef tile::Product<bf16, 2, 1, tile::kPairsMN, tile::kRowsK, true, 1, 4, 3> P;
+  const auto at = P::place();
+  const int tm = blockIdx.x, tn = blockIdx.y;
+  f32x16 acc[2][1];
+  P::run(acc, W, X, 2 * a.f, a.n, a.k, tm * P::TM, tn * P::TN, at);
+  if (at.group) return;
+  const int lane = at.lane, first = tn * P::TN + 32 * at.wn, token = first + (lane & 31);
+  const int f0 = tm * (P::TM / 2) + 32 * at.wm, feature = f0 + 16 * (lane >> 5);
+  float g[16], u[16], h[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    g[i] = acc[0][0][i];
+    u[i] = acc[1][0][i];
+    h[i] = act_f<kAct>(g[i]) * u[i];
+    if (i == 7) GEMM_SCHED_FENCE();  // (sixteen at once pass the registers of 16 waves)
+  }
+  if (kKeep) {
+    // (Powers are laid out by blocks of 64 features.)
+    const int block = (f0 >> 5) & 1;
+    const int power_g = power_of(g), power_u = power_of(u);
+    a.kept.put_power(0, block, power_g, f0 & ~63, first, a.n, a.f, lane);
+    a.kept.put_power(1, block, power_u, f0 & ~63, first, a.n, a.f, lane);
+    if (token < a.n) {
+      short* const row = (short*)a.kept.values + (int64_t)token * 2 * a.f + feature;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (feature + 8 * e < a.f) {
+          *(i16x8*)(row + 8 * e) = f16_run(g + 8 * e, scale_down(power_g));
+          *(i16x8*)(row + a.f + 8 * e) = f16_run(u + 8 * e, scale_down(power_u));
+        }
+    }
+  }
+  if (token < a.n) store_run(a.h + (int64_t)token * a.f, feature, a.f, h);
+}
+
+template <int kAct>
+__global__ void __launch_bounds__(1024) gated_down_bwd_few_kernel(tile::Operand V, tile::Operand DY, DownBwdArgs a) {
+  typedef tile::Product<bf16, 1, 1, tile::kRowsK, tile::kRowsK, true, 1, 4> P;
+  const auto at = P::place();
+  const int tm = blockIdx.x, tn = blockIdx.y;
+  f32x16 acc[1][1];
+  P::run(acc, V, DY, a.f, a.n, a.k, tm * P::TM, tn * P::TN, at);
+  if (at.group) return;
+  const int lane = at.lane, first = tn * P::TN + 32 * at.wn, token = first + (lane & 31);
+  const int f0 = tm * P::TM + 32 * at.wm, feature = f0 + 16 * (lane >> 5), block = (f0 >> 5) & 1;
+  const float scale_g = scale_up(a.kept.get_power(0, block, f0 & ~63, first, a.n, a.f, lane));
+  const float scale_u = scale_up(a.kept.get_power(1, block, f0 & ~63, first, a.n, a.f, lane));
+  if (token >= a.n) return;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (feature + 8 * e >= a.f) continue;
+    const int64_t own = (int64_t)token * 2 * a.f + feature + 8 * e;
+    const f16x8 g = *(const f16x8*)(a.kept.values + own), u = *(const f16x8*)(a.kept.values + own + a.f);
+    float dg[8], du[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float dh = acc[0][0][8 * e + i];
+      float value, slope;
+      act_both<kAct>((float)g[i] * scale_g, value, slope);
+      dg[i] = dh * ((float)u[i] * scale_u) * slope;
+      du[i] = dh * value;
+    }
+    *reinterpret_cast<bf16x8*>(a.d_gate_up + own) = pack8(dg);
+    *reinterpret_cast<bf16x8*>(a.d_gate_up + own + a.f) = pack8(du);
+  }
+}
+
+// y [n][m] = x [n][k] w, w [k][m] (kRowsMN) or [m][k] (kRowsK), in tiles of 64 T x 64 T.
+template <tile::Layout kW, int T, int kGroups>
+__global__ void __launch_bounds__(256 * kGroups, kGroups == 1 ? 2 : 1)
+    gated_linear_few_kernel(tile::Operand W, tile::Operand X, bf16* y, int n, int k, int m) {
+  typedef tile::Product<bf16, T, T, kW, tile::kRowsK, true, 1, kGroups> P;
+  const auto at = P::place();
+  const int tm = blockIdx.x, tn = blockIdx.y;
+  f32x16 acc[T][T];
+  P::run(acc, W, X, m, n, k, tm * P::TM, tn * P::TN, at);
+  if (at.group) return;
+#pragma unroll
+  for (int nb = 0; nb < T; ++nb) {
+    const int token = tn * P::TN + 32 * (T * at.wn + nb) + (at.lane & 31);
+    if (token >= n) continue;
+#pragma unroll
+    for (int mb = 0; mb < T; ++mb) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = acc[mb][nb][i];
+      store_run(y + (int64_t)token * m, tm * P::TM + 32 * (T * at.wm + mb) + 16 * (at.lane >> 5), m, v);
+    }
+  }
+}
+
 // ---- weight gradients ----
 
 struct GradItem {
@@ -414,12 +519,73 @@ bool rows_ok(const void* p, int64_t ld, int width) {
   return ld >= width && ld % 8 == 0 && ld <= kMostStride && ((uintptr_t)p & 15) == 0;
 }
 
+// Tiles of 256 x 256 from which a product takes them.  Measured at d 768, f 2048 (us, by
+// tokens; the larger tiles against 64 x 64 with four sets of waves, or 128 x 128):
+//   x W      1024 (64 tiles) 26.7 / 19.9, 2048 (128) 28.1 / 35.3
+//   dy V^T   1024 (32) 33.8 / 18.8, 2048 (64) 33.9 / 32.7, 4096 (128) 36.5 / 62.3
+//   h V      1 42 / 7, 1024 (12) 44 / 11.6 / 17.3, 2048 (24) 44 / 22.9 / 18.3,
+//            4096 (48) 47 / 36 / 21, 8192 (96) 52 / 72 / 39, 16384 (192) 63 / 140 / 76
+constexpr int kPairTiles = 68;                   // x W and dy V^T, against 64 tokens
+constexpr int kLinearTiles = 110, kLinearFew = 18;  // h V and dx, against 128 x 128; those against 64 x 64
+
 unsigned persistent_grid(int tiles) {
   const int cus = gemm::device_cus();
   return (unsigned)(tiles < cus ? tiles : cus);
 }
 
 int tile_group(int m_tiles) { return m_tiles <= 16 ? m_tiles : gemm::kGroupM; }
+
+// Whether the product of m features over n tokens with g and u at its end goes to the tiles of 64 tokens.
+bool few(int n, int m) { return tiles_of(m, n) < kPairTiles; }
+
+dim3 few_grid(int m, int tile_m, int n) { return dim3(ceil_div(m, tile_m), ceil_div(n, 64)); }
+
+template <tile::Layout kW>
+void launch_linear_few(const tile::Operand& W, const tile::Operand& X, void* y, int n, int k, int m, bool wide,
+                       hipStream_t s) {
+  if (wide)
+    gated_linear_few_kernel<kW, 2, 1><<<dim3(ceil_div(m, 128), ceil_div(n, 128)), 256, 0, s>>>(W, X, (bf16*)y, n, k, m);
+  else
+    gated_linear_few_kernel<kW, 1, 4><<<dim3(ceil_div(m, 64), ceil_div(n, 64)), 1024, 0, s>>>(W, X, (bf16*)y, n, k, m);
+}
+
+int linear(const void* x, int64_t ldx, const void* w, int64_t ldw, bool w_kmajor, void* y, int n, int k, int m,
+           hipStream_t s) {
+  const int tiles = tiles_of(m, n);
+  if (tiles >= kLinearTiles) return gptrig_linear(x, ldx, w, ldw, w_kmajor, nullptr, y, m, n, k, m, s);
+  const tile::Operand W{w, ldw}, X{x, ldx};
+  if (w_kmajor)
+    launch_linear_few<tile::kRowsK>(W, X, y, n, k, m, tiles >= kLinearFew, s);
+  else
+    launch_linear_few<tile::kRowsMN>(W, X, y, n, k, m, tiles >= kLinearFew, s);
+  GPTRIG_CHECK_LAUNCH();
+  return GPTRIG_OK;
+}
+
+template <int kAct>
+void launch_up(const Operand& W, const Operand& X, const UpArgs& a, hipStream_t s) {
+  if (few(a.n, 2 * a.f)) {
+    const tile::Operand w{W.p, W.ld, W.pair}, x{X.p, X.ld};
+    if (a.kept.values)
+      gated_up_few_kernel<kAct, true><<<few_grid(2 * a.f, 128, a.n), 1024, 0, s>>>(w, x, a);
+    else
+      gated_up_few_kernel<kAct, false><<<few_grid(2 * a.f, 128, a.n), 1024, 0, s>>>(w, x, a);
+    return;
+  }
+  const unsigned grid = persistent_grid(tiles_of(2 * a.f, a.n));
+  if (a.kept.values)
+    gated_up_kernel<kAct, true><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
+  else
+    gated_up_kernel<kAct, false><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
+}
+
+template <int kAct>
+void launch_down_bwd(const Operand& V, const Operand& DY, const DownBwdArgs& a, hipStream_t s) {
+  if (few(a.n, a.f))
+    gated_down_bwd_few_kernel<kAct><<<few_grid(a.f, 64, a.n), 1024, 0, s>>>({V.p, V.ld}, {DY.p, DY.ld}, a);
+  else
+    gated_down_bwd_kernel<kAct><<<persistent_grid(tiles_of(a.f, a.n)), gemm::THREADS, 0, s>>>(V, DY, a);
+}
 
 }  // namespace
 
@@ -437,17 +603,12 @@ int gptrig_gated_mlp_fwd(const void* x, int64_t ldx, const void* gate_up_w, int6
   const hipStream_t s = (hipStream_t)stream;
   const Operand W{(const bf16*)gate_up_w, ldw, 0, f}, X{(const bf16*)x, ldx};
   const UpArgs a{kept_at(kept, n, f), (bf16*)h, n, d, f, tile_group(ceil_div(2 * f, BM))};
-  const unsigned grid = persistent_grid(tiles_of(2 * f, n));
-  if (activation == kSilu && kept)
-    gated_up_kernel<kSilu, true><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
-  else if (activation == kSilu)
-    gated_up_kernel<kSilu, false><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
-  else if (kept)
-    gated_up_kernel<kGelu, true><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
+  if (activation == kSilu)
+    launch_up<kSilu>(W, X, a, s);
   else
-    gated_up_kernel<kGelu, false><<<grid, gemm::THREADS, 0, s>>>(W, X, a);
+    launch_up<kGelu>(W, X, a, s);
   GPTRIG_CHECK_LAUNCH();
-  return gptrig_linear(h, f, down_w, ldv, 0, nullptr, y, d_out, n, f, d_out, stream);
+  return linear(h, f, down_w, ldv, false, y, n, f, d_out, s);
 }
 
 size_t gptrig_gated_mlp_kept_bytes(int n, int f) {
@@ -480,15 +641,14 @@ int gptrig_gated_mlp_bwd(const void* dy, int64_t lddy, const void* x, int64_t ld
   if (dx || d_gate_up_w) {
     const Operand V{(const bf16*)down_w, ldv}, DY{(const bf16*)dy, lddy};
     const DownBwdArgs a{kept_at(const_cast<void*>(kept), n, f), dgu, n, d_out, f, tile_group(ceil_div(f, BM))};
-    const unsigned grid = persistent_grid(tiles_of(f, n));
     if (activation == kSilu)
-      gated_down_bwd_kernel<kSilu><<<grid, gemm::THREADS, 0, s>>>(V, DY, a);
+      launch_down_bwd<kSilu>(V, DY, a, s);
     else
-      gated_down_bwd_kernel<kGelu><<<grid, gemm::THREADS, 0, s>>>(V, DY, a);
+      launch_down_bwd<kGelu>(V, DY, a, s);
     GPTRIG_CHECK_LAUNCH();
   }
   if (dx) {
-    const int status = gptrig_linear(dgu, 2 * (int64_t)f, gate_up_w, ldw, 1, nullptr, dx, d, n, 2 * f, d, stream);
+    const int status = linear(dgu, 2 * (int64_t)f, gate_up_w, ldw, true, dx, n, 2 * f, d, s);
     if (status != GPTRIG_OK) return status;
   }
   GradItems g{};

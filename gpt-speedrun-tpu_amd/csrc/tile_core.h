@@ -41,11 +41,14 @@ __device__ __forceinline__ f32x16 mma(i16x8 a, i16x8 b, f32x16 c, f16) {
 // rows of 64 bytes.  A copy takes 1 KB: of a blocked operand 16 rows of a block, one
 // run of whole lines, for which the address unit needs some 20 cycles; 64-byte pieces
 // of lines (K-major rows) take it 40 to 50.
-enum Layout { kRowsK, kRowsMN, kBlockedK, kBlockedMN };
+// kPairsMN: two kRowsMN matrices side by side, the second `pair` elements after the
+// first, whose columns take turns in the tile in blocks of 32 (gemm::Operand's).
+enum Layout { kRowsK, kRowsMN, kPairsMN, kBlockedK, kBlockedMN };
 
 struct Operand {
   const void* p;
   int64_t ld;
+  int64_t pair = 0;
 };
 
 template <int kBytes, int kStage>
@@ -75,6 +78,10 @@ struct Source {
   // mn0: the tile's first row, MN: the operand's rows; K range [k_begin, k_end).
   // (k_begin is a multiple of 32 and mn0 of 64: blocked stages and tiles start on a block.)
   __device__ __forceinline__ void init(Operand op, int mn0, int MN, int k_begin, int k_end, int wave, int lane) {
+    if (kLayout == kPairsMN) {  // columns of one of the two matrices
+      mn0 >>= 1;
+      MN >>= 1;
+    }
     const int r0 = kK ? mn0 : k_begin, c0 = kK ? k_begin : mn0;  // as the memory has rows and columns
     if (kBlocked) {
       base = (const char*)op.p + ((int64_t)(c0 >> 5) * op.ld + r0) * 64;
@@ -87,20 +94,26 @@ struct Source {
     for (int j = 0; j < P; ++j) {
       const int b = wave * P + j, slab = b / (TM / 16), blk = b % (TM / 16);
       int k, m;
+      bool second = false;
       if (kK) {
         m = blk * 16 + (lane >> 2);
         k = 32 * slab + 8 * ((lane & 3) ^ ((m >> 2) & 3));
-      } else if (kLayout == kRowsMN) {
+      } else if (!kBlocked) {
         constexpr int kChunks = TM / 8;
         const int row = blk * (512 / TM) + lane / kChunks;
         k = 32 * slab + row;
         m = 8 * ((lane % kChunks) ^ swizzle(row));
+        if (kLayout == kPairsMN) {
+          second = (m >> 5) & 1;
+          m = 32 * (m >> 6) + (m & 31);
+        }
       } else {
         k = 32 * slab + 16 * (blk & 1) + (lane >> 2);
         m = 32 * (blk >> 1) + 8 * (lane & 3);
       }
       const int r = kK ? m : k, c = kK ? k : m;
-      off[j] = 2u * (uint32_t)(kBlocked ? ((int64_t)(c >> 5) * op.ld + r) * 32 + (c & 31) : (int64_t)r * op.ld + c);
+      off[j] = 2u * (uint32_t)(kBlocked ? ((int64_t)(c >> 5) * op.ld + r) * 32 + (c & 31)
+                                        : (int64_t)r * op.ld + c + (second ? op.pair : 0));
       const int rem = k_end - k_begin - k;
       nvalid[j] = (mn0 + m < MN && rem > 0) ? (rem + kDepth - 1) / kDepth : 0;
     }
@@ -348,13 +361,13 @@ struct Product {
       };
       if (at.group == 1) put(stage_array<kStageBytes, 1>());
       if (kGroups > 2 && at.group == 2) put(stage_array<kStageBytes, 2>());
-      if (kGroups > 3 && at.group == 3) put(stage_array<kStageBytes, 3>());
+      if (kGroups > 3 && at.group == 3) put(stage_array<kStageBytes, 3 % kRing>());
       GPTRIG_WAIT_LGKM0();
       wg_barrier();
       if (at.group == 0) {
         add(stage_array<kStageBytes, 1>());
         if (kGroups > 2) add(stage_array<kStageBytes, 2>());
-        if (kGroups > 3) add(stage_array<kStageBytes, 3>());
+        if (kGroups > 3) add(stage_array<kStageBytes, 3 % kRing>());
       }
     }
 #endif

@@ -100,7 +100,8 @@ def test_sizes(n, sizes, kind):
     check(kernels(*args, kind), exact(*args, kind), bounds(*args, kind))
 
 
-@pytest.mark.parametrize("n,d,f,kind", [(1000, 1000, 2664, "gelu"), (4097, 512, 1360, "silu"), (129, 768, 2048, "silu")])
+@pytest.mark.parametrize("n,d,f,kind", [(1000, 1000, 2664, "gelu"), (4097, 512, 1360, "silu"), (129, 768, 2048, "silu"),
+                                        (5000, 264, 136, "silu"), (9001, 200, 2056, "gelu"), (2049, 1032, 520, "silu")])
 def test_larger(n, d, f, kind):
     args = data(n, d, f, d)
     check(kernels(*args, kind), exact(*args, kind), bounds(*args, kind))

@@ -19,7 +19,8 @@
 //      float32; rows that lie inside the chunk are written, of a row that crosses
 //      its start or its end the part goes to the workspace (at most two a chunk).
 //      The same launch writes zeros to the rows that no token names.
-//   3. Rows that cross chunks are joined from their parts, in order.
+//   3. Rows that cross chunks are joined from their parts, in order.  The launch before
+//      lists them; the list's order changes nothing.
 #include <algorithm>
 
 #include "common.h"
@@ -27,7 +28,10 @@
 namespace {
 
 constexpr int kDigits = 256;      // bins of a pass
-constexpr int kOneBlock = 8192;   // most tokens that one workgroup sorts
+// Most tokens that one workgroup sorts: 34 us for 8191 of them against 23 in four
+// launches, but those cost the host more than they save the GPU (a pass 79 us against
+// 111), until there are more.
+constexpr int kOneBlock = 8192;
 constexpr int kMostBlocks = 256;  // most workgroups of a pass
 constexpr int kSlab = 256;        // columns of a row that a wave holds: four a lane
 
@@ -36,8 +40,9 @@ struct Sort {
   int wide;  // tokens are int64
   int vocab;
   int n;
-  int seg;     // positions of a block, a multiple of 64 per wave
+  int seg;  // positions of a block
   int blocks;
+  int* crossing;  // a number that the sort leaves 0
 };
 
 template <bool kWide>
@@ -52,17 +57,17 @@ __device__ __forceinline__ int load_key(const Sort& s, const int* keys, int i) {
 }
 
 // counts[block][digit] of the digit at `shift`; keys NULL: the tokens themselves.
-__global__ void __launch_bounds__(256) radix_histogram_kernel(Sort s, const int* __restrict__ keys,
+__global__ void __launch_bounds__(1024) radix_histogram_kernel(Sort s, const int* __restrict__ keys,
                                                               int* __restrict__ counts, int shift) {
   __shared__ int bins[kDigits];
-  bins[threadIdx.x] = 0;
+  if (threadIdx.x < kDigits) bins[threadIdx.x] = 0;
   __syncthreads();
   const int64_t begin = (int64_t)blockIdx.x * s.seg;
   const int end = (int)min((int64_t)s.n, begin + s.seg);
-  for (int i = (int)begin + (int)threadIdx.x; i < end; i += 256)
+  for (int i = (int)begin + (int)threadIdx.x; i < end; i += 1024)
     atomicAdd(&bins[(load_key(s, keys, i) >> shift) & (kDigits - 1)], 1);
   __syncthreads();
-  counts[blockIdx.x * kDigits + threadIdx.x] = bins[threadIdx.x];
+  if (threadIdx.x < kDigits) counts[blockIdx.x * kDigits + threadIdx.x] = bins[threadIdx.x];
 }
 
 // One block's stable scatter of positions [begin, end) by the digit at `shift`.
@@ -130,27 +135,32 @@ __device__ void exclusive_scan(int* totals, int tid) {
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
     radix_scatter_kernel(Sort s, const int* __restrict__ keys, const int* __restrict__ positions,
                          const int* __restrict__ counts, int* __restrict__ keys_out, int* __restrict__ positions_out,
                          int shift) {
-  __shared__ int place[4][kDigits];
-  __shared__ int bases[kDigits];
-  const int tid = threadIdx.x;
-  int before = 0, total = 0;
+  __shared__ int place[16][kDigits];
+  __shared__ int bases[kDigits], before[kDigits];
+  const int tid = threadIdx.x, digit = tid & (kDigits - 1);
+  if (tid < kDigits) bases[tid] = before[tid] = 0;
+  if (blockIdx.x == 0 && tid == 0) *s.crossing = 0;
+  __syncthreads();
+  // Four threads a digit share the blocks.
+  int mine = 0, total = 0;
 #pragma unroll 8
-  for (int b = 0; b < s.blocks; ++b) {
-    const int c = counts[b * kDigits + tid];
+  for (int b = tid / kDigits; b < s.blocks; b += 4) {
+    const int c = counts[b * kDigits + digit];
     total += c;
-    before += b < (int)blockIdx.x ? c : 0;
+    mine += b < (int)blockIdx.x ? c : 0;
   }
-  bases[tid] = total;
+  atomicAdd(&bases[digit], total);
+  atomicAdd(&before[digit], mine);
   __syncthreads();
   exclusive_scan(bases, tid);
-  bases[tid] += before;
+  if (tid < kDigits) bases[tid] += before[tid];
   const int64_t begin = (int64_t)blockIdx.x * s.seg;
-  scatter_block<4>(s, keys, positions, keys_out, positions_out, shift, (int)begin,
-                   (int)min((int64_t)s.n, begin + s.seg), place, bases);
+  scatter_block<16>(s, keys, positions, keys_out, positions_out, shift, (int)begin,
+                    (int)min((int64_t)s.n, begin + s.seg), place, bases);
 }
 
 // All passes of a short sort; the buffers change roles after each.
@@ -159,6 +169,7 @@ __global__ void __launch_bounds__(1024) radix_one_block_kernel(Sort s, int* keys
   __shared__ int place[16][kDigits];
   __shared__ int bases[kDigits];
   const int tid = threadIdx.x;
+  if (tid == 0) *s.crossing = 0;
   for (int p = 0; p < passes; ++p) {
     // The last pass writes b.
     const bool to_b = ((passes - p) & 1) != 0;
@@ -227,19 +238,28 @@ __global__ void __launch_bounds__(256)
                           OT* __restrict__ y, int64_t n, int d, int vocab, float scale) {
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * 4;
-  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += waves) {
-    int key = wide ? token_key<true>(tokens, i, vocab) : token_key<false>(tokens, i, vocab);
-    key = __builtin_amdgcn_readfirstlane(key);
+  int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  auto key_of = [&](int64_t at) {
+    return wide ? token_key<true>(tokens, min(at, n - 1), vocab) : token_key<false>(tokens, min(at, n - 1), vocab);
+  };
+  for (int ahead = key_of(i); i < n; i += waves) {
+    const int key = __builtin_amdgcn_readfirstlane(ahead);
+    ahead = key_of(i + waves);
     const TT* row = table + (int64_t)key * ldt;
     OT* out = y + i * d;
-    for (int column = 0; column < d; column += kSlab) {
-      f32x4 v{};
+    // Four slabs in flight: a wave's rows wait for each other otherwise.
+    for (int column = 0; column < d; column += 4 * kSlab) {
+      f32x4 v[4]{};
       if (key < vocab) {
-        v = load_columns<TT, kVec>(row, column, lane, d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= scale;
+        for (int k = 0; k < 4; ++k) v[k] = load_columns<TT, kVec>(row, column + k * kSlab, lane, d);
       }
-      store_columns<OT, kVec>(out, v, column, lane, d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[k][j] *= scale;
+        store_columns<OT, kVec>(out, v[k], column + k * kSlab, lane, d);
+      }
     }
   }
 }
@@ -248,6 +268,7 @@ struct Reduce {
   const int* keys;       // sorted
   const int* positions;  // of each key, ascending within a key
   float* parts;          // [chunks][2][d]: of a row that began before the chunk, of one that goes on after it
+  int* crossing;         // the number of rows that cross chunks, then the chunks where they begin (in any order)
   int n, d, vocab, chunk, chunks, slabs;
   float scale;
 };
@@ -300,15 +321,17 @@ __device__ __forceinline__ void add_chunk(const Reduce& r, const GT* __restrict_
       }
     }
   }
-  flush(current, head, current == first_after);
+  const bool goes_on = current == first_after && current < r.vocab;
+  flush(current, head, goes_on);
+  if (goes_on && !head && column == 0 && lane == 0) r.crossing[1 + atomicAdd(r.crossing, 1)] = chunk;
 }
 
-// First index of the sorted keys that is at least (kAfter: above) k.
-template <bool kAfter>
-__device__ __forceinline__ int key_bound(const int* keys, int low, int high, int k) {
+// First index of the sorted keys that is at least k.
+__device__ __forceinline__ int key_bound(const int* keys, int high, int k) {
+  int low = 0;
   while (low < high) {
     const int mid = low + ((high - low) >> 1);
-    if (kAfter ? keys[mid] <= k : keys[mid] < k) low = mid + 1;
+    if (keys[mid] < k) low = mid + 1;
     else high = mid;
   }
   return low;
@@ -329,7 +352,7 @@ __global__ void __launch_bounds__(256) embedding_reduce_kernel(Reduce r, const G
     }
     const int64_t first = (w - add_waves) * kZeroRows;
     const int row = (int)min(first + (lane & (kZeroRows - 1)), (int64_t)r.vocab - 1);
-    const int at = key_bound<false>(r.keys, 0, r.n, row);
+    const int at = key_bound(r.keys, r.n, row);
     const bool absent = at >= r.n || r.keys[at] != row;
     uint64_t rows = __ballot(absent && lane < kZeroRows && first + lane < r.vocab);
     while (rows) {  // uniform
@@ -341,38 +364,45 @@ __global__ void __launch_bounds__(256) embedding_reduce_kernel(Reduce r, const G
   }
 }
 
-// Rows that cross chunks: the workgroup of the chunk where such a row begins adds
-// its parts, each wave those of every fourth chunk, the waves' sums in order.
+constexpr int kJoin = 8;  // waves that join a row's parts
+
+// Rows that cross chunks: a workgroup for each (and each slab of it) adds its parts,
+// each wave those of every eighth chunk, the waves' sums in order.
 template <typename OT, bool kVec>
-__global__ void __launch_bounds__(256) embedding_join_kernel(Reduce r, OT* __restrict__ dtable, int64_t items) {
-  __shared__ f32x4 sums[4][64];
+__global__ void __launch_bounds__(64 * kJoin) embedding_join_kernel(Reduce r, OT* __restrict__ dtable) {
+  __shared__ f32x4 sums[kJoin][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t items = (int64_t)*r.crossing * r.slabs;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int chunk = (int)(item / r.slabs), column = (int)(item % r.slabs) * kSlab;
-    const int64_t begin = (int64_t)chunk * r.chunk, end = begin + r.chunk;
-    if (end >= r.n) continue;  // (uniform, here and below)
+    const int chunk = r.crossing[1 + item / r.slabs], column = (int)(item % r.slabs) * kSlab;
+    const int64_t end = ((int64_t)chunk + 1) * r.chunk;
     const int key = r.keys[end - 1];
-    if (key >= r.vocab || key != r.keys[end]) continue;
-    if (r.keys[begin] == key && begin > 0 && r.keys[begin - 1] == key) continue;  // it began earlier
-    const int stop = key_bound<true>(r.keys, (int)end, r.n, key);
-    const int last = (stop - 1) / r.chunk;  // the chunk where it ends
+    // The chunk where it ends: the last that begins with it, looked for 64 at a time.
+    int last = chunk;
+    for (uint64_t more = ~0ull; more == ~0ull;) {
+      const int64_t at = ((int64_t)last + 1 + lane) * r.chunk;
+      more = __ballot(at < r.n && r.keys[min(at, (int64_t)r.n - 1)] == key);
+      last += more == ~0ull ? 64 : __builtin_ctzll(~more);
+    }
     f32x4 sum{};
     if (wave == 0) sum = load_columns<float, kVec>(r.parts + ((int64_t)chunk * 2 + 1) * r.d, column, lane, r.d);
     int c = chunk + 1 + wave;
-    for (; c + 12 <= last; c += 16) {
-      f32x4 v[4];
+    constexpr int kAhead = 8;  // parts in flight
+    for (; c + (kAhead - 1) * kJoin <= last; c += kAhead * kJoin) {
+      f32x4 v[kAhead];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[j] = load_columns<float, kVec>(r.parts + (int64_t)(c + 4 * j) * 2 * r.d, column, lane, r.d);
+      for (int j = 0; j < kAhead; ++j)
+        v[j] = load_columns<float, kVec>(r.parts + (int64_t)(c + kJoin * j) * 2 * r.d, column, lane, r.d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += v[j];
+      for (int j = 0; j < kAhead; ++j) sum += v[j];
     }
-    for (; c <= last; c += 4) sum += load_columns<float, kVec>(r.parts + (int64_t)c * 2 * r.d, column, lane, r.d);
+    for (; c <= last; c += kJoin) sum += load_columns<float, kVec>(r.parts + (int64_t)c * 2 * r.d, column, lane, r.d);
     __syncthreads();  // (the last item's sums are read)
     sums[wave][lane] = sum;
     __syncthreads();
     if (wave == 0) {
-      sum = ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane];
+#pragma unroll
+      for (int w = 1; w < kJoin; ++w) sum += sums[w][lane];
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] *= r.scale;
       store_columns<OT, kVec>(dtable + (int64_t)key * r.d, sum, column, lane, r.d);
@@ -384,7 +414,7 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(Reduce r, OT* __res
 
 struct Plan {
   int passes, seg, blocks, chunk, chunks, slabs;
-  size_t pairs, counts, parts, total;  // bytes: one int array, the histograms, the parts; all of it
+  size_t pairs, counts, crossing, parts, total;  // bytes: one int array, the histograms, ...; all of it
 };
 
 size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -394,7 +424,7 @@ Plan make_plan(int n, int d, int vocab) {
   int bits = 0;
   while (bits < 31 && (vocab >> bits) != 0) ++bits;  // (the key `vocab` is one of them)
   p.passes = std::max(1, (bits + 7) / 8);
-  p.seg = std::max(1024, ceil_div(ceil_div(n, kMostBlocks), 1024) * 1024);
+  p.seg = std::max(2048, ceil_div(ceil_div(n, kMostBlocks), 2048) * 2048);
   p.blocks = n <= kOneBlock ? 1 : ceil_div(n, p.seg);
   // Pairs a chunk: enough waves for the chip where there are few, fewer parts where there are many.
   p.chunk = 4;
@@ -403,8 +433,9 @@ Plan make_plan(int n, int d, int vocab) {
   p.slabs = ceil_div(d, kSlab);
   p.pairs = round_up((size_t)n * 4);
   p.counts = round_up((size_t)p.blocks * kDigits * 4);
+  p.crossing = round_up(((size_t)p.chunks + 1) * 4);
   p.parts = round_up((size_t)p.chunks * 2 * d * 4);
-  p.total = 4 * p.pairs + p.counts + p.parts;
+  p.total = 4 * p.pairs + p.counts + p.crossing + p.parts;
   return p;
 }
 
@@ -416,6 +447,9 @@ bool aligned(const void* p, int64_t ld, int type) { return ld % 4 == 0 && (uintp
 
 constexpr int64_t kMostGrid = 1 << 20;  // workgroups a launch; more work is looped over
 
+constexpr unsigned kJoinGrid = 1024;    // of the join, which learns on the GPU how much there is
+constexpr unsigned kRowsGrid = 2048;    // of the lookup: eight a CU, which is all that a CU holds
+
 unsigned grid_of(int64_t items, int per_block) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>(kMostGrid, (items + per_block - 1) / per_block));
 }
@@ -423,7 +457,7 @@ unsigned grid_of(int64_t items, int per_block) {
 template <typename TT, typename OT>
 void launch_rows(bool vec, const void* tokens, int wide, const void* table, int64_t ldt, void* y, int64_t n, int d,
                  int vocab, float scale, hipStream_t s) {
-  const unsigned grid = grid_of(n, 4);
+  const unsigned grid = std::min(grid_of(n, 4), kRowsGrid);
   if (vec)
     embedding_rows_kernel<TT, OT, true><<<grid, 256, 0, s>>>(tokens, wide, (const TT*)table, ldt, (OT*)y, n, d, vocab, scale);
   else
@@ -436,7 +470,8 @@ int launch_reduce_as(const Reduce& r, const void* dy, int64_t lddy, void* dtable
   embedding_reduce_kernel<GT, OT, kVec><<<grid_of(add + zero, 4), 256, 0, s>>>(r, (const GT*)dy, lddy, (OT*)dtable, add,
                                                                               zero);
   GPTRIG_CHECK_LAUNCH();
-  embedding_join_kernel<OT, kVec><<<grid_of(add, 1), 256, 0, s>>>(r, (OT*)dtable, add);
+  if (!add) return GPTRIG_OK;
+  embedding_join_kernel<OT, kVec><<<std::min(grid_of(add, 1), kJoinGrid), 64 * kJoin, 0, s>>>(r, (OT*)dtable);
   GPTRIG_CHECK_LAUNCH();
   return GPTRIG_OK;
 }
@@ -499,6 +534,7 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
   Plan p{};
   int* keys = nullptr;
   int* positions = nullptr;
+  int* crossing = nullptr;
   float* parts = nullptr;
   if (n > 0) {
     p = make_plan((int)n, d, vocab);
@@ -510,8 +546,9 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
     int* const keys_b = (int*)(at + 2 * p.pairs);
     int* const positions_b = (int*)(at + 3 * p.pairs);
     int* const counts = (int*)(at + 4 * p.pairs);
-    parts = (float*)(at + 4 * p.pairs + p.counts);
-    const Sort sort{tokens, tokens_are_int64, vocab, (int)n, p.seg, p.blocks};
+    crossing = (int*)(at + 4 * p.pairs + p.counts);
+    parts = (float*)(at + 4 * p.pairs + p.counts + p.crossing);
+    const Sort sort{tokens, tokens_are_int64, vocab, (int)n, p.seg, p.blocks, crossing};
     if (p.blocks == 1) {
       radix_one_block_kernel<<<1, 1024, 0, s>>>(sort, keys_a, positions_a, keys_b, positions_b, p.passes);
       GPTRIG_CHECK_LAUNCH();
@@ -521,16 +558,16 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
       for (int pass = 0; pass < p.passes; ++pass) {
         int* const keys_to = pass & 1 ? keys_a : keys_b;
         int* const positions_to = pass & 1 ? positions_a : positions_b;
-        radix_histogram_kernel<<<p.blocks, 256, 0, s>>>(sort, keys, counts, 8 * pass);
+        radix_histogram_kernel<<<p.blocks, 1024, 0, s>>>(sort, keys, counts, 8 * pass);
         GPTRIG_CHECK_LAUNCH();
-        radix_scatter_kernel<<<p.blocks, 256, 0, s>>>(sort, keys, positions, counts, keys_to, positions_to, 8 * pass);
+        radix_scatter_kernel<<<p.blocks, 1024, 0, s>>>(sort, keys, positions, counts, keys_to, positions_to, 8 * pass);
         GPTRIG_CHECK_LAUNCH();
         keys = keys_to;
         positions = positions_to;
       }
     }
   }
-  const Reduce r{keys, positions, parts, (int)n, d, vocab, std::max(1, p.chunk), p.chunks, ceil_div(d, kSlab), scale};
+  const Reduce r{keys, positions, parts, crossing, (int)n, d, vocab, std::max(1, p.chunk), p.chunks, ceil_div(d, kSlab), scale};
   const bool vec = d % 4 == 0 && (n == 0 || aligned(dy, lddy, dy_type)) && aligned(dtable, d, table_type);
   if (dy_type == GPTRIG_TYPE_F32 && table_type == GPTRIG_TYPE_F32)
     return launch_reduce<float, float>(vec, r, dy, lddy, dtable, s);

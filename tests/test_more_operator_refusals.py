@@ -61,11 +61,12 @@ def test_embedding_entry_points_check_their_arguments():
 
 @pytest.mark.parametrize("n", [1, 1000, 8192, 8193, 65536, 131072, 10 ** 6, 2 ** 31 - 65537])
 def test_embedding_workspace(n):
-    """Two buffers of pairs, the histograms of at most 256 blocks, two partial rows a chunk of four pairs or more."""
+    """Two buffers of pairs, the histograms of at most 256 blocks, two partial rows a chunk of four pairs or more, and
+    its number."""
 
     size = _lib.query("gptrig_scaled_embedding_bwd_workspace_bytes", n, 16, 1000)
     chunks = [-(-n // c) for c in (4, 32)]
-    assert 16 * n + 128 * chunks[1] <= size <= 16 * n + 128 * chunks[0] + 256 * 1024 + 6 * 256
+    assert 16 * n + 132 * chunks[1] <= size <= 16 * n + 132 * chunks[0] + 256 * 1024 + 7 * 256
 
 
 def test_gated_mlp_refusals():

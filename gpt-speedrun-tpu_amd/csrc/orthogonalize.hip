@@ -18,10 +18,13 @@
 // an error of X in the directions of small singular values grows by a each step (485
 // times in five), but only through the term a X, which is computed from all 22 bits;
 // in B X the rounding of X meets B, which is small in those directions, and the
-// rounding of B multiplies what is there.  In simulations over spectra from flat to
-// falling by 10^6 the result differs from the exact one by 0.1 to 0.9 times the
-// rounding to bfloat16 that follows; with X in one float16 by up to 24 times, in
-// one bfloat16 by up to 200 times.
+// rounding of B multiplies what is there.  The diagonals of A and B stay in float32
+// and out of the products (A = D + O: A A = D D + D O + O D + O O; a X + B X = (a +
+// diag B) X + the rest): the more alike the singular values, the more of A and B lies
+// there.  In simulations, of 1 to 2000 rows and of spectra from flat to falling by
+// 10^6, the result is then off by 1.0 to 1.2 times the rounding to bfloat16 alone (1.6
+// for some of five rows); with the diagonals in float16 by 1.0 to 2.8 times, with X in
+// one float16 by up to 24, in one bfloat16 by up to 200.
 //
 // One launch does a product for every matrix of a list (48 matrices of a model of 12
 // layers fill the chip where one would not); matrices of one shape are a group, laid
@@ -48,6 +51,7 @@ struct Group {
   int sum0;      // the first one's index
   int64_t x0;    // first element in hi and lo
   int64_t a0;    // in A and B
+  int64_t d0;    // in their diagonals
   // Columns of X and of A with their padding: whole blocks of 32.
   __host__ __device__ int ldx() const { return (n + 31) & ~31; }
   __host__ __device__ int lda() const { return (m + 31) & ~31; }
@@ -69,6 +73,7 @@ struct Args {
   int groups, tensors;
   double* sums;
   f16 *hi, *hi_next, *lo, *A, *B;
+  float *diag_a, *diag_b;  // of A, and a more than of B; A and B themselves have zeros there
   float a, b, c, eps;
 };
 
@@ -297,6 +302,8 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
   const int lane = at.lane, ld = kSymmetric ? lda : ldx;
   const tile::Block block = P::block(at, 0), block_low = P::block(at, 1);
   f16* const lo = s.lo + (hi - s.hi);
+  float* const diag_a = s.diag_a + g.d0 + (int64_t)matrix * lda;
+  float* const diag_b = s.diag_b + g.d0 + (int64_t)matrix * lda;
   bf16* out = nullptr;
   if constexpr (kKind == kLast) {
     const Tensor& t = find_tensor(s, gi, matrix);
@@ -330,6 +337,17 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
 #pragma unroll
     for (int b = 0; b < kAhead; ++b) fetch(b);
   }
+  // The diagonals at the lane's rows, and (of A) at the wave's features: a feature a lane.
+  float at_row[NB], at_feature[(MB + 1) / 2];
+  if constexpr (kKind != kGram) {
+    const float* const from = kKind == kSquare ? diag_a : diag_b;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) at_row[nb] = from[min(row_first + 32 * nb + (lane & 31), lda - 1)];
+  }
+  if constexpr (kKind == kSquare) {
+#pragma unroll
+    for (int k = 0; k < (MB + 1) / 2; ++k) at_feature[k] = diag_a[min(f_first + 64 * k + lane, lda - 1)];
+  }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int row0 = row_first + 32 * nb;
@@ -353,9 +371,31 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
         for (int e = 0; e < 8; ++e) {
           float& r = v[8 * h + e];
           r = acc[mb][nb][8 * h + e];
-          if constexpr (kKind == kSquare) r = __builtin_fmaf(s.c, r, s.b * (float)x[e]);
+          if constexpr (kKind == kSquare) {
+            // b A + c A A off the diagonal, A = D + O: (b + c (D_i + D_j)) O + c O O.
+            const float other = __shfl(at_feature[mb / 2], 32 * (mb & 1) + 16 * (lane >> 5) + 8 * h + e);
+            r = __builtin_fmaf(__builtin_fmaf(s.c, at_row[nb] + other, s.b), (float)x[e], s.c * r);
+          }
           if constexpr (!kSymmetric)
-            r = settled(__builtin_fmaf(s.a, __builtin_fmaf((float)x_low[e], 1.0f / kLow, (float)x[e]), r));
+            r = settled(__builtin_fmaf(at_row[nb], __builtin_fmaf((float)x_low[e], 1.0f / kLow, (float)x[e]), r));
+        }
+      }
+      if (kSymmetric && row0 == j0) {
+        // The diagonal leaves in float32: of A as it is, of B as b D + c (D D + O O) + a.
+        // (Rows past the last are written too, zeros of A: what lies there is read.)
+        float own_diag = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (e == (lane & 31) - 16 * (lane >> 5)) {
+            own_diag = v[e];
+            v[e] = 0.f;
+          }
+        if (((lane & 31) >> 4) == (lane >> 5)) {
+          if constexpr (kKind == kGram)
+            diag_a[row0 + (lane & 31)] = own_diag;
+          else
+            diag_b[row0 + (lane & 31)] =
+                __builtin_fmaf(at_row[nb], __builtin_fmaf(s.c, at_row[nb], s.b), own_diag) + s.a;
         }
       }
       const int rows = m - row0;
@@ -409,9 +449,10 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
 size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct Sizes {
-  int64_t x = 0, a = 0, sums = 0;  // elements of hi (and lo, hi_next), of A (and B), of the sums
+  int64_t x = 0, a = 0, d = 0, sums = 0;  // elements of hi (and lo, hi_next), of A (and B), a diagonal, of the sums
   size_t bytes() const {
-    return 3 * round_up((size_t)x * 2) + 2 * round_up((size_t)a * 2) + round_up((size_t)sums * 8);
+    return 3 * round_up((size_t)x * 2) + 2 * round_up((size_t)a * 2) + 2 * round_up((size_t)d * 4) +
+           round_up((size_t)sums * 8);
   }
 };
 
@@ -428,6 +469,7 @@ Sizes size_of(const Group& g, int64_t count) {
   Sizes s;
   s.x = count * g.m * g.ldx();
   s.a = count * g.m * g.lda();
+  s.d = count * g.lda();
   s.sums = count * g.parts;
   return s;
 }
@@ -456,7 +498,7 @@ struct Walk {
       if (gi == kMostGroups) break;
       const Sizes one = size_of(shape, 1);
       const int64_t left = kMostBytes - (int64_t)total.bytes();
-      int64_t take = left / (6 * one.x + 4 * one.a + 8 * one.sums);
+      int64_t take = left / (6 * one.x + 4 * one.a + 8 * one.d + 8 * one.sums);
       if (take <= 0) {
         if (s.tensors) break;
         take = 1;
@@ -477,6 +519,7 @@ struct Walk {
       const Sizes more = size_of(shape, take);
       total.x += more.x;
       total.a += more.a;
+      total.d += more.d;
       total.sums += more.sums;
       inside += take;
       if (inside < t.count) break;
@@ -488,10 +531,12 @@ struct Walk {
       Group& g = s.g[i];
       g.x0 = from.x;
       g.a0 = from.a;
+      g.d0 = from.d;
       g.sum0 = (int)from.sums;
       const Sizes more = size_of(g, g.count);
       from.x += more.x;
       from.a += more.a;
+      from.d += more.d;
       from.sums += more.sums;
     }
     return s.groups > 0;
@@ -590,7 +635,10 @@ int gptrig_orthogonalize(const gptrig_matrices* list, int count, int type, int s
     s.lo = (f16*)(at + 2 * x);
     s.A = (f16*)(at + 3 * x);
     s.B = (f16*)(at + 3 * x + sq);
-    s.sums = (double*)(at + 3 * x + 2 * sq);
+    const size_t diag = round_up((size_t)total.d * 4);
+    s.diag_a = (float*)(at + 3 * x + 2 * sq);
+    s.diag_b = (float*)(at + 3 * x + 2 * sq + diag);
+    s.sums = (double*)(at + 3 * x + 2 * sq + 2 * diag);
     int64_t grid = count_groups(s, [](const Group& g) -> int64_t { return g.parts; });
     if (type == GPTRIG_TYPE_F32)
       ortho_norm_kernel<float><<<(unsigned)grid, 256, 0, st>>>(s);

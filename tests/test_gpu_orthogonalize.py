@@ -1,7 +1,7 @@
 """``optim.orthogonalize_tensors`` against its formula in 64 bits on the CPU.
 
-``stepped`` computes it a second time in 64 bits with the kernels' roundings: the operands, A and B to float16, the rest
-of X to float16 at 2^11 times its size, the result to bfloat16.  Its distance from the exact result is what the types
+``stepped`` computes it a second time in 64 bits with the kernels' roundings: the operands, A and B (without their
+diagonals) to float16, the rest of X to float16 at 2^11 times its size, the result to bfloat16.  Its distance from the exact result is what the types
 lose; the kernels' own roundings differ from its in their errors, not in their number or size, so two such distances lie
 between them, and a third over for the float32 sums.  A single value may be eight times the root mean square off (as far
 as a sum of many roundings hardly ever gets), and half a step of bfloat16 of its own.
@@ -41,8 +41,13 @@ def stepped(u, steps=5, coefficients=MUON, eps=1e-7, rounded=False):
     x = x.T if tall else x
     hi, lo = r(x), r((x - r(x)) * 2048)
     for _ in range(steps):
-        gram = r(hi @ hi.T)
-        x = a * (hi + lo / 2048) + r(b * gram + c * gram @ gram) @ hi
+        gram = hi @ hi.T
+        d = gram.diagonal()
+        o = r(gram - torch.diag(d))
+        square = o @ o
+        rest = (b + c * (d[:, None] + d)) * o + c * square
+        more = a + b * d + c * (d * d + square.diagonal())
+        x = more[:, None] * (hi + lo / 2048) + r(rest - torch.diag(rest.diagonal())) @ hi
         hi, lo = r(x), r((x - r(x)) * 2048)
     x = x.T if tall else x
     return x.to(F32).to(BF16).to(F64) if rounded else x

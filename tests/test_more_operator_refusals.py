@@ -184,16 +184,16 @@ def test_orthogonalize_entry_points_check_their_arguments():
 
 
 def test_orthogonalize_workspace():
-    """Three times X, A and B in 16 bits, rows padded to 32, and the sums: of one launch's tensors, which more matrices
+    """Three times X, A and B in 16 bits, rows padded to 32, two diagonals, and the sums: of one launch's tensors, which more matrices
     than fit 2 GiB do not make larger."""
 
     size = lambda *rows: _lib.lib().gptrig_orthogonalize_workspace_bytes(matrices(*rows), len(rows))  # noqa: E731
     assert size() == 0 and size((0, 0, 0, 5, 5)) == 0
-    one = 3 * 2 * 30 * 64 + 2 * 2 * 30 * 32 + 8
-    assert one <= size((0, 0, 1, 30, 50)) <= one + 6 * 255
+    one = 3 * 2 * 30 * 64 + 2 * 2 * 30 * 32 + 2 * 4 * 32 + 8
+    assert one <= size((0, 0, 1, 30, 50)) <= one + 8 * 255
     assert size((0, 0, 1, 30, 50)) == size((0, 0, 1, 50, 30))
-    assert 7 * one <= size((0, 0, 3, 30, 50), (0, 0, 4, 50, 30)) <= 7 * one + 6 * 255
-    assert 64 * one <= size(*[(0, 0, 1, 30, 50)] * 100) <= 64 * one + 6 * 255
+    assert 7 * one <= size((0, 0, 3, 30, 50), (0, 0, 4, 50, 30)) <= 7 * one + 8 * 255
+    assert 64 * one <= size(*[(0, 0, 1, 30, 50)] * 100) <= 64 * one + 8 * 255
     for rows in ([(0, 0, 1000, 2048, 2048)], [(0, 0, 1, 4096, 4096)] * 60, [(0, 0, 10 ** 9, 100, 100)]):
         assert (1 << 30) < size(*rows) <= (1 << 31) + 4096
     big = size((0, 0, 3, 65536, 65536))

@@ -292,6 +292,7 @@ def orthogonalize_tensors(updates: Sequence[torch.Tensor], *, steps: int = 5,
     for i, shape in enumerate(shapes):
         if len(shape) < 2 or max(shape[-2:]) > _MOST_SIDE:
             raise ValueError(f"updates[{i}] must be matrices of at most 65536 rows and columns, got {tuple(shape)}")
+    steps = operator.index(steps)
     if not 1 <= steps <= 1000:
         raise ValueError(f"steps must be between 1 and 1000, got {steps}")
     if len(coefficients) != 3 or not all(-_MOST_F32 <= c <= _MOST_F32 for c in coefficients):
@@ -312,5 +313,5 @@ def orthogonalize_tensors(updates: Sequence[torch.Tensor], *, steps: int = 5,
     table[1::4] = map(torch.Tensor.data_ptr, out)
     table = array.array("q", table)
     _lib.call_on(updates[0].get_device(), "gptrig_orthogonalize", table.buffer_info()[0], len(out),
-                 _MATRIX_TYPES[kind], int(steps), *map(float, coefficients), float(eps), ws.data_ptr(), size)
+                 _MATRIX_TYPES[kind], steps, *map(float, coefficients), float(eps), ws.data_ptr(), size)
     return out

@@ -301,6 +301,18 @@ __global__ void __launch_bounds__(gemm::THREADS) gated_down_bwd_kernel(Operand V
 // most of the chip idle.  Four sets of waves share a tile's K and add their parts
 // through LDS: a workgroup's time is that of its loads, one after the other.
 
+// A workgroup's tile.  kByTokens: those of one token tile follow one another on one
+// XCD, whose L2 then reads the tokens once (h V and dx of 8192 tokens 39 -> 33 and 79
+// -> 68 us); else they are dealt out to the XCDs in turn, which spreads the weights
+// (x W of 1024 tokens 20 against 26 us).
+template <bool kByTokens>
+__device__ __forceinline__ void few_tile(int features, int tile_m, int& tm, int& tn) {
+  const int across = (features + tile_m - 1) / tile_m;
+  const int pid = kByTokens ? gemm::xcd_swizzle(blockIdx.x, gridDim.x) : blockIdx.x;
+  tm = pid % across;
+  tn = pid / across;
+}
+
 // A lane's run of 16 features of a row.
 __device__ __forceinline__ void store_run(bf16* row, int feature, int features, const float* v) {
   if (feature < features) *reinterpret_cast<bf16x8*>(row + feature) = pack8(v);
@@ -311,7 +323,8 @@ template <int kAct, bool kKeep>
 __global__ void __launch_bounds__(1024) gated_up_few_kernel(tile::Operand W, tile::Operand X, UpArgs a) {
   typedef tile::Product<bf16, 2, 1, tile::kPairsMN, tile::kRowsK, true, 1, 4, 3> P;
   const auto at = P::place();
-  const int tm = blockIdx.x, tn = blockIdx.y;
+  int tm, tn;
+  few_tile<false>(2 * a.f, P::TM, tm, tn);
   f32x16 acc[2][1];
   P::run(acc, W, X, 2 * a.f, a.n, a.k, tm * P::TM, tn * P::TN, at);
   if (at.group) return;
@@ -348,7 +361,8 @@ template <int kAct>
 __global__ void __launch_bounds__(1024) gated_down_bwd_few_kernel(tile::Operand V, tile::Operand DY, DownBwdArgs a) {
   typedef tile::Product<bf16, 1, 1, tile::kRowsK, tile::kRowsK, true, 1, 4> P;
   const auto at = P::place();
-  const int tm = blockIdx.x, tn = blockIdx.y;
+  int tm, tn;
+  few_tile<false>(a.f, P::TM, tm, tn);
   f32x16 acc[1][1];
   P::run(acc, V, DY, a.f, a.n, a.k, tm * P::TM, tn * P::TN, at);
   if (at.group) return;
@@ -382,7 +396,8 @@ __global__ void __launch_bounds__(256 * kGroups, kGroups == 1 ? 2 : 1)
     gated_linear_few_kernel(tile::Operand W, tile::Operand X, bf16* y, int n, int k, int m) {
   typedef tile::Product<bf16, T, T, kW, tile::kRowsK, true, 1, kGroups> P;
   const auto at = P::place();
-  const int tm = blockIdx.x, tn = blockIdx.y;
+  int tm, tn;
+  few_tile<true>(m, P::TM, tm, tn);
   f32x16 acc[T][T];
   P::run(acc, W, X, m, n, k, tm * P::TM, tn * P::TN, at);
   if (at.group) return;
@@ -520,13 +535,15 @@ bool rows_ok(const void* p, int64_t ld, int width) {
 }
 
 // Tiles of 256 x 256 from which a product takes them.  Measured at d 768, f 2048 (us, by
-// tokens; the larger tiles against 64 x 64 with four sets of waves, or 128 x 128):
-//   x W      1024 (64 tiles) 26.7 / 19.9, 2048 (128) 28.1 / 35.3
-//   dy V^T   1024 (32) 33.8 / 18.8, 2048 (64) 33.9 / 32.7, 4096 (128) 36.5 / 62.3
-//   h V      1 42 / 7, 1024 (12) 44 / 11.6 / 17.3, 2048 (24) 44 / 22.9 / 18.3,
-//            4096 (48) 47 / 36 / 21, 8192 (96) 52 / 72 / 39, 16384 (192) 63 / 140 / 76
+// tokens, their number behind; the large tiles against 64 tokens with four sets of
+// waves, against 128 x 128):
+//   x W      1024 (64) 26 / 20, 2048 (128) 28 / 37
+//   dy V^T   1024 (32) 33 / 18, 2048 (64) 33 / 33, 4096 (128) 36 / 63
+//   h V      1 (3) 42 / 7 / 16, 1024 (12) 44 / 12 / 18, 2048 (24) 45 / 21 / 19,
+//            4096 (48) 46 / 33 / 20, 8192 (96) 53 / 65 / 33, 16384 (192) 63 / 129 / 63
+//   dx       1 77 / 12 / 28, 1024 82 / 21 / 31, 8192 91 / 130 / 68, 16384 114 / 264 / 127
 constexpr int kPairTiles = 68;                   // x W and dy V^T, against 64 tokens
-constexpr int kLinearTiles = 110, kLinearFew = 18;  // h V and dx, against 128 x 128; those against 64 x 64
+constexpr int kLinearTiles = 150, kLinearFew = 18;  // h V and dx, against 128 x 128; those against 64 x 64
 
 unsigned persistent_grid(int tiles) {
   const int cus = gemm::device_cus();
@@ -538,15 +555,15 @@ int tile_group(int m_tiles) { return m_tiles <= 16 ? m_tiles : gemm::kGroupM; }
 // Whether the product of m features over n tokens with g and u at its end goes to the tiles of 64 tokens.
 bool few(int n, int m) { return tiles_of(m, n) < kPairTiles; }
 
-dim3 few_grid(int m, int tile_m, int n) { return dim3(ceil_div(m, tile_m), ceil_div(n, 64)); }
+unsigned few_grid(int m, int tile_m, int n, int tile_n = 64) { return (unsigned)(ceil_div(m, tile_m) * ceil_div(n, tile_n)); }
 
 template <tile::Layout kW>
 void launch_linear_few(const tile::Operand& W, const tile::Operand& X, void* y, int n, int k, int m, bool wide,
                        hipStream_t s) {
   if (wide)
-    gated_linear_few_kernel<kW, 2, 1><<<dim3(ceil_div(m, 128), ceil_div(n, 128)), 256, 0, s>>>(W, X, (bf16*)y, n, k, m);
+    gated_linear_few_kernel<kW, 2, 1><<<few_grid(m, 128, n, 128), 256, 0, s>>>(W, X, (bf16*)y, n, k, m);
   else
-    gated_linear_few_kernel<kW, 1, 4><<<dim3(ceil_div(m, 64), ceil_div(n, 64)), 1024, 0, s>>>(W, X, (bf16*)y, n, k, m);
+    gated_linear_few_kernel<kW, 1, 4><<<few_grid(m, 64, n), 1024, 0, s>>>(W, X, (bf16*)y, n, k, m);
 }
 
 int linear(const void* x, int64_t ldx, const void* w, int64_t ldw, bool w_kmajor, void* y, int n, int k, int m,

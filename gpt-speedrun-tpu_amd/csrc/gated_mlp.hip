@@ -319,7 +319,7 @@ __device__ __forceinline__ void store_run(bf16* row, int feature, int features, 
   if (feature + 8 < features) *reinterpret_cast<bf16x8*>(row + feature + 8) = pack8(v + 8);
 }
 
-template <int kAct, bool kKeep>
+template <int kAct>
 __global__ void __launch_bounds__(1024) gated_up_few_kernel(tile::Operand W, tile::Operand X, UpArgs a) {
   typedef tile::Product<bf16, 2, 1, tile::kPairsMN, tile::kRowsK, true, 1, 4, 3> P;
   const auto at = P::place();
@@ -330,15 +330,13 @@ __global__ void __launch_bounds__(1024) gated_up_few_kernel(tile::Operand W, til
   if (at.group) return;
   const int lane = at.lane, first = tn * P::TN + 32 * at.wn, token = first + (lane & 31);
   const int f0 = tm * (P::TM / 2) + 32 * at.wm, feature = f0 + 16 * (lane >> 5);
-  float g[16], u[16], h[16];
+  float g[16], u[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     g[i] = acc[0][0][i];
     u[i] = acc[1][0][i];
-    h[i] = act_f<kAct>(g[i]) * u[i];
-    if (i == 7) GEMM_SCHED_FENCE();  // (sixteen at once pass the registers of 16 waves)
   }
-  if (kKeep) {
+  if (a.kept.values) {
     // (Powers are laid out by blocks of 64 features.)
     const int block = (f0 >> 5) & 1;
     const int power_g = power_of(g), power_u = power_of(u);
@@ -354,7 +352,15 @@ __global__ void __launch_bounds__(1024) gated_up_few_kernel(tile::Operand W, til
         }
     }
   }
-  if (token < a.n) store_run(a.h + (int64_t)token * a.f, feature, a.f, h);
+  if (token >= a.n) return;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (feature + 8 * e >= a.f) continue;
+    float h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = act_f<kAct>(g[8 * e + i]) * u[8 * e + i];
+    *reinterpret_cast<bf16x8*>(a.h + (int64_t)token * a.f + feature + 8 * e) = pack8(h);
+  }
 }
 
 template <int kAct>
@@ -583,10 +589,7 @@ template <int kAct>
 void launch_up(const Operand& W, const Operand& X, const UpArgs& a, hipStream_t s) {
   if (few(a.n, 2 * a.f)) {
     const tile::Operand w{W.p, W.ld, W.pair}, x{X.p, X.ld};
-    if (a.kept.values)
-      gated_up_few_kernel<kAct, true><<<few_grid(2 * a.f, 128, a.n), 1024, 0, s>>>(w, x, a);
-    else
-      gated_up_few_kernel<kAct, false><<<few_grid(2 * a.f, 128, a.n), 1024, 0, s>>>(w, x, a);
+    gated_up_few_kernel<kAct><<<few_grid(2 * a.f, 128, a.n), 1024, 0, s>>>(w, x, a);
     return;
   }
   const unsigned grid = persistent_grid(tiles_of(2 * a.f, a.n));

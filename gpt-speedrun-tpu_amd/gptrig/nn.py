@@ -1,8 +1,9 @@
 """Model primitives on gfx950, mirroring ``rig/nn.py``.
 
 ``rms_norm``, ``apply_rotary`` and ``gelu`` run the HIP kernels of
-``csrc/elementwise.hip`` with hand-written backward passes, ``layer_norm`` (not
-in ``rig/nn.py``) those of ``csrc/layernorm.hip``; ``linear`` is a
+``csrc/elementwise.hip`` with hand-written backward passes, ``layer_norm``,
+``embedding`` and ``gated_mlp`` (not in ``rig/nn.py``) those of
+``csrc/layernorm.hip``, ``embedding.hip`` and ``gated_mlp.hip``; ``linear`` is a
 plain library GEMM (hipBLASLt through torch) with the reference's bf16
 rounding points.
 """

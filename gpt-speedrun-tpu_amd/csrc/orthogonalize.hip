@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(256) ortho_load_kernel(Args s) {
   double sum = 0.0;
   for (int i = threadIdx.x; i < g.parts; i += 256) sum += s.sums[g.sum0 + (int64_t)matrix * g.parts + i];
   sum = block_sum(sum, shared);
-  const float scale = (float)(1.0 / (sqrt(sum) + (double)s.eps));
+  // (In 64 bits: the norm of large float32, and the inverse of a small one, are none.)
+  const double scale = 1.0 / (sqrt(sum) + (double)s.eps);
   if (g.tall) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(256) ortho_load_kernel(Args s) {
     f16x4 high, low;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = settled(v[k][e] * scale);
+      const float x = settled((float)((double)v[k][e] * scale));
       high[e] = (f16)x;
       low[e] = (f16)((x - (float)high[e]) * kLow);
     }
@@ -252,7 +253,6 @@ __device__ __forceinline__ void triangle(int t, int& ti, int& tj) {
   ti = kWide * p + rest / (p + 1);
   tj = rest % (p + 1);
 }
-
 
 enum { kGram = 0, kSquare = 1, kUpdate = 2, kLast = 3 };
 

@@ -99,6 +99,21 @@ def test_scales(scale):
     check(one(u), u)
 
 
+@pytest.mark.parametrize("shape", [(40, 72), (72, 40), (7, 9)])
+def test_a_power_of_two_changes_nothing(shape):
+    """Without eps: from multiples of the smallest float32 (the norm's inverse is none then) to its largest (the norm
+    itself is none)."""
+
+    g = torch.Generator().manual_seed(5)
+    u = torch.randint(-127, 128, shape, generator=g).to(F32)
+    want = one(u, eps=0.0)
+    check(want, u, eps=0.0)
+    for power in (-149, -130, 121):
+        scaled = torch.ldexp(u.to(F64), torch.tensor(power)).to(F32)
+        assert torch.equal(torch.ldexp(scaled.to(F64), torch.tensor(-power)), u.to(F64))
+        assert torch.equal(one(scaled, eps=0.0), want), power
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 8])
 def test_steps(steps):
     u = matrix(90, 140, 2.0)

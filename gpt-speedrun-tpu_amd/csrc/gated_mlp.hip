@@ -19,6 +19,11 @@
 // The weight gradients cut the tokens into slices where the tiles alone do not
 // fill the chip; each slice writes its float32 sums to the workspace and a small
 // pass adds them in order, so the result does not depend on timing.
+//
+// Measured, 65536 tokens, d 768, f 2048 (a large library product reaches 1000 to 1200
+// TFLOP/s): x W with what is kept 472 us (873 TFLOP/s; 0.8 GB written), h V 208 (991),
+// dy V^T 399 (517; 1.1 GB read and written), dx 374 (1103), both weights' gradients 622
+// (994) and 26 for their parts.
 #include "tile_core.h"
 
 namespace {

@@ -1,9 +1,9 @@
 """``optim.orthogonalize_tensors`` against its formula in 64 bits on the CPU.
 
 ``stepped`` computes it a second time in 64 bits with the kernels' roundings: the operands, A and B (without their
-diagonals) to float16, the rest of X to float16 at 2^11 times its size, the result to bfloat16.  Its distance from the exact result is what the types
-lose; the kernels' own roundings differ from its in their errors, not in their number or size, so two such distances lie
-between them, and a third over for the float32 sums.  A single value may be eight times the root mean square off (as far
+diagonals) to float16, the rest of X to float16 at 2^11 times its size, the result to bfloat16.  Its distance from the
+exact result is what the types lose; the kernels' own roundings differ from its in their errors, not in their number or
+size, so two such distances lie between them, and a third over for the float32 sums.  A single value may be eight times the root mean square off (as far
 as a sum of many roundings hardly ever gets), and half a step of bfloat16 of its own.
 """
 

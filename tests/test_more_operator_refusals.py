@@ -184,8 +184,8 @@ def test_orthogonalize_entry_points_check_their_arguments():
 
 
 def test_orthogonalize_workspace():
-    """Three times X, A and B in 16 bits, rows padded to 32, two diagonals, and the sums: of one launch's tensors, which more matrices
-    than fit 2 GiB do not make larger."""
+    """Three times X, A and B in 16 bits, rows padded to 32, two diagonals, and the sums: of one launch's
+    tensors, which more matrices than fit 2 GiB do not make larger."""
 
     size = lambda *rows: _lib.lib().gptrig_orthogonalize_workspace_bytes(matrices(*rows), len(rows))  # noqa: E731
     assert size() == 0 and size((0, 0, 0, 5, 5)) == 0

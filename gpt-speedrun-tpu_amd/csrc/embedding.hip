@@ -31,9 +31,8 @@
 namespace {
 
 constexpr int kDigits = 256;      // bins of a pass
-// Most tokens that one workgroup sorts: 34 us for 8191 of them against 23 in four
-// launches, but those cost the host more than they save the GPU (a pass 79 us against
-// 111), until there are more.
+// Most tokens that one workgroup sorts, in LDS: 22 us for 8191 of them against 23 in
+// four launches, which cost the host more besides.
 constexpr int kOneBlock = 8192;
 constexpr int kMostBlocks = 256;  // most workgroups of a pass
 constexpr int kSlab = 256;        // columns of a row that a wave holds: four a lane
@@ -73,10 +72,41 @@ __global__ void __launch_bounds__(1024) radix_histogram_kernel(Sort s, const int
   if (threadIdx.x < kDigits) counts[blockIdx.x * kDigits + threadIdx.x] = bins[threadIdx.x];
 }
 
+// Where a lane's key goes: place[digit] is where the wave's next key of that digit
+// does.  The lanes of one digit find each other by eight ballots, and their order is
+// the lanes' order.
+__device__ __forceinline__ int take_place(int* place, int digit, bool valid, int lane) {
+  uint64_t same = __ballot(valid);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const uint64_t set = __ballot((digit >> b) & 1);
+    same &= (digit >> b) & 1 ? set : ~set;
+  }
+  const int rank = __popcll(same & ((1ull << lane) - 1));
+  int at = 0;
+  if (valid) at = place[digit] + rank;
+  // (Every lane has read its place before the last of each digit moves it on;
+  // the fences order the lanes' accesses for the compiler and cost nothing.)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (valid && (same >> lane) == 1) place[digit] = at + 1;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return at;
+}
+
+// place[wave][digit] from the number of the wave's keys to where they begin.
+template <int kWaves>
+__device__ __forceinline__ void begin_places(int (*place)[kDigits], const int* bases, int tid) {
+  if (tid >= kDigits) return;
+  int at = bases[tid];
+  for (int w = 0; w < kWaves; ++w) {
+    const int c = place[w][tid];
+    place[w][tid] = at;
+    at += c;
+  }
+}
+
 // One block's stable scatter of positions [begin, end) by the digit at `shift`.
-// Each wave owns a contiguous share of them; place[wave][digit] is where its next
-// key of that digit goes.  Within 64 keys the lanes of one digit find each other
-// by eight ballots, and their order is the lanes' order.
+// Each wave owns a contiguous share of them.
 template <int kWaves>
 __device__ void scatter_block(const Sort& s, const int* keys, const int* positions, int* keys_out, int* positions_out,
                               int shift, int begin, int end, int (*place)[kDigits], int* bases) {
@@ -87,34 +117,14 @@ __device__ void scatter_block(const Sort& s, const int* keys, const int* positio
   __syncthreads();
   for (int i = from + lane; i < to; i += 64) atomicAdd(&place[wave][(load_key(s, keys, i) >> shift) & (kDigits - 1)], 1);
   __syncthreads();
-  if (tid < kDigits) {
-    int at = bases[tid];
-    for (int w = 0; w < kWaves; ++w) {
-      const int c = place[w][tid];
-      place[w][tid] = at;
-      at += c;
-    }
-  }
+  begin_places<kWaves>(place, bases, tid);
   __syncthreads();
   for (int i0 = from; i0 < to; i0 += 64) {
     const int i = i0 + lane;
     const bool valid = i < to;
     const int key = valid ? load_key(s, keys, i) : 0;
     const int digit = (key >> shift) & (kDigits - 1);
-    uint64_t same = __ballot(valid);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const uint64_t set = __ballot((digit >> b) & 1);
-      same &= (digit >> b) & 1 ? set : ~set;
-    }
-    const int rank = __popcll(same & ((1ull << lane) - 1));
-    int at = 0;
-    if (valid) at = place[wave][digit] + rank;
-    // (Every lane has read its place before the last of each digit moves it on;
-    // the fences order the lanes' accesses for the compiler and cost nothing.)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (valid && (same >> lane) == 1) place[wave][digit] = at + 1;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int at = take_place(place[wave], digit, valid, lane);
     if (valid) {
       keys_out[at] = key;
       positions_out[at] = positions ? positions[i] : i;
@@ -166,28 +176,63 @@ __global__ void __launch_bounds__(1024)
                     (int)min((int64_t)s.n, begin + s.seg), place, bases);
 }
 
-// All passes of a short sort; the buffers change roles after each.
-__global__ void __launch_bounds__(1024) radix_one_block_kernel(Sort s, int* keys_a, int* positions_a, int* keys_b,
-                                                               int* positions_b, int passes) {
-  __shared__ int place[16][kDigits];
+// All passes of a short sort.  The pairs stay in LDS, where a pass puts them in a new
+// order without the address unit's 170 cycles for 64 places (in memory: 34 us for 8191
+// pairs, 22 now); a lane holds the eight it is to place.
+__global__ void __launch_bounds__(1024) radix_one_block_kernel(Sort s, int* keys_out, int* positions_out, int passes) {
+  constexpr int kWaves = 16, kHeld = kOneBlock / (64 * kWaves);
+  __shared__ int place[kWaves][kDigits];
   __shared__ int bases[kDigits];
-  const int tid = threadIdx.x;
+  __shared__ int keys[kOneBlock], positions[kOneBlock];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int first = wave * 64 * kHeld + lane;
   if (tid == 0) *s.crossing = 0;
+  int key[kHeld], position[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    position[j] = first + 64 * j;
+    key[j] = load_key(s, nullptr, min(position[j], s.n - 1));
+  }
   for (int p = 0; p < passes; ++p) {
-    // The last pass writes b.
-    const bool to_b = ((passes - p) & 1) != 0;
-    const int* keys = p == 0 ? nullptr : to_b ? keys_a : keys_b;
-    const int* positions = p == 0 ? nullptr : to_b ? positions_a : positions_b;
-    if (tid < kDigits) bases[tid] = 0;
+    auto digit = [&](int j) { return (key[j] >> (8 * p)) & (kDigits - 1); };
+    for (int i = tid; i < kWaves * kDigits; i += 64 * kWaves) (&place[0][0])[i] = 0;
     __syncthreads();
-    for (int i = tid; i < s.n; i += 1024) atomicAdd(&bases[(load_key(s, keys, i) >> (8 * p)) & (kDigits - 1)], 1);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (first + 64 * j < s.n) atomicAdd(&place[wave][digit(j)], 1);
+    __syncthreads();
+    if (tid < kDigits) {
+      int total = 0;
+      for (int w = 0; w < kWaves; ++w) total += place[w][tid];
+      bases[tid] = total;
+    }
     __syncthreads();
     exclusive_scan(bases, tid);
-    scatter_block<16>(s, keys, positions, to_b ? keys_b : keys_a, to_b ? positions_b : positions_a, 8 * p, 0, s.n,
-                      place, bases);
-    __threadfence_block();
+    begin_places<kWaves>(place, bases, tid);
     __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const bool valid = first + 64 * j < s.n;
+      const int at = take_place(place[wave], digit(j), valid, lane);
+      if (valid) {
+        keys[at] = key[j];
+        positions[at] = position[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (first + 64 * j < s.n) {
+        key[j] = keys[first + 64 * j];
+        position[j] = positions[first + 64 * j];
+      }
   }
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (first + 64 * j < s.n) {
+      keys_out[first + 64 * j] = key[j];
+      positions_out[first + 64 * j] = position[j];
+    }
 }
 
 // ---- rows ----
@@ -553,7 +598,7 @@ int gptrig_scaled_embedding_bwd(const void* tokens, int tokens_are_int64, const 
     parts = (float*)(at + 4 * p.pairs + p.counts + p.crossing);
     const Sort sort{tokens, tokens_are_int64, vocab, (int)n, p.seg, p.blocks, crossing};
     if (p.blocks == 1) {
-      radix_one_block_kernel<<<1, 1024, 0, s>>>(sort, keys_a, positions_a, keys_b, positions_b, p.passes);
+      radix_one_block_kernel<<<1, 1024, 0, s>>>(sort, keys_b, positions_b, p.passes);
       GPTRIG_CHECK_LAUNCH();
       keys = keys_b;
       positions = positions_b;

@@ -279,8 +279,9 @@ def orthogonalize_tensors(updates: Sequence[torch.Tensor], *, steps: int = 5,
     than columns.  That moves its singular values towards 1.  The default
     coefficients move them fast, to between 0.7 and 1.2.  The products take float16
     operands: coefficients that make a value pass 65504 give infinities.  A matrix of
-    zeros stays one, or is NaN where ``eps`` is 0 too.  ``updates``: all float32 or all bfloat16, of two dimensions or more, sides at most 65536.
-    The results hold no gradient: updates that ask for one are refused.
+    zeros stays one, or is NaN where ``eps`` is 0 too.  ``updates``: all float32 or
+    all bfloat16, of two dimensions or more, sides at most 65536.  The results hold
+    no gradient: updates that ask for one are refused.
     """
 
     if not updates:

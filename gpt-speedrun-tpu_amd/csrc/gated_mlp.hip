@@ -60,8 +60,8 @@ __device__ __forceinline__ void act_both(float x, float& a, float& slope) {
 // last may be shorter) scaled by a power of two that brings its largest to 2^14 ..
 // 2^15, and those powers, a byte each, [2][runs][n].  11 bits where bfloat16 has 8,
 // in the same space: with bfloat16 the gradients of x and W were 1.76 times as far
-// off as their own rounding alone, which is 1.41 times now.  (What is 2^-25 of its
-// run's largest or less is lost.)
+// off as their own rounding alone, which is 1.41 times now.  (What is 2^-39 of its
+// run's largest or less is lost: float16 ends at 2^-25.)
 __host__ __device__ inline int runs_of(int f) { return (f + 15) / 16; }
 
 struct Kept {
@@ -89,16 +89,17 @@ struct Kept {
 };
 
 // The float32 exponent field of a run's largest value, and the factor that goes with it.
+// The lowest power is 15, whose factor 2^126 and its reciprocal are both normal numbers: a
+// run whose largest is below 2^-112 stays below 2^14.
 __device__ __forceinline__ int power_of(const float (&v)[16]) {
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
-  return max(14, __builtin_bit_cast(int, most) >> 23);
+  return max(15, __builtin_bit_cast(int, most) >> 23);
 }
 __device__ __forceinline__ float scale_down(int power) { return __builtin_bit_cast(float, (268 - power) << 23); }
-__device__ __forceinline__ float scale_up(int power) {  // its reciprocal; in two steps where that is no normal number
-  return __builtin_bit_cast(float, max(power - 14, 1) << 23);
-}
+// Its reciprocal.  (Of a power that is not there, and reads 0, any number: its values are zeros.)
+__device__ __forceinline__ float scale_up(int power) { return __builtin_bit_cast(float, (uint32_t)(power - 14) << 23); }
 
 // A wave's 32 rows of 64 features of 16 bits in LDS, on the way between its
 // accumulators' layout (runs of 16 features of a row) and lines: eight lanes hold 128

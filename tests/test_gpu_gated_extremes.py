@@ -1,0 +1,50 @@
+"""``nn.gated_mlp`` at the ends of its values' range, against its formula in 64 bits on the CPU.
+
+The bounds are those of the block's other tests (``bounds`` there), which are relative, and ``slack``: what float32 and
+bfloat16 may flush below 2^-126 of g, u, dg and du and of each product on the way.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_gpu_gated_mlp import BF16, F64, NAMES, bounds, data, exact, kernels
+
+pytestmark = pytest.mark.gpu
+
+LEAST = 2.0 ** -126
+# A few tokens, and enough tiles of 256 x 256 in x W (153) and dy V^T (85) that the kernels of those tiles take them.
+SIZES = [(40, 64, 72, 64), (4097, 64, 1032, 64)]
+
+
+def slack(x, w, v, dy):
+    x, w, v, dy = (t.to(F64).abs() for t in (x, w, v, dy))
+    n, (f, _) = len(x), v.shape
+    each = 4 * LEAST * (1 + dy @ v.T)  # of dg and du: a flushed u or g times dh, and their own
+    both = torch.cat((each, each), 1)
+    return [LEAST * (f + v.sum(0, keepdim=True).expand(n, -1)), both @ w.T + 2 * f * LEAST, x.T @ both + n * LEAST,
+            LEAST * (n + dy.sum(0, keepdim=True).expand(f, -1))]
+
+
+def off_by(a, b):
+    return (a.cpu().to(F64) - b).abs()
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("which", ["x", "gate_up_w"])
+@pytest.mark.parametrize("scale", [1e-33, 5e-35, 2e-35])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_tiny_values(sizes, scale, which, kind):
+    """g and u of some 1e-35: the gradient of what is not tiny is as small, and no less exact."""
+
+    x, w, v, dy = data(*sizes)
+    if which == "x":
+        x = (x.to(F64) * scale).to(BF16)
+    else:
+        w = (w.to(F64) * scale).to(BF16)
+    args = (x, w, v, dy)
+    wanted, limits, more = exact(*args, kind), bounds(*args, kind), slack(*args)
+    assert wanted[1 if which == "x" else 2].abs().max() > scale / 10
+    for name, a, b, limit, least in zip(NAMES, kernels(*args, kind), wanted, limits, more):
+        off = off_by(a, b)
+        assert (off <= 1.1 * limit + least).all(), (name, (off / (1.1 * limit + least)).max().item())

@@ -90,11 +90,17 @@ struct Kept {
 
 // The float32 exponent field of a run's largest value, and the factor that goes with it.
 // The lowest power is 15, whose factor 2^126 and its reciprocal are both normal numbers: a
-// run whose largest is below 2^-112 stays below 2^14.
+// run whose largest is below 2^-112 stays below 2^14.  Infinities and NaN stay what they are
+// at any power and do not count.
 __device__ __forceinline__ int power_of(const float (&v)[16]) {
   float most = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]));
+  if (most == __builtin_inff()) {
+    most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i]) == __builtin_inff() ? 0.f : fabsf(v[i]));
+  }
   return max(15, __builtin_bit_cast(int, most) >> 23);
 }
 __device__ __forceinline__ float scale_down(int power) { return __builtin_bit_cast(float, (268 - power) << 23); }

@@ -48,3 +48,26 @@ def test_tiny_values(sizes, scale, which, kind):
     for name, a, b, limit, least in zip(NAMES, kernels(*args, kind), wanted, limits, more):
         off = off_by(a, b)
         assert (off <= 1.1 * limit + least).all(), (name, (off / (1.1 * limit + least)).max().item())
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("column", [5, 64 + 37])
+@pytest.mark.parametrize("sizes", [(n, d, 64 if n == 40 else f, o) for n, d, f, o in SIZES])
+def test_a_feature_is_its_own(sizes, column, value, kind):
+    """One infinity (or NaN) of the projection spoils one feature's g or u; the weights' gradients of all others, its
+    neighbours in a run of 16 among them, are the formula's."""
+
+    n, d, f, _ = sizes
+    column = column if column < 64 else f + column - 64
+    x, w, v, dy = data(*sizes)
+    clean = (x, w.clone(), v, dy)
+    clean[1][3, column] = 0
+    w[3, column] = value
+    x[:, 3] += (x[:, 3] == 0).to(BF16)
+    wanted, limits = exact(*clean, kind), bounds(*clean, kind)
+    got = kernels(x, w, v, dy, kind)
+    others = torch.arange(f) != column % f
+    for i, at in ((2, (slice(None), others.repeat(2))), (3, (others,))):
+        off = off_by(got[i], wanted[i])[at]
+        assert (off <= 1.1 * limits[i][at] + 1e-30).all(), (NAMES[i], (off / (limits[i][at] + 1e-30)).max().item())

@@ -62,7 +62,11 @@ __device__ __forceinline__ float wave_max(float v) {
 // 1 / (1 + e) one v_rcp_f32 (1 ulp, far below the bf16 rounding of every
 // caller's result): 5 and 10 full-rate operations plus the two
 // transcendentals, against 10 and 18 for the tanh form.  Both saturate like
-// the tanh form: e = inf gives s = 0 (gelu -> -0), e = 0 gives s = 1.
+// the tanh form: e = inf gives s = 0 (gelu -> -0), e = 0 gives s = 1.  From |x| =
+// 1.1e13 on x 2u' passes float32; there s is 0 or 1, and the largest float32 in its
+// place leaves the derivative's limits 0 and 1 where infinity would make NaN.  (A
+// minimum and a maximum, whose constants are literals; the median of three holds them
+// in registers, 6 of which the persistent product with this at its end spilled.)
 __device__ __forceinline__ float gelu_f(float x) {
   constexpr float a = -2.0f * 0.7978845608028654f * GPTRIG_LOG2E;  // -2k log2(e)
   constexpr float b = a * 0.044715f;
@@ -76,7 +80,7 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
   constexpr float b2 = a2 * 3.0f * 0.044715f;       // 6kc
   const float x2 = x * x;
   const float s = __builtin_amdgcn_rcpf(1.0f + fast_exp2(x * __builtin_fmaf(x2, b, a)));
-  const float w = x * __builtin_fmaf(x2, b2, a2);
+  const float w = fmaxf(fminf(x * __builtin_fmaf(x2, b2, a2), __FLT_MAX__), -__FLT_MAX__);
   return s * __builtin_fmaf(w, 1.0f - s, 1.0f);
 }
 

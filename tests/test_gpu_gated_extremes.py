@@ -8,7 +8,9 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_gpu_gated_mlp import BF16, F64, NAMES, bounds, data, exact, kernels
+from test_gpu_gated_mlp import BF16, DEV, F64, NAMES, bounds, data, exact, kernels
+
+from gptrig.nn import gelu
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +73,34 @@ def test_a_feature_is_its_own(sizes, column, value, kind):
     for i, at in ((2, (slice(None), others.repeat(2))), (3, (others,))):
         off = off_by(got[i], wanted[i])[at]
         assert (off <= 1.1 * limits[i][at] + 1e-30).all(), (NAMES[i], (off / (limits[i][at] + 1e-30)).max().item())
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+@pytest.mark.parametrize("which,scale", [("x", 1e6), ("x", 1e13), ("x", 1e14), ("x", 1e17), ("gate", 1e14), ("gate", 1e30)])
+@pytest.mark.parametrize("sizes", [(40, 64, 64, 64), (4097, 64, 1032, 64)])
+def test_far_gates(sizes, which, scale, kind):
+    """Gates so far out that the cube in GELU's argument passes float32: its limits 0 and 1, no NaN."""
+
+    x, w, v, dy = data(*sizes)
+    if which == "x":
+        x = (x.to(F64) * scale).to(BF16)
+    else:
+        f = len(v)
+        w[:, :f] = (w[:, :f].to(F64) * scale).to(BF16)
+    args = (x, w, v, dy)
+    for name, a, b, limit in zip(NAMES, kernels(*args, kind), exact(*args, kind), bounds(*args, kind)):
+        off = off_by(a, b)
+        assert torch.isfinite(a).all() and (off <= 1.1 * limit + 1e-30).all(), name
+
+
+def test_gelu_of_far_values():
+    """``nn.gelu`` and its gradient, the same functions: 0 or x, 0 or 1."""
+
+    size = torch.tensor([20.0, 1e4, 1e6, 1e12, 1.3e13, 1.6e13, 1e14, 1e18, 1.9e19, 1e20, 1e30, 3e38], dtype=F64).to(BF16)
+    x = torch.cat((size, -size)).to(DEV).requires_grad_()
+    y = gelu(x)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(y, torch.where(x > 0, x, 0)) and torch.equal(dx, (x > 0).to(BF16))
+    x = torch.full((8,), float("nan"), dtype=BF16, device=DEV, requires_grad=True)
+    (dx,) = torch.autograd.grad(gelu(x), x, torch.ones_like(x))
+    assert torch.isnan(dx).all()

@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
     const f16* const from = kSymmetric ? A : hi;
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
-      // (Of the last row and block again where there are none: those are not used.)
+      // (Of the last row and block again where there are none: results of those are not kept.)
       const int row = min(row_first + 32 * (b / MB) + tile::Block::line_row(it, lane), m - 1);
       const int64_t own = blocked(m, row, min(f_first + 32 * (b % MB), ld - 32) + tile::Block::line_feature(lane));
       old[b % kAhead][it] = *(const i16x8*)(from + own);
@@ -417,9 +417,11 @@ __global__ void __launch_bounds__(256, 2) ortho_product_kernel(Args s) {
           block_low.put_run(lane, __builtin_bit_cast(i16x8, to_f16(v)), __builtin_bit_cast(i16x8, to_f16(v + 8)));
           store(block_low, lo + own, rows);
         }
-        // The mirrored tile.  (Past the last row and column both operands read zeros, and so are the rows' ends.)
+        // The mirrored tile, in which rows past the last are the rows' ends: zeros.  (Those
+        // lanes have v of operands that read zeros, but of another row's elements of A.)
         if (kSymmetric && past < 0) {
-          block.put_turned(lane, low, high);
+          const bool there = row0 + (lane & 31) < m;
+          block.put_turned(lane, there ? low : i16x8{}, there ? high : i16x8{});
           store(block, result + blocked(m, j0, row0), m - j0);
         }
       } else {

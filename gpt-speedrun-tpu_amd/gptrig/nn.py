@@ -266,7 +266,8 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, 
     ``tokens``: int32 or int64 of any shape; a token outside ``[0, vocab)``, such
     as -1 for padding, gives a row of zeros and takes no part in the gradient.
     ``table``: float32 or bfloat16 ``[vocab, width]``, any row stride; ``dtype``:
-    bfloat16 or float32.  Differentiable once in ``table``: the gradient has its
+    bfloat16 or float32; ``scale``: a number (read at the call; one that asks for a
+    gradient is refused).  Differentiable once in ``table``: the gradient has its
     shape and type, each row the float32 sum of its tokens' gradients in a fixed
     order, so that the same call gives the same bits.
     """
@@ -280,8 +281,11 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, 
     if table.shape[0] >= 2 ** 31 - 1 or table.shape[1] > 1 << 24 or tokens.numel() >= 2 ** 31 - 65536:
         raise ValueError(f"at most 2^31 - 2 rows of 2^24 columns and fewer than 2^31 - 65536 tokens, got "
                          f"{tuple(table.shape)} and {tuple(tokens.shape)}")
+    if isinstance(scale, torch.Tensor) and _lib.needs_autograd(scale):
+        raise RuntimeError("embedding has no derivative in scale: give it a number, or multiply the result")
     if not -_MOST_F32 <= scale <= _MOST_F32:
         raise ValueError(f"scale must be a finite float32, got {scale}")
+    scale = float(scale)
     _lib.require_one_device(table, tokens)
     if _lib.needs_autograd(table):
         return _Embedding.apply(table, tokens, scale, dtype)

@@ -47,3 +47,24 @@ def test_rows_past_the_last(m, n, count, turned):
     assert torch.isfinite(got).all()
     off = (got - want).abs()
     assert (off <= 14 * 2.0 ** -11 * C * d ** 2.5 + 2.0 ** -8 * want.abs()).all(), off.max() / (C * d ** 2.5)
+
+
+def test_on_another_stream():
+    updates = [torch.randn(s, generator=torch.Generator().manual_seed(1)).to(DEV) for s in ((70, 100), (3, 200, 40))]
+    wanted = orthogonalize_tensors(updates)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = orthogonalize_tensors(updates)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, wanted))
+
+
+def test_transforms_are_refused():
+    u = torch.randn((4, 20, 30), device=DEV)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: orthogonalize_tensors([t])[0], (u,), (u,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: orthogonalize_tensors([t])[0].float().sum())(u)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: orthogonalize_tensors([t])[0])(u)

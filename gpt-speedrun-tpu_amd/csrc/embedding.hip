@@ -5,7 +5,7 @@
 //
 // Both move rows and compute next to nothing: HBM bounds them, or the launches
 // where there are few tokens.  Measured, 65536 tokens of 768 columns: bfloat16 rows of
-// a float32 table of 50304 38 us (3.6 TB/s with each row of the table that is named
+// a float32 table of 50304 38 us (3.9 TB/s with each row of the table that is named
 // read once), the sums of the gradient 64 us (255 MB, 4.0 TB/s; a large copy 5.1), the
 // four launches of its sort 22 us, the join 9.
 //

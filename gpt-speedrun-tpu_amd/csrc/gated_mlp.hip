@@ -563,6 +563,9 @@ bool rows_ok(const void* p, int64_t ld, int width) {
 //   h V      1 (3) 42 / 7 / 16, 1024 (12) 44 / 12 / 18, 2048 (24) 45 / 21 / 19,
 //            4096 (48) 46 / 33 / 20, 8192 (96) 53 / 65 / 33, 16384 (192) 63 / 129 / 63
 //   dx       1 77 / 12 / 28, 1024 82 / 21 / 31, 8192 91 / 130 / 68, 16384 114 / 264 / 127
+// That is one pair of widths: the rule knows the number of tiles, not the depth K, and
+// elsewhere the better form may be another (dx of 5001 x 1000 with K 5328, 80 tiles: 111
+// in 128 x 128, 82 in large tiles cut along K with their parts added after).
 constexpr int kPairTiles = 68;                   // x W and dy V^T, against 64 tokens
 constexpr int kLinearTiles = 150, kLinearFew = 18;  // h V and dx, against 128 x 128; those against 64 x 64
 

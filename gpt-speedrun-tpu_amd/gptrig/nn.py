@@ -269,7 +269,9 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, 
     bfloat16 or float32; ``scale``: a number (read at the call; one that asks for a
     gradient is refused).  Differentiable once in ``table``: the gradient has its
     shape and type, each row the float32 sum of its tokens' gradients in a fixed
-    order, so that the same call gives the same bits.
+    order, so that the same call gives the same bits.  (``train.GPTTrainer`` keeps a
+    lookup of its own, the reference's: tokens clamped, the gradient added with
+    atomics.)
     """
 
     if tokens.dtype not in (torch.int32, torch.int64):

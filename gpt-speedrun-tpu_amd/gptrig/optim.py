@@ -278,10 +278,14 @@ def orthogonalize_tensors(updates: Sequence[torch.Tensor], *, steps: int = 5,
     x^T`` and ``coefficients = (a, b, c)``, on the transpose where it has more rows
     than columns.  That moves its singular values towards 1.  The default
     coefficients move them fast, to between 0.7 and 1.2.  The products take float16
-    operands: coefficients that make a value pass 65504 give infinities.  A matrix of
-    zeros stays one, or is NaN where ``eps`` is 0 too.  ``updates``: all float32 or
-    all bfloat16, of two dimensions or more, sides at most 65536.  The results hold
-    no gradient: updates that ask for one are refused.
+    operands: coefficients that make a value pass 65504 give infinities, or NaN where
+    two meet.  A matrix of zeros stays one, or is NaN where ``eps`` is 0 too.
+    ``updates``: all float32 or all bfloat16, of two dimensions or more, sides at most
+    65536.  The results hold no gradient: updates that ask for one are refused.
+
+    A call takes a workspace beside the results: six bytes an element and four for each
+    pair of a matrix's rows (its shorter side), for up to 64 tensors at a time and at
+    most 2 GiB unless one matrix alone needs more.
     """
 
     if not updates:

@@ -397,7 +397,9 @@ int gptrig_embedding_bwd(const int32_t* tokens, const void* dout, float* dtable,
  * repeats a row), y and dtable contiguous.  Pointers aligned to their element, n
  * below 2^31 - 65536 (0 allowed), d at most 2^24, vocab below 2^31 - 1.  The
  * backward takes gptrig_scaled_embedding_bwd_workspace_bytes of workspace, 16-byte
- * aligned.
+ * aligned.  (The pair above is the training step's: bf16 rows as they are, a token
+ * outside the vocabulary read as the nearest one inside, and a gradient that is added
+ * to dtable with atomics, in any order.)
  * ---------------------------------------------------------------------- */
 int gptrig_scaled_embedding_fwd(const void* tokens, int tokens_are_int64, const void* table, int64_t ldt,
                                 int table_type, void* y, int y_type, int64_t n, int d, int vocab, float scale,

@@ -14,7 +14,8 @@
 // every value here is below 2 in size, the normalised X's around (m n)^-1/2, and
 // what float16 flushes near 2^-25 is far below the sums' own rounding) and add in
 // float32.  X itself is held in two float16, the operand `hi` and the rest `lo`,
-// scaled by 2^11 so that it keeps its bits: 22 bits.  That is what the result needs:
+// scaled by 2^11 so that it keeps its bits: 22 bits, or 2^-36 where that is more (values
+// below 2^-14).  That is what the result needs:
 // an error of X in the directions of small singular values grows by a each step (485
 // times in five), but only through the term a X, which is computed from all 22 bits;
 // in B X the rounding of X meets B, which is small in those directions, and the

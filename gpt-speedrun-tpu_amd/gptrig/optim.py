@@ -279,7 +279,8 @@ def orthogonalize_tensors(updates: Sequence[torch.Tensor], *, steps: int = 5,
     than columns.  That moves its singular values towards 1.  The default
     coefficients move them fast, to between 0.7 and 1.2.  The products take float16
     operands: coefficients that make a value pass 65504 give infinities, or NaN where
-    two meet.  A matrix of zeros stays one, or is NaN where ``eps`` is 0 too.
+    two meet.  A matrix of zeros stays one, or is NaN where ``eps`` is 0 too; one whose
+    norm is far below ``eps`` gives small results, held to about 2^-36 times a^steps.
     ``updates``: all float32 or all bfloat16, of two dimensions or more, sides at most
     65536.  The results hold no gradient: updates that ask for one are refused.
 
